@@ -166,6 +166,117 @@ int tos_attention_noalloc_dev(float *out, const float *q, const void *k_cache, c
                               int kv_type, int n_heads, int n_kv, int head_dim, int pos, int max_ctx,
                               int mode, void *stream);
 
+/* ------------------------------------------- serving from a paged cache
+ * Batches of sequences of different lengths, whose keys and values lie in
+ * pages of a pool (no counterpart in the reference, which decodes one
+ * sequence over one contiguous cache, llm.c:641-743).  A step of a layer is
+ * tos_kv_append_paged_dev (per-head norm, rotation, K/V into their pages, q
+ * rotated) and then tos_attention_prompt_paged_dev for prompts or
+ * tos_attention_decode_paged_dev for single tokens.  All are asynchronous on
+ * `stream`, allocate nothing, keep nothing between calls (workspaces are
+ * written before they are read: no initialisation needed, but calls or
+ * captured graphs that may overlap need one each) and give the same bits
+ * run to run.  Lengths, positions and tables are device arrays, so a
+ * captured call may be replayed after they changed within the bounds given.
+ * The calls run on the library's device, whatever the caller's current one. */
+
+/* Rows of tokens: token t's heads lie at ptr + t * stride elements, head h
+ * at h * head_dim from there.  type: TOS_TYPE_F32 or TOS_TYPE_F16. */
+typedef struct {
+    void *ptr;
+    int64_t stride;          /* elements; at least heads * head_dim */
+    int type;
+} tos_rows_t;
+
+/* A pool of pages: row r of page p is at ((p * page_size + r) * n_kv + head)
+ * * head_dim of k and of v.  table[s * table_stride + i] is the page that
+ * holds rows [i * page_size, (i + 1) * page_size) of sequence s.  Entries that
+ * cover rows in use lie in [0, n_pages); others are not read.  A row of a
+ * page outside that range is not written, and reads as zeros. */
+typedef struct {
+    void *k, *v;
+    int type;                /* TOS_TYPE_F32 or TOS_TYPE_F16 */
+    int n_pages, page_size, n_kv, head_dim;   /* head_dim <= 256 */
+    const int *table;        /* device */
+    int n_seqs, table_stride;
+} tos_paged_kv_t;
+
+/* Rotary positions: pair i < rot_dim/2 of a head turns by pos * theta_i,
+ * theta_i = base^(-2i/rot_dim) / freq_factors[i]; elements from rot_dim on
+ * stay.  LINEAR divides theta_i by `factor`.  YARN (Peng et al. 2023) blends
+ * theta_i (fast pairs) with theta_i / factor (slow ones) along the ramp
+ * between the pairs that turn beta_fast and beta_slow times in orig_ctx
+ * positions, and multiplies the rotated elements by attn_factor * (1 + 0.1
+ * ln factor).  Angles are kept as 64-bit fractions of a turn, so far positions
+ * lose nothing.  (tos_rope_dev keeps the reference's own sine and cosine.) */
+enum { TOS_ROTARY_INTERLEAVED = 0,   /* pairs (2i, 2i + 1), as llm_rope */
+       TOS_ROTARY_HALF = 1 };        /* pairs (i, i + rot_dim/2) */
+enum { TOS_ROTARY_SCALE_NONE = 0, TOS_ROTARY_SCALE_LINEAR = 1, TOS_ROTARY_SCALE_YARN = 2 };
+typedef struct {
+    int rot_dim;             /* even, 2..256 */
+    int layout;              /* TOS_ROTARY_INTERLEAVED or TOS_ROTARY_HALF */
+    float base;
+    int scaling;             /* TOS_ROTARY_SCALE_* */
+    float factor;            /* LINEAR, YARN: >= 1 */
+    int orig_ctx;            /* YARN */
+    float beta_fast, beta_slow, attn_factor;   /* YARN: 32, 1, 1 are usual */
+    const float *freq_factors;   /* host, rot_dim/2 positive values, or NULL */
+} tos_rotary_desc_t;
+typedef struct tos_rotary tos_rotary_t;
+/* Uploads the frequencies; complete on return (not during a stream capture). */
+int tos_rotary_create(tos_rotary_t **r, const tos_rotary_desc_t *d);
+void tos_rotary_destroy(tos_rotary_t *r);   /* after the work that uses it */
+
+/* RMS norm of every head of q and k (x / sqrt(mean x^2 + eps) * w, w fp32
+ * [head_dim]; NULL: none) and its rotation at pos[t] (rot NULL: none), in one
+ * pass.  q_out / k_out may be q / k themselves (same type and stride) but not
+ * overlap them otherwise; types may differ (F32 rounded to F16 once, at the
+ * end).  q and q_out NULL with n_heads 0, likewise k.  head_dim even, <= 256. */
+int tos_qk_norm_rotary_dev(const tos_rows_t *q, const tos_rows_t *q_out, const tos_rows_t *k,
+                           const tos_rows_t *k_out, int n_tokens, int n_heads, int n_kv, int head_dim,
+                           const float *q_norm, const float *k_norm, float eps, const tos_rotary_t *rot,
+                           const int *pos, void *stream);
+
+/* Stores token t's keys (normed and rotated as above) and values as row
+ * slot[t] of sequence seq[t]; optionally q likewise into q_out (NULL both:
+ * k and v only, n_heads 0).  pos[t] is the rotation's position (the slot plus
+ * the length of a shared prefix, if any).  A token with seq[t] outside
+ * [0, kv->n_seqs) or slot[t] outside its table row stores nothing (padding).
+ * Two tokens of one call must not name the same row. */
+int tos_kv_append_paged_dev(const tos_paged_kv_t *kv, const tos_rows_t *k, const tos_rows_t *v,
+                            const tos_rows_t *q, const tos_rows_t *q_out, int n_tokens, int n_heads,
+                            const int *seq, const int *slot, const int *pos, const float *q_norm,
+                            const float *k_norm, float eps, const tos_rotary_t *rot, void *stream);
+
+/* Causal attention of packed prompts (or chunks of them): the rows
+ * cu_q[i]..cu_q[i+1]-1 of q are the last ones of sequence i, which holds
+ * kv_len[i] rows in the cache, these included; row r sees keys 0 ..
+ * kv_len[i] - (cu_q[i+1] - cu_q[i]) + r, and gives zeros where that is
+ * none.  n_seqs <= kv->n_seqs; cu_q: n_seqs + 1 ascending device ints.
+ * max_q, max_kv: no sequence has more rows / keys (what is beyond is not
+ * computed / not seen).  Rows outside the sequences stay as they were.  Heads
+ * are grouped: query head h reads key/value head h / (n_heads / n_kv).  out
+ * and q have one type and must not overlap.  Keys and values that a row does
+ * not see never reach it, infinities and NaN included. */
+size_t tos_attention_prompt_paged_workspace_bytes(int n_seqs, int total_q, int max_q, int max_kv, int n_heads,
+                                                  int n_kv, int head_dim);
+int tos_attention_prompt_paged_dev(const tos_rows_t *out, const tos_rows_t *q, const tos_paged_kv_t *kv,
+                                   const int *cu_q, const int *kv_len, int n_seqs, int total_q, int max_q,
+                                   int max_kv, int n_heads, float scale, void *workspace, size_t workspace_bytes,
+                                   void *stream);
+
+/* Attention of one token for each of n_seqs sequences: row i of q sees the
+ * prefix_len rows in the pages prefix_table[0..] (shared by all; read once
+ * for all) and then kv_len[i] rows of sequence i's own pages (at most
+ * max_kv).  prefix_len 0 (prefix_table may be NULL): plain paged decoding.
+ * A row that sees nothing gives zeros. */
+size_t tos_attention_decode_paged_workspace_bytes(int n_seqs, int max_kv, int prefix_len, int n_heads, int n_kv,
+                                                  int head_dim);
+int tos_attention_decode_paged_dev(const tos_rows_t *out, const tos_rows_t *q, const tos_paged_kv_t *kv,
+                                   const int *kv_len, int n_seqs, int max_kv, const int *prefix_table,
+                                   int prefix_len, int n_heads, float scale, void *workspace,
+                                   size_t workspace_bytes, void *stream);
+
 /* --------------------- host-pointer drop-ins for runtime/nn/llm.c statics */
 void tos_gemv(float *out, const void *weight, const float *x, int out_dim, int in_dim, int type); /* llm.c:329 */
 float tos_vec_dot(const void *weight, const float *x, int n, int type);                           /* llm.c:221 */

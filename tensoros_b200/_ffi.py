@@ -50,6 +50,24 @@ class TfDesc(C.Structure):
                [("tok_embed", vp), ("rms_final", vp)]
 
 
+class Rows(C.Structure):
+    """tos_rows_t"""
+    _fields_ = [("ptr", vp), ("stride", C.c_int64), ("type", i32)]
+
+
+class PagedKv(C.Structure):
+    """tos_paged_kv_t"""
+    _fields_ = [("k", vp), ("v", vp), ("type", i32), ("n_pages", i32), ("page_size", i32), ("n_kv", i32),
+                ("head_dim", i32), ("table", vp), ("n_seqs", i32), ("table_stride", i32)]
+
+
+class RotaryDesc(C.Structure):
+    """tos_rotary_desc_t"""
+    _fields_ = [("rot_dim", i32), ("layout", i32), ("base", f32), ("scaling", i32), ("factor", f32),
+                ("orig_ctx", i32), ("beta_fast", f32), ("beta_slow", f32), ("attn_factor", f32),
+                ("freq_factors", vp)]
+
+
 class TensorDesc(C.Structure):
     """tos_tensor_desc_t (tensor_desc_t of kernel/core/kernel.h:30-40)"""
     _fields_ = [("ndim", C.c_uint32), ("shape", C.c_uint64 * 8), ("strides", C.c_uint64 * 8), ("dtype", C.c_int32),
@@ -139,6 +157,14 @@ NN_FUNCS = {
     "tos_argmax_sharded_dev": (i32, [vp, i32, i32, vp, vp]),
     "tos_gemm_workspace_bytes": (sz, [i32, i32, i32]),
     "tos_gemm_dev": (i32, [vp, vp, i32, vp, vp, sz, vp]),
+    "tos_rotary_create": (i32, [C.POINTER(vp), C.POINTER(RotaryDesc)]),
+    "tos_rotary_destroy": (None, [vp]),
+    "tos_qk_norm_rotary_dev": (i32, [vp, vp, vp, vp, i32, i32, i32, i32, vp, vp, f32, vp, vp, vp]),
+    "tos_kv_append_paged_dev": (i32, [vp, vp, vp, vp, vp, i32, i32, vp, vp, vp, vp, vp, f32, vp, vp]),
+    "tos_attention_prompt_paged_workspace_bytes": (sz, [i32] * 7),
+    "tos_attention_prompt_paged_dev": (i32, [vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, f32, vp, sz, vp]),
+    "tos_attention_decode_paged_workspace_bytes": (sz, [i32] * 6),
+    "tos_attention_decode_paged_dev": (i32, [vp, vp, vp, vp, i32, i32, vp, i32, i32, f32, vp, sz, vp]),
     "tos_tf_rmsnorm": (None, [vp, vp, vp, i32]),
     "tos_tf_swiglu_ffn": (None, [vp, vp, vp, vp, vp, i32, i32]),
     "tos_tf_model_create": (i32, [C.POINTER(vp), C.POINTER(TfDesc)]),

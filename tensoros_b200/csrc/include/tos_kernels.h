@@ -252,6 +252,63 @@ size_t tosk_step_sync_bytes(void);
 int tosk_step_check(const tosk_step_t *s);
 int tosk_step_launch(const tosk_step_t *s, cudaStream_t st);
 
+/* ------------------------------------------------ paged cache (paged_*.cu) */
+typedef struct {
+    const void *src;             /* tokens' rows (NULL: none) */
+    void *dst;
+    long long sstride, dstride;  /* elements from one token to the next */
+    int stype, dtype;
+} tosk_rows_t;
+
+typedef struct {
+    void *k, *v;
+    int type, n_pages, page_size, n_kv, hd;
+    const int *table;
+    int n_seqs, table_stride;
+} tosk_paged_t;
+
+/* Frequencies of a rotation: turns per position of each pair in units of
+ * 2^-64 (device), and the magnitude of the rotated elements. */
+typedef struct {
+    unsigned long long *turn;
+    int rot, half;
+    float mag;
+} tosk_rotary_t;
+
+typedef struct {
+    tosk_rows_t q, k, v;         /* v: append only */
+    int n_tokens, n_heads, n_kv, hd;
+    const float *q_norm, *k_norm;
+    float eps;
+    tosk_rotary_t rot;           /* turn NULL: no rotation */
+    const int *pos;
+    int append;                  /* 1: k and v go to the pages of kv */
+    tosk_paged_t kv;
+    const int *seq, *slot;
+} tosk_rotary_args_t;
+int tosk_rotary_rows(const tosk_rotary_args_t *a, cudaStream_t st);
+
+typedef struct {
+    void *out;
+    const void *q;
+    long long out_stride, q_stride;
+    int type;                    /* of q and out */
+    tosk_paged_t kv;
+    const int *cu_q;             /* NULL: one row a sequence (decode) */
+    const int *kv_len;
+    int n_seqs, total_q, max_q, max_kv, n_heads;
+    const int *prefix_table;     /* decode */
+    int prefix_len;
+    float scale;
+    void *ws;
+    size_t ws_bytes;
+    int *err;
+} tosk_paged_attn_t;
+size_t tosk_paged_prompt_ws_bytes(int n_seqs, int total_q, int max_q, int max_kv, int n_heads, int n_kv, int hd);
+size_t tosk_paged_decode_ws_bytes(int n_seqs, int max_kv, int prefix_len, int n_heads, int n_kv, int hd);
+int tosk_paged_prompt(const tosk_paged_attn_t *a, cudaStream_t st);
+int tosk_paged_decode(const tosk_paged_attn_t *a, cudaStream_t st);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,442 @@
+// paged_attention.cu - attention over a paged K/V cache: the general kernel
+// (any head dimension up to 256, fp32 or fp16 cache, any page size), the
+// joining of a split key axis, and the launch plans.
+//
+//   o_r = sum_j w_j v_j / sum_j w_j,  w_j = 2^(c q_r.k_j - m),  c = scale log2 e
+//
+// in one pass over the keys with a running maximum m and sum per row; a new
+// maximum scales what was summed so far by 2^(m_old - m_new).
+//
+// general kernel.  A CTA takes R packed rows (token, query head of the group)
+// of one sequence and one key/value head, so a K/V row read serves all of the
+// group's heads, and walks the keys in tiles of 64 staged in shared memory as
+// fp32.  256 threads as 16 x 16: thread (ty, tx) owns rows ty + 16 i and, for
+// the scores, keys tx + 16 j, for the sums, dims 4 tx + 64 j.  All arithmetic
+// is fp32 FMA.  R = 64 for prompts, 16 where a sequence brings few rows.
+#include <cuda_runtime.h>
+
+#include "paged_common.cuh"
+
+namespace tos {
+
+constexpr int kKT = 64;      // keys a tile
+constexpr int kGenThreads = 256;
+
+__device__ __forceinline__ float4 load4(const void* p, int type, long long i, bool vec) {
+  if (type == TOSK_F32) {
+    const float* f = reinterpret_cast<const float*>(p) + i;
+    if (vec) return *reinterpret_cast<const float4*>(f);
+    return make_float4(f[0], f[1], f[2], f[3]);
+  }
+  const __half* h = reinterpret_cast<const __half*>(p) + i;
+  if (vec) {
+    const uint2 u = *reinterpret_cast<const uint2*>(h);
+    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&u.x));
+    const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
+    return make_float4(a.x, a.y, b.x, b.y);
+  }
+  return make_float4(__half2float(h[0]), __half2float(h[1]), __half2float(h[2]), __half2float(h[3]));
+}
+// four elements from i on of a row of hd, zeros behind its end
+__device__ __forceinline__ float4 load4_tail(const void* p, int type, long long row, int d, int hd, bool vec) {
+  if (d + 4 <= hd) return load4(p, type, row + d, vec);
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (d < hd) v.x = load_elem(p, type, row + d);
+  if (d + 1 < hd) v.y = load_elem(p, type, row + d + 1);
+  if (d + 2 < hd) v.z = load_elem(p, type, row + d + 2);
+  return v;
+}
+
+struct GenArgs {
+  PagedProblem p;
+  int rtiles;                // row tiles of the longest sequence
+  int q_vec, kv_vec;         // four-element accesses are aligned
+};
+
+template <int R, int NJ>
+__global__ void __launch_bounds__(kGenThreads) paged_attn_general_kernel(const GenArgs a) {
+  constexpr int RI = R / 16, LD = 64 * NJ + 4, LP = kKT + 4;
+  extern __shared__ float sm[];
+  float* sq = sm;                       // [R][LD]
+  float* sk = sq + R * LD;              // [kKT][LD]
+  float* sv = sk + kKT * LD;            // [kKT][LD]
+  float* sp = sv + kKT * LD;            // [R][LP]
+  __shared__ int s_bad[R];
+  const PagedProblem& p = a.p;
+  pdl_wait();
+  pdl_trigger();
+  int b = blockIdx.x;
+  const int kvh = b % p.n_kv;
+  b /= p.n_kv;
+  const int seq = b % p.n_seqs;
+  b /= p.n_seqs;
+  const int split = p.splits ? b % p.splits : 0;
+  const int rt = a.rtiles - 1 - (p.splits ? b / p.splits : b);   // long rows first
+  const SeqTask t = seq_task(p, seq);
+  const int rows = t.qn * p.group, r0 = rt * R;
+  if (r0 >= rows) return;
+  const int nr = min(R, rows - r0);
+  int k0 = 0, k1 = seen(p, t, (r0 + nr - 1) / p.group);
+  if (p.splits) {
+    k0 = split * p.chunk;
+    k1 = min(k1, k0 + p.chunk);
+    if (k0 >= k1) return;               // no row of the tile sees a key of this split
+  }
+  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+  const int hd4 = (p.hd + 3) / 4;
+  for (int i = tid; i < R; i += kGenThreads) s_bad[i] = 0;
+  for (int i = tid; i < R * 16 * NJ; i += kGenThreads) {
+    const int r = i / (16 * NJ), c = i % (16 * NJ);
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (r < nr && c < hd4) {
+      const int rr = r0 + r;
+      v = load4_tail(p.q, p.type, (long long)(t.q0 + rr / p.group) * p.q_stride +
+                                      (long long)(kvh * p.group + rr % p.group) * p.hd, 4 * c, p.hd, a.q_vec);
+    }
+    *reinterpret_cast<float4*>(sq + r * LD + 4 * c) = v;
+  }
+  int lim[RI];
+  float m[RI], l[RI], o[RI][NJ][4];
+#pragma unroll
+  for (int i = 0; i < RI; ++i) {
+    const int r = ty + 16 * i;
+    lim[i] = r < nr ? seen(p, t, (r0 + r) / p.group) : 0;
+    m[i] = -INFINITY;
+    l[i] = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[i][j][e] = 0.0f;
+  }
+  for (int kt = k0; kt < k1; kt += kKT) {
+    __syncthreads();
+    for (int i = tid; i < kKT * 16 * NJ; i += kGenThreads) {
+      const int r = i / (16 * NJ), c = i % (16 * NJ);
+      float4 kx = make_float4(0.f, 0.f, 0.f, 0.f), vx = kx;
+      if (kt + r < k1 && c < hd4) {
+        const long long off = kv_off(p, t.table, kt + r, kvh);
+        if (off >= 0) {
+          kx = load4_tail(p.k, p.kv_type, off, 4 * c, p.hd, a.kv_vec);
+          vx = load4_tail(p.v, p.kv_type, off, 4 * c, p.hd, a.kv_vec);
+        }
+      }
+      *reinterpret_cast<float4*>(sk + r * LD + 4 * c) = kx;
+      *reinterpret_cast<float4*>(sv + r * LD + 4 * c) = vx;
+    }
+    __syncthreads();
+    float s[RI][4];
+#pragma unroll
+    for (int i = 0; i < RI; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[i][j] = 0.0f;
+    for (int c = 0; c < hd4; ++c) {
+      float4 kx[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) kx[j] = *reinterpret_cast<const float4*>(sk + (tx + 16 * j) * LD + 4 * c);
+#pragma unroll
+      for (int i = 0; i < RI; ++i) {
+        const float4 qx = *reinterpret_cast<const float4*>(sq + (ty + 16 * i) * LD + 4 * c);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          s[i][j] = fmaf(qx.w, kx[j].w, fmaf(qx.z, kx[j].z, fmaf(qx.y, kx[j].y, fmaf(qx.x, kx[j].x, s[i][j]))));
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < RI; ++i) {
+      float mx = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        s[i][j] = kt + tx + 16 * j < min(lim[i], k1) ? s[i][j] * p.scale_log2 : -INFINITY;
+        mx = fmaxf(mx, s[i][j]);
+      }
+#pragma unroll
+      for (int x = 8; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+      const float mn = fmaxf(m[i], mx), base = mn == -INFINITY ? 0.0f : mn;
+      const float c = exp2f(m[i] - base);       // 2^-inf = 0 on a row's first keys
+      m[i] = mn;
+      float sum = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float w = exp2f(s[i][j] - base);
+        sum += w;
+        sp[(ty + 16 * i) * LP + tx + 16 * j] = w;
+      }
+      l[i] = fmaf(l[i], c, sum);                // this thread's keys; joined at the end
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[i][j][e] *= c;
+    }
+    __syncwarp();                               // a row's weights come from its own half warp
+    const int kn = min(kKT, k1 - kt);
+    for (int kk = 0; kk < kn; ++kk) {
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const float4 vx = *reinterpret_cast<const float4*>(sv + kk * LD + 4 * tx + 64 * j);
+#pragma unroll
+        for (int i = 0; i < RI; ++i) {
+          const float w = sp[(ty + 16 * i) * LP + kk];
+          o[i][j][0] = fmaf(w, vx.x, o[i][j][0]);
+          o[i][j][1] = fmaf(w, vx.y, o[i][j][1]);
+          o[i][j][2] = fmaf(w, vx.z, o[i][j][2]);
+          o[i][j][3] = fmaf(w, vx.w, o[i][j][3]);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < RI; ++i) {
+    float sum = l[i];
+#pragma unroll
+    for (int x = 8; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+    const int r = ty + 16 * i;
+    if (r >= nr) continue;
+    const int rr = r0 + r, tok = t.q0 + rr / p.group, h = kvh * p.group + rr % p.group;
+    if (p.splits) {
+      const long long row = (long long)(p.slot0 + split) * p.total_q * p.heads + (long long)tok * p.heads + h;
+      if (tx == 0) p.part_ml[row] = make_float2(m[i], sum);
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (4 * tx + 64 * j + e < p.hd) p.part_o[row * p.hd + 4 * tx + 64 * j + e] = o[i][j][e];
+    } else {
+      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+      const long long oo = (long long)tok * p.out_stride + (long long)h * p.hd;
+      bool bad = false;
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float v = o[i][j][e] * inv;
+          if (4 * tx + 64 * j + e < p.hd) {
+            store_elem(p.out, p.type, oo + 4 * tx + 64 * j + e, v);
+            bad |= isnan(v);
+          }
+        }
+      if (bad) s_bad[r] = 1;
+    }
+  }
+  if (p.splits) return;
+  __syncthreads();
+  for (int r = tid >> 5; r < nr; r += kGenThreads / 32)
+    if (s_bad[r]) {
+      const int rr = r0 + r;
+      attn_row_plain(p, nullptr, 0, t.table, seen(p, t, rr / p.group), t.q0 + rr / p.group,
+                     kvh * p.group + rr % p.group);
+    }
+}
+
+// Joins the partial rows of a split key axis: o = sum_s 2^(m_s - M) o_s /
+// sum_s 2^(m_s - M) l_s.  A warp a row; the slots of the prefix come first.
+struct JoinArgs {
+  PagedProblem p;              // of the sequences' own keys; splits: slots they have
+  int pre_splits;              // slots of the prefix, all of them written
+  const int* prefix_table;
+  int prefix_len;
+};
+
+__global__ void __launch_bounds__(128) paged_attn_join_kernel(const JoinArgs a) {
+  const PagedProblem& p = a.p;
+  pdl_wait();
+  pdl_trigger();
+  const int lane = threadIdx.x & 31;
+  const int seq = blockIdx.y;
+  const SeqTask t = seq_task(p, seq);
+  const int w = blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (w >= t.qn * p.heads) return;
+  const int r = w / p.heads, h = w % p.heads, tok = t.q0 + r;
+  const int n = seen(p, t, r);
+  const int own = (n + p.chunk - 1) / p.chunk;
+  const long long row = (long long)tok * p.heads + h, step = (long long)p.total_q * p.heads;
+  const int cnt = a.pre_splits + own;
+  float M = -INFINITY;
+  for (int s = lane; s < cnt; s += 32) M = fmaxf(M, p.part_ml[s * step + row].x);
+  for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
+  const float base = M == -INFINITY ? 0.0f : M;
+  float L = 0.0f, o[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) o[i] = 0.0f;
+  for (int s = 0; s < cnt; ++s) {
+    const float2 ml = p.part_ml[s * step + row];
+    const float c = exp2f(ml.x - base);
+    L = fmaf(ml.y, c, L);
+    const float* src = p.part_o + (s * step + row) * p.hd;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (lane + 32 * i < p.hd) o[i] = fmaf(src[lane + 32 * i], c, o[i]);
+  }
+  const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+  const long long oo = (long long)tok * p.out_stride + (long long)h * p.hd;
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float v = o[i] * inv;
+    if (lane + 32 * i < p.hd) {
+      store_elem(p.out, p.type, oo + lane + 32 * i, v);
+      bad |= isnan(v);
+    }
+  }
+  if (__any_sync(0xffffffffu, bad)) attn_row_plain(p, a.prefix_table, a.prefix_len, t.table, n, tok, h);
+}
+
+}  // namespace tos
+
+using namespace tos;
+
+namespace {
+constexpr int kSms = 148;
+
+int launch(const void* func, dim3 grid, int threads, size_t smem, const void* arg, cudaStream_t st) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  void* args[] = {const_cast<void*>(arg)};
+  return (int)cudaLaunchKernelExC(&cfg, func, args);
+}
+
+PagedProblem problem_of(const tosk_paged_attn_t* a) {
+  PagedProblem p = {};
+  p.out = a->out; p.q = a->q;
+  p.out_stride = a->out_stride; p.q_stride = a->q_stride;
+  p.type = a->type;
+  p.k = a->kv.k; p.v = a->kv.v;
+  p.kv_type = a->kv.type; p.n_pages = a->kv.n_pages; p.page_size = a->kv.page_size;
+  p.n_kv = a->kv.n_kv; p.hd = a->kv.hd;
+  p.heads = a->n_heads; p.group = a->n_heads / a->kv.n_kv;
+  p.table = a->kv.table; p.table_stride = a->kv.table_stride;
+  p.cu_q = a->cu_q; p.kv_len = a->kv_len;
+  p.n_seqs = a->n_seqs; p.total_q = a->total_q; p.max_q = a->max_q; p.max_kv = a->max_kv;
+  p.fixed_kv = -1;
+  p.causal = 1;
+  p.scale_log2 = a->scale * 1.4426950408889634f;
+  p.err = a->err;
+  return p;
+}
+
+size_t slot_bytes(int total_q, int heads, int hd) {
+  return (((size_t)total_q * heads * ((size_t)hd * 4 + 8)) + 15) & ~(size_t)15;
+}
+
+// ------------------------------------------------------------ general kernel
+bool aligned4(const void* p, long long stride, int type, int hd) {
+  return ((uintptr_t)p & (type == TOSK_F32 ? 15 : 7)) == 0 && stride % 4 == 0 && hd % 4 == 0;
+}
+
+template <int R, int NJ>
+int general_launch(const GenArgs& g, long long grid, cudaStream_t st) {
+  const size_t smem = ((size_t)(R + 2 * kKT) * (64 * NJ + 4) + (size_t)R * (kKT + 4)) * 4;
+  const void* f = (const void*)paged_attn_general_kernel<R, NJ>;
+  // per call: the attribute belongs to the device, and setting it is a host-side store
+  const cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return (int)e;
+  return launch(f, dim3((unsigned)grid), kGenThreads, smem, &g, st);
+}
+
+template <int R>
+int general_rows(const PagedProblem& p, cudaStream_t st) {
+  GenArgs g;
+  g.p = p;
+  const long long rows = (long long)(p.fixed_kv >= 0 ? p.total_q : p.max_q) * p.group;
+  g.rtiles = (int)((rows + R - 1) / R);
+  g.q_vec = aligned4(p.q, p.q_stride, p.type, p.hd);
+  g.kv_vec = aligned4(p.k, 4, p.kv_type, p.hd) && aligned4(p.v, 4, p.kv_type, p.hd);
+  const long long grid = (long long)g.rtiles * (p.splits ? p.splits : 1) * p.n_seqs * p.n_kv;
+  if (grid > 0x7fffffffll) return (int)cudaErrorInvalidValue;
+  if (p.hd <= 64) return general_launch<R, 1>(g, grid, st);
+  if (p.hd <= 128) return general_launch<R, 2>(g, grid, st);
+  return general_launch<R, 4>(g, grid, st);
+}
+
+int run_general(const PagedProblem& p, cudaStream_t st) {
+  const long long rows = (long long)(p.fixed_kv >= 0 ? p.total_q : p.max_q) * p.group;
+  return rows <= 32 ? general_rows<16>(p, st) : general_rows<64>(p, st);
+}
+
+// Splits of a key axis: enough CTAs for two rounds over the SMs, at least 256
+// keys each.
+int plan_splits(long long tiles, int keys) {
+  const long long want = (2 * kSms + tiles - 1) / tiles;
+  const long long most = (keys + 255) / 256;
+  const long long s = want < most ? want : most;
+  return s < 1 ? 1 : (int)s;
+}
+int chunk_of(int keys, int splits) { return ((keys + splits - 1) / splits + kKT - 1) / kKT * kKT; }
+
+struct DecodePlan {
+  int own, own_chunk, pre, pre_chunk;   // own 0: straight to out
+};
+DecodePlan plan_decode(int n_seqs, int max_kv, int prefix_len, int heads, int n_kv) {
+  DecodePlan d;
+  const long long rows = (long long)n_seqs * (heads / n_kv);
+  d.pre = prefix_len > 0 ? plan_splits((rows + 63) / 64 * n_kv, prefix_len) : 0;
+  d.pre_chunk = d.pre ? chunk_of(prefix_len, d.pre) : 0;
+  if (d.pre) d.pre = (prefix_len + d.pre_chunk - 1) / d.pre_chunk;
+  d.own = max_kv > 0 ? plan_splits((long long)n_seqs * n_kv, max_kv) : 1;
+  d.own_chunk = max_kv > 0 ? chunk_of(max_kv, d.own) : kKT;
+  if (max_kv > 0) d.own = (max_kv + d.own_chunk - 1) / d.own_chunk;
+  if (!d.pre && d.own == 1) d.own = 0;
+  return d;
+}
+
+int run_join(const PagedProblem& own, int pre, const int* prefix_table, int prefix_len, cudaStream_t st) {
+  JoinArgs j;
+  j.p = own;
+  j.pre_splits = pre;
+  j.prefix_table = prefix_table;
+  j.prefix_len = prefix_len;
+  const long long gx = ((long long)own.max_q * own.heads + 3) / 4;
+  if (gx > 0x7fffffffll || own.n_seqs > 65535) return (int)cudaErrorInvalidValue;
+  return launch((const void*)paged_attn_join_kernel, dim3((unsigned)gx, own.n_seqs), 128, 0, &j, st);
+}
+
+void part_views(PagedProblem& p, void* ws, int slots) {
+  p.part_ml = reinterpret_cast<float2*>(ws);
+  p.part_o = reinterpret_cast<float*>(p.part_ml + (size_t)slots * p.total_q * p.heads);
+}
+}  // namespace
+
+extern "C" size_t tosk_paged_prompt_ws_bytes(int, int, int, int, int, int, int) { return 0; }
+
+extern "C" size_t tosk_paged_decode_ws_bytes(int n_seqs, int max_kv, int prefix_len, int n_heads, int n_kv, int hd) {
+  const DecodePlan d = plan_decode(n_seqs, max_kv, prefix_len, n_heads, n_kv);
+  return (size_t)(d.own + d.pre) * slot_bytes(n_seqs, n_heads, hd);
+}
+
+extern "C" int tosk_paged_prompt(const tosk_paged_attn_t* a, cudaStream_t st) {
+  return run_general(problem_of(a), st);
+}
+
+extern "C" int tosk_paged_decode(const tosk_paged_attn_t* a, cudaStream_t st) {
+  PagedProblem p = problem_of(a);
+  const DecodePlan d = plan_decode(a->n_seqs, a->max_kv, a->prefix_len, a->n_heads, a->kv.n_kv);
+  if (!d.own) return run_general(p, st);
+  part_views(p, a->ws, d.own + d.pre);
+  if (d.pre) {
+    PagedProblem x = p;
+    x.table = a->prefix_table;
+    x.n_seqs = 1;
+    x.cu_q = nullptr;
+    x.fixed_kv = a->prefix_len;
+    x.causal = 0;
+    x.splits = d.pre;
+    x.chunk = d.pre_chunk;
+    const int e = run_general(x, st);
+    if (e) return e;
+  }
+  p.splits = d.own;
+  p.chunk = d.own_chunk;
+  p.slot0 = d.pre;
+  if (a->max_kv > 0) {
+    const int e = run_general(p, st);
+    if (e) return e;
+  }
+  return run_join(p, d.pre, a->prefix_table, a->prefix_len, st);
+}
