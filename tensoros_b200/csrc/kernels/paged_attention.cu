@@ -16,6 +16,7 @@
 #include <cuda_runtime.h>
 
 #include "paged_common.cuh"
+#include "paged_tc.cuh"
 
 namespace tos {
 
@@ -322,7 +323,7 @@ PagedProblem problem_of(const tosk_paged_attn_t* a) {
 }
 
 size_t slot_bytes(int total_q, int heads, int hd) {
-  return (((size_t)total_q * heads * ((size_t)hd * 4 + 8)) + 15) & ~(size_t)15;
+  return (size_t)total_q * heads * ((size_t)hd * 4 + 8) + 16;
 }
 
 // ------------------------------------------------------------ general kernel
@@ -368,7 +369,8 @@ int plan_splits(long long tiles, int keys) {
   const long long s = want < most ? want : most;
   return s < 1 ? 1 : (int)s;
 }
-int chunk_of(int keys, int splits) { return ((keys + splits - 1) / splits + kKT - 1) / kKT * kKT; }
+// Keys a split, a multiple of the tensor-core kernel's tile.
+int chunk_of(int keys, int splits) { return ((keys + splits - 1) / splits + 127) / 128 * 128; }
 
 struct DecodePlan {
   int own, own_chunk, pre, pre_chunk;   // own 0: straight to out
@@ -376,11 +378,11 @@ struct DecodePlan {
 DecodePlan plan_decode(int n_seqs, int max_kv, int prefix_len, int heads, int n_kv) {
   DecodePlan d;
   const long long rows = (long long)n_seqs * (heads / n_kv);
-  d.pre = prefix_len > 0 ? plan_splits((rows + 63) / 64 * n_kv, prefix_len) : 0;
+  d.pre = prefix_len > 0 ? plan_splits((rows + 255) / 256 * n_kv, prefix_len) : 0;
   d.pre_chunk = d.pre ? chunk_of(prefix_len, d.pre) : 0;
   if (d.pre) d.pre = (prefix_len + d.pre_chunk - 1) / d.pre_chunk;
   d.own = max_kv > 0 ? plan_splits((long long)n_seqs * n_kv, max_kv) : 1;
-  d.own_chunk = max_kv > 0 ? chunk_of(max_kv, d.own) : kKT;
+  d.own_chunk = max_kv > 0 ? chunk_of(max_kv, d.own) : 128;
   if (max_kv > 0) d.own = (max_kv + d.own_chunk - 1) / d.own_chunk;
   if (!d.pre && d.own == 1) d.own = 0;
   return d;
@@ -398,12 +400,32 @@ int run_join(const PagedProblem& own, int pre, const int* prefix_table, int pref
 }
 
 void part_views(PagedProblem& p, void* ws, int slots) {
-  p.part_ml = reinterpret_cast<float2*>(ws);
-  p.part_o = reinterpret_cast<float*>(p.part_ml + (size_t)slots * p.total_q * p.heads);
+  const size_t rows = (size_t)slots * p.total_q * p.heads;
+  p.part_o = reinterpret_cast<float*>(ws);
+  p.part_ml = reinterpret_cast<float2*>(reinterpret_cast<uint8_t*>(ws) + ((rows * p.hd * 4 + 15) & ~(size_t)15));
+}
+
+// Many rows a sequence: the tensor cores where the cache allows it.
+int run_tiles(const PagedProblem& p, cudaStream_t st) { return paged_tc_ok(p) ? paged_tc_run(p, st) : run_general(p, st); }
+
+// Splits of a prompt call's keys (0: none): row tiles of 256 that leave SMs
+// without work are cut along the keys, at least 512 a split.
+int plan_prompt(int n_seqs, int total_q, int max_q, int max_kv, int heads, int n_kv) {
+  const long long g = heads / n_kv;
+  long long tiles = ((long long)max_q * g + 255) / 256 * n_seqs;
+  const long long most = ((long long)total_q * g + 255) / 256 + n_seqs;
+  if (most < tiles) tiles = most;
+  tiles *= n_kv;
+  long long s = kSms / tiles;
+  if (s > (max_kv + 511) / 512) s = (max_kv + 511) / 512;
+  return s > 1 ? (int)s : 0;
 }
 }  // namespace
 
-extern "C" size_t tosk_paged_prompt_ws_bytes(int, int, int, int, int, int, int) { return 0; }
+extern "C" size_t tosk_paged_prompt_ws_bytes(int n_seqs, int total_q, int max_q, int max_kv, int n_heads, int n_kv,
+                                             int hd) {
+  return (size_t)plan_prompt(n_seqs, total_q, max_q, max_kv, n_heads, n_kv) * slot_bytes(total_q, n_heads, hd);
+}
 
 extern "C" size_t tosk_paged_decode_ws_bytes(int n_seqs, int max_kv, int prefix_len, int n_heads, int n_kv, int hd) {
   const DecodePlan d = plan_decode(n_seqs, max_kv, prefix_len, n_heads, n_kv);
@@ -411,7 +433,13 @@ extern "C" size_t tosk_paged_decode_ws_bytes(int n_seqs, int max_kv, int prefix_
 }
 
 extern "C" int tosk_paged_prompt(const tosk_paged_attn_t* a, cudaStream_t st) {
-  return run_general(problem_of(a), st);
+  PagedProblem p = problem_of(a);
+  p.splits = plan_prompt(a->n_seqs, a->total_q, a->max_q, a->max_kv, a->n_heads, a->kv.n_kv);
+  if (!p.splits) return run_tiles(p, st);
+  p.chunk = chunk_of(a->max_kv, p.splits);
+  part_views(p, a->ws, p.splits);
+  const int e = run_tiles(p, st);
+  return e ? e : run_join(p, 0, nullptr, 0, st);
 }
 
 extern "C" int tosk_paged_decode(const tosk_paged_attn_t* a, cudaStream_t st) {
@@ -428,7 +456,7 @@ extern "C" int tosk_paged_decode(const tosk_paged_attn_t* a, cudaStream_t st) {
     x.causal = 0;
     x.splits = d.pre;
     x.chunk = d.pre_chunk;
-    const int e = run_general(x, st);
+    const int e = run_tiles(x, st);
     if (e) return e;
   }
   p.splits = d.own;

@@ -1,0 +1,567 @@
+// paged_attention_tc.cu - attention of many query rows over an fp16 paged
+// cache on the tensor cores (tcgen05): prompts, and a decode batch over its
+// shared prefix.
+//
+//   S = Q K^T,  P = 2^(c S - m),  O += P V,  l += sum P     (128 x 128 tiles)
+//
+// A CTA takes 256 packed rows (token, query head of the group) of one
+// sequence and one key/value head as two tiles of 128 and walks the keys in
+// tiles of 128:
+//   * warp 8 brings K and V tiles, page by page, into a ring of shared memory
+//     slots (TMA boxes of a page's rows x 64 columns, swizzled 128 B; lane i
+//     takes page i of the tile);
+//   * warp 9 issues the MMAs in the order PV0(j) S0(j+1) PV1(j) S1(j+1), so
+//     the tensor cores work on one row tile while the other's softmax runs;
+//     accumulators in tensor memory: S0, S1 (128 columns each), O0, O1;
+//   * warps 0-3 and 4-7 hold one row tile each, a row a thread: S from tensor
+//     memory, the row's maximum and sum without any exchange, P back into
+//     S's columns as the A operand of P V.
+// The maximum in use follows the true one only when that has grown by more
+// than 2^8 (O is then scaled in tensor memory), so O is touched rarely.
+// P carries a factor 2^7, at most 2^15, which keeps small weights out of
+// fp16's subnormals; it cancels in O / l.
+//
+// Precision.  fp16 rows: P is rounded to fp16 (half a step, 2^-11, of each
+// weight, which is what the output's own rounding costs; sums and maxima are
+// fp32).  fp32 rows: q, scaled by a power of two per row, and P go in as
+// exact fp16 pairs hi + lo (22 bits), two MMAs each, so results are fp32's.
+//
+// Keys behind a row's last one are masked in S; value rows behind the key
+// range are zeroed in shared memory (a page's unused rows may hold
+// anything), and a row that shows NaN is computed again key by key
+// (attn_row_plain), so an unseen infinity never reaches it.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+#include <cuda_runtime.h>
+
+#include "paged_common.cuh"
+#include "paged_tc.cuh"
+
+namespace tos {
+
+constexpr int kTcThreads = 320;
+constexpr int kRows = 128;            // rows of a tile
+constexpr int kKeys = 128;            // keys of a tile
+constexpr float kBias = 7.0f;         // log2 of the factor that P carries
+constexpr float kSlack = 8.0f;        // log2 by which the maximum may grow unfollowed
+
+struct TcArgs {
+  CUtensorMap mk, mv;                 // [page][row][kv head][dim]: boxes of box_rows rows x 64 dims
+  PagedProblem p;
+  int rtiles, box_rows, q_vec, out_vec;
+};
+
+template <int HD, bool SPLIT>
+struct TcShape {
+  static constexpr int kHalves = HD / 64;
+  static constexpr int kTile = kHalves * 16384;                 // bytes of a 128 x HD fp16 tile
+  static constexpr int kQ = 2 * (SPLIT ? 2 : 1) * kTile;
+  static constexpr int kSlots = HD == 128 ? (SPLIT ? 3 : 5) : 8;
+  static constexpr int kBars = 2 * kSlots + 1 + 6;
+  static constexpr int kSmem = 1024 + kQ + kSlots * kTile + kBars * 8 + 16;
+  static_assert(kSmem <= 227 * 1024, "shared memory");
+};
+
+__device__ __forceinline__ void tc_ld32(uint32_t addr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr));
+}
+__device__ __forceinline__ void tc_st32(uint32_t addr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+
+__device__ __forceinline__ void tma_page(void* dst, const CUtensorMap* m, int x, int head, int row, int page,
+                                         uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+      "[%6];" ::"r"(smem_u32(dst)),
+      "l"(m), "r"(x), "r"(head), "r"(row), "r"(page), "r"(smem_u32(bar))
+      : "memory");
+}
+
+template <int HD, bool SPLIT>
+__global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __grid_constant__ TcArgs a) {
+  using T = TcShape<HD, SPLIT>;
+  extern __shared__ uint8_t raw[];
+  uint8_t* sm = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
+  uint8_t* sq = sm;                                   // [tile][hi, lo][half][128 rows x 128 B]
+  uint8_t* ring = sm + T::kQ;
+  uint64_t* full = reinterpret_cast<uint64_t*>(ring + T::kSlots * T::kTile);
+  uint64_t* empty = full + T::kSlots;
+  uint64_t* qfull = empty + T::kSlots;
+  uint64_t* sfull = qfull + 1;                        // [2]: S of tile t is there
+  uint64_t* pfull = sfull + 2;                        // [2]: P of tile t is there
+  uint64_t* odone = pfull + 2;                        // [2]: O of tile t has taken P in
+  uint32_t* tmem_at = reinterpret_cast<uint32_t*>(odone + 2);
+  const PagedProblem& p = a.p;
+  pdl_wait();
+  pdl_trigger();
+
+  int b = blockIdx.x;
+  const int kvh = b % p.n_kv;
+  b /= p.n_kv;
+  const int seq = b % p.n_seqs;
+  b /= p.n_seqs;
+  const int split = p.splits ? b % p.splits : 0;
+  const int rt = a.rtiles - 1 - (p.splits ? b / p.splits : b);      // long rows first
+  const SeqTask t = seq_task(p, seq);
+  const int rows = t.qn * p.group, r0 = rt * 2 * kRows;
+  if (r0 >= rows) return;
+  int k0 = 0, k1 = seen(p, t, (min(rows, r0 + 2 * kRows) - 1) / p.group);
+  if (p.splits) {
+    k0 = split * p.chunk;
+    k1 = min(k1, k0 + p.chunk);
+    if (k0 >= k1) return;
+  }
+  // key tiles that each row tile needs
+  int nt[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int last = min(rows, r0 + (i + 1) * kRows) - 1;
+    const int e = last >= r0 + i * kRows ? min(k1, seen(p, t, last / p.group)) : 0;
+    nt[i] = e > k0 ? (e - k0 + kKeys - 1) / kKeys : 0;
+  }
+  const int nmax = max(nt[0], nt[1]);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (warp == 9) tmem_alloc(tmem_at, 512);
+  if (tid == 0) {
+    for (int i = 0; i < T::kSlots; ++i) {
+      mbar_init(full + i, 1);
+      mbar_init(empty + i, 1);
+    }
+    mbar_init(qfull, 2 * kRows);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(sfull + i, 1);
+      mbar_init(pfull + i, kRows);
+      mbar_init(odone + i, 1);
+    }
+    mbar_fence_init();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_at;
+
+  if (warp == 8) {
+    // ------------------------------------------------------------ K, V tiles
+    bool ok = true;
+    int used = 0;                                     // slots filled
+    for (int j = 0; j < nmax && ok; ++j) {
+      const int kt = k0 + j * kKeys;
+      const int need = (min(kKeys, k1 - kt) + a.box_rows - 1) / a.box_rows;
+      int page = -1, row = 0;
+      if (lane < need) {
+        const int key = kt + lane * a.box_rows;
+        page = t.table[key / p.page_size];
+        row = key % p.page_size;
+      }
+      for (int v = 0; v < 2 && ok; ++v) {
+        const int s = used % T::kSlots;
+        if (used >= T::kSlots) ok = mbar_wait(empty + s, (used / T::kSlots - 1) & 1, p.err, 31);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (lane == 0) mbar_arrive_expect_tx(full + s, need * a.box_rows * HD * 2);
+        __syncwarp();
+        if (lane < need) {
+          uint8_t* dst = ring + s * T::kTile + lane * a.box_rows * 128;
+#pragma unroll
+          for (int h = 0; h < T::kHalves; ++h)
+            tma_page(dst + h * 16384, v ? &a.mv : &a.mk, 64 * h, kvh, row, page, full + s);
+        }
+        ++used;
+      }
+    }
+    // every copy lands before the CTA may end
+    for (int i = max(0, used - T::kSlots); i < used; ++i)
+      mbar_wait(full + i % T::kSlots, (i / T::kSlots) & 1, p.err, 32);
+  } else if (warp == 9) {
+    // ------------------------------------------------------------------ MMAs
+    constexpr uint32_t kIdS = (1u << 4) | (8u << 24) | ((uint32_t)(kKeys >> 3) << 17);
+    constexpr uint32_t kIdO = (1u << 4) | (8u << 24) | ((uint32_t)(HD >> 3) << 17) | (1u << 16);   // V is N-major
+    bool ok = mbar_wait(qfull, 0, p.err, 33);
+    ok = __all_sync(0xffffffffu, ok);
+    tc_fence_after();
+    auto wait_slot = [&](int i) {
+      if (ok) ok = mbar_wait(full + i % T::kSlots, (i / T::kSlots) & 1, p.err, 34);
+      ok = __all_sync(0xffffffffu, ok);
+    };
+    auto issue_s = [&](int i, int j) {
+      wait_slot(2 * j);
+      if (!ok) return;
+      if (lane == 0) {
+        const uint32_t kb = smem_u32(ring + (2 * j % T::kSlots) * T::kTile);
+        const uint32_t qb = smem_u32(sq + i * (SPLIT ? 2 : 1) * T::kTile);
+#pragma unroll
+        for (int part = 0; part < (SPLIT ? 2 : 1); ++part)
+#pragma unroll
+          for (int k = 0; k < HD / 16; ++k) {
+            const uint32_t off = (k >> 2) * 16384 + (k & 3) * 32;
+            mma_f16_ss(tmem + i * kKeys, desc_k(qb + part * T::kTile + off), desc_k(kb + off), kIdS, part + k > 0);
+          }
+        mma_commit(sfull + i);
+        if (i == 1 || j >= nt[1]) mma_commit(empty + 2 * j % T::kSlots);
+      }
+      __syncwarp();
+    };
+    for (int i = 0; i < 2; ++i)
+      if (nt[i] > 0 && ok) issue_s(i, 0);
+    for (int j = 0; j < nmax && ok; ++j)
+      for (int i = 0; i < 2 && ok; ++i) {
+        if (j >= nt[i]) continue;
+        const int slot = (2 * j + 1) % T::kSlots;
+        wait_slot(2 * j + 1);
+        const int have = min(kKeys, k1 - (k0 + j * kKeys));
+        if (ok && have < kKeys && (i == 0 || j >= nt[0])) {
+          // value rows behind the range count with weight 0: they must be finite
+          for (int h = 0; h < T::kHalves; ++h) {
+            uint8_t* base = ring + slot * T::kTile + h * 16384;
+            for (int o = have * 128 + lane * 16; o < kKeys * 128; o += 512)
+              *reinterpret_cast<uint4*>(base + o) = make_uint4(0, 0, 0, 0);
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+        }
+        if (ok) ok = mbar_wait(pfull + i, j & 1, p.err, 35);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        if (lane == 0) {
+          const uint32_t vb = smem_u32(ring + slot * T::kTile);
+#pragma unroll
+          for (int part = 0; part < (SPLIT ? 2 : 1); ++part)
+#pragma unroll
+            for (int k = 0; k < kKeys / 16; ++k)
+              mma_f16_ts(tmem + 256 + i * HD, tmem + i * kKeys + part * 64 + k * 8, desc_mn(vb + k * 2048, 16384),
+                         kIdO, j > 0 || part + k > 0);
+          mma_commit(odone + i);
+          if (i == 1 || j >= nt[1]) mma_commit(empty + slot);
+        }
+        __syncwarp();
+        if (j + 1 < nt[i]) issue_s(i, j + 1);
+      }
+    __syncwarp();
+  } else {
+    // --------------------------------------------------------------- softmax
+    const int i = warp >> 2, wq = warp & 3, r = tid & 127;      // row tile, TMEM quarter, row of the tile
+    const int base_row = r0 + i * kRows;
+    // Q rows of the tile into the swizzled K-major layout: 8 or 16 lanes a
+    // row, eight elements each; fp32 rows scaled by a power of two and split
+    float my_inv = 1.0f;                                         // undoes the scale of row r
+    const float sgn = p.scale_log2 < 0.0f ? -1.0f : 1.0f;        // a negative scale goes into q
+    {
+      constexpr int CH = HD / 8;
+      const int c = lane % CH, rr0 = lane / CH;
+#pragma unroll 4
+      for (int step = 0; step < 32 * CH / 32; ++step) {
+        const int row = wq * 32 + step * (32 / CH) + rr0;        // this warp's 32 rows
+        const int pr = base_row + row;
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = 0.0f;
+        if (pr < rows) {
+          const long long at = (long long)(t.q0 + pr / p.group) * p.q_stride +
+                               (long long)(kvh * p.group + pr % p.group) * p.hd + 8 * c;
+          if (8 * c < p.hd) {
+            if (a.q_vec) {
+              if (p.type == TOSK_F32) {
+                const float4 u = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p.q) + at);
+                const float4 v = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p.q) + at + 4);
+                x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
+                x[4] = v.x; x[5] = v.y; x[6] = v.z; x[7] = v.w;
+              } else {
+                const uint4 u = *reinterpret_cast<const uint4*>(reinterpret_cast<const __half*>(p.q) + at);
+                const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
+                  x[2 * e] = f.x;
+                  x[2 * e + 1] = f.y;
+                }
+              }
+            } else {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) x[e] = load_elem(p.q, p.type, at + e);   // hd is a multiple of 8
+            }
+          }
+        }
+        float sc = sgn;
+        if (SPLIT) {
+          float mx = 0.0f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(x[e]));
+#pragma unroll
+          for (int o = CH / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+          const float s2 = pow2_to_2p13(mx);
+          sc *= s2;
+          const float inv = 1.0f / s2;                           // exact: a power of two
+#pragma unroll
+          for (int q = 0; q < 32 / CH; ++q) {
+            const float v = __shfl_sync(0xffffffffu, inv, q * CH);
+            if (lane == step * (32 / CH) + q) my_inv = v;
+          }
+        }
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float u = x[2 * e] * sc, v = x[2 * e + 1] * sc;
+          const __half2 H = __floats2half2_rn(u, v);
+          hi[e] = *reinterpret_cast<const uint32_t*>(&H);
+          if (SPLIT) {
+            const float2 f = __half22float2(H);
+            const __half2 L = __floats2half2_rn(u - f.x, v - f.y);
+            lo[e] = *reinterpret_cast<const uint32_t*>(&L);
+          }
+        }
+        uint8_t* dst = sq + i * (SPLIT ? 2 : 1) * T::kTile + (c >> 3) * 16384 + sw128(row, c & 7);
+        *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        if (SPLIT) *reinterpret_cast<uint4*>(dst + T::kTile) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      mbar_arrive(qfull);
+    }
+    const int pr = base_row + r;
+    const bool live = pr < rows;
+    const int tok = t.q0 + pr / p.group, head = kvh * p.group + pr % p.group;
+    const int lim = live ? min(seen(p, t, pr / p.group), k1) : 0;      // keys this row sees
+    const float sc = fmaxf(fabsf(p.scale_log2) * my_inv, 1.2e-38f);   // not 0: a masked score is -inf * sc
+    const uint32_t lanes = (uint32_t)wq << 21;                          // TMEM lane of the warp's first row, << 16
+    const uint32_t ts = tmem + lanes + i * kKeys, to = tmem + lanes + 256 + i * HD;
+    float m = -INFINITY, l = 0.0f;
+    bool ok = true;
+    for (int j = 0; j < nt[i]; ++j) {
+      if (ok) ok = mbar_wait(sfull + i, j & 1, p.err, 36);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t s[4][32];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tc_ld32(ts + 32 * c, s[c]);
+      asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+      const int left = lim - (k0 + j * kKeys);                          // keys of this tile that the row sees
+      if (__any_sync(0xffffffffu, left < kKeys)) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (32 * c + e >= left) s[c][e] = 0xff800000u;              // -inf
+      }
+      float mx[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        mx[c] = __uint_as_float(s[c][0]);
+#pragma unroll
+        for (int e = 1; e < 32; ++e) mx[c] = fmaxf(mx[c], __uint_as_float(s[c][e]));
+      }
+      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;
+      if (j == 0) {
+        m = top;
+      } else if (__any_sync(0xffffffffu, top > m + kSlack)) {
+        // scale O and l to the new maximum (lanes that need not: by 1)
+        const float mn = top > m + kSlack ? top : m;
+        const float f = mn == m ? 1.0f : exp2f(m - mn);
+        if (ok) ok = mbar_wait(odone + i, (j - 1) & 1, p.err, 37);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < HD / 32; ++c) {
+          uint32_t o[32];
+          tc_ld32(to + 32 * c, o);
+          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+          tc_st32(to + 32 * c, o);
+        }
+        l *= f;
+        m = mn;
+      }
+      const float bias = kBias - (m == -INFINITY ? 0.0f : m);
+      float sum[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t hi[16], lo[16];
+        sum[c] = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float u = ex2(fmaf(__uint_as_float(s[c][2 * e]), sc, bias));
+          const float v = ex2(fmaf(__uint_as_float(s[c][2 * e + 1]), sc, bias));
+          sum[c] += u;
+          sum[c] += v;
+          const __half2 H = __floats2half2_rn(u, v);
+          hi[e] = *reinterpret_cast<const uint32_t*>(&H);
+          if (SPLIT) {
+            const float2 f = __half22float2(H);
+            const __half2 L = __floats2half2_rn(u - f.x, v - f.y);
+            lo[e] = *reinterpret_cast<const uint32_t*>(&L);
+          }
+        }
+        tmem_st16(ts + 16 * c, hi);
+        if (SPLIT) tmem_st16(ts + 64 + 16 * c, lo);
+      }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(pfull + i);
+    }
+    if (ok && nt[i] > 0) ok = mbar_wait(odone + i, (nt[i] - 1) & 1, p.err, 38);
+    ok = __all_sync(0xffffffffu, ok);
+    tc_fence_after();
+    // ------------------------------------------------------------- output
+    bool bad = false;
+    if (ok) {
+      const float inv = p.splits ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+      const long long part = (long long)(p.slot0 + split) * p.total_q * p.heads + (long long)tok * p.heads + head;
+      if (p.splits && live) p.part_ml[part] = make_float2(m - kBias, l);
+      const long long oo = (long long)tok * p.out_stride + (long long)head * p.hd;
+#pragma unroll
+      for (int c = 0; c < HD / 32; ++c) {
+        uint32_t o[32];
+        if (nt[i] > 0) {
+          tc_ld32(to + 32 * c, o);
+          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = 0;
+        }
+        if (!live) continue;
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          const float v = l == 0.0f ? 0.0f : __uint_as_float(o[e]) * inv;
+          o[e] = __float_as_uint(v);
+          bad |= isnan(v);
+        }
+        if (p.splits) {
+          float* dst = p.part_o + part * p.hd + 32 * c;
+#pragma unroll
+          for (int e = 0; e < 32; e += 4)
+            if (32 * c + e < p.hd) *reinterpret_cast<uint4*>(dst + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+        } else {
+          if (a.out_vec && p.type == TOSK_F32) {
+            float* dst = reinterpret_cast<float*>(p.out) + oo + 32 * c;
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+              if (32 * c + e < p.hd) *reinterpret_cast<uint4*>(dst + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+          } else if (a.out_vec) {
+            __half* dst = reinterpret_cast<__half*>(p.out) + oo + 32 * c;
+#pragma unroll
+            for (int e = 0; e < 32; e += 8) {
+              uint32_t h[4];
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                const __half2 H = __floats2half2_rn(__uint_as_float(o[e + 2 * q]), __uint_as_float(o[e + 2 * q + 1]));
+                h[q] = *reinterpret_cast<const uint32_t*>(&H);
+              }
+              if (32 * c + e < p.hd) *reinterpret_cast<uint4*>(dst + e) = make_uint4(h[0], h[1], h[2], h[3]);
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (32 * c + e < p.hd) store_elem(p.out, p.type, oo + 32 * c + e, __uint_as_float(o[e]));
+          }
+        }
+      }
+    }
+    if (!p.splits) {
+      uint32_t todo = __ballot_sync(0xffffffffu, bad && live);
+      while (todo) {
+        const int w = __ffs(todo) - 1;
+        todo &= todo - 1;
+        const int pw = base_row + wq * 32 + w;
+        attn_row_plain(p, nullptr, 0, t.table, seen(p, t, pw / p.group), t.q0 + pw / p.group,
+                       kvh * p.group + pw % p.group);
+      }
+    }
+    tc_fence_before();
+  }
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+}  // namespace tos
+
+using namespace tos;
+
+namespace {
+// K or V pool as [page][row][kv head][dim], boxes of box_rows rows of one
+// head x 64 dims (dims past hd read as zeros).
+bool pool_map(CUtensorMap* m, const void* base, const PagedProblem& p, int box_rows) {
+  const PFN_cuTensorMapEncodeTiled_v12000 enc = tensor_map_encoder();
+  if (!enc) return false;
+  const cuuint64_t dim[4] = {(cuuint64_t)p.hd, (cuuint64_t)p.n_kv, (cuuint64_t)p.page_size, (cuuint64_t)p.n_pages};
+  const cuuint64_t row = (cuuint64_t)p.n_kv * p.hd * 2;
+  const cuuint64_t str[3] = {(cuuint64_t)p.hd * 2, row, row * p.page_size};
+  const cuuint32_t box[4] = {64, 1, (cuuint32_t)box_rows, 1};
+  const cuuint32_t es[4] = {1, 1, 1, 1};
+  return enc(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), dim, str, box, es,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int HD, bool SPLIT>
+int tc_launch(const TcArgs& a, unsigned grid, cudaStream_t st) {
+  const void* f = (const void*)paged_attn_tc_kernel<HD, SPLIT>;
+  const cudaError_t e =
+      cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, TcShape<HD, SPLIT>::kSmem);
+  if (e != cudaSuccess) return (int)e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(kTcThreads);
+  cfg.dynamicSmemBytes = TcShape<HD, SPLIT>::kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  void* args[] = {const_cast<TcArgs*>(&a)};
+  return (int)cudaLaunchKernelExC(&cfg, f, args);
+}
+}  // namespace
+
+namespace tos {
+
+// What the tensor-core kernel takes: an fp16 cache in 16-byte rows of at most
+// 128 elements, pages that tile 128 keys or are tiled by them.
+bool paged_tc_ok(const PagedProblem& p) {
+  const int ps = p.page_size;
+  return p.kv_type == TOSK_F16 && p.hd % 8 == 0 && p.hd <= 128 && ps >= 8 &&
+         (ps < kKeys ? kKeys % ps == 0 : ps % kKeys == 0) && ((uintptr_t)p.k & 15) == 0 && ((uintptr_t)p.v & 15) == 0 &&
+         (long long)ps * p.n_kv * p.hd * 2 < (1ll << 39);
+}
+
+int paged_tc_run(const PagedProblem& p, cudaStream_t st) {
+  TcArgs a;
+  a.p = p;
+  a.box_rows = p.page_size < kKeys ? p.page_size : kKeys;
+  const long long rows = (long long)(p.fixed_kv >= 0 ? p.total_q : p.max_q) * p.group;
+  const long long rt = (rows + 2 * kRows - 1) / (2 * kRows);
+  const long long grid = rt * (p.splits ? p.splits : 1) * p.n_seqs * p.n_kv;
+  if (grid > 0x7fffffffll) return (int)cudaErrorInvalidValue;
+  a.rtiles = (int)rt;
+  a.q_vec = ((uintptr_t)p.q & 15) == 0 && p.q_stride % (p.type == TOSK_F32 ? 4 : 8) == 0;
+  a.out_vec = ((uintptr_t)p.out & 15) == 0 && p.out_stride % (p.type == TOSK_F32 ? 4 : 8) == 0;
+  if (!pool_map(&a.mk, p.k, p, a.box_rows) || !pool_map(&a.mv, p.v, p, a.box_rows)) return (int)cudaErrorNotSupported;
+  const bool split = p.type == TOSK_F32;
+  if (p.hd <= 64) return split ? tc_launch<64, true>(a, (unsigned)grid, st) : tc_launch<64, false>(a, (unsigned)grid, st);
+  return split ? tc_launch<128, true>(a, (unsigned)grid, st) : tc_launch<128, false>(a, (unsigned)grid, st);
+}
+
+}  // namespace tos

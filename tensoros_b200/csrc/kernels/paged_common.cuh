@@ -94,7 +94,7 @@ __device__ __forceinline__ void store_elem(void* p, int type, long long i, float
 // in the row.  Such rows are computed again here, where an unseen key is not
 // read at all (a row with a NaN of its own gets it again).  prefix: keys
 // before the sequence's own (decode).
-__device__ __noinline__ void attn_row_plain(const PagedProblem& p, const int* prefix_table, int prefix_len,
+static __device__ __noinline__ void attn_row_plain(const PagedProblem& p, const int* prefix_table, int prefix_len,
                                             const int* table, int n, int tok, int h) {
   const int lane = threadIdx.x & 31;
   const long long qo = (long long)tok * p.q_stride + (long long)h * p.hd;
