@@ -361,10 +361,9 @@ int run_general(const PagedProblem& p, cudaStream_t st) {
   return rows <= 32 ? general_rows<16>(p, st) : general_rows<64>(p, st);
 }
 
-// Splits of a key axis: enough CTAs for two rounds over the SMs, at least 256
-// keys each.
-int plan_splits(long long tiles, int keys) {
-  const long long want = (2 * kSms + tiles - 1) / tiles;
+// Splits of a key axis: `rounds` CTAs for every SM, at least 256 keys each.
+int plan_splits(long long tiles, int keys, int rounds) {
+  const long long want = (rounds * kSms + tiles - 1) / tiles;
   const long long most = (keys + 255) / 256;
   const long long s = want < most ? want : most;
   return s < 1 ? 1 : (int)s;
@@ -378,10 +377,10 @@ struct DecodePlan {
 DecodePlan plan_decode(int n_seqs, int max_kv, int prefix_len, int heads, int n_kv) {
   DecodePlan d;
   const long long rows = (long long)n_seqs * (heads / n_kv);
-  d.pre = prefix_len > 0 ? plan_splits((rows + 255) / 256 * n_kv, prefix_len) : 0;
+  d.pre = prefix_len > 0 ? plan_splits((rows + 255) / 256 * n_kv, prefix_len, 1) : 0;
   d.pre_chunk = d.pre ? chunk_of(prefix_len, d.pre) : 0;
   if (d.pre) d.pre = (prefix_len + d.pre_chunk - 1) / d.pre_chunk;
-  d.own = max_kv > 0 ? plan_splits((long long)n_seqs * n_kv, max_kv) : 1;
+  d.own = max_kv > 0 ? plan_splits((long long)n_seqs * n_kv, max_kv, 12) : 1;
   d.own_chunk = max_kv > 0 ? chunk_of(max_kv, d.own) : 128;
   if (max_kv > 0) d.own = (max_kv + d.own_chunk - 1) / d.own_chunk;
   if (!d.pre && d.own == 1) d.own = 0;
@@ -445,8 +444,10 @@ extern "C" int tosk_paged_prompt(const tosk_paged_attn_t* a, cudaStream_t st) {
 extern "C" int tosk_paged_decode(const tosk_paged_attn_t* a, cudaStream_t st) {
   PagedProblem p = problem_of(a);
   const DecodePlan d = plan_decode(a->n_seqs, a->max_kv, a->prefix_len, a->n_heads, a->kv.n_kv);
-  if (!d.own) return run_general(p, st);
+  const bool fast = paged_decode_ok(p);
+  if (!d.own) return fast ? paged_decode_run(p, 0, st) : run_general(p, st);
   part_views(p, a->ws, d.own + d.pre);
+  bool beside = false;
   if (d.pre) {
     PagedProblem x = p;
     x.table = a->prefix_table;
@@ -458,12 +459,13 @@ extern "C" int tosk_paged_decode(const tosk_paged_attn_t* a, cudaStream_t st) {
     x.chunk = d.pre_chunk;
     const int e = run_tiles(x, st);
     if (e) return e;
+    beside = true;
   }
   p.splits = d.own;
   p.chunk = d.own_chunk;
   p.slot0 = d.pre;
   if (a->max_kv > 0) {
-    const int e = run_general(p, st);
+    const int e = fast ? paged_decode_run(p, beside, st) : run_general(p, st);
     if (e) return e;
   }
   return run_join(p, d.pre, a->prefix_table, a->prefix_len, st);

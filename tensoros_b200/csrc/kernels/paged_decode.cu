@@ -1,0 +1,333 @@
+// paged_decode.cu - attention of single tokens over an fp16 paged cache.
+//
+// A CTA takes a chunk of one sequence's keys for one key/value head and the
+// (up to 8 or 16) query heads that share it; its four warps take every fourth
+// 16-key step each and run alone, without any exchange until the end:
+//   * the step's K and V rows stream through the warp's own ring in shared
+//     memory (cp.async, 16-byte pieces, 8 KB a step at 128 dims; pages by the
+//     table entry fetched one step ahead).  Rows past the end and pages that
+//     are none come as zeros;
+//   * S = Q K^T and O += P V by mma.sync m16n8k16: eight queries' fp16 high
+//     parts are rows 0-7 of A and their low parts rows 8-15, so fp32 queries
+//     and weights cost no extra instruction and the two row halves are added
+//     afterwards.  tcgen05 wants 128 rows; here there are 8 or 16;
+//   * running maximum and sum per query as in the prompt kernel (followed
+//     only beyond a factor 2^8, weights biased by 2^7).
+// The four warps' results are joined in shared memory; with a split key axis
+// (or a prefix) the joining kernel adds the chunks.
+//
+// Bound: HBM.  A 16-key step is 8 KB and 32 MMAs (HD 128), ~1/16 of what the
+// tensor pipe does in the time the bytes take.
+#include <cuda_runtime.h>
+
+#include "paged_common.cuh"
+#include "paged_tc.cuh"
+
+namespace tos {
+
+constexpr int kDecWarps = 4;
+constexpr int kStep = 16;             // keys a warp step
+
+template <int HD>
+struct DecShape {
+  static constexpr int kRow = HD * 2;                            // bytes of a key row in shared memory
+  static constexpr int kStage = 2 * kStep * kRow;                // K and V
+  static constexpr int kDepth = HD == 64 ? 6 : 3;
+  static constexpr int kSmem = kDecWarps * kDepth * kStage;
+};
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool have) {
+  const int n = have ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// two floats as packed fp16 high parts and what they leave
+__device__ __forceinline__ void split_pair(float x, float y, uint32_t& hi, uint32_t& lo) {
+  const __half2 H = __floats2half2_rn(x, y);
+  const float2 f = __half22float2(H);
+  const __half2 L = __floats2half2_rn(x - f.x, y - f.y);
+  hi = *reinterpret_cast<const uint32_t*>(&H);
+  lo = *reinterpret_cast<const uint32_t*>(&L);
+}
+
+struct DecArgs {
+  PagedProblem p;
+  int qblocks;             // blocks of 8 * NQ query heads of a group
+  int late_wait;           // 1: runs beside the prefix kernel, whose end it awaits at its own end
+};
+
+template <int HD, int NQ>
+__global__ void __launch_bounds__(32 * kDecWarps) paged_decode_kernel(const DecArgs a) {
+  using T = DecShape<HD>;
+  extern __shared__ __align__(128) uint8_t sm[];
+  const PagedProblem& p = a.p;
+  if (!a.late_wait) {
+    pdl_wait();
+    pdl_trigger();
+  }
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
+  int b = blockIdx.x;
+  const int qb = b % a.qblocks;
+  b /= a.qblocks;
+  const int kvh = b % p.n_kv;
+  b /= p.n_kv;
+  const int splits = p.splits ? p.splits : 1, split = b % splits, seq = b / splits;
+  const SeqTask t = seq_task(p, seq);
+  int k0 = 0, k1 = t.kvn;
+  if (p.splits) {
+    k0 = split * p.chunk;
+    k1 = min(k1, k0 + p.chunk);
+  }
+  const int h0 = kvh * p.group + qb * 8 * NQ;                    // first query head
+  const int nh = min(8 * NQ, p.group - qb * 8 * NQ);
+  if (k0 < k1 || !p.splits) {
+    const int steps = (k1 - k0 + kStep - 1) / kStep;
+    const uint32_t ring = smem_u32(sm) + warp * T::kDepth * T::kStage;
+    const __half* kb = reinterpret_cast<const __half*>(p.k);
+    const __half* vb = reinterpret_cast<const __half*>(p.v);
+    constexpr int CH = HD / 8;                                   // 16-byte pieces of a row
+    const int chs = p.hd / 8;
+    // Row offset of key (step, lane): lanes 0..15 hold one each
+    auto fetch_row = [&](int st) -> long long {
+      const int key = k0 + st * kStep + (lane & 15);
+      return st < steps && key < k1 ? kv_off(p, t.table, key, kvh) : -1;
+    };
+    auto issue = [&](int st, long long row) {
+      if (st < steps) {
+        const uint32_t dst = ring + (st / kDecWarps % T::kDepth) * T::kStage;
+#pragma unroll
+        for (int i = 0; i < kStep * CH / 32; ++i) {
+          const int idx = i * 32 + lane, key = idx / CH, c = idx % CH;
+          const long long off = __shfl_sync(0xffffffffu, row, key);
+          const bool have = off >= 0 && c < chs;
+          const long long o = have ? off + 8 * c : 0;
+          const uint32_t d = dst + key * T::kRow + ((c ^ (key & 7)) << 4);
+          cp16(d, kb + o, have);
+          cp16(d + kStep * T::kRow, vb + o, have);
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    // the ring's first stages, then the queries while they fly
+    long long rows[T::kDepth];
+#pragma unroll
+    for (int d = 0; d < T::kDepth; ++d) rows[d] = fetch_row(warp + d * kDecWarps);
+#pragma unroll
+    for (int d = 0; d < T::kDepth - 1; ++d) issue(warp + d * kDecWarps, rows[d]);
+    long long nrow = rows[T::kDepth - 1];
+
+    uint32_t qa[NQ][HD / 16][4];
+    float sc[NQ], m[NQ], l[NQ], o[NQ][HD / 8][4];
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+      const int h = n * 8 + g;                                    // this lane's query
+      const bool live = h < nh;
+      const long long qo = (long long)t.q0 * p.q_stride + (long long)(h0 + (live ? h : 0)) * p.hd;
+      float x[HD / 16][4];
+      float mx = 0.0f;
+#pragma unroll
+      for (int k = 0; k < HD / 16; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int d = 16 * k + 2 * t4 + (e & 1) + 8 * (e >> 1);
+          x[k][e] = live && d < p.hd ? load_elem(p.q, p.type, qo + d) : 0.0f;
+          mx = fmaxf(mx, fabsf(x[k][e]));
+        }
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      const float s2 = pow2_to_2p13(mx);                          // exact scaling of the row
+      const float sg = p.scale_log2 < 0.0f ? -s2 : s2;
+      sc[n] = fmaxf(fabsf(p.scale_log2) * (1.0f / s2), 1.2e-38f);  // not 0: a masked score is -inf * sc
+#pragma unroll
+      for (int k = 0; k < HD / 16; ++k) {
+        split_pair(x[k][0] * sg, x[k][1] * sg, qa[n][k][0], qa[n][k][1]);
+        split_pair(x[k][2] * sg, x[k][3] * sg, qa[n][k][2], qa[n][k][3]);
+      }
+      m[n] = -INFINITY;
+      l[n] = 0.0f;
+#pragma unroll
+      for (int d = 0; d < HD / 8; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[n][d][e] = 0.0f;
+    }
+    // ldmatrix row addresses: K: lanes 0-7 / 8-15 keys 0-7 at the two halves
+    // of 16 dims, 16-31 keys 8-15; V (transposed): 0-15 keys, 16-31 the next 8 dims
+    const int krow = (lane & 7) + ((lane >> 4) << 3), kch = (lane >> 3) & 1;
+    const int vrow = lane & 15, vch = lane >> 4;
+
+    for (int st = warp; st < steps; st += kDecWarps) {
+      issue(st + (T::kDepth - 1) * kDecWarps, nrow);
+      nrow = fetch_row(st + T::kDepth * kDecWarps);
+      asm volatile("cp.async.wait_group %0;" ::"n"(T::kDepth - 1) : "memory");
+      __syncwarp();
+      const uint32_t kbase = ring + (st / kDecWarps % T::kDepth) * T::kStage, vbase = kbase + kStep * T::kRow;
+      float s[NQ][2][4];
+#pragma unroll
+      for (int n = 0; n < NQ; ++n)
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[n][c][e] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < HD / 16; ++k) {
+        uint32_t bk[4];
+        ldsm4(bk, kbase + krow * T::kRow + (((2 * k + kch) ^ (krow & 7)) << 4));
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+          mma16816(s[n][0], qa[n][k], bk[0], bk[1]);
+          mma16816(s[n][1], qa[n][k], bk[2], bk[3]);
+        }
+      }
+      const int left = k1 - (k0 + st * kStep);                    // keys of the step that count
+      uint32_t pa[NQ][4];
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) {
+        float w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int key = (e >> 1) * 8 + 2 * t4 + (e & 1);
+          w[e] = key < left ? (s[n][e >> 1][e & 1] + s[n][e >> 1][2 + (e & 1)]) * sc[n] : -INFINITY;
+        }
+        float top = fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3]));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        if (__any_sync(0xffffffffu, top > m[n] + 8.0f)) {
+          const float mn = top > m[n] + 8.0f ? top : m[n];
+          const float f = mn == m[n] ? 1.0f : exp2f(m[n] - mn);   // 0 on the first keys
+          m[n] = mn;
+          l[n] *= f;
+#pragma unroll
+          for (int d = 0; d < HD / 8; ++d)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[n][d][e] *= f;
+        }
+        const float bias = 7.0f - (m[n] == -INFINITY ? 0.0f : m[n]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = ex2(w[e] + bias);
+        l[n] += (w[0] + w[1]) + (w[2] + w[3]);
+        split_pair(w[0], w[1], pa[n][0], pa[n][1]);
+        split_pair(w[2], w[3], pa[n][2], pa[n][3]);
+      }
+#pragma unroll
+      for (int d = 0; d < HD / 16; ++d) {
+        uint32_t bv[4];
+        ldsm4t(bv, vbase + vrow * T::kRow + (((2 * d + vch) ^ (vrow & 7)) << 4));
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+          mma16816(o[n][2 * d], pa[n], bv[0], bv[1]);
+          mma16816(o[n][2 * d + 1], pa[n], bv[2], bv[3]);
+        }
+      }
+      __syncwarp();                                               // the stage may be filled again
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();                                              // the rings are free: join the warps there
+    float* so = reinterpret_cast<float*>(sm);                     // [warp][8 NQ queries][HD]
+    __shared__ float2 sml[kDecWarps][8 * NQ];
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+      l[n] += __shfl_xor_sync(0xffffffffu, l[n], 1);
+      l[n] += __shfl_xor_sync(0xffffffffu, l[n], 2);
+      if (t4 == 0) sml[warp][n * 8 + g] = make_float2(m[n] - 7.0f, l[n]);
+#pragma unroll
+      for (int d = 0; d < HD / 8; ++d)
+        *reinterpret_cast<float2*>(so + ((warp * NQ + n) * 8 + g) * HD + 8 * d + 2 * t4) =
+            make_float2(o[n][d][0] + o[n][d][2], o[n][d][1] + o[n][d][3]);
+    }
+    __syncthreads();
+    // a warp a query
+    for (int h = warp; h < nh; h += kDecWarps) {
+      float M = -INFINITY, L = 0.0f, f[kDecWarps];
+#pragma unroll
+      for (int w = 0; w < kDecWarps; ++w) M = fmaxf(M, sml[w][h].x);
+#pragma unroll
+      for (int w = 0; w < kDecWarps; ++w) {
+        f[w] = M == -INFINITY ? 0.0f : exp2f(sml[w][h].x - M);
+        L += f[w] * sml[w][h].y;
+      }
+      const int head = h0 + h;
+      const long long part = (long long)(p.slot0 + split) * p.total_q * p.heads + (long long)t.q0 * p.heads + head;
+      const long long oo = (long long)t.q0 * p.out_stride + (long long)head * p.hd;
+      const float inv = p.splits ? 1.0f : L == 0.0f ? 0.0f : 1.0f / L;
+      if (p.splits && lane == 0) p.part_ml[part] = make_float2(M, L);
+      for (int d = lane; d < p.hd; d += 32) {
+        float v = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kDecWarps; ++w) v = fmaf(f[w], so[(w * NQ * 8 + h) * HD + d], v);
+        if (p.splits) p.part_o[part * p.hd + d] = v;
+        else store_elem(p.out, p.type, oo + d, L == 0.0f ? 0.0f : v * inv);
+      }
+    }
+  }
+  if (a.late_wait) {
+    pdl_trigger();
+    pdl_wait();
+  }
+}
+
+}  // namespace tos
+
+using namespace tos;
+
+namespace {
+template <int HD, int NQ>
+int dec_launch(const DecArgs& a, unsigned grid, cudaStream_t st) {
+  const void* f = (const void*)paged_decode_kernel<HD, NQ>;
+  const cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, DecShape<HD>::kSmem);
+  if (e != cudaSuccess) return (int)e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(32 * kDecWarps);
+  cfg.dynamicSmemBytes = DecShape<HD>::kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  void* args[] = {const_cast<DecArgs*>(&a)};
+  return (int)cudaLaunchKernelExC(&cfg, f, args);
+}
+}  // namespace
+
+namespace tos {
+
+// What this kernel takes: an fp16 cache whose rows are whole 16-byte pieces.
+bool paged_decode_ok(const PagedProblem& p) {
+  return p.kv_type == TOSK_F16 && p.hd % 8 == 0 && ((uintptr_t)p.k & 15) == 0 && ((uintptr_t)p.v & 15) == 0;
+}
+
+// One token a sequence.  Groups of up to 8 query heads in one block of 8,
+// larger ones in blocks of 16 (256 dims: of 8, for the registers).
+int paged_decode_run(const PagedProblem& p, int late_wait, cudaStream_t st) {
+  DecArgs a;
+  a.p = p;
+  a.late_wait = late_wait;
+  const int nq = p.group > 8 && p.hd <= 128 ? 2 : 1;
+  a.qblocks = (p.group + 8 * nq - 1) / (8 * nq);
+  const long long grid = (long long)a.qblocks * p.n_kv * (p.splits ? p.splits : 1) * p.n_seqs;
+  if (grid > 0x7fffffffll) return (int)cudaErrorInvalidValue;
+  const unsigned n = (unsigned)grid;
+  if (p.hd <= 64) return nq == 1 ? dec_launch<64, 1>(a, n, st) : dec_launch<64, 2>(a, n, st);
+  if (p.hd <= 128) return nq == 1 ? dec_launch<128, 1>(a, n, st) : dec_launch<128, 2>(a, n, st);
+  return dec_launch<256, 1>(a, n, st);
+}
+
+}  // namespace tos

@@ -13,6 +13,9 @@ namespace tos {
 
 bool paged_tc_ok(const PagedProblem& p);
 int paged_tc_run(const PagedProblem& p, cudaStream_t st);
+// paged_decode.cu
+bool paged_decode_ok(const PagedProblem& p);
+int paged_decode_run(const PagedProblem& p, int late_wait, cudaStream_t st);
 
 #ifdef __CUDACC__
 // Shared-memory operand, rows of 128 bytes swizzled 128 B.  K-major (Q, K:
