@@ -39,7 +39,9 @@
 
 namespace tos {
 
-constexpr int kTcThreads = 320;
+constexpr int kTcThreads = 384;        // two softmax warpgroups; K/V copies, MMAs, two idle warps
+constexpr int kTcRegsSoftmax = 208, kTcRegsRest = 88;   // of the launch's 168 a thread: 2 * 208 + 88 = 3 * 168
+static_assert(2 * kTcRegsSoftmax + kTcRegsRest <= 3 * 168, "registers of the launch");
 constexpr int kRows = 128;            // rows of a tile
 constexpr int kKeys = 128;            // keys of a tile
 constexpr float kBias = 7.0f;         // log2 of the factor that P carries
@@ -57,7 +59,7 @@ struct TcShape {
   static constexpr int kTile = kHalves * 16384;                 // bytes of a 128 x HD fp16 tile
   static constexpr int kQ = 2 * (SPLIT ? 2 : 1) * kTile;
   static constexpr int kSlots = HD == 128 ? (SPLIT ? 3 : 5) : 8;
-  static constexpr int kBars = 2 * kSlots + 1 + 6;
+  static constexpr int kBars = 2 * kSlots + 1 + 8;
   static constexpr int kSmem = 1024 + kQ + kSlots * kTile + kBars * 8 + 16;
   static_assert(kSmem <= 227 * 1024, "shared memory");
 };
@@ -72,6 +74,37 @@ __device__ __forceinline__ void tc_ld32(uint32_t addr, uint32_t (&r)[32]) {
         "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
         "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(addr));
+}
+#define TOS_R8(r, i) \
+  "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7])
+// The registers of a tcgen05.ld hold their values only after the wait; tying
+// them to it keeps every use behind it.
+__device__ __forceinline__ void tc_wait_ld(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : TOS_R8(r, 0), TOS_R8(r, 8), TOS_R8(r, 16), TOS_R8(r, 24)::"memory");
+}
+__device__ __forceinline__ void tc_tie(uint32_t (&r)[32]) {
+  asm volatile("" : TOS_R8(r, 0), TOS_R8(r, 8), TOS_R8(r, 16), TOS_R8(r, 24)::"memory");
+}
+#undef TOS_R8
+// 2^x of two values on the FMA pipe, which has room beside the 16 exponentials
+// a clock of the SFU.  x = n + f, |f| <= 1/2: n by adding 1.5 2^23, 2^f by a
+// degree-4 polynomial fitted here for least relative error (2.6e-6, far below
+// the weights' fp16 rounding), 2^n into the exponent.  Below 2^-126: 2^-126.
+__device__ __forceinline__ float2 exp2_fma(float2 x) {
+  x.x = fmaxf(x.x, -126.0f);
+  x.y = fmaxf(x.y, -126.0f);
+  const float2 big = make_float2(12582912.0f, 12582912.0f), nbig = make_float2(-12582912.0f, -12582912.0f);
+  const float2 n = __fadd2_rn(x, big);
+  const float2 r = __fadd2_rn(n, nbig);
+  const float2 f = __ffma2_rn(r, make_float2(-1.0f, -1.0f), x);
+  float2 y = make_float2(0.00957010146f, 0.00957010146f);
+  y = __ffma2_rn(y, f, make_float2(0.0559178603f, 0.0559178603f));
+  y = __ffma2_rn(y, f, make_float2(0.240247488f, 0.240247488f));
+  y = __ffma2_rn(y, f, make_float2(0.693121815f, 0.693121815f));
+  y = __ffma2_rn(y, f, make_float2(0.999999261f, 0.999999261f));
+  y.x = __uint_as_float(__float_as_uint(y.x) + (__float_as_uint(n.x) << 23));
+  y.y = __uint_as_float(__float_as_uint(y.y) + (__float_as_uint(n.y) << 23));
+  return y;
 }
 __device__ __forceinline__ void tc_st32(uint32_t addr, const uint32_t (&r)[32]) {
   asm volatile(
@@ -105,8 +138,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
   uint64_t* empty = full + T::kSlots;
   uint64_t* qfull = empty + T::kSlots;
   uint64_t* sfull = qfull + 1;                        // [2]: S of tile t is there
-  uint64_t* pfull = sfull + 2;                        // [2]: P of tile t is there
-  uint64_t* odone = pfull + 2;                        // [2]: O of tile t has taken P in
+  uint64_t* pfull = sfull + 2;                        // [2][2]: half the keys of tile t's P are there
+  uint64_t* odone = pfull + 4;                        // [2]: O of tile t has taken P in
   uint32_t* tmem_at = reinterpret_cast<uint32_t*>(odone + 2);
   const PagedProblem& p = a.p;
   pdl_wait();
@@ -147,7 +180,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
     mbar_init(qfull, 2 * kRows);
     for (int i = 0; i < 2; ++i) {
       mbar_init(sfull + i, 1);
-      mbar_init(pfull + i, kRows);
+      mbar_init(pfull + 2 * i, kRows);
+      mbar_init(pfull + 2 * i + 1, kRows);
       mbar_init(odone + i, 1);
     }
     mbar_fence_init();
@@ -157,6 +191,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
   tc_fence_after();
   const uint32_t tmem = *tmem_at;
 
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTcRegsRest));
   if (warp == 8) {
     // ------------------------------------------------------------ K, V tiles
     bool ok = true;
@@ -236,100 +272,108 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
         }
-        if (ok) ok = mbar_wait(pfull + i, j & 1, p.err, 35);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        tc_fence_after();
-        if (lane == 0) {
-          const uint32_t vb = smem_u32(ring + slot * T::kTile);
+        for (int half = 0; half < 2; ++half) {
+          if (ok) ok = mbar_wait(pfull + 2 * i + half, j & 1, p.err, 35);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          tc_fence_after();
+          if (lane == 0) {
+            const uint32_t vb = smem_u32(ring + slot * T::kTile);
 #pragma unroll
-          for (int part = 0; part < (SPLIT ? 2 : 1); ++part)
+            for (int part = 0; part < (SPLIT ? 2 : 1); ++part)
 #pragma unroll
-            for (int k = 0; k < kKeys / 16; ++k)
-              mma_f16_ts(tmem + 256 + i * HD, tmem + i * kKeys + part * 64 + k * 8, desc_mn(vb + k * 2048, 16384),
-                         kIdO, j > 0 || part + k > 0);
-          mma_commit(odone + i);
-          if (i == 1 || j >= nt[1]) mma_commit(empty + slot);
+              for (int k = 0; k < kKeys / 32; ++k) {
+                const int kk = half * (kKeys / 32) + k;
+                mma_f16_ts(tmem + 256 + i * HD, tmem + i * kKeys + part * 64 + kk * 8, desc_mn(vb + kk * 2048, 16384),
+                           kIdO, j + half + part + k > 0);
+              }
+            if (half) {
+              mma_commit(odone + i);
+              if (i == 1 || j >= nt[1]) mma_commit(empty + slot);
+            }
+          }
+          __syncwarp();
         }
-        __syncwarp();
+        if (!ok) break;
         if (j + 1 < nt[i]) issue_s(i, j + 1);
       }
     __syncwarp();
+  }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kTcRegsSoftmax));
     // --------------------------------------------------------------- softmax
     const int i = warp >> 2, wq = warp & 3, r = tid & 127;      // row tile, TMEM quarter, row of the tile
     const int base_row = r0 + i * kRows;
     // Q rows of the tile into the swizzled K-major layout: 8 or 16 lanes a
-    // row, eight elements each; fp32 rows scaled by a power of two and split
+    // row, eight elements each; fp32 rows scaled by a power of two and split.
+    // A batch of rows is in flight at once; a lane works out one row's place.
     float my_inv = 1.0f;                                         // undoes the scale of row r
-    const float sgn = p.scale_log2 < 0.0f ? -1.0f : 1.0f;        // a negative scale goes into q
     {
-      constexpr int CH = HD / 8;
+      constexpr int CH = HD / 8, RPS = 32 / CH, BATCH = SPLIT ? 4 : 8;
+      const float sgn = p.scale_log2 < 0.0f ? -1.0f : 1.0f;      // a negative scale goes into q
       const int c = lane % CH, rr0 = lane / CH;
-#pragma unroll 4
-      for (int step = 0; step < 32 * CH / 32; ++step) {
-        const int row = wq * 32 + step * (32 / CH) + rr0;        // this warp's 32 rows
-        const int pr = base_row + row;
-        float x[8];
+      const int pr = base_row + wq * 32 + lane;
+      const long long my_at = pr < rows ? (long long)(t.q0 + pr / p.group) * p.q_stride +
+                                              (long long)(kvh * p.group + pr % p.group) * p.hd
+                                        : -1;
+      for (int s0 = 0; s0 < CH; s0 += BATCH) {
+        uint4 u[BATCH][SPLIT ? 2 : 1];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = 0.0f;
-        if (pr < rows) {
-          const long long at = (long long)(t.q0 + pr / p.group) * p.q_stride +
-                               (long long)(kvh * p.group + pr % p.group) * p.hd + 8 * c;
-          if (8 * c < p.hd) {
+        for (int q = 0; q < BATCH; ++q) {
+          const long long row_at = __shfl_sync(0xffffffffu, my_at, (s0 + q) * RPS + rr0);
+          const long long at = row_at + 8 * c;
+#pragma unroll
+          for (int w = 0; w < (SPLIT ? 2 : 1); ++w) u[q][w] = make_uint4(0, 0, 0, 0);
+          if (row_at >= 0 && 8 * c < p.hd) {                     // hd is a multiple of 8
             if (a.q_vec) {
-              if (p.type == TOSK_F32) {
-                const float4 u = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p.q) + at);
-                const float4 v = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p.q) + at + 4);
-                x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
-                x[4] = v.x; x[5] = v.y; x[6] = v.z; x[7] = v.w;
-              } else {
-                const uint4 u = *reinterpret_cast<const uint4*>(reinterpret_cast<const __half*>(p.q) + at);
-                const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
-                  x[2 * e] = f.x;
-                  x[2 * e + 1] = f.y;
+              for (int w = 0; w < (SPLIT ? 2 : 1); ++w)
+                u[q][w] = SPLIT ? *reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(p.q) + at + 4 * w)
+                                : *reinterpret_cast<const uint4*>(reinterpret_cast<const __half*>(p.q) + at);
+            } else {
+              uint32_t* x = reinterpret_cast<uint32_t*>(&u[q][0]);
+#pragma unroll
+              for (int e = 0; e < (SPLIT ? 8 : 4); ++e) {
+                if (SPLIT) {
+                  x[e] = reinterpret_cast<const uint32_t*>(p.q)[at + e];
+                } else {
+                  const uint16_t* h = reinterpret_cast<const uint16_t*>(p.q) + at + 2 * e;
+                  x[e] = (uint32_t)h[0] | (uint32_t)h[1] << 16;
                 }
               }
-            } else {
-#pragma unroll
-              for (int e = 0; e < 8; ++e) x[e] = load_elem(p.q, p.type, at + e);   // hd is a multiple of 8
             }
           }
         }
-        float sc = sgn;
-        if (SPLIT) {
-          float mx = 0.0f;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(x[e]));
-#pragma unroll
-          for (int o = CH / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-          const float s2 = pow2_to_2p13(mx);
-          sc *= s2;
-          const float inv = 1.0f / s2;                           // exact: a power of two
-#pragma unroll
-          for (int q = 0; q < 32 / CH; ++q) {
-            const float v = __shfl_sync(0xffffffffu, inv, q * CH);
-            if (lane == step * (32 / CH) + q) my_inv = v;
-          }
-        }
-        uint32_t hi[4], lo[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float u = x[2 * e] * sc, v = x[2 * e + 1] * sc;
-          const __half2 H = __floats2half2_rn(u, v);
-          hi[e] = *reinterpret_cast<const uint32_t*>(&H);
+        for (int q = 0; q < BATCH; ++q) {
+          const int row = wq * 32 + (s0 + q) * RPS + rr0;
+          uint8_t* dst = sq + i * (SPLIT ? 2 : 1) * T::kTile + (c >> 3) * 16384 + sw128(row, c & 7);
           if (SPLIT) {
-            const float2 f = __half22float2(H);
-            const __half2 L = __floats2half2_rn(u - f.x, v - f.y);
-            lo[e] = *reinterpret_cast<const uint32_t*>(&L);
+            const uint4 &v0 = u[q][0], &v1 = u[q][SPLIT ? 1 : 0];
+            float x[8] = {__uint_as_float(v0.x), __uint_as_float(v0.y), __uint_as_float(v0.z), __uint_as_float(v0.w),
+                          __uint_as_float(v1.x), __uint_as_float(v1.y), __uint_as_float(v1.z), __uint_as_float(v1.w)};
+            float mx = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(x[e]));
+#pragma unroll
+            for (int o = CH / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+            const float s2 = pow2_to_2p13(mx), sc2 = sgn * s2, inv = 1.0f / s2;   // exact: powers of two
+#pragma unroll
+            for (int w = 0; w < RPS; ++w) {
+              const float v = __shfl_sync(0xffffffffu, inv, w * CH);
+              if (lane == (s0 + q) * RPS + w) my_inv = v;
+            }
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) split_pair(x[2 * e] * sc2, x[2 * e + 1] * sc2, hi[e], lo[e]);
+            *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            *reinterpret_cast<uint4*>(dst + T::kTile) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+          } else {
+            const uint32_t flip = sgn < 0.0f ? 0x80008000u : 0u;
+            *reinterpret_cast<uint4*>(dst) =
+                make_uint4(u[q][0].x ^ flip, u[q][0].y ^ flip, u[q][0].z ^ flip, u[q][0].w ^ flip);
           }
         }
-        uint8_t* dst = sq + i * (SPLIT ? 2 : 1) * T::kTile + (c >> 3) * 16384 + sw128(row, c & 7);
-        *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        if (SPLIT) *reinterpret_cast<uint4*>(dst + T::kTile) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       mbar_arrive(qfull);
@@ -351,7 +395,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
       uint32_t s[4][32];
 #pragma unroll
       for (int c = 0; c < 4; ++c) tc_ld32(ts + 32 * c, s[c]);
-      asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+      tc_wait_ld(s[0]);
+#pragma unroll
+      for (int c = 1; c < 4; ++c) tc_tie(s[c]);
       const int left = lim - (k0 + j * kKeys);                          // keys of this tile that the row sees
       if (__any_sync(0xffffffffu, left < kKeys)) {
 #pragma unroll
@@ -363,9 +409,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
       float mx[4];
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        mx[c] = __uint_as_float(s[c][0]);
+        mx[c] = fmaxf(__uint_as_float(s[c][0]), __uint_as_float(s[c][1]));
 #pragma unroll
-        for (int e = 1; e < 32; ++e) mx[c] = fmaxf(mx[c], __uint_as_float(s[c][e]));
+        for (int e = 2; e < 32; e += 2)
+          mx[c] = fmaxf(fmaxf(mx[c], __uint_as_float(s[c][e])), __uint_as_float(s[c][e + 1]));
       }
       const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;
       if (j == 0) {
@@ -382,7 +429,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
         for (int c = 0; c < HD / 32; ++c) {
           uint32_t o[32];
           tc_ld32(to + 32 * c, o);
-          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+          tc_wait_ld(o);
 #pragma unroll
           for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
           tc_st32(to + 32 * c, o);
@@ -391,37 +438,39 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
         m = mn;
       }
       const float bias = kBias - (m == -INFINITY ? 0.0f : m);
-      float sum[4];
+      const float2 sc2 = make_float2(sc, sc), bias2 = make_float2(bias, bias);
+      float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         uint32_t hi[16], lo[16];
-        sum[c] = 0.0f;
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const float u = ex2(fmaf(__uint_as_float(s[c][2 * e]), sc, bias));
-          const float v = ex2(fmaf(__uint_as_float(s[c][2 * e + 1]), sc, bias));
-          sum[c] += u;
-          sum[c] += v;
-          const __half2 H = __floats2half2_rn(u, v);
-          hi[e] = *reinterpret_cast<const uint32_t*>(&H);
+          const float2 x =
+              __ffma2_rn(make_float2(__uint_as_float(s[c][2 * e]), __uint_as_float(s[c][2 * e + 1])), sc2, bias2);
+          const float2 w = !SPLIT && (e & 3) == 3 ? exp2_fma(x) : make_float2(ex2(x.x), ex2(x.y));
+          sum[e & 1] = __fadd2_rn(sum[e & 1], w);
           if (SPLIT) {
-            const float2 f = __half22float2(H);
-            const __half2 L = __floats2half2_rn(u - f.x, v - f.y);
-            lo[e] = *reinterpret_cast<const uint32_t*>(&L);
+            split_pair(w.x, w.y, hi[e], lo[e]);
+          } else {
+            const __half2 H = __floats2half2_rn(w.x, w.y);
+            hi[e] = *reinterpret_cast<const uint32_t*>(&H);
           }
         }
         tmem_st16(ts + 16 * c, hi);
         if (SPLIT) tmem_st16(ts + 64 + 16 * c, lo);
+        if (c & 1) {                                                    // half the keys: the MMAs may start on them
+          tmem_st_wait();
+          tc_fence_before();
+          mbar_arrive(pfull + 2 * i + (c >> 1));
+        }
       }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-      tmem_st_wait();
-      tc_fence_before();
-      mbar_arrive(pfull + i);
+      l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
     }
     if (ok && nt[i] > 0) ok = mbar_wait(odone + i, (nt[i] - 1) & 1, p.err, 38);
     ok = __all_sync(0xffffffffu, ok);
     tc_fence_after();
     // ------------------------------------------------------------- output
+    if (lim <= k0) l = 0.0f;                                            // sees nothing here, whatever exp2 made of -inf
     bool bad = false;
     if (ok) {
       const float inv = p.splits ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
@@ -433,7 +482,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
         uint32_t o[32];
         if (nt[i] > 0) {
           tc_ld32(to + 32 * c, o);
-          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+          tc_wait_ld(o);
         } else {
 #pragma unroll
           for (int e = 0; e < 32; ++e) o[e] = 0;

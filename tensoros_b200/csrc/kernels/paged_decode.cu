@@ -58,15 +58,6 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// two floats as packed fp16 high parts and what they leave
-__device__ __forceinline__ void split_pair(float x, float y, uint32_t& hi, uint32_t& lo) {
-  const __half2 H = __floats2half2_rn(x, y);
-  const float2 f = __half22float2(H);
-  const __half2 L = __floats2half2_rn(x - f.x, y - f.y);
-  hi = *reinterpret_cast<const uint32_t*>(&H);
-  lo = *reinterpret_cast<const uint32_t*>(&L);
-}
-
 struct DecArgs {
   PagedProblem p;
   int qblocks;             // blocks of 8 * NQ query heads of a group

@@ -67,6 +67,14 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// two floats as packed fp16 high parts and what they leave
+__device__ __forceinline__ void split_pair(float x, float y, uint32_t& hi, uint32_t& lo) {
+  const __half2 H = __floats2half2_rn(x, y);
+  const float2 f = __half22float2(H);
+  const __half2 L = __floats2half2_rn(x - f.x, y - f.y);
+  hi = *reinterpret_cast<const uint32_t*>(&H);
+  lo = *reinterpret_cast<const uint32_t*>(&L);
+}
 // Power of two 2^k with m * 2^k in [2^13, 2^14) (m > 0 finite), else 1.
 __device__ __forceinline__ float pow2_to_2p13(float m) {
   const int eb = (int)((__float_as_uint(m) >> 23) & 0xFF);
