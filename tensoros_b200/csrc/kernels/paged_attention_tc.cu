@@ -59,7 +59,7 @@ struct TcShape {
   static constexpr int kTile = kHalves * 16384;                 // bytes of a 128 x HD fp16 tile
   static constexpr int kQ = 2 * (SPLIT ? 2 : 1) * kTile;
   static constexpr int kSlots = HD == 128 ? (SPLIT ? 3 : 5) : 8;
-  static constexpr int kBars = 2 * kSlots + 1 + 8;
+  static constexpr int kBars = 2 * kSlots + 2 + 8;
   static constexpr int kSmem = 1024 + kQ + kSlots * kTile + kBars * 8 + 16;
   static_assert(kSmem <= 227 * 1024, "shared memory");
 };
@@ -140,7 +140,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
   uint64_t* sfull = qfull + 1;                        // [2]: S of tile t is there
   uint64_t* pfull = sfull + 2;                        // [2][2]: half the keys of tile t's P are there
   uint64_t* odone = pfull + 4;                        // [2]: O of tile t has taken P in
-  uint32_t* tmem_at = reinterpret_cast<uint32_t*>(odone + 2);
+  uint64_t* vtail = odone + 2;                        // the last V tile's unused rows are zero
+  uint32_t* tmem_at = reinterpret_cast<uint32_t*>(vtail + 1);
   const PagedProblem& p = a.p;
   pdl_wait();
   pdl_trigger();
@@ -170,6 +171,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
     nt[i] = e > k0 ? (e - k0 + kKeys - 1) / kKeys : 0;
   }
   const int nmax = max(nt[0], nt[1]);
+  const bool tail = nmax > 0 && k0 + nmax * kKeys > k1;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (warp == 9) tmem_alloc(tmem_at, 512);
   if (tid == 0) {
@@ -178,6 +180,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
       mbar_init(empty + i, 1);
     }
     mbar_init(qfull, 2 * kRows);
+    mbar_init(vtail, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(sfull + i, 1);
       mbar_init(pfull + 2 * i, kRows);
@@ -224,79 +227,72 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
     }
     // every copy lands before the CTA may end
     for (int i = max(0, used - T::kSlots); i < used; ++i)
-      mbar_wait(full + i % T::kSlots, (i / T::kSlots) & 1, p.err, 32);
-  } else if (warp == 9) {
-    // ------------------------------------------------------------------ MMAs
-    constexpr uint32_t kIdS = (1u << 4) | (8u << 24) | ((uint32_t)(kKeys >> 3) << 17);
-    constexpr uint32_t kIdO = (1u << 4) | (8u << 24) | ((uint32_t)(HD >> 3) << 17) | (1u << 16);   // V is N-major
-    bool ok = mbar_wait(qfull, 0, p.err, 33);
+      ok = mbar_wait(full + i % T::kSlots, (i / T::kSlots) & 1, p.err, 32) && ok;
     ok = __all_sync(0xffffffffu, ok);
-    tc_fence_after();
-    auto wait_slot = [&](int i) {
-      if (ok) ok = mbar_wait(full + i % T::kSlots, (i / T::kSlots) & 1, p.err, 34);
-      ok = __all_sync(0xffffffffu, ok);
-    };
-    auto issue_s = [&](int i, int j) {
-      wait_slot(2 * j);
-      if (!ok) return;
-      if (lane == 0) {
-        const uint32_t kb = smem_u32(ring + (2 * j % T::kSlots) * T::kTile);
-        const uint32_t qb = smem_u32(sq + i * (SPLIT ? 2 : 1) * T::kTile);
+    if (tail && ok) {
+      // value rows of the last tile behind the key range count with weight 0:
+      // they must be finite
+      const int have = k1 - (k0 + (nmax - 1) * kKeys);
+      for (int h = 0; h < T::kHalves; ++h)
+        for (int o = have * 128 + lane * 16; o < kKeys * 128; o += 512)
+          *reinterpret_cast<uint4*>(ring + (used - 1) % T::kSlots * T::kTile + h * 16384 + o) = make_uint4(0, 0, 0, 0);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(vtail);
+    }
+  } else if (warp == 9) {
+    // ------------------------------------------------------- MMAs, one thread
+    if (elect_one()) {
+      constexpr uint32_t kIdS = (1u << 4) | (8u << 24) | ((uint32_t)(kKeys >> 3) << 17);
+      constexpr uint32_t kIdO = (1u << 4) | (8u << 24) | ((uint32_t)(HD >> 3) << 17) | (1u << 16);   // V is N-major
+      bool ok = mbar_wait(qfull, 0, p.err, 33);
+      tc_fence_after();
+      // S of row tile i on key tile j (the first of the two row tiles waits for K)
+      auto issue_s = [&](int i, int j) {
+        if (i == 0 || j >= nt[0]) ok = ok && mbar_wait(full + 2 * j % T::kSlots, (2 * j / T::kSlots) & 1, p.err, 34);
+        if (!ok) return;
+        const uint32_t kd = desc_k(smem_u32(ring + (2 * j % T::kSlots) * T::kTile));
+        const uint32_t qd = desc_k(smem_u32(sq + i * (SPLIT ? 2 : 1) * T::kTile));
+        const uint32_t d = tmem + i * kKeys;
 #pragma unroll
         for (int part = 0; part < (SPLIT ? 2 : 1); ++part)
 #pragma unroll
           for (int k = 0; k < HD / 16; ++k) {
-            const uint32_t off = (k >> 2) * 16384 + (k & 3) * 32;
-            mma_f16_ss(tmem + i * kKeys, desc_k(qb + part * T::kTile + off), desc_k(kb + off), kIdS, part + k > 0);
+            const uint32_t off = ((k >> 2) * 16384 + (k & 3) * 32) >> 4;
+            mma_f16_ss(d, qd + (part * T::kTile >> 4) + off, kd + off, kIdS, part + k > 0);
           }
         mma_commit(sfull + i);
         if (i == 1 || j >= nt[1]) mma_commit(empty + 2 * j % T::kSlots);
-      }
-      __syncwarp();
-    };
-    for (int i = 0; i < 2; ++i)
-      if (nt[i] > 0 && ok) issue_s(i, 0);
-    for (int j = 0; j < nmax && ok; ++j)
-      for (int i = 0; i < 2 && ok; ++i) {
-        if (j >= nt[i]) continue;
-        const int slot = (2 * j + 1) % T::kSlots;
-        wait_slot(2 * j + 1);
-        const int have = min(kKeys, k1 - (k0 + j * kKeys));
-        if (ok && have < kKeys && (i == 0 || j >= nt[0])) {
-          // value rows behind the range count with weight 0: they must be finite
-          for (int h = 0; h < T::kHalves; ++h) {
-            uint8_t* base = ring + slot * T::kTile + h * 16384;
-            for (int o = have * 128 + lane * 16; o < kKeys * 128; o += 512)
-              *reinterpret_cast<uint4*>(base + o) = make_uint4(0, 0, 0, 0);
+      };
+      for (int i = 0; i < 2; ++i)
+        if (nt[i] > 0) issue_s(i, 0);
+      for (int j = 0; j < nmax && ok; ++j)
+        for (int i = 0; i < 2 && ok; ++i) {
+          if (j >= nt[i]) continue;
+          const int slot = (2 * j + 1) % T::kSlots;
+          if (i == 0 || j >= nt[0]) {
+            ok = mbar_wait(full + slot, ((2 * j + 1) / T::kSlots) & 1, p.err, 34);
+            if (j == nmax - 1 && tail) ok = ok && mbar_wait(vtail, 0, p.err, 39);
           }
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          __syncwarp();
-        }
-        for (int half = 0; half < 2; ++half) {
-          if (ok) ok = mbar_wait(pfull + 2 * i + half, j & 1, p.err, 35);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          tc_fence_after();
-          if (lane == 0) {
-            const uint32_t vb = smem_u32(ring + slot * T::kTile);
+          const uint32_t vd0 = desc_mn(smem_u32(ring + slot * T::kTile), 16384);
+          const uint32_t d = tmem + 256 + i * HD;
+          for (int half = 0; half < 2 && ok; ++half) {
+            ok = mbar_wait(pfull + 2 * i + half, j & 1, p.err, 35);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t vd = vd0 + half * (kKeys / 2 * 128 >> 4), pa = tmem + i * kKeys + half * (kKeys / 4);
 #pragma unroll
             for (int part = 0; part < (SPLIT ? 2 : 1); ++part)
 #pragma unroll
-              for (int k = 0; k < kKeys / 32; ++k) {
-                const int kk = half * (kKeys / 32) + k;
-                mma_f16_ts(tmem + 256 + i * HD, tmem + i * kKeys + part * 64 + kk * 8, desc_mn(vb + kk * 2048, 16384),
-                           kIdO, j + half + part + k > 0);
-              }
-            if (half) {
-              mma_commit(odone + i);
-              if (i == 1 || j >= nt[1]) mma_commit(empty + slot);
-            }
+              for (int k = 0; k < kKeys / 32; ++k)
+                mma_f16_ts(d, pa + part * 64 + k * 8, vd + (k * 2048 >> 4), kIdO, part + k > 0 ? true : j + half > 0);
           }
-          __syncwarp();
+          if (!ok) break;
+          mma_commit(odone + i);
+          if (i == 1 || j >= nt[1]) mma_commit(empty + slot);
+          if (j + 1 < nt[i]) issue_s(i, j + 1);
         }
-        if (!ok) break;
-        if (j + 1 < nt[i]) issue_s(i, j + 1);
-      }
+    }
     __syncwarp();
   }
   } else {

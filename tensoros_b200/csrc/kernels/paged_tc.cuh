@@ -18,31 +18,39 @@ bool paged_decode_ok(const PagedProblem& p);
 int paged_decode_run(const PagedProblem& p, int late_wait, cudaStream_t st);
 
 #ifdef __CUDACC__
-// Shared-memory operand, rows of 128 bytes swizzled 128 B.  K-major (Q, K:
-// the contraction runs along the row): 8-row groups 1024 bytes apart.
-__device__ __forceinline__ uint64_t desc_k(uint32_t saddr) {
-  return (uint64_t)((saddr >> 4) & 0x3FFF) | (uint64_t)1 << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 |
-         (uint64_t)2 << 61;
+// Shared-memory operands, rows of 128 bytes swizzled 128 B, eight rows every
+// 1024 bytes (the stride offset): the descriptors differ in their low word
+// only, and an address within the tile is added to that.  K-major (Q, K: the
+// contraction runs along the row) has no leading offset; N-major (V: down the
+// rows) has the next 64 columns `lead` bytes on.
+constexpr uint32_t kDescHi = (1024u >> 4) | 1u << 14 | 2u << 29;
+__device__ __forceinline__ uint32_t desc_k(uint32_t saddr) { return (saddr >> 4) | 1u << 16; }
+__device__ __forceinline__ uint32_t desc_mn(uint32_t saddr, uint32_t lead) { return (saddr >> 4) | (lead >> 4) << 16; }
+// One lane of a converged warp.  The tensor instructions take their operands
+// from uniform registers; behind this predicate the compiler knows that one
+// thread runs and moves them there directly (behind lane == 0 an MMA took
+// ~100 cycles to issue, whatever its size).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
+  return p != 0;
 }
-// N-major (V: the contraction runs down the rows): 8-row groups of the
-// contraction 1024 bytes apart (stride offset), the next 64 columns `lead`
-// bytes on (leading offset).
-__device__ __forceinline__ uint64_t desc_mn(uint32_t saddr, uint32_t lead) {
-  return (uint64_t)((saddr >> 4) & 0x3FFF) | (uint64_t)(lead >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 |
-         (uint64_t)1 << 46 | (uint64_t)2 << 61;
-}
-__device__ __forceinline__ void mma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+// D (tensor memory) = A B or += A B; A and B in shared memory, or A in tensor
+// memory
+__device__ __forceinline__ void mma_f16_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool acc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "mov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)acc), "n"(kDescHi)
       : "memory");
 }
-__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a_tmem, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a_tmem, uint32_t b, uint32_t idesc, bool acc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a_tmem), "l"(b), "r"(idesc), "r"(acc)
+      "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "mov.b64 db, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}" ::"r"(d),
+      "r"(a_tmem), "r"(b), "r"(idesc), "r"((uint32_t)acc), "n"(kDescHi)
       : "memory");
 }
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {
