@@ -258,15 +258,35 @@ __global__ void __launch_bounds__(128) paged_attn_join_kernel(const JoinArgs a) 
   float L = 0.0f, o[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) o[i] = 0.0f;
-  for (int s = 0; s < cnt; ++s) {
-    const float2 ml = p.part_ml[s * step + row];
-    const float c = exp2f(ml.x - base);
-    L = fmaf(ml.y, c, L);
-    const float* src = p.part_o + (s * step + row) * p.hd;
+  for (int s0 = 0; s0 < cnt; s0 += 32) {
+    // lane i: the weight of slot s0 + i; the slots' rows four at a time, so
+    // that their loads are in flight together
+    float c = 0.0f;
+    if (s0 + lane < cnt) {
+      const float2 ml = p.part_ml[(s0 + lane) * step + row];
+      c = exp2f(ml.x - base);
+      L = fmaf(ml.y, c, L);
+    }
+    const int m = min(32, cnt - s0);
+    for (int s = 0; s < m; s += 4) {
+      float x[4][8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (lane + 32 * i < p.hd) o[i] = fmaf(src[lane + 32 * i], c, o[i]);
+      for (int u = 0; u < 4; ++u) {
+        const float* src = p.part_o + ((s0 + s + u) * step + row) * p.hd;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[u][i] = s + u < m && lane + 32 * i < p.hd ? src[lane + 32 * i] : 0.0f;
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const float cu = __shfl_sync(0xffffffffu, c, (s + u) & 31);
+        if (s + u < m) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) o[i] = fmaf(x[u][i], cu, o[i]);
+        }
+      }
+    }
   }
+  for (int x = 16; x > 0; x >>= 1) L += __shfl_xor_sync(0xffffffffu, L, x);
   const float inv = L == 0.0f ? 0.0f : 1.0f / L;
   const long long oo = (long long)tok * p.out_stride + (long long)h * p.hd;
   bool bad = false;
@@ -407,17 +427,23 @@ void part_views(PagedProblem& p, void* ws, int slots) {
 // Many rows a sequence: the tensor cores where the cache allows it.
 int run_tiles(const PagedProblem& p, cudaStream_t st) { return paged_tc_ok(p) ? paged_tc_run(p, st) : run_general(p, st); }
 
-// Splits of a prompt call's keys (0: none): row tiles of 256 that leave SMs
-// without work are cut along the keys, at least 512 a split.
+// Splits of a prompt call's keys (0: none).  Fewer row tiles than SMs leave
+// SMs without work: the keys are cut, at least 512 a split, into the number
+// of splits with the shortest schedule (rounds over the SMs, each 1/s of the
+// keys), at ~3% of a round a split for the partial rows' way through memory.
 int plan_prompt(int n_seqs, int total_q, int max_q, int max_kv, int heads, int n_kv) {
-  const long long g = heads / n_kv;
-  long long tiles = ((long long)max_q * g + 255) / 256 * n_seqs;
-  const long long most = ((long long)total_q * g + 255) / 256 + n_seqs;
-  if (most < tiles) tiles = most;
-  tiles *= n_kv;
-  long long s = kSms / tiles;
-  if (s > (max_kv + 511) / 512) s = (max_kv + 511) / 512;
-  return s > 1 ? (int)s : 0;
+  const long long tiles = paged_tc_tiles(n_seqs, total_q, max_q, heads / n_kv) * n_kv;
+  if (tiles >= kSms) return 0;
+  int best = 1;
+  float cost = 1.0f;
+  for (int s = 2; s <= 16 && s <= max_kv / 512; ++s) {
+    const float c = (float)((s * tiles + kSms - 1) / kSms) / s + 0.03f * s;
+    if (c < cost) {
+      cost = c;
+      best = s;
+    }
+  }
+  return best > 1 ? best : 0;
 }
 }  // namespace
 

@@ -39,9 +39,12 @@
 
 namespace tos {
 
-constexpr int kTcThreads = 384;        // two softmax warpgroups; K/V copies, MMAs, two idle warps
-constexpr int kTcRegsSoftmax = 208, kTcRegsRest = 88;   // of the launch's 168 a thread: 2 * 208 + 88 = 3 * 168
-static_assert(2 * kTcRegsSoftmax + kTcRegsRest <= 3 * 168, "registers of the launch");
+constexpr int kTcThreads = 640;        // four softmax warpgroups; K/V copies, MMAs, two idle warps
+constexpr int kTcRegs = 96;            // a thread at launch, moved to the softmax warps afterwards
+constexpr int kTcRegsSoftmax = 104, kTcRegsRest = 64;
+static_assert(4 * kTcRegsSoftmax + kTcRegsRest <= 5 * kTcRegs, "registers of the launch");
+constexpr int kCopyWarp = 16, kMmaWarp = 17;
+constexpr int kSetupBar = 9;           // named barriers: 1..8 pair the two warps of 32 rows, 9 the set-up
 constexpr int kRows = 128;            // rows of a tile
 constexpr int kKeys = 128;            // keys of a tile
 constexpr float kBias = 7.0f;         // log2 of the factor that P carries
@@ -50,7 +53,7 @@ constexpr float kSlack = 8.0f;        // log2 by which the maximum may grow unfo
 struct TcArgs {
   CUtensorMap mk, mv;                 // [page][row][kv head][dim]: boxes of box_rows rows x 64 dims
   PagedProblem p;
-  int rtiles, box_rows, q_vec, out_vec;
+  int box_rows, q_vec, out_vec;
 };
 
 template <int HD, bool SPLIT>
@@ -59,8 +62,9 @@ struct TcShape {
   static constexpr int kTile = kHalves * 16384;                 // bytes of a 128 x HD fp16 tile
   static constexpr int kQ = 2 * (SPLIT ? 2 : 1) * kTile;
   static constexpr int kSlots = HD == 128 ? (SPLIT ? 3 : 5) : 8;
-  static constexpr int kBars = 2 * kSlots + 2 + 8;
-  static constexpr int kSmem = 1024 + kQ + kSlots * kTile + kBars * 8 + 16;
+  static constexpr int kBars = 2 * kSlots + 1 + 8;
+  static constexpr int kStage = kQ >= 16 * 4096 ? 0 : 16 * 4096;     // output rows, where Q's place is too small for them
+  static constexpr int kSmem = kQ + kSlots * kTile + kStage + kBars * 8 + 16 + 4 * kRows * 4;
   static_assert(kSmem <= 227 * 1024, "shared memory");
 };
 
@@ -127,21 +131,183 @@ __device__ __forceinline__ void tma_page(void* dst, const CUtensorMap* m, int x,
       : "memory");
 }
 
+struct TileId {
+  int seq, rt;                        // seq < 0: no such tile
+};
+
+// The f-th row tile of the call in falling order of its key tiles, so that
+// the long ones start first whatever the sequences' order, and no CTA is
+// spent on tiles that the longest sequence would have.  In sequence s the
+// tiles with at least w key tiles are the last count(s, w); the w of rank f
+// is found by bisection over their sum (lanes take sequences), the sequence
+// by a prefix sum.
+__device__ __forceinline__ TileId pick_tile(const PagedProblem& p, int f) {
+  TileId id = {-1, 0};
+  if (p.n_seqs == 1) {
+    const SeqTask t = seq_task(p, 0);
+    const int n = (t.qn * p.group + 2 * kRows - 1) / (2 * kRows);
+    if (f < n) id = {0, n - 1 - f};
+    return id;
+  }
+  const int lane = threadIdx.x & 31;
+  auto tiles = [&](const SeqTask& t) { return (t.qn * p.group + 2 * kRows - 1) / (2 * kRows); };
+  const SeqTask none = {0, 0, 0, 0, nullptr};
+  const SeqTask mine = lane < p.n_seqs ? seq_task(p, lane) : none;    // the first 32 sequences stay in registers
+  auto task = [&](int s) { return s < 32 ? mine : s < p.n_seqs ? seq_task(p, s) : none; };
+  auto count = [&](const SeqTask& t, int w) {
+    const int n = tiles(t);
+    if (w <= 0) return n;
+    if (kKeys * (w - 1) >= t.kvn) return 0;
+    const long long tok = (long long)kKeys * (w - 1) - t.off;    // first token that sees key kKeys (w - 1)
+    const long long first = tok <= 0 ? 0 : tok * p.group / (2 * kRows);
+    return first >= n ? 0 : n - (int)first;
+  };
+  auto total = [&](int w) {
+    int c = count(mine, w);
+    for (int s = lane + 32; s < p.n_seqs; s += 32) c += count(seq_task(p, s), w);
+    return __reduce_add_sync(0xffffffffu, c);
+  };
+  if (f >= total(0)) return id;
+  int lo = 0, hi = (p.max_kv + kKeys - 1) / kKeys + 1;            // total(lo) > f >= total(hi)
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (total(mid) > f) lo = mid;
+    else hi = mid;
+  }
+  f -= total(lo + 1);
+  for (int s0 = 0; s0 < p.n_seqs; s0 += 32) {
+    const int s = s0 + lane;
+    const SeqTask t = task(s);
+    const int c0 = count(t, lo), c1 = count(t, lo + 1);
+    int sum = c0 - c1;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += v;
+    }
+    const uint32_t hit = __ballot_sync(0xffffffffu, sum > f);
+    if (hit) {
+      const int w = __ffs(hit) - 1;
+      const int before = __shfl_sync(0xffffffffu, sum - (c0 - c1), w);
+      const int rt = tiles(t) - c0;                               // first tile with that many
+      return {s0 + w, __shfl_sync(0xffffffffu, rt, w) + f - before};
+    }
+    f -= __shfl_sync(0xffffffffu, sum, 31);
+  }
+  return id;
+}
+
+// Scores from the n-th on (of 32) count for nothing.
+__device__ __forceinline__ void mask32(uint32_t (&s)[32], int n) {
+#pragma unroll
+  for (int e = 0; e < 32; ++e)
+    if (e >= n) s[e] = 0xff800000u;                                     // -inf
+}
+__device__ __forceinline__ float max32(const uint32_t (&s)[32]) {
+  float a = fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1])), b = fmaxf(__uint_as_float(s[2]), __uint_as_float(s[3]));
+#pragma unroll
+  for (int e = 4; e < 32; e += 4) {
+    a = fmaxf(fmaxf(a, __uint_as_float(s[e])), __uint_as_float(s[e + 1]));
+    b = fmaxf(fmaxf(b, __uint_as_float(s[e + 2])), __uint_as_float(s[e + 3]));
+  }
+  return fmaxf(a, b);
+}
+// The two warps that share 32 rows.
+__device__ __forceinline__ void pair_sync(int bar) { asm volatile("bar.sync %0, 64;" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ bool pair_any(int bar, bool x) {
+  uint32_t y;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %2, 0;\n\tbar.red.or.pred q, %1, 64, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(y)
+      : "r"(bar), "r"((uint32_t)x)
+      : "memory");
+  return y != 0;
+}
+
+// The two row tiles of Q into the swizzled K-major layout, 16 rows a warp, 8
+// or 16 lanes a row, eight elements each, all rows in flight at once.  fp32
+// rows are scaled by a power of two and split; what undoes the scale goes to
+// sx[tile][0][row].  A lane works out one row's place.
+template <int HD, bool SPLIT>
+__device__ __forceinline__ void load_q(const PagedProblem& p, const SeqTask& t, int kvh, int rows, int r0, int vec,
+                                       uint8_t* sq, float* sx) {
+  using T = TcShape<HD, SPLIT>;
+  constexpr int CH = HD / 8, RPS = 32 / CH, STEPS = 16 / RPS, PARTS = SPLIT ? 2 : 1, BATCH = 8 / PARTS < STEPS ? 8 / PARTS : STEPS;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, i = warp >> 3, w0 = (warp & 7) * 16;
+  const float sgn = p.scale_log2 < 0.0f ? -1.0f : 1.0f;        // a negative scale goes into q
+  const int c = lane % CH, rr0 = lane / CH;
+  const int pr = r0 + i * kRows + w0 + (lane & 15);
+  const long long my_at = pr < rows ? (long long)(t.q0 + pr / p.group) * p.q_stride +
+                                          (long long)(kvh * p.group + pr % p.group) * p.hd
+                                    : -1;
+#pragma unroll
+  for (int s0 = 0; s0 < STEPS; s0 += BATCH) {
+    uint4 u[BATCH][PARTS];
+#pragma unroll
+    for (int q = 0; q < BATCH; ++q) {
+      const long long row_at = __shfl_sync(0xffffffffu, my_at, (s0 + q) * RPS + rr0);
+      const long long at = row_at + 8 * c;
+#pragma unroll
+      for (int w = 0; w < PARTS; ++w) u[q][w] = make_uint4(0, 0, 0, 0);
+      if (row_at >= 0 && 8 * c < p.hd) {                         // hd is a multiple of 8
+        if (vec) {
+#pragma unroll
+          for (int w = 0; w < PARTS; ++w)
+            u[q][w] = SPLIT ? *reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(p.q) + at + 4 * w)
+                            : *reinterpret_cast<const uint4*>(reinterpret_cast<const __half*>(p.q) + at);
+        } else if (SPLIT) {
+          const uint32_t* x = reinterpret_cast<const uint32_t*>(p.q) + at;
+          u[q][0] = make_uint4(x[0], x[1], x[2], x[3]);
+          u[q][PARTS - 1] = make_uint4(x[4], x[5], x[6], x[7]);
+        } else {
+          const uint16_t* h = reinterpret_cast<const uint16_t*>(p.q) + at;
+          u[q][0] = make_uint4(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16, h[4] | (uint32_t)h[5] << 16,
+                               h[6] | (uint32_t)h[7] << 16);
+        }
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < BATCH; ++q) {
+      const int row = w0 + (s0 + q) * RPS + rr0;
+      uint8_t* dst = sq + i * PARTS * T::kTile + (c >> 3) * 16384 + sw128(row, c & 7);
+      if (SPLIT) {
+        const uint4 v0 = u[q][0], v1 = u[q][PARTS - 1];
+        const float x[8] = {__uint_as_float(v0.x), __uint_as_float(v0.y), __uint_as_float(v0.z), __uint_as_float(v0.w),
+                            __uint_as_float(v1.x), __uint_as_float(v1.y), __uint_as_float(v1.z), __uint_as_float(v1.w)};
+        float mx = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(x[e]));
+#pragma unroll
+        for (int o = CH / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        const float s2 = pow2_to_2p13(mx), f = sgn * s2;         // exact: powers of two
+        if (c == 0) sx[i * 2 * kRows + row] = 1.0f / s2;
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) split_pair(x[2 * e] * f, x[2 * e + 1] * f, hi[e], lo[e]);
+        *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        *reinterpret_cast<uint4*>(dst + T::kTile) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      } else {
+        const uint32_t flip = sgn < 0.0f ? 0x80008000u : 0u;
+        *reinterpret_cast<uint4*>(dst) = make_uint4(u[q][0].x ^ flip, u[q][0].y ^ flip, u[q][0].z ^ flip, u[q][0].w ^ flip);
+      }
+    }
+  }
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+
 template <int HD, bool SPLIT>
 __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __grid_constant__ TcArgs a) {
   using T = TcShape<HD, SPLIT>;
-  extern __shared__ uint8_t raw[];
-  uint8_t* sm = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
-  uint8_t* sq = sm;                                   // [tile][hi, lo][half][128 rows x 128 B]
+  extern __shared__ __align__(1024) uint8_t sm[];
+  uint8_t* sq = sm;                                   // [tile][hi, lo][half][128 rows x 128 B]; then output rows
   uint8_t* ring = sm + T::kQ;
-  uint64_t* full = reinterpret_cast<uint64_t*>(ring + T::kSlots * T::kTile);
+  uint64_t* full = reinterpret_cast<uint64_t*>(ring + T::kSlots * T::kTile + T::kStage);
   uint64_t* empty = full + T::kSlots;
-  uint64_t* qfull = empty + T::kSlots;
-  uint64_t* sfull = qfull + 1;                        // [2]: S of tile t is there
+  uint64_t* sfull = empty + T::kSlots;                // [2]: S of tile t is there
   uint64_t* pfull = sfull + 2;                        // [2][2]: half the keys of tile t's P are there
   uint64_t* odone = pfull + 4;                        // [2]: O of tile t has taken P in
   uint64_t* vtail = odone + 2;                        // the last V tile's unused rows are zero
   uint32_t* tmem_at = reinterpret_cast<uint32_t*>(vtail + 1);
+  float* sx = reinterpret_cast<float*>(tmem_at + 4);  // [tile][half of the keys][row]: exchange of the two halves
   const PagedProblem& p = a.p;
   pdl_wait();
   pdl_trigger();
@@ -149,13 +315,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
   int b = blockIdx.x;
   const int kvh = b % p.n_kv;
   b /= p.n_kv;
-  const int seq = b % p.n_seqs;
-  b /= p.n_seqs;
   const int split = p.splits ? b % p.splits : 0;
-  const int rt = a.rtiles - 1 - (p.splits ? b / p.splits : b);      // long rows first
-  const SeqTask t = seq_task(p, seq);
-  const int rows = t.qn * p.group, r0 = rt * 2 * kRows;
-  if (r0 >= rows) return;
+  const TileId id = pick_tile(p, p.splits ? b / p.splits : b);
+  if (id.seq < 0) return;
+  const SeqTask t = seq_task(p, id.seq);
+  const int rows = t.qn * p.group, r0 = id.rt * 2 * kRows;
   int k0 = 0, k1 = seen(p, t, (min(rows, r0 + 2 * kRows) - 1) / p.group);
   if (p.splits) {
     k0 = split * p.chunk;
@@ -173,276 +337,213 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
   const int nmax = max(nt[0], nt[1]);
   const bool tail = nmax > 0 && k0 + nmax * kKeys > k1;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  if (warp == 9) tmem_alloc(tmem_at, 512);
-  if (tid == 0) {
-    for (int i = 0; i < T::kSlots; ++i) {
-      mbar_init(full + i, 1);
-      mbar_init(empty + i, 1);
-    }
-    mbar_init(qfull, 2 * kRows);
-    mbar_init(vtail, 1);
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(sfull + i, 1);
-      mbar_init(pfull + 2 * i, kRows);
-      mbar_init(pfull + 2 * i + 1, kRows);
-      mbar_init(odone + i, 1);
-    }
-    mbar_fence_init();
+  if (smem_u32(sm) & 1023) {                          // the swizzled tiles need it; the launch gives it
+    if (tid == 0) atomicCAS(p.err, 0, 41);
+    return;
   }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = *tmem_at;
-
-  if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTcRegsRest));
-  if (warp == 8) {
-    // ------------------------------------------------------------ K, V tiles
-    bool ok = true;
-    int used = 0;                                     // slots filled
-    for (int j = 0; j < nmax && ok; ++j) {
-      const int kt = k0 + j * kKeys;
-      const int need = (min(kKeys, k1 - kt) + a.box_rows - 1) / a.box_rows;
-      int page = -1, row = 0;
-      if (lane < need) {
-        const int key = kt + lane * a.box_rows;
-        page = t.table[key / p.page_size];
-        row = key % p.page_size;
+  if (warp == kCopyWarp) {
+    // the copies start before the other warps are ready
+    if (lane == 0) {
+      for (int i = 0; i < T::kSlots; ++i) {
+        mbar_init(full + i, 1);
+        mbar_init(empty + i, 1);
       }
-      for (int v = 0; v < 2 && ok; ++v) {
-        const int s = used % T::kSlots;
-        if (used >= T::kSlots) ok = mbar_wait(empty + s, (used / T::kSlots - 1) & 1, p.err, 31);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        if (lane == 0) mbar_arrive_expect_tx(full + s, need * a.box_rows * HD * 2);
-        __syncwarp();
-        if (lane < need) {
-          uint8_t* dst = ring + s * T::kTile + lane * a.box_rows * 128;
-#pragma unroll
-          for (int h = 0; h < T::kHalves; ++h)
-            tma_page(dst + h * 16384, v ? &a.mv : &a.mk, 64 * h, kvh, row, page, full + s);
-        }
-        ++used;
+      mbar_init(vtail, 1);
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(sfull + i, 1);
+        mbar_init(pfull + 2 * i, kRows);
+        mbar_init(pfull + 2 * i + 1, kRows);
+        mbar_init(odone + i, 1);
       }
-    }
-    // every copy lands before the CTA may end
-    for (int i = max(0, used - T::kSlots); i < used; ++i)
-      ok = mbar_wait(full + i % T::kSlots, (i / T::kSlots) & 1, p.err, 32) && ok;
-    ok = __all_sync(0xffffffffu, ok);
-    if (tail && ok) {
-      // value rows of the last tile behind the key range count with weight 0:
-      // they must be finite
-      const int have = k1 - (k0 + (nmax - 1) * kKeys);
-      for (int h = 0; h < T::kHalves; ++h)
-        for (int o = have * 128 + lane * 16; o < kKeys * 128; o += 512)
-          *reinterpret_cast<uint4*>(ring + (used - 1) % T::kSlots * T::kTile + h * 16384 + o) = make_uint4(0, 0, 0, 0);
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) mbar_arrive(vtail);
-    }
-  } else if (warp == 9) {
-    // ------------------------------------------------------- MMAs, one thread
-    if (elect_one()) {
-      constexpr uint32_t kIdS = (1u << 4) | (8u << 24) | ((uint32_t)(kKeys >> 3) << 17);
-      constexpr uint32_t kIdO = (1u << 4) | (8u << 24) | ((uint32_t)(HD >> 3) << 17) | (1u << 16);   // V is N-major
-      bool ok = mbar_wait(qfull, 0, p.err, 33);
-      tc_fence_after();
-      // S of row tile i on key tile j (the first of the two row tiles waits for K)
-      auto issue_s = [&](int i, int j) {
-        if (i == 0 || j >= nt[0]) ok = ok && mbar_wait(full + 2 * j % T::kSlots, (2 * j / T::kSlots) & 1, p.err, 34);
-        if (!ok) return;
-        const uint32_t kd = desc_k(smem_u32(ring + (2 * j % T::kSlots) * T::kTile));
-        const uint32_t qd = desc_k(smem_u32(sq + i * (SPLIT ? 2 : 1) * T::kTile));
-        const uint32_t d = tmem + i * kKeys;
-#pragma unroll
-        for (int part = 0; part < (SPLIT ? 2 : 1); ++part)
-#pragma unroll
-          for (int k = 0; k < HD / 16; ++k) {
-            const uint32_t off = ((k >> 2) * 16384 + (k & 3) * 32) >> 4;
-            mma_f16_ss(d, qd + (part * T::kTile >> 4) + off, kd + off, kIdS, part + k > 0);
-          }
-        mma_commit(sfull + i);
-        if (i == 1 || j >= nt[1]) mma_commit(empty + 2 * j % T::kSlots);
-      };
-      for (int i = 0; i < 2; ++i)
-        if (nt[i] > 0) issue_s(i, 0);
-      for (int j = 0; j < nmax && ok; ++j)
-        for (int i = 0; i < 2 && ok; ++i) {
-          if (j >= nt[i]) continue;
-          const int slot = (2 * j + 1) % T::kSlots;
-          if (i == 0 || j >= nt[0]) {
-            ok = mbar_wait(full + slot, ((2 * j + 1) / T::kSlots) & 1, p.err, 34);
-            if (j == nmax - 1 && tail) ok = ok && mbar_wait(vtail, 0, p.err, 39);
-          }
-          const uint32_t vd0 = desc_mn(smem_u32(ring + slot * T::kTile), 16384);
-          const uint32_t d = tmem + 256 + i * HD;
-          for (int half = 0; half < 2 && ok; ++half) {
-            ok = mbar_wait(pfull + 2 * i + half, j & 1, p.err, 35);
-            if (!ok) break;
-            tc_fence_after();
-            const uint32_t vd = vd0 + half * (kKeys / 2 * 128 >> 4), pa = tmem + i * kKeys + half * (kKeys / 4);
-#pragma unroll
-            for (int part = 0; part < (SPLIT ? 2 : 1); ++part)
-#pragma unroll
-              for (int k = 0; k < kKeys / 32; ++k)
-                mma_f16_ts(d, pa + part * 64 + k * 8, vd + (k * 2048 >> 4), kIdO, part + k > 0 ? true : j + half > 0);
-          }
-          if (!ok) break;
-          mma_commit(odone + i);
-          if (i == 1 || j >= nt[1]) mma_commit(empty + slot);
-          if (j + 1 < nt[i]) issue_s(i, j + 1);
-        }
+      mbar_fence_init();
     }
     __syncwarp();
+    asm volatile("bar.arrive %0, %1;" ::"n"(kSetupBar), "n"(kTcThreads) : "memory");
+  } else {
+    if (warp == kMmaWarp) tmem_alloc(tmem_at, 512);
+    if (warp < kCopyWarp) load_q<HD, SPLIT>(p, t, kvh, rows, r0, a.q_vec, sq, sx);
+    tc_fence_before();
+    asm volatile("bar.sync %0, %1;" ::"n"(kSetupBar), "n"(kTcThreads) : "memory");
+    tc_fence_after();
   }
+
+  if (warp >= kCopyWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTcRegsRest));
+    if (warp == kCopyWarp) {
+      // ------------------------------------------------------------ K, V tiles
+      bool ok = true;
+      int used = 0;                                     // slots filled
+      for (int j = 0; j < nmax && ok; ++j) {
+        const int kt = k0 + j * kKeys;
+        const int need = (min(kKeys, k1 - kt) + a.box_rows - 1) / a.box_rows;
+        int page = -1, row = 0;
+        if (lane < need) {
+          const int key = kt + lane * a.box_rows;
+          page = t.table[key / p.page_size];
+          row = key % p.page_size;
+        }
+        for (int v = 0; v < 2 && ok; ++v) {
+          const int s = used % T::kSlots;
+          if (used >= T::kSlots) ok = mbar_wait(empty + s, (used / T::kSlots - 1) & 1, p.err, 31);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          if (lane == 0) mbar_arrive_expect_tx(full + s, need * a.box_rows * HD * 2);
+          __syncwarp();
+          if (lane < need) {
+            uint8_t* dst = ring + s * T::kTile + lane * a.box_rows * 128;
+  #pragma unroll
+            for (int h = 0; h < T::kHalves; ++h)
+              tma_page(dst + h * 16384, v ? &a.mv : &a.mk, 64 * h, kvh, row, page, full + s);
+          }
+          ++used;
+        }
+      }
+      // every copy lands before the CTA may end
+      for (int i = max(0, used - T::kSlots); i < used; ++i)
+        ok = mbar_wait(full + i % T::kSlots, (i / T::kSlots) & 1, p.err, 32) && ok;
+      ok = __all_sync(0xffffffffu, ok);
+      if (tail && ok) {
+        // value rows of the last tile behind the key range count with weight 0:
+        // they must be finite
+        const int have = k1 - (k0 + (nmax - 1) * kKeys);
+        for (int h = 0; h < T::kHalves; ++h)
+          for (int o = have * 128 + lane * 16; o < kKeys * 128; o += 512)
+            *reinterpret_cast<uint4*>(ring + (used - 1) % T::kSlots * T::kTile + h * 16384 + o) = make_uint4(0, 0, 0, 0);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(vtail);
+      }
+    } else if (warp == kMmaWarp) {
+      // ------------------------------------------------------- MMAs, one thread
+      if (elect_one()) {
+        constexpr uint32_t kIdS = (1u << 4) | (8u << 24) | ((uint32_t)(kKeys >> 3) << 17);
+        constexpr uint32_t kIdO = (1u << 4) | (8u << 24) | ((uint32_t)(HD >> 3) << 17) | (1u << 16);   // V is N-major
+        const uint32_t tmem = *tmem_at;
+        bool ok = true;
+        // S of row tile i on key tile j (the first of the two row tiles waits for K)
+        auto issue_s = [&](int i, int j) {
+          if (i == 0 || j >= nt[0]) ok = ok && mbar_wait(full + 2 * j % T::kSlots, (2 * j / T::kSlots) & 1, p.err, 34);
+          if (!ok) return;
+          const uint32_t kd = desc_k(smem_u32(ring + (2 * j % T::kSlots) * T::kTile));
+          const uint32_t qd = desc_k(smem_u32(sq + i * (SPLIT ? 2 : 1) * T::kTile));
+          const uint32_t d = tmem + i * kKeys;
+  #pragma unroll
+          for (int part = 0; part < (SPLIT ? 2 : 1); ++part)
+  #pragma unroll
+            for (int k = 0; k < HD / 16; ++k) {
+              const uint32_t off = ((k >> 2) * 16384 + (k & 3) * 32) >> 4;
+              mma_f16_ss(d, qd + (part * T::kTile >> 4) + off, kd + off, kIdS, part + k > 0);
+            }
+          mma_commit(sfull + i);
+          if (i == 1 || j >= nt[1]) mma_commit(empty + 2 * j % T::kSlots);
+        };
+        for (int i = 0; i < 2; ++i)
+          if (nt[i] > 0) issue_s(i, 0);
+        for (int j = 0; j < nmax && ok; ++j)
+          for (int i = 0; i < 2 && ok; ++i) {
+            if (j >= nt[i]) continue;
+            const int slot = (2 * j + 1) % T::kSlots;
+            if (i == 0 || j >= nt[0]) {
+              ok = mbar_wait(full + slot, ((2 * j + 1) / T::kSlots) & 1, p.err, 34);
+              if (j == nmax - 1 && tail) ok = ok && mbar_wait(vtail, 0, p.err, 39);
+            }
+            const uint32_t vd0 = desc_mn(smem_u32(ring + slot * T::kTile), 16384);
+            const uint32_t d = tmem + 256 + i * HD;
+            for (int half = 0; half < 2 && ok; ++half) {
+              ok = mbar_wait(pfull + 2 * i + half, j & 1, p.err, 35);
+              if (!ok) break;
+              tc_fence_after();
+              const uint32_t vd = vd0 + half * (kKeys / 2 * 128 >> 4), pa = tmem + i * kKeys + half * 64;
+#pragma unroll
+              for (int part = 0; part < (SPLIT ? 2 : 1); ++part)
+#pragma unroll
+                for (int k = 0; k < kKeys / 32; ++k)
+                  mma_f16_ts(d, pa + (k >> 1) * 32 + part * 16 + (k & 1) * 8, vd + (k * 2048 >> 4), kIdO,
+                             part + k > 0 ? true : j + half > 0);
+            }
+            if (!ok) break;
+            mma_commit(odone + i);
+            if (i == 1 || j >= nt[1]) mma_commit(empty + slot);
+            if (j + 1 < nt[i]) issue_s(i, j + 1);
+          }
+      }
+      __syncwarp();
+    }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kTcRegsSoftmax));
     // --------------------------------------------------------------- softmax
-    const int i = warp >> 2, wq = warp & 3, r = tid & 127;      // row tile, TMEM quarter, row of the tile
-    const int base_row = r0 + i * kRows;
-    // Q rows of the tile into the swizzled K-major layout: 8 or 16 lanes a
-    // row, eight elements each; fp32 rows scaled by a power of two and split.
-    // A batch of rows is in flight at once; a lane works out one row's place.
-    float my_inv = 1.0f;                                         // undoes the scale of row r
-    {
-      constexpr int CH = HD / 8, RPS = 32 / CH, BATCH = SPLIT ? 4 : 8;
-      const float sgn = p.scale_log2 < 0.0f ? -1.0f : 1.0f;      // a negative scale goes into q
-      const int c = lane % CH, rr0 = lane / CH;
-      const int pr = base_row + wq * 32 + lane;
-      const long long my_at = pr < rows ? (long long)(t.q0 + pr / p.group) * p.q_stride +
-                                              (long long)(kvh * p.group + pr % p.group) * p.hd
-                                        : -1;
-      for (int s0 = 0; s0 < CH; s0 += BATCH) {
-        uint4 u[BATCH][SPLIT ? 2 : 1];
-#pragma unroll
-        for (int q = 0; q < BATCH; ++q) {
-          const long long row_at = __shfl_sync(0xffffffffu, my_at, (s0 + q) * RPS + rr0);
-          const long long at = row_at + 8 * c;
-#pragma unroll
-          for (int w = 0; w < (SPLIT ? 2 : 1); ++w) u[q][w] = make_uint4(0, 0, 0, 0);
-          if (row_at >= 0 && 8 * c < p.hd) {                     // hd is a multiple of 8
-            if (a.q_vec) {
-#pragma unroll
-              for (int w = 0; w < (SPLIT ? 2 : 1); ++w)
-                u[q][w] = SPLIT ? *reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(p.q) + at + 4 * w)
-                                : *reinterpret_cast<const uint4*>(reinterpret_cast<const __half*>(p.q) + at);
-            } else {
-              uint32_t* x = reinterpret_cast<uint32_t*>(&u[q][0]);
-#pragma unroll
-              for (int e = 0; e < (SPLIT ? 8 : 4); ++e) {
-                if (SPLIT) {
-                  x[e] = reinterpret_cast<const uint32_t*>(p.q)[at + e];
-                } else {
-                  const uint16_t* h = reinterpret_cast<const uint16_t*>(p.q) + at + 2 * e;
-                  x[e] = (uint32_t)h[0] | (uint32_t)h[1] << 16;
-                }
-              }
-            }
-          }
-        }
-#pragma unroll
-        for (int q = 0; q < BATCH; ++q) {
-          const int row = wq * 32 + (s0 + q) * RPS + rr0;
-          uint8_t* dst = sq + i * (SPLIT ? 2 : 1) * T::kTile + (c >> 3) * 16384 + sw128(row, c & 7);
-          if (SPLIT) {
-            const uint4 &v0 = u[q][0], &v1 = u[q][SPLIT ? 1 : 0];
-            float x[8] = {__uint_as_float(v0.x), __uint_as_float(v0.y), __uint_as_float(v0.z), __uint_as_float(v0.w),
-                          __uint_as_float(v1.x), __uint_as_float(v1.y), __uint_as_float(v1.z), __uint_as_float(v1.w)};
-            float mx = 0.0f;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(x[e]));
-#pragma unroll
-            for (int o = CH / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-            const float s2 = pow2_to_2p13(mx), sc2 = sgn * s2, inv = 1.0f / s2;   // exact: powers of two
-#pragma unroll
-            for (int w = 0; w < RPS; ++w) {
-              const float v = __shfl_sync(0xffffffffu, inv, w * CH);
-              if (lane == (s0 + q) * RPS + w) my_inv = v;
-            }
-            uint32_t hi[4], lo[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) split_pair(x[2 * e] * sc2, x[2 * e + 1] * sc2, hi[e], lo[e]);
-            *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-            *reinterpret_cast<uint4*>(dst + T::kTile) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-          } else {
-            const uint32_t flip = sgn < 0.0f ? 0x80008000u : 0u;
-            *reinterpret_cast<uint4*>(dst) =
-                make_uint4(u[q][0].x ^ flip, u[q][0].y ^ flip, u[q][0].z ^ flip, u[q][0].w ^ flip);
-          }
-        }
-      }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      mbar_arrive(qfull);
-    }
-    const int pr = base_row + r;
+    // row tile, half of a tile's keys (and of the output's dims), 32 rows
+    const int i = warp >> 3, hf = (warp >> 2) & 1, wq = warp & 3, r = wq * 32 + lane;
+    const int bar = 1 + i * 4 + wq;                                      // this warp and the other half's
+    const uint32_t tmem = *tmem_at;
+    const int pr = r0 + i * kRows + r;
     const bool live = pr < rows;
     const int tok = t.q0 + pr / p.group, head = kvh * p.group + pr % p.group;
     const int lim = live ? min(seen(p, t, pr / p.group), k1) : 0;      // keys this row sees
-    const float sc = fmaxf(fabsf(p.scale_log2) * my_inv, 1.2e-38f);   // not 0: a masked score is -inf * sc
+    float* mine = sx + (i * 2 + hf) * kRows + r;
+    float* other = sx + (i * 2 + (hf ^ 1)) * kRows + r;
+    const float inv_q = SPLIT ? sx[i * 2 * kRows + r] : 1.0f;           // undoes the row's scale
+    const float sc = fmaxf(fabsf(p.scale_log2) * inv_q, 1.2e-38f);     // not 0: a masked score is -inf * sc
+    pair_sync(bar);                                                     // the scales are read: sx is free
     const uint32_t lanes = (uint32_t)wq << 21;                          // TMEM lane of the warp's first row, << 16
-    const uint32_t ts = tmem + lanes + i * kKeys, to = tmem + lanes + 256 + i * HD;
+    const uint32_t ts = tmem + lanes + i * kKeys, to = tmem + lanes + 256 + i * HD + hf * (HD / 2);
     float m = -INFINITY, l = 0.0f;
-    bool ok = true;
+    bool ok = true;     // a wait that ran out: go on without waiting, so that the two warps' barriers stay paired
     for (int j = 0; j < nt[i]; ++j) {
       if (ok) ok = mbar_wait(sfull + i, j & 1, p.err, 36);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
+      __syncwarp();
       tc_fence_after();
-      uint32_t s[4][32];
+      const int left = lim - (k0 + j * kKeys) - 64 * hf;                // keys of this half tile that the row sees
+      const bool cut = __any_sync(0xffffffffu, left < 64);
+      // S is read twice, for the maximum and for the weights: two reads of
+      // tensor memory cost less than 64 registers
+      float top = -INFINITY;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) tc_ld32(ts + 32 * c, s[c]);
-      tc_wait_ld(s[0]);
-#pragma unroll
-      for (int c = 1; c < 4; ++c) tc_tie(s[c]);
-      const int left = lim - (k0 + j * kKeys);                          // keys of this tile that the row sees
-      if (__any_sync(0xffffffffu, left < kKeys)) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (32 * c + e >= left) s[c][e] = 0xff800000u;              // -inf
+      for (int c = 0; c < 2; ++c) {
+        uint32_t s[32];
+        tc_ld32(ts + 64 * hf + 32 * c, s);
+        tc_wait_ld(s);
+        if (cut) mask32(s, left - 32 * c);
+        top = fmaxf(top, max32(s));
       }
-      float mx[4];
+      top *= sc;
+      if (pair_any(bar, j == 0 || top > m + kSlack)) {
+        // a first or a much larger maximum: agree on the row's over both
+        // halves, scale O (each half its dims) and l to it
+        *mine = top;
+        pair_sync(bar);
+        top = fmaxf(top, *other);
+        const float mn = j == 0 || top > m + kSlack ? top : m;
+        if (j > 0) {
+          const float f = mn == m ? 1.0f : exp2f(m - mn);
+          if (ok) ok = mbar_wait(odone + i, (j - 1) & 1, p.err, 37);
+          __syncwarp();
+          tc_fence_after();
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        mx[c] = fmaxf(__uint_as_float(s[c][0]), __uint_as_float(s[c][1]));
+          for (int c = 0; c < HD / 64; ++c) {
+            uint32_t o[32];
+            tc_ld32(to + 32 * c, o);
+            tc_wait_ld(o);
 #pragma unroll
-        for (int e = 2; e < 32; e += 2)
-          mx[c] = fmaxf(fmaxf(mx[c], __uint_as_float(s[c][e])), __uint_as_float(s[c][e + 1]));
-      }
-      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;
-      if (j == 0) {
-        m = top;
-      } else if (__any_sync(0xffffffffu, top > m + kSlack)) {
-        // scale O and l to the new maximum (lanes that need not: by 1)
-        const float mn = top > m + kSlack ? top : m;
-        const float f = mn == m ? 1.0f : exp2f(m - mn);
-        if (ok) ok = mbar_wait(odone + i, (j - 1) & 1, p.err, 37);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        tc_fence_after();
-#pragma unroll
-        for (int c = 0; c < HD / 32; ++c) {
-          uint32_t o[32];
-          tc_ld32(to + 32 * c, o);
-          tc_wait_ld(o);
-#pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-          tc_st32(to + 32 * c, o);
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+            tc_st32(to + 32 * c, o);
+          }
+          l *= f;
         }
-        l *= f;
         m = mn;
       }
       const float bias = kBias - (m == -INFINITY ? 0.0f : m);
       const float2 sc2 = make_float2(sc, sc), bias2 = make_float2(bias, bias);
       float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t hi[16], lo[16];
+      for (int c = 0; c < 2; ++c) {
+        uint32_t s[32], hi[16], lo[16];
+        tc_ld32(ts + 64 * hf + 32 * c, s);
+        tc_wait_ld(s);
+        if (cut) mask32(s, left - 32 * c);
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const float2 x =
-              __ffma2_rn(make_float2(__uint_as_float(s[c][2 * e]), __uint_as_float(s[c][2 * e + 1])), sc2, bias2);
+          const float2 x = __ffma2_rn(make_float2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), sc2, bias2);
           const float2 w = !SPLIT && (e & 3) == 3 ? exp2_fma(x) : make_float2(ex2(x.x), ex2(x.y));
           sum[e & 1] = __fadd2_rn(sum[e & 1], w);
           if (SPLIT) {
@@ -452,81 +553,106 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
             hi[e] = *reinterpret_cast<const uint32_t*>(&H);
           }
         }
-        tmem_st16(ts + 16 * c, hi);
-        if (SPLIT) tmem_st16(ts + 64 + 16 * c, lo);
-        if (c & 1) {                                                    // half the keys: the MMAs may start on them
-          tmem_st_wait();
-          tc_fence_before();
-          mbar_arrive(pfull + 2 * i + (c >> 1));
-        }
+        // over these 32 keys' own S: high parts, then low parts
+        tmem_st16(ts + 64 * hf + 32 * c, hi);
+        if (SPLIT) tmem_st16(ts + 64 * hf + 32 * c + 16, lo);
       }
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(pfull + 2 * i + hf);
       l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
     }
     if (ok && nt[i] > 0) ok = mbar_wait(odone + i, (nt[i] - 1) & 1, p.err, 38);
     ok = __all_sync(0xffffffffu, ok);
     tc_fence_after();
+    pair_sync(bar);
+    *mine = l;
+    pair_sync(bar);
+    l += *other;
     // ------------------------------------------------------------- output
+    // A row a thread in tensor memory; 32 dims (fp32) or the half's dims
+    // (fp16) go through shared memory (Q's, which no MMA reads any more), 128
+    // bytes a row, so that eight lanes write a row's pieces side by side.
     if (lim <= k0) l = 0.0f;                                            // sees nothing here, whatever exp2 made of -inf
+    const bool f32 = p.splits || p.type == TOSK_F32;
+    const int es = f32 ? 4 : 2;
+    const float inv = l == 0.0f || nt[i] == 0 ? 0.0f : p.splits ? 1.0f : 1.0f / l;
+    const long long slot = (long long)(p.slot0 + split) * p.total_q * p.heads + (long long)tok * p.heads + head;
+    if (p.splits && live && hf == 0 && ok) p.part_ml[slot] = make_float2(m - kBias, l);
+    const long long row_at = !live ? -1 : p.splits ? slot * p.hd : (long long)tok * p.out_stride + (long long)head * p.hd;
+    uint8_t* stage = (T::kStage ? ring + T::kSlots * T::kTile : sq + i * (T::kQ / 2)) + ((T::kStage ? i * 8 : 0) + hf * 4 + wq) * 4096;
     bool bad = false;
-    if (ok) {
-      const float inv = p.splits ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
-      const long long part = (long long)(p.slot0 + split) * p.total_q * p.heads + (long long)tok * p.heads + head;
-      if (p.splits && live) p.part_ml[part] = make_float2(m - kBias, l);
-      const long long oo = (long long)tok * p.out_stride + (long long)head * p.hd;
-#pragma unroll
-      for (int c = 0; c < HD / 32; ++c) {
-        uint32_t o[32];
-        if (nt[i] > 0) {
-          tc_ld32(to + 32 * c, o);
-          tc_wait_ld(o);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = 0;
-        }
-        if (!live) continue;
-#pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          const float v = l == 0.0f ? 0.0f : __uint_as_float(o[e]) * inv;
-          o[e] = __float_as_uint(v);
-          bad |= isnan(v);
-        }
+    // the staged rows' `n` bytes to dims from dim0 on
+    auto flush = [&](int dim0, int n) {
+      __syncwarp();
+      const int c = lane & 7, dim = dim0 + c * (16 / es);
+#pragma unroll 4
+      for (int q = 0; q < 8; ++q) {
+        const int row = q * 4 + (lane >> 3);
+        const long long at = __shfl_sync(0xffffffffu, row_at, row);
+        if (at < 0 || c * 16 >= n || dim >= p.hd) continue;
+        const uint4 v = *reinterpret_cast<const uint4*>(stage + sw128(row, c));
         if (p.splits) {
-          float* dst = p.part_o + part * p.hd + 32 * c;
-#pragma unroll
-          for (int e = 0; e < 32; e += 4)
-            if (32 * c + e < p.hd) *reinterpret_cast<uint4*>(dst + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+          *reinterpret_cast<uint4*>(p.part_o + at + dim) = v;
+        } else if (a.out_vec) {
+          *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(p.out) + (at + dim) * es) = v;
         } else {
-          if (a.out_vec && p.type == TOSK_F32) {
-            float* dst = reinterpret_cast<float*>(p.out) + oo + 32 * c;
+          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-            for (int e = 0; e < 32; e += 4)
-              if (32 * c + e < p.hd) *reinterpret_cast<uint4*>(dst + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-          } else if (a.out_vec) {
-            __half* dst = reinterpret_cast<__half*>(p.out) + oo + 32 * c;
-#pragma unroll
-            for (int e = 0; e < 32; e += 8) {
-              uint32_t h[4];
-#pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                const __half2 H = __floats2half2_rn(__uint_as_float(o[e + 2 * q]), __uint_as_float(o[e + 2 * q + 1]));
-                h[q] = *reinterpret_cast<const uint32_t*>(&H);
-              }
-              if (32 * c + e < p.hd) *reinterpret_cast<uint4*>(dst + e) = make_uint4(h[0], h[1], h[2], h[3]);
+          for (int e = 0; e < 4; ++e) {
+            if (f32) {
+              reinterpret_cast<uint32_t*>(p.out)[at + dim + e] = w[e];
+            } else {
+              reinterpret_cast<uint16_t*>(p.out)[at + dim + 2 * e] = (uint16_t)w[e];
+              reinterpret_cast<uint16_t*>(p.out)[at + dim + 2 * e + 1] = (uint16_t)(w[e] >> 16);
             }
-          } else {
-#pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (32 * c + e < p.hd) store_elem(p.out, p.type, oo + 32 * c + e, __uint_as_float(o[e]));
           }
         }
       }
+      __syncwarp();
+    };
+    if (ok) {
+#pragma unroll
+      for (int c32 = 0; c32 < HD / 64; ++c32) {
+        uint32_t o[32];
+        tc_ld32(to + 32 * c32, o);
+        tc_wait_ld(o);
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          const float v = inv == 0.0f ? 0.0f : __uint_as_float(o[e]) * inv;
+          o[e] = __float_as_uint(v);
+          bad |= isnan(v);
+        }
+        if (f32) {
+#pragma unroll
+          for (int c = 0; c < 8; ++c)
+            *reinterpret_cast<uint4*>(stage + sw128(lane, c)) = make_uint4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
+          flush(hf * (HD / 2) + 32 * c32, 128);
+        } else {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t h[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const __half2 H = __floats2half2_rn(__uint_as_float(o[8 * c + 2 * q]), __uint_as_float(o[8 * c + 2 * q + 1]));
+              h[q] = *reinterpret_cast<const uint32_t*>(&H);
+            }
+            *reinterpret_cast<uint4*>(stage + sw128(lane, 4 * c32 + c)) = make_uint4(h[0], h[1], h[2], h[3]);
+          }
+        }
+      }
+      if (!f32) flush(hf * (HD / 2), HD);
     }
-    if (!p.splits) {
-      uint32_t todo = __ballot_sync(0xffffffffu, bad && live);
+    if (!p.splits && pair_any(bar, bad && live)) {
+      // rows that show NaN in either half, once both halves are written
+      pair_sync(bar);                                                   // l is read: sx is free
+      *mine = bad && live ? 1.0f : 0.0f;
+      pair_sync(bar);
+      uint32_t todo = hf == 0 ? __ballot_sync(0xffffffffu, *mine != 0.0f || *other != 0.0f) : 0;
       while (todo) {
         const int w = __ffs(todo) - 1;
         todo &= todo - 1;
-        const int pw = base_row + wq * 32 + w;
+        const int pw = r0 + i * kRows + wq * 32 + w;
         attn_row_plain(p, nullptr, 0, t.table, seen(p, t, pw / p.group), t.q0 + pw / p.group,
                        kvh * p.group + pw % p.group);
       }
@@ -534,9 +660,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
     tc_fence_before();
   }
   __syncthreads();
-  if (warp == 9) {
+  if (warp == kMmaWarp) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc(*tmem_at, 512);
   }
 }
 
@@ -592,15 +718,19 @@ bool paged_tc_ok(const PagedProblem& p) {
          (long long)ps * p.n_kv * p.hd * 2 < (1ll << 39);
 }
 
+// Row tiles of one key/value head that a call can have at most.
+long long paged_tc_tiles(int n_seqs, int total_q, int max_q, int group) {
+  const long long each = ((long long)max_q * group + 2 * kRows - 1) / (2 * kRows) * n_seqs;
+  const long long all = (long long)total_q * group / (2 * kRows) + n_seqs;
+  return each < all ? each : all;
+}
+
 int paged_tc_run(const PagedProblem& p, cudaStream_t st) {
   TcArgs a;
   a.p = p;
   a.box_rows = p.page_size < kKeys ? p.page_size : kKeys;
-  const long long rows = (long long)(p.fixed_kv >= 0 ? p.total_q : p.max_q) * p.group;
-  const long long rt = (rows + 2 * kRows - 1) / (2 * kRows);
-  const long long grid = rt * (p.splits ? p.splits : 1) * p.n_seqs * p.n_kv;
+  const long long grid = paged_tc_tiles(p.n_seqs, p.total_q, p.max_q, p.group) * (p.splits ? p.splits : 1) * p.n_kv;
   if (grid > 0x7fffffffll) return (int)cudaErrorInvalidValue;
-  a.rtiles = (int)rt;
   a.q_vec = ((uintptr_t)p.q & 15) == 0 && p.q_stride % (p.type == TOSK_F32 ? 4 : 8) == 0;
   a.out_vec = ((uintptr_t)p.out & 15) == 0 && p.out_stride % (p.type == TOSK_F32 ? 4 : 8) == 0;
   if (!pool_map(&a.mk, p.k, p, a.box_rows) || !pool_map(&a.mv, p.v, p, a.box_rows)) return (int)cudaErrorNotSupported;
