@@ -39,12 +39,13 @@
 
 namespace tos {
 
+constexpr int kTcCtas = 148;           // one a SM, each takes pieces of work in turn
 constexpr int kTcThreads = 640;        // four softmax warpgroups; K/V copies, MMAs, two idle warps
 constexpr int kTcRegs = 96;            // a thread at launch, moved to the softmax warps afterwards
 constexpr int kTcRegsSoftmax = 104, kTcRegsRest = 64;
 static_assert(4 * kTcRegsSoftmax + kTcRegsRest <= 5 * kTcRegs, "registers of the launch");
-constexpr int kCopyWarp = 16, kMmaWarp = 17;
-constexpr int kSetupBar = 9;           // named barriers: 1..8 pair the two warps of 32 rows, 9 the set-up
+constexpr int kCopyWarp = 16, kMmaWarp = 17, kPlanWarp = 18;
+constexpr int kTileBar = 9;            // named barriers: 1..8 pair the two warps of 32 rows, 9 and 10 a row tile's eight
 constexpr int kRows = 128;            // rows of a tile
 constexpr int kKeys = 128;            // keys of a tile
 constexpr float kBias = 7.0f;         // log2 of the factor that P carries
@@ -62,9 +63,9 @@ struct TcShape {
   static constexpr int kTile = kHalves * 16384;                 // bytes of a 128 x HD fp16 tile
   static constexpr int kQ = 2 * (SPLIT ? 2 : 1) * kTile;
   static constexpr int kSlots = HD == 128 ? (SPLIT ? 3 : 5) : 8;
-  static constexpr int kBars = 2 * kSlots + 1 + 8;
+  static constexpr int kBars = 2 * kSlots + 17;
   static constexpr int kStage = kQ >= 16 * 4096 ? 0 : 16 * 4096;     // output rows, where Q's place is too small for them
-  static constexpr int kSmem = kQ + kSlots * kTile + kStage + kBars * 8 + 16 + 4 * kRows * 4;
+  static constexpr int kSmem = kQ + kSlots * kTile + kStage + kBars * 8 + 8 + 2 * 64 + 4 * kRows * 4;
   static_assert(kSmem <= 227 * 1024, "shared memory");
 };
 
@@ -223,32 +224,56 @@ __device__ __forceinline__ bool pair_any(int bar, bool x) {
   return y != 0;
 }
 
-// The two row tiles of Q into the swizzled K-major layout, 16 rows a warp, 8
-// or 16 lanes a row, eight elements each, all rows in flight at once.  fp32
-// rows are scaled by a power of two and split; what undoes the scale goes to
-// sx[tile][0][row].  A lane works out one row's place.
+__device__ __forceinline__ bool tile_any(int bar, bool x) {
+  uint32_t y;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %2, 0;\n\tbar.red.or.pred q, %1, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(y)
+      : "r"(bar), "r"((uint32_t)x)
+      : "memory");
+  return y != 0;
+}
+
+// One piece of work: 256 packed rows of a sequence, one key/value head, keys
+// [k0, k1).
+struct __align__(16) Work {
+  int seq, kvh, split, r0;            // seq < 0: no more
+  int rows, q0, off, kvn;             // the sequence's packed rows and first token; its SeqTask's off, kvn
+  int k0, k1, nt[2];                  // key tiles of the two row tiles
+  int pad[4];
+};
+
+// Q rows of a row tile, 16 rows a warp, 8 or 16 lanes a row, eight elements
+// each: asked into L2 early, then through registers into the swizzled K-major
+// layout.  fp32 rows are scaled by a power of two and split into fp16 pairs.
 template <int HD, bool SPLIT>
-__device__ __forceinline__ void load_q(const PagedProblem& p, const SeqTask& t, int kvh, int rows, int r0, int vec,
-                                       uint8_t* sq, float* sx) {
-  using T = TcShape<HD, SPLIT>;
-  constexpr int CH = HD / 8, RPS = 32 / CH, STEPS = 16 / RPS, PARTS = SPLIT ? 2 : 1, BATCH = 8 / PARTS < STEPS ? 8 / PARTS : STEPS;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, i = warp >> 3, w0 = (warp & 7) * 16;
-  const float sgn = p.scale_log2 < 0.0f ? -1.0f : 1.0f;        // a negative scale goes into q
-  const int c = lane % CH, rr0 = lane / CH;
-  const int pr = r0 + i * kRows + w0 + (lane & 15);
-  const long long my_at = pr < rows ? (long long)(t.q0 + pr / p.group) * p.q_stride +
-                                          (long long)(kvh * p.group + pr % p.group) * p.hd
-                                    : -1;
-#pragma unroll
-  for (int s0 = 0; s0 < STEPS; s0 += BATCH) {
-    uint4 u[BATCH][PARTS];
+struct QRows {
+  static constexpr int CH = HD / 8, RPS = 32 / CH, STEPS = 16 / RPS, PARTS = SPLIT ? 2 : 1;
+  static constexpr int BATCH = 8 / PARTS < STEPS ? 8 / PARTS : STEPS;
+  long long my_at;                    // lane i: element offset of row i (of the warp's 16), -1: none
+
+  __device__ __forceinline__ void place(const PagedProblem& p, const Work& w, int row0) {
+    const int pr = w.r0 + row0 + (threadIdx.x & 15);
+    my_at = pr < w.rows ? (long long)(w.q0 + pr / p.group) * p.q_stride +
+                              (long long)(w.kvh * p.group + pr % p.group) * p.hd
+                        : -1;
+  }
+  // the rows' 128-byte lines into L2 (a row's first and second half of the warp each take every other one)
+  __device__ __forceinline__ void ask(const PagedProblem& p) {
+    const int es = SPLIT ? 4 : 2, first = (threadIdx.x >> 4) & 1;
+    if (my_at >= 0)
+      for (int o = first * 128; o < p.hd * es; o += 256)
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(reinterpret_cast<const uint8_t*>(p.q) + my_at * es + o));
+  }
+  __device__ __forceinline__ void fetch(const PagedProblem& p, int s0, int vec, uint4 (&u)[BATCH][PARTS]) {
+    const int lane = threadIdx.x & 31, c = lane % CH, rr0 = lane / CH;
 #pragma unroll
     for (int q = 0; q < BATCH; ++q) {
       const long long row_at = __shfl_sync(0xffffffffu, my_at, (s0 + q) * RPS + rr0);
       const long long at = row_at + 8 * c;
 #pragma unroll
       for (int w = 0; w < PARTS; ++w) u[q][w] = make_uint4(0, 0, 0, 0);
-      if (row_at >= 0 && 8 * c < p.hd) {                         // hd is a multiple of 8
+      if (row_at >= 0 && 8 * c < p.hd) {                       // hd is a multiple of 8
         if (vec) {
 #pragma unroll
           for (int w = 0; w < PARTS; ++w)
@@ -265,10 +290,17 @@ __device__ __forceinline__ void load_q(const PagedProblem& p, const SeqTask& t, 
         }
       }
     }
+  }
+  // dst: the row tile's high parts (low parts follow); what undoes a row's
+  // scale goes to inv[row]
+  __device__ __forceinline__ void store(const PagedProblem& p, int s0, int row0, uint8_t* dst, float* inv,
+                                        const uint4 (&u)[BATCH][PARTS]) {
+    const int lane = threadIdx.x & 31, c = lane % CH, rr0 = lane / CH;
+    const float sgn = p.scale_log2 < 0.0f ? -1.0f : 1.0f;      // a negative scale goes into q
 #pragma unroll
     for (int q = 0; q < BATCH; ++q) {
-      const int row = w0 + (s0 + q) * RPS + rr0;
-      uint8_t* dst = sq + i * PARTS * T::kTile + (c >> 3) * 16384 + sw128(row, c & 7);
+      const int row = row0 + (s0 + q) * RPS + rr0;
+      uint8_t* d = dst + (c >> 3) * 16384 + sw128(row, c & 7);
       if (SPLIT) {
         const uint4 v0 = u[q][0], v1 = u[q][PARTS - 1];
         const float x[8] = {__uint_as_float(v0.x), __uint_as_float(v0.y), __uint_as_float(v0.z), __uint_as_float(v0.w),
@@ -278,21 +310,21 @@ __device__ __forceinline__ void load_q(const PagedProblem& p, const SeqTask& t, 
         for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(x[e]));
 #pragma unroll
         for (int o = CH / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-        const float s2 = pow2_to_2p13(mx), f = sgn * s2;         // exact: powers of two
-        if (c == 0) sx[i * 2 * kRows + row] = 1.0f / s2;
+        const float s2 = pow2_to_2p13(mx), f = sgn * s2;       // exact: powers of two
+        if (c == 0) inv[row] = 1.0f / s2;
         uint32_t hi[4], lo[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) split_pair(x[2 * e] * f, x[2 * e + 1] * f, hi[e], lo[e]);
-        *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        *reinterpret_cast<uint4*>(dst + T::kTile) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        *reinterpret_cast<uint4*>(d) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        *reinterpret_cast<uint4*>(d + TcShape<HD, SPLIT>::kTile) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
       } else {
         const uint32_t flip = sgn < 0.0f ? 0x80008000u : 0u;
-        *reinterpret_cast<uint4*>(dst) = make_uint4(u[q][0].x ^ flip, u[q][0].y ^ flip, u[q][0].z ^ flip, u[q][0].w ^ flip);
+        *reinterpret_cast<uint4*>(d) =
+            make_uint4(u[q][0].x ^ flip, u[q][0].y ^ flip, u[q][0].z ^ flip, u[q][0].w ^ flip);
       }
     }
   }
-  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-}
+};
 
 template <int HD, bool SPLIT>
 __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __grid_constant__ TcArgs a) {
@@ -305,167 +337,219 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
   uint64_t* sfull = empty + T::kSlots;                // [2]: S of tile t is there
   uint64_t* pfull = sfull + 2;                        // [2][2]: half the keys of tile t's P are there
   uint64_t* odone = pfull + 4;                        // [2]: O of tile t has taken P in
-  uint64_t* vtail = odone + 2;                        // the last V tile's unused rows are zero
-  uint32_t* tmem_at = reinterpret_cast<uint32_t*>(vtail + 1);
-  float* sx = reinterpret_cast<float*>(tmem_at + 4);  // [tile][half of the keys][row]: exchange of the two halves
+  uint64_t* qfull = odone + 2;                        // [2][2]: Q of tile t of an even, an odd piece of work
+  uint64_t* wfull = qfull + 4;                        // [2]: a piece of work is posted
+  uint64_t* wempty = wfull + 2;                       // [2]: and read by all
+  uint64_t* tailbar = wempty + 2;                     // the copy warp's own
+  uint32_t& tmem_at = *reinterpret_cast<uint32_t*>(tailbar + 1);
+  static_assert(T::kBars % 2 == 1, "work lies on 16 bytes");
+  Work* work = reinterpret_cast<Work*>(tailbar + 2);  // [2]
+  float* sx = reinterpret_cast<float*>(work + 2);     // [tile][half of the keys][row]: exchange of the two halves
   const PagedProblem& p = a.p;
-  pdl_wait();
-  pdl_trigger();
-
-  int b = blockIdx.x;
-  const int kvh = b % p.n_kv;
-  b /= p.n_kv;
-  const int split = p.splits ? b % p.splits : 0;
-  const TileId id = pick_tile(p, p.splits ? b / p.splits : b);
-  if (id.seq < 0) return;
-  const SeqTask t = seq_task(p, id.seq);
-  const int rows = t.qn * p.group, r0 = id.rt * 2 * kRows;
-  int k0 = 0, k1 = seen(p, t, (min(rows, r0 + 2 * kRows) - 1) / p.group);
-  if (p.splits) {
-    k0 = split * p.chunk;
-    k1 = min(k1, k0 + p.chunk);
-    if (k0 >= k1) return;
-  }
-  // key tiles that each row tile needs
-  int nt[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int last = min(rows, r0 + (i + 1) * kRows) - 1;
-    const int e = last >= r0 + i * kRows ? min(k1, seen(p, t, last / p.group)) : 0;
-    nt[i] = e > k0 ? (e - k0 + kKeys - 1) / kKeys : 0;
-  }
-  const int nmax = max(nt[0], nt[1]);
-  const bool tail = nmax > 0 && k0 + nmax * kKeys > k1;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (smem_u32(sm) & 1023) {                          // the swizzled tiles need it; the launch gives it
     if (tid == 0) atomicCAS(p.err, 0, 41);
     return;
   }
-  if (warp == kCopyWarp) {
-    // the copies start before the other warps are ready
-    if (lane == 0) {
-      for (int i = 0; i < T::kSlots; ++i) {
-        mbar_init(full + i, 1);
-        mbar_init(empty + i, 1);
-      }
-      mbar_init(vtail, 1);
-      for (int i = 0; i < 2; ++i) {
-        mbar_init(sfull + i, 1);
-        mbar_init(pfull + 2 * i, kRows);
-        mbar_init(pfull + 2 * i + 1, kRows);
-        mbar_init(odone + i, 1);
-      }
-      mbar_fence_init();
+  if (warp == kMmaWarp) tmem_alloc(&tmem_at, 512);
+  if (tid == 0) {
+    for (int i = 0; i < T::kSlots; ++i) {
+      mbar_init(full + i, 1);
+      mbar_init(empty + i, 1);
     }
-    __syncwarp();
-    asm volatile("bar.arrive %0, %1;" ::"n"(kSetupBar), "n"(kTcThreads) : "memory");
-  } else {
-    if (warp == kMmaWarp) tmem_alloc(tmem_at, 512);
-    if (warp < kCopyWarp) load_q<HD, SPLIT>(p, t, kvh, rows, r0, a.q_vec, sq, sx);
-    tc_fence_before();
-    asm volatile("bar.sync %0, %1;" ::"n"(kSetupBar), "n"(kTcThreads) : "memory");
-    tc_fence_after();
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(sfull + i, 1);
+      mbar_init(pfull + 2 * i, kRows);
+      mbar_init(pfull + 2 * i + 1, kRows);
+      mbar_init(odone + i, 1);
+      mbar_init(qfull + 2 * i, 2 * kRows);
+      mbar_init(qfull + 2 * i + 1, 2 * kRows);
+      mbar_init(wfull + i, 1);
+      mbar_init(wempty + i, kCopyWarp + 2);           // the softmax warps, the copy warp, the MMA thread
+    }
+    mbar_init(tailbar, 1);
+    mbar_fence_init();
   }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  pdl_wait();
+  pdl_trigger();
 
   if (warp >= kCopyWarp) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTcRegsRest));
-    if (warp == kCopyWarp) {
-      // ------------------------------------------------------------ K, V tiles
-      bool ok = true;
-      int used = 0;                                     // slots filled
-      for (int j = 0; j < nmax && ok; ++j) {
-        const int kt = k0 + j * kKeys;
-        const int need = (min(kKeys, k1 - kt) + a.box_rows - 1) / a.box_rows;
-        int page = -1, row = 0;
-        if (lane < need) {
-          const int key = kt + lane * a.box_rows;
-          page = t.table[key / p.page_size];
-          row = key % p.page_size;
-        }
-        for (int v = 0; v < 2 && ok; ++v) {
-          const int s = used % T::kSlots;
-          if (used >= T::kSlots) ok = mbar_wait(empty + s, (used / T::kSlots - 1) & 1, p.err, 31);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          if (lane == 0) mbar_arrive_expect_tx(full + s, need * a.box_rows * HD * 2);
-          __syncwarp();
-          if (lane < need) {
-            uint8_t* dst = ring + s * T::kTile + lane * a.box_rows * 128;
-  #pragma unroll
-            for (int h = 0; h < T::kHalves; ++h)
-              tma_page(dst + h * 16384, v ? &a.mv : &a.mk, 64 * h, kvh, row, page, full + s);
+    if (warp == kPlanWarp) {
+      // ------------------------------------------------------------ the plan
+      // The pieces, longest first, go round the CTAs there and back, which
+      // evens out the CTAs' sums.
+      bool ok = true, more = true;
+      int posted = 0;
+      const int splits = p.splits ? p.splits : 1;
+      for (int k = 0; more && ok; ++k) {
+        const int g = k * (int)gridDim.x + (k & 1 ? (int)gridDim.x - 1 - (int)blockIdx.x : (int)blockIdx.x);
+        Work w;
+        w.seq = -1;
+        w.kvh = g % p.n_kv;
+        w.split = g / p.n_kv % splits;
+        const TileId id = pick_tile(p, g / p.n_kv / splits);
+        more = id.seq >= 0;
+        if (more) {
+          const SeqTask t = seq_task(p, id.seq);
+          w.seq = id.seq;
+          w.r0 = id.rt * 2 * kRows;
+          w.rows = t.qn * p.group;
+          w.q0 = t.q0;
+          w.off = t.off;
+          w.kvn = t.kvn;
+          w.k0 = 0;
+          w.k1 = seen(p, t, (min(w.rows, w.r0 + 2 * kRows) - 1) / p.group);
+          if (p.splits) {
+            w.k0 = w.split * p.chunk;
+            w.k1 = min(w.k1, w.k0 + p.chunk);
+            if (w.k0 >= w.k1) continue;               // no row of the tile sees a key of this split
           }
-          ++used;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int last = min(w.rows, w.r0 + (i + 1) * kRows) - 1;
+            const int e = last >= w.r0 + i * kRows ? min(w.k1, seen(p, t, last / p.group)) : 0;
+            w.nt[i] = e > w.k0 ? (e - w.k0 + kKeys - 1) / kKeys : 0;
+          }
+        }
+        if (posted >= 2) ok = mbar_wait(wempty + (posted & 1), (posted / 2 - 1) & 1, p.err, 42);
+        ok = __all_sync(0xffffffffu, ok);
+        if (ok && lane == 0) {
+          work[posted & 1] = w;
+          mbar_arrive(wfull + (posted & 1));
+        }
+        ++posted;
+      }
+    } else if (warp == kCopyWarp) {
+      // ---------------------------------------------------------- K, V tiles
+      bool ok = true;
+      int used = 0, tails = 0;                        // slots filled; tiles cut off by the key range
+      for (int n = 0; ok; ++n) {
+        ok = mbar_wait(wfull + (n & 1), (n >> 1) & 1, p.err, 43);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        const Work& w = work[n & 1];
+        const int seq = w.seq, kvh = w.kvh, k0 = w.k0, k1 = w.k1, nmax = max(w.nt[0], w.nt[1]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(wempty + (n & 1));
+        if (seq < 0) break;
+        const int* table = p.table + (long long)seq * p.table_stride;
+        for (int j = 0; j < nmax && ok; ++j) {
+          const int kt = k0 + j * kKeys, have = min(kKeys, k1 - kt);
+          const int need = (have + a.box_rows - 1) / a.box_rows;
+          int page = -1, row = 0;
+          if (lane < need) {
+            const int key = kt + lane * a.box_rows;
+            page = table[key / p.page_size];
+            row = key % p.page_size;
+          }
+          for (int v = 0; v < 2 && ok; ++v) {
+            const int s = used % T::kSlots;
+            if (used >= T::kSlots) ok = mbar_wait(empty + s, (used / T::kSlots - 1) & 1, p.err, 31);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            const bool cut = v && have < kKeys;
+            uint64_t* bar = cut ? tailbar : full + s;
+            if (lane == 0) mbar_arrive_expect_tx(bar, need * a.box_rows * HD * 2);
+            __syncwarp();
+            if (lane < need) {
+              uint8_t* dst = ring + s * T::kTile + lane * a.box_rows * 128;
+#pragma unroll
+              for (int h = 0; h < T::kHalves; ++h)
+                tma_page(dst + h * 16384, v ? &a.mv : &a.mk, 64 * h, kvh, row, page, bar);
+            }
+            if (cut) {
+              // value rows behind the key range count with weight 0: they
+              // must be finite
+              ok = mbar_wait(tailbar, tails & 1, p.err, 32);
+              ok = __all_sync(0xffffffffu, ok);
+              if (!ok) break;
+              ++tails;
+              for (int h = 0; h < T::kHalves; ++h)
+                for (int o = have * 128 + lane * 16; o < kKeys * 128; o += 512)
+                  *reinterpret_cast<uint4*>(ring + s * T::kTile + h * 16384 + o) = make_uint4(0, 0, 0, 0);
+              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+              __syncwarp();
+              if (lane == 0) mbar_arrive(full + s);
+            }
+            ++used;
+          }
         }
       }
       // every copy lands before the CTA may end
       for (int i = max(0, used - T::kSlots); i < used; ++i)
-        ok = mbar_wait(full + i % T::kSlots, (i / T::kSlots) & 1, p.err, 32) && ok;
-      ok = __all_sync(0xffffffffu, ok);
-      if (tail && ok) {
-        // value rows of the last tile behind the key range count with weight 0:
-        // they must be finite
-        const int have = k1 - (k0 + (nmax - 1) * kKeys);
-        for (int h = 0; h < T::kHalves; ++h)
-          for (int o = have * 128 + lane * 16; o < kKeys * 128; o += 512)
-            *reinterpret_cast<uint4*>(ring + (used - 1) % T::kSlots * T::kTile + h * 16384 + o) = make_uint4(0, 0, 0, 0);
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) mbar_arrive(vtail);
-      }
+        mbar_wait(full + i % T::kSlots, (i / T::kSlots) & 1, p.err, 33);
     } else if (warp == kMmaWarp) {
-      // ------------------------------------------------------- MMAs, one thread
+      // ----------------------------------------------------- MMAs, one thread
       if (elect_one()) {
         constexpr uint32_t kIdS = (1u << 4) | (8u << 24) | ((uint32_t)(kKeys >> 3) << 17);
         constexpr uint32_t kIdO = (1u << 4) | (8u << 24) | ((uint32_t)(HD >> 3) << 17) | (1u << 16);   // V is N-major
-        const uint32_t tmem = *tmem_at;
+        const uint32_t tmem = tmem_at;
         bool ok = true;
-        // S of row tile i on key tile j (the first of the two row tiles waits for K)
-        auto issue_s = [&](int i, int j) {
-          if (i == 0 || j >= nt[0]) ok = ok && mbar_wait(full + 2 * j % T::kSlots, (2 * j / T::kSlots) & 1, p.err, 34);
-          if (!ok) return;
-          const uint32_t kd = desc_k(smem_u32(ring + (2 * j % T::kSlots) * T::kTile));
-          const uint32_t qd = desc_k(smem_u32(sq + i * (SPLIT ? 2 : 1) * T::kTile));
-          const uint32_t d = tmem + i * kKeys;
-  #pragma unroll
-          for (int part = 0; part < (SPLIT ? 2 : 1); ++part)
-  #pragma unroll
-            for (int k = 0; k < HD / 16; ++k) {
-              const uint32_t off = ((k >> 2) * 16384 + (k & 3) * 32) >> 4;
-              mma_f16_ss(d, qd + (part * T::kTile >> 4) + off, kd + off, kIdS, part + k > 0);
-            }
-          mma_commit(sfull + i);
-          if (i == 1 || j >= nt[1]) mma_commit(empty + 2 * j % T::kSlots);
-        };
-        for (int i = 0; i < 2; ++i)
-          if (nt[i] > 0) issue_s(i, 0);
-        for (int j = 0; j < nmax && ok; ++j)
+        int base = 0, c0 = 0, c1 = 0;                 // ring uses and key tiles of the two row tiles before this piece
+        for (int n = 0; ok; ++n) {
+          ok = mbar_wait(wfull + (n & 1), (n >> 1) & 1, p.err, 44);
+          if (!ok) break;
+          const Work& w = work[n & 1];
+          if (w.seq < 0) break;
+          const int n0 = w.nt[0], n1 = w.nt[1], nmax = max(n0, n1);
+          // S of row tile i on key tile j (the first of the two row tiles waits for K)
+          auto issue_s = [&](int i, int j) {
+            const int u = base + 2 * j, slot = u % T::kSlots;
+            if (i == 0 || j >= n0) ok = ok && mbar_wait(full + slot, (u / T::kSlots) & 1, p.err, 34);
+            if (!ok) return;
+            const uint32_t kd = desc_k(smem_u32(ring + slot * T::kTile));
+            const uint32_t qd = desc_k(smem_u32(sq + i * (T::kQ / 2)));
+            const uint32_t d = tmem + i * kKeys;
+#pragma unroll
+            for (int part = 0; part < (SPLIT ? 2 : 1); ++part)
+#pragma unroll
+              for (int k = 0; k < HD / 16; ++k) {
+                const uint32_t off = ((k >> 2) * 16384 + (k & 3) * 32) >> 4;
+                mma_f16_ss(d, qd + (part * T::kTile >> 4) + off, kd + off, kIdS, part + k > 0);
+              }
+            mma_commit(sfull + i);
+            if (i == 1 || j >= n1) mma_commit(empty + slot);
+          };
           for (int i = 0; i < 2 && ok; ++i) {
-            if (j >= nt[i]) continue;
-            const int slot = (2 * j + 1) % T::kSlots;
-            if (i == 0 || j >= nt[0]) {
-              ok = mbar_wait(full + slot, ((2 * j + 1) / T::kSlots) & 1, p.err, 34);
-              if (j == nmax - 1 && tail) ok = ok && mbar_wait(vtail, 0, p.err, 39);
-            }
-            const uint32_t vd0 = desc_mn(smem_u32(ring + slot * T::kTile), 16384);
-            const uint32_t d = tmem + 256 + i * HD;
-            for (int half = 0; half < 2 && ok; ++half) {
-              ok = mbar_wait(pfull + 2 * i + half, j & 1, p.err, 35);
-              if (!ok) break;
-              tc_fence_after();
-              const uint32_t vd = vd0 + half * (kKeys / 2 * 128 >> 4), pa = tmem + i * kKeys + half * 64;
-#pragma unroll
-              for (int part = 0; part < (SPLIT ? 2 : 1); ++part)
-#pragma unroll
-                for (int k = 0; k < kKeys / 32; ++k)
-                  mma_f16_ts(d, pa + (k >> 1) * 32 + part * 16 + (k & 1) * 8, vd + (k * 2048 >> 4), kIdO,
-                             part + k > 0 ? true : j + half > 0);
-            }
-            if (!ok) break;
-            mma_commit(odone + i);
-            if (i == 1 || j >= nt[1]) mma_commit(empty + slot);
-            if (j + 1 < nt[i]) issue_s(i, j + 1);
+            ok = mbar_wait(qfull + 2 * i + (n & 1), (n >> 1) & 1, p.err, 35);
+            tc_fence_after();
+            if (ok && (i ? n1 : n0) > 0) issue_s(i, 0);
           }
+          if (!ok) break;
+          mbar_arrive(wempty + (n & 1));
+          for (int j = 0; j < nmax && ok; ++j)
+            for (int i = 0; i < 2 && ok; ++i) {
+              if (j >= (i ? n1 : n0)) continue;
+              const int u = base + 2 * j + 1, slot = u % T::kSlots;
+              if (i == 0 || j >= n0) ok = mbar_wait(full + slot, (u / T::kSlots) & 1, p.err, 36);
+              const uint32_t vd0 = desc_mn(smem_u32(ring + slot * T::kTile), 16384);
+              const uint32_t d = tmem + 256 + i * HD;
+              const uint32_t ph = ((i ? c1 : c0) + j) & 1;
+              for (int half = 0; half < 2 && ok; ++half) {
+                ok = mbar_wait(pfull + 2 * i + half, ph, p.err, 37);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t vd = vd0 + half * (kKeys / 2 * 128 >> 4), pa = tmem + i * kKeys + half * 64;
+#pragma unroll
+                for (int part = 0; part < (SPLIT ? 2 : 1); ++part)
+#pragma unroll
+                  for (int k = 0; k < kKeys / 32; ++k)
+                    mma_f16_ts(d, pa + (k >> 1) * 32 + part * 16 + (k & 1) * 8, vd + (k * 2048 >> 4), kIdO,
+                               part + k > 0 ? true : j + half > 0);
+              }
+              if (!ok) break;
+              mma_commit(odone + i);
+              if (i == 1 || j >= n1) mma_commit(empty + slot);
+              if (j + 1 < (i ? n1 : n0)) issue_s(i, j + 1);
+            }
+          base += 2 * nmax;
+          c0 += n0;
+          c1 += n1;
+        }
       }
       __syncwarp();
     }
@@ -475,153 +559,194 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
     // row tile, half of a tile's keys (and of the output's dims), 32 rows
     const int i = warp >> 3, hf = (warp >> 2) & 1, wq = warp & 3, r = wq * 32 + lane;
     const int bar = 1 + i * 4 + wq;                                      // this warp and the other half's
-    const uint32_t tmem = *tmem_at;
-    const int pr = r0 + i * kRows + r;
-    const bool live = pr < rows;
-    const int tok = t.q0 + pr / p.group, head = kvh * p.group + pr % p.group;
-    const int lim = live ? min(seen(p, t, pr / p.group), k1) : 0;      // keys this row sees
+    const int row0 = i * kRows + (warp & 7) * 16;                        // Q rows this warp brings (of 256)
+    uint8_t* q_tile = sq + i * (T::kQ / 2);
     float* mine = sx + (i * 2 + hf) * kRows + r;
     float* other = sx + (i * 2 + (hf ^ 1)) * kRows + r;
-    const float inv_q = SPLIT ? sx[i * 2 * kRows + r] : 1.0f;           // undoes the row's scale
-    const float sc = fmaxf(fabsf(p.scale_log2) * inv_q, 1.2e-38f);     // not 0: a masked score is -inf * sc
-    pair_sync(bar);                                                     // the scales are read: sx is free
     const uint32_t lanes = (uint32_t)wq << 21;                          // TMEM lane of the warp's first row, << 16
-    const uint32_t ts = tmem + lanes + i * kKeys, to = tmem + lanes + 256 + i * HD + hf * (HD / 2);
-    float m = -INFINITY, l = 0.0f;
-    bool ok = true;     // a wait that ran out: go on without waiting, so that the two warps' barriers stay paired
-    for (int j = 0; j < nt[i]; ++j) {
-      if (ok) ok = mbar_wait(sfull + i, j & 1, p.err, 36);
+    const uint32_t ts = tmem_at + lanes + i * kKeys, to = tmem_at + lanes + 256 + i * HD + hf * (HD / 2);
+    uint8_t* stage = (T::kStage ? ring + T::kSlots * T::kTile + i * 32768 : q_tile) + (hf * 4 + wq) * 4096;
+    bool ok = true;     // a wait that ran out: no more waiting, and all warps of the row tile leave together
+    int cnt = 0;                                                        // key tiles so far
+    QRows<HD, SPLIT> qr;
+    Work w;
+    // the n-th piece of work, and its Q rows on their way to L2
+    auto take = [&](int n) {
+      if (ok) ok = mbar_wait(wfull + (n & 1), (n >> 1) & 1, p.err, 38);
+      w = work[n & 1];
+      if (!__all_sync(0xffffffffu, ok)) w.seq = -1;
+      __syncwarp();
+      if (w.seq >= 0) {
+        if (lane == 0) mbar_arrive(wempty + (n & 1));
+        qr.place(p, w, row0);
+        qr.ask(p);
+      }
+    };
+    take(0);
+    for (int n = 0;; ++n) {
+      // also: every warp of the row tile has written its last output rows
+      if (tile_any(kTileBar + i, !ok) || w.seq < 0) break;
+#pragma unroll
+      for (int s0 = 0; s0 < QRows<HD, SPLIT>::STEPS; s0 += QRows<HD, SPLIT>::BATCH) {
+        uint4 u[QRows<HD, SPLIT>::BATCH][QRows<HD, SPLIT>::PARTS];
+        qr.fetch(p, s0, a.q_vec, u);
+        qr.store(p, s0, (warp & 7) * 16, q_tile, sx + i * 2 * kRows, u);
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      mbar_arrive(qfull + 2 * i + (n & 1));
+      float inv_q = 1.0f;                                                // undoes the row's scale
+      if (SPLIT) {
+        tile_any(kTileBar + i, false);
+        inv_q = sx[i * 2 * kRows + r];
+        tile_any(kTileBar + i, false);                                   // read by all: sx is free
+      }
+      const int pr = w.r0 + i * kRows + r, nt = w.nt[i], k0 = w.k0;
+      const bool live = pr < w.rows;
+      const int tok = w.q0 + pr / p.group, head = w.kvh * p.group + pr % p.group, seq = w.seq;
+      const SeqTask st = {w.q0, 0, w.kvn, w.off, nullptr};
+      const int all = live ? seen(p, st, pr / p.group) : 0, lim = min(all, w.k1);   // keys this row sees, here
+      const long long slot = (long long)(p.slot0 + w.split) * p.total_q * p.heads + (long long)tok * p.heads + head;
+      const float sc = fmaxf(fabsf(p.scale_log2) * inv_q, 1.2e-38f);   // not 0: a masked score is -inf * sc
+      float m = -INFINITY, l = 0.0f;
+      for (int j = 0; j < nt; ++j) {
+        if (ok) ok = mbar_wait(sfull + i, (cnt + j) & 1, p.err, 39);
+        __syncwarp();
+        tc_fence_after();
+        const int left = lim - (k0 + j * kKeys) - 64 * hf;              // keys of this half tile that the row sees
+        const bool cut = __any_sync(0xffffffffu, left < 64);
+        // S is read twice, for the maximum and for the weights: two reads of
+        // tensor memory cost less than 64 registers
+        float top = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t s[32];
+          tc_ld32(ts + 64 * hf + 32 * c, s);
+          tc_wait_ld(s);
+          if (cut) mask32(s, left - 32 * c);
+          top = fmaxf(top, max32(s));
+        }
+        top *= sc;
+        if (pair_any(bar, j == 0 || top > m + kSlack)) {
+          // a first or a much larger maximum: agree on the row's over both
+          // halves, scale O (each half its dims) and l to it
+          *mine = top;
+          pair_sync(bar);
+          top = fmaxf(top, *other);
+          const float mn = j == 0 || top > m + kSlack ? top : m;
+          if (j > 0) {
+            const float f = mn == m ? 1.0f : exp2f(m - mn);
+            if (ok) ok = mbar_wait(odone + i, (cnt + j - 1) & 1, p.err, 40);
+            __syncwarp();
+            tc_fence_after();
+#pragma unroll
+            for (int c = 0; c < HD / 64; ++c) {
+              uint32_t o[32];
+              tc_ld32(to + 32 * c, o);
+              tc_wait_ld(o);
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              tc_st32(to + 32 * c, o);
+            }
+            l *= f;
+          }
+          m = mn;
+        }
+        const float bias = kBias - (m == -INFINITY ? 0.0f : m);
+        const float2 sc2 = make_float2(sc, sc), bias2 = make_float2(bias, bias);
+        float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t s[32], hi[16], lo[16];
+          tc_ld32(ts + 64 * hf + 32 * c, s);
+          tc_wait_ld(s);
+          if (cut) mask32(s, left - 32 * c);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const float2 x = __ffma2_rn(make_float2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), sc2, bias2);
+            const float2 v = !SPLIT && (e & 3) == 3 ? exp2_fma(x) : make_float2(ex2(x.x), ex2(x.y));
+            sum[e & 1] = __fadd2_rn(sum[e & 1], v);
+            if (SPLIT) {
+              split_pair(v.x, v.y, hi[e], lo[e]);
+            } else {
+              const __half2 H = __floats2half2_rn(v.x, v.y);
+              hi[e] = *reinterpret_cast<const uint32_t*>(&H);
+            }
+          }
+          // over these 32 keys' own S: high parts, then low parts
+          tmem_st16(ts + 64 * hf + 32 * c, hi);
+          if (SPLIT) tmem_st16(ts + 64 * hf + 32 * c + 16, lo);
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(pfull + 2 * i + hf);
+        l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+      }
+      cnt += nt;
+      take(n + 1);
+      if (ok && nt > 0) ok = mbar_wait(odone + i, (cnt - 1) & 1, p.err, 45);
       __syncwarp();
       tc_fence_after();
-      const int left = lim - (k0 + j * kKeys) - 64 * hf;                // keys of this half tile that the row sees
-      const bool cut = __any_sync(0xffffffffu, left < 64);
-      // S is read twice, for the maximum and for the weights: two reads of
-      // tensor memory cost less than 64 registers
-      float top = -INFINITY;
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t s[32];
-        tc_ld32(ts + 64 * hf + 32 * c, s);
-        tc_wait_ld(s);
-        if (cut) mask32(s, left - 32 * c);
-        top = fmaxf(top, max32(s));
-      }
-      top *= sc;
-      if (pair_any(bar, j == 0 || top > m + kSlack)) {
-        // a first or a much larger maximum: agree on the row's over both
-        // halves, scale O (each half its dims) and l to it
-        *mine = top;
-        pair_sync(bar);
-        top = fmaxf(top, *other);
-        const float mn = j == 0 || top > m + kSlack ? top : m;
-        if (j > 0) {
-          const float f = mn == m ? 1.0f : exp2f(m - mn);
-          if (ok) ok = mbar_wait(odone + i, (j - 1) & 1, p.err, 37);
-          __syncwarp();
-          tc_fence_after();
-#pragma unroll
-          for (int c = 0; c < HD / 64; ++c) {
-            uint32_t o[32];
-            tc_ld32(to + 32 * c, o);
-            tc_wait_ld(o);
-#pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-            tc_st32(to + 32 * c, o);
-          }
-          l *= f;
-        }
-        m = mn;
-      }
-      const float bias = kBias - (m == -INFINITY ? 0.0f : m);
-      const float2 sc2 = make_float2(sc, sc), bias2 = make_float2(bias, bias);
-      float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t s[32], hi[16], lo[16];
-        tc_ld32(ts + 64 * hf + 32 * c, s);
-        tc_wait_ld(s);
-        if (cut) mask32(s, left - 32 * c);
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float2 x = __ffma2_rn(make_float2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), sc2, bias2);
-          const float2 w = !SPLIT && (e & 3) == 3 ? exp2_fma(x) : make_float2(ex2(x.x), ex2(x.y));
-          sum[e & 1] = __fadd2_rn(sum[e & 1], w);
-          if (SPLIT) {
-            split_pair(w.x, w.y, hi[e], lo[e]);
-          } else {
-            const __half2 H = __floats2half2_rn(w.x, w.y);
-            hi[e] = *reinterpret_cast<const uint32_t*>(&H);
-          }
-        }
-        // over these 32 keys' own S: high parts, then low parts
-        tmem_st16(ts + 64 * hf + 32 * c, hi);
-        if (SPLIT) tmem_st16(ts + 64 * hf + 32 * c + 16, lo);
-      }
-      tmem_st_wait();
-      tc_fence_before();
-      mbar_arrive(pfull + 2 * i + hf);
-      l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-    }
-    if (ok && nt[i] > 0) ok = mbar_wait(odone + i, (nt[i] - 1) & 1, p.err, 38);
-    ok = __all_sync(0xffffffffu, ok);
-    tc_fence_after();
-    pair_sync(bar);
-    *mine = l;
-    pair_sync(bar);
-    l += *other;
-    // ------------------------------------------------------------- output
-    // A row a thread in tensor memory; 32 dims (fp32) or the half's dims
-    // (fp16) go through shared memory (Q's, which no MMA reads any more), 128
-    // bytes a row, so that eight lanes write a row's pieces side by side.
-    if (lim <= k0) l = 0.0f;                                            // sees nothing here, whatever exp2 made of -inf
-    const bool f32 = p.splits || p.type == TOSK_F32;
-    const int es = f32 ? 4 : 2;
-    const float inv = l == 0.0f || nt[i] == 0 ? 0.0f : p.splits ? 1.0f : 1.0f / l;
-    const long long slot = (long long)(p.slot0 + split) * p.total_q * p.heads + (long long)tok * p.heads + head;
-    if (p.splits && live && hf == 0 && ok) p.part_ml[slot] = make_float2(m - kBias, l);
-    const long long row_at = !live ? -1 : p.splits ? slot * p.hd : (long long)tok * p.out_stride + (long long)head * p.hd;
-    uint8_t* stage = (T::kStage ? ring + T::kSlots * T::kTile : sq + i * (T::kQ / 2)) + ((T::kStage ? i * 8 : 0) + hf * 4 + wq) * 4096;
-    bool bad = false;
-    // the staged rows' `n` bytes to dims from dim0 on
-    auto flush = [&](int dim0, int n) {
-      __syncwarp();
-      const int c = lane & 7, dim = dim0 + c * (16 / es);
+      pair_sync(bar);
+      *mine = l;
+      pair_sync(bar);
+      l += *other;
+      // ----------------------------------------------------------- output
+      // A row a thread in tensor memory; 32 dims (fp32) or the half's dims
+      // (fp16) go through shared memory (Q's, which no MMA reads any more),
+      // 128 bytes a row, so that eight lanes write a row's pieces side by side.
+      if (lim <= k0) l = 0.0f;                                          // sees nothing here, whatever exp2 made of -inf
+      const bool f32 = p.splits || p.type == TOSK_F32;
+      const int es = f32 ? 4 : 2;
+      const float inv = l == 0.0f || nt == 0 ? 0.0f : p.splits ? 1.0f : 1.0f / l;
+      if (p.splits && live && hf == 0) p.part_ml[slot] = make_float2(m - kBias, l);
+      const long long row_at =
+          !live ? -1 : p.splits ? slot * p.hd : (long long)tok * p.out_stride + (long long)head * p.hd;
+      float2 odd = make_float2(0.0f, 0.0f);                             // NaN once an infinity or NaN was seen
+      const bool none = __any_sync(0xffffffffu, inv == 0.0f);
+      // the staged rows' `bytes` to dims from dim0 on
+      auto flush = [&](int dim0, int bytes) {
+        __syncwarp();
+        const int c = lane & 7, dim = dim0 + c * (16 / es);
 #pragma unroll 4
-      for (int q = 0; q < 8; ++q) {
-        const int row = q * 4 + (lane >> 3);
-        const long long at = __shfl_sync(0xffffffffu, row_at, row);
-        if (at < 0 || c * 16 >= n || dim >= p.hd) continue;
-        const uint4 v = *reinterpret_cast<const uint4*>(stage + sw128(row, c));
-        if (p.splits) {
-          *reinterpret_cast<uint4*>(p.part_o + at + dim) = v;
-        } else if (a.out_vec) {
-          *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(p.out) + (at + dim) * es) = v;
-        } else {
-          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        for (int q = 0; q < 8; ++q) {
+          const int row = q * 4 + (lane >> 3);
+          const long long at = __shfl_sync(0xffffffffu, row_at, row);
+          if (at < 0 || c * 16 >= bytes || dim >= p.hd) continue;
+          const uint4 v = *reinterpret_cast<const uint4*>(stage + sw128(row, c));
+          if (p.splits) {
+            *reinterpret_cast<uint4*>(p.part_o + at + dim) = v;
+          } else if (a.out_vec) {
+            *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(p.out) + (at + dim) * es) = v;
+          } else {
+            const uint32_t x[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            if (f32) {
-              reinterpret_cast<uint32_t*>(p.out)[at + dim + e] = w[e];
-            } else {
-              reinterpret_cast<uint16_t*>(p.out)[at + dim + 2 * e] = (uint16_t)w[e];
-              reinterpret_cast<uint16_t*>(p.out)[at + dim + 2 * e + 1] = (uint16_t)(w[e] >> 16);
+            for (int e = 0; e < 4; ++e) {
+              if (f32) {
+                reinterpret_cast<uint32_t*>(p.out)[at + dim + e] = x[e];
+              } else {
+                reinterpret_cast<uint16_t*>(p.out)[at + dim + 2 * e] = (uint16_t)x[e];
+                reinterpret_cast<uint16_t*>(p.out)[at + dim + 2 * e + 1] = (uint16_t)(x[e] >> 16);
+              }
             }
           }
         }
-      }
-      __syncwarp();
-    };
-    if (ok) {
+        __syncwarp();
+      };
 #pragma unroll
       for (int c32 = 0; c32 < HD / 64; ++c32) {
         uint32_t o[32];
         tc_ld32(to + 32 * c32, o);
         tc_wait_ld(o);
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          const float v = inv == 0.0f ? 0.0f : __uint_as_float(o[e]) * inv;
-          o[e] = __float_as_uint(v);
-          bad |= isnan(v);
+        for (int e = 0; e < 32; e += 2) {
+          const float2 v = __fmul2_rn(make_float2(__uint_as_float(o[e]), __uint_as_float(o[e + 1])), make_float2(inv, inv));
+          odd = __ffma2_rn(v, make_float2(0.0f, 0.0f), odd);
+          o[e] = __float_as_uint(v.x);
+          o[e + 1] = __float_as_uint(v.y);
+        }
+        if (none) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = inv == 0.0f ? 0u : o[e];
         }
         if (f32) {
 #pragma unroll
@@ -642,27 +767,27 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
         }
       }
       if (!f32) flush(hf * (HD / 2), HD);
-    }
-    if (!p.splits && pair_any(bar, bad && live)) {
-      // rows that show NaN in either half, once both halves are written
-      pair_sync(bar);                                                   // l is read: sx is free
-      *mine = bad && live ? 1.0f : 0.0f;
-      pair_sync(bar);
-      uint32_t todo = hf == 0 ? __ballot_sync(0xffffffffu, *mine != 0.0f || *other != 0.0f) : 0;
-      while (todo) {
-        const int w = __ffs(todo) - 1;
-        todo &= todo - 1;
-        const int pw = r0 + i * kRows + wq * 32 + w;
-        attn_row_plain(p, nullptr, 0, t.table, seen(p, t, pw / p.group), t.q0 + pw / p.group,
-                       kvh * p.group + pw % p.group);
+      tc_fence_before();                                                // O and S are read: the next piece's MMAs may come
+      const bool bad = live && inv != 0.0f && isnan(odd.x + odd.y);
+      if (!p.splits && pair_any(bar, bad)) {
+        // rows that show one in either half, once both halves are written
+        pair_sync(bar);                                                 // l is read: sx is free
+        *mine = bad ? 1.0f : 0.0f;
+        pair_sync(bar);
+        uint32_t todo = hf == 0 ? __ballot_sync(0xffffffffu, *mine != 0.0f || *other != 0.0f) : 0;
+        while (todo) {
+          const int x = __ffs(todo) - 1;
+          todo &= todo - 1;
+          attn_row_plain(p, nullptr, 0, p.table + (long long)seq * p.table_stride, __shfl_sync(0xffffffffu, all, x),
+                         __shfl_sync(0xffffffffu, tok, x), __shfl_sync(0xffffffffu, head, x));
+        }
       }
     }
-    tc_fence_before();
   }
   __syncthreads();
   if (warp == kMmaWarp) {
     tc_fence_after();
-    tmem_dealloc(*tmem_at, 512);
+    tmem_dealloc(tmem_at, 512);
   }
 }
 
@@ -689,6 +814,12 @@ bool pool_map(CUtensorMap* m, const void* base, const PagedProblem& p, int box_r
 template <int HD, bool SPLIT>
 int tc_launch(const TcArgs& a, unsigned grid, cudaStream_t st) {
   const void* f = (const void*)paged_attn_tc_kernel<HD, SPLIT>;
+  // the softmax warps wait for registers that the launch must have brought
+  static const int regs = [f] {
+    cudaFuncAttributes fa;
+    return cudaFuncGetAttributes(&fa, f) == cudaSuccess ? fa.numRegs : 0;
+  }();
+  if (regs < kTcRegs) return (int)cudaErrorNotSupported;
   const cudaError_t e =
       cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, TcShape<HD, SPLIT>::kSmem);
   if (e != cudaSuccess) return (int)e;
@@ -729,8 +860,9 @@ int paged_tc_run(const PagedProblem& p, cudaStream_t st) {
   TcArgs a;
   a.p = p;
   a.box_rows = p.page_size < kKeys ? p.page_size : kKeys;
-  const long long grid = paged_tc_tiles(p.n_seqs, p.total_q, p.max_q, p.group) * (p.splits ? p.splits : 1) * p.n_kv;
-  if (grid > 0x7fffffffll) return (int)cudaErrorInvalidValue;
+  long long grid = paged_tc_tiles(p.n_seqs, p.total_q, p.max_q, p.group) * (p.splits ? p.splits : 1) * p.n_kv;
+  if (grid > 0x3fffffffll) return (int)cudaErrorInvalidValue;    // the plan counts pieces in 32 bits
+  if (grid > kTcCtas) grid = kTcCtas;
   a.q_vec = ((uintptr_t)p.q & 15) == 0 && p.q_stride % (p.type == TOSK_F32 ? 4 : 8) == 0;
   a.out_vec = ((uintptr_t)p.out & 15) == 0 && p.out_stride % (p.type == TOSK_F32 ? 4 : 8) == 0;
   if (!pool_map(&a.mk, p.k, p, a.box_rows) || !pool_map(&a.mv, p.v, p, a.box_rows)) return (int)cudaErrorNotSupported;
