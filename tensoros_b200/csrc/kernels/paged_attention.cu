@@ -428,16 +428,19 @@ void part_views(PagedProblem& p, void* ws, int slots) {
 int run_tiles(const PagedProblem& p, cudaStream_t st) { return paged_tc_ok(p) ? paged_tc_run(p, st) : run_general(p, st); }
 
 // Splits of a prompt call's keys (0: none).  Fewer row tiles than SMs leave
-// SMs without work: the keys are cut, at least 512 a split, into the number
-// of splits with the shortest schedule (rounds over the SMs, each 1/s of the
-// keys), at ~3% of a round a split for the partial rows' way through memory.
-int plan_prompt(int n_seqs, int total_q, int max_q, int max_kv, int heads, int n_kv) {
-  const long long tiles = paged_tc_tiles(n_seqs, total_q, max_q, heads / n_kv) * n_kv;
+// SMs without work, so the keys are cut into the number of splits with the
+// shortest schedule, counted in key tiles of 128: rounds over the SMs, each
+// its share of the keys and ~3.5 tiles' worth of starting and ending a piece;
+// the joining ~2, and a tile's worth for every 1.1 M elements of partial rows.
+// (Measured: a key tile 1.75 us, a piece ~6 us beside its tiles.)
+int plan_prompt(int total_q, int max_kv, int heads, int n_kv, int hd) {
+  const long long tiles = ((long long)total_q * (heads / n_kv) + 255) / 256 * n_kv;
   if (tiles >= kSms) return 0;
+  const float keys = max_kv / 128.0f, rows = (float)total_q * heads * hd / 1.1e6f;
   int best = 1;
-  float cost = 1.0f;
+  float cost = keys + 3.5f;
   for (int s = 2; s <= 16 && s <= max_kv / 512; ++s) {
-    const float c = (float)((s * tiles + kSms - 1) / kSms) / s + 0.03f * s;
+    const float c = (float)((s * tiles + kSms - 1) / kSms) * (keys / s + 3.5f) + 2.0f + s * rows;
     if (c < cost) {
       cost = c;
       best = s;
@@ -447,9 +450,8 @@ int plan_prompt(int n_seqs, int total_q, int max_q, int max_kv, int heads, int n
 }
 }  // namespace
 
-extern "C" size_t tosk_paged_prompt_ws_bytes(int n_seqs, int total_q, int max_q, int max_kv, int n_heads, int n_kv,
-                                             int hd) {
-  return (size_t)plan_prompt(n_seqs, total_q, max_q, max_kv, n_heads, n_kv) * slot_bytes(total_q, n_heads, hd);
+extern "C" size_t tosk_paged_prompt_ws_bytes(int total_q, int max_kv, int n_heads, int n_kv, int hd) {
+  return (size_t)plan_prompt(total_q, max_kv, n_heads, n_kv, hd) * slot_bytes(total_q, n_heads, hd);
 }
 
 extern "C" size_t tosk_paged_decode_ws_bytes(int n_seqs, int max_kv, int prefix_len, int n_heads, int n_kv, int hd) {
@@ -459,7 +461,7 @@ extern "C" size_t tosk_paged_decode_ws_bytes(int n_seqs, int max_kv, int prefix_
 
 extern "C" int tosk_paged_prompt(const tosk_paged_attn_t* a, cudaStream_t st) {
   PagedProblem p = problem_of(a);
-  p.splits = plan_prompt(a->n_seqs, a->total_q, a->max_q, a->max_kv, a->n_heads, a->kv.n_kv);
+  p.splits = plan_prompt(a->total_q, a->max_kv, a->n_heads, a->kv.n_kv, a->kv.hd);
   if (!p.splits) return run_tiles(p, st);
   p.chunk = chunk_of(a->max_kv, p.splits);
   part_views(p, a->ws, p.splits);

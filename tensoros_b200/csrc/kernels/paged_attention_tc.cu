@@ -49,6 +49,10 @@ constexpr int kTileBar = 9;            // named barriers: 1..8 pair the two warp
 constexpr int kRows = 128;            // rows of a tile
 constexpr int kKeys = 128;            // keys of a tile
 constexpr float kBias = 7.0f;         // log2 of the factor that P carries
+#ifndef TOS_POLY
+#define TOS_POLY 4
+#endif
+constexpr int kPoly = TOS_POLY;       // one of so many pairs of exponentials goes to the FMA pipe
 constexpr float kSlack = 8.0f;        // log2 by which the maximum may grow unfollowed
 
 struct TcArgs {
@@ -87,8 +91,11 @@ __device__ __forceinline__ void tc_ld32(uint32_t addr, uint32_t (&r)[32]) {
 __device__ __forceinline__ void tc_wait_ld(uint32_t (&r)[32]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" : TOS_R8(r, 0), TOS_R8(r, 8), TOS_R8(r, 16), TOS_R8(r, 24)::"memory");
 }
-__device__ __forceinline__ void tc_tie(uint32_t (&r)[32]) {
-  asm volatile("" : TOS_R8(r, 0), TOS_R8(r, 8), TOS_R8(r, 16), TOS_R8(r, 24)::"memory");
+__device__ __forceinline__ void tc_wait_ld16(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : TOS_R8(r, 0), TOS_R8(r, 8)::"memory");
+}
+__device__ __forceinline__ void tc_wait_ld8(uint32_t (&r)[8]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : TOS_R8(r, 0)::"memory");
 }
 #undef TOS_R8
 // 2^x of two values on the FMA pipe, which has room beside the 16 exponentials
@@ -110,6 +117,24 @@ __device__ __forceinline__ float2 exp2_fma(float2 x) {
   y.x = __uint_as_float(__float_as_uint(y.x) + (__float_as_uint(n.x) << 23));
   y.y = __uint_as_float(__float_as_uint(y.y) + (__float_as_uint(n.y) << 23));
   return y;
+}
+__device__ __forceinline__ void tc_ld16(uint32_t addr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr));
+}
+__device__ __forceinline__ void tc_ld8(uint32_t addr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(addr));
+}
+__device__ __forceinline__ void tc_st4(uint32_t addr, const uint32_t (&r)[4]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+               "r"(r[3])
+               : "memory");
 }
 __device__ __forceinline__ void tc_st32(uint32_t addr, const uint32_t (&r)[32]) {
   asm volatile(
@@ -197,20 +222,35 @@ __device__ __forceinline__ TileId pick_tile(const PagedProblem& p, int f) {
   return id;
 }
 
-// Scores from the n-th on (of 32) count for nothing.
-__device__ __forceinline__ void mask32(uint32_t (&s)[32], int n) {
+// Scores from the n-th on count for nothing.
+template <int N>
+__device__ __forceinline__ void mask_from(uint32_t (&s)[N], int n) {
 #pragma unroll
-  for (int e = 0; e < 32; ++e)
+  for (int e = 0; e < N; ++e)
     if (e >= n) s[e] = 0xff800000u;                                     // -inf
 }
-__device__ __forceinline__ float max32(const uint32_t (&s)[32]) {
+template <int N>
+__device__ __forceinline__ float max_of(const uint32_t (&s)[N]) {
   float a = fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1])), b = fmaxf(__uint_as_float(s[2]), __uint_as_float(s[3]));
 #pragma unroll
-  for (int e = 4; e < 32; e += 4) {
+  for (int e = 4; e < N; e += 4) {
     a = fmaxf(fmaxf(a, __uint_as_float(s[e])), __uint_as_float(s[e + 1]));
     b = fmaxf(fmaxf(b, __uint_as_float(s[e + 2])), __uint_as_float(s[e + 3]));
   }
   return fmaxf(a, b);
+}
+// Multiplies n columns of this warp's 32 rows in tensor memory.  Rarely
+// called: out of line, so that its registers cost the loop around it none.
+static __device__ __noinline__ void scale_cols(uint32_t addr, int n, float f) {
+#pragma unroll 1
+  for (int c = 0; c < n; c += 16) {
+    uint32_t o[16];
+    tc_ld16(addr + c, o);
+    tc_wait_ld16(o);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+    tmem_st16(addr + c, o);
+  }
 }
 // The two warps that share 32 rows.
 __device__ __forceinline__ void pair_sync(int bar) { asm volatile("bar.sync %0, 64;" ::"r"(bar) : "memory"); }
@@ -586,7 +626,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
     for (int n = 0;; ++n) {
       // also: every warp of the row tile has written its last output rows
       if (tile_any(kTileBar + i, !ok) || w.seq < 0) break;
-#pragma unroll
+#pragma unroll 1
       for (int s0 = 0; s0 < QRows<HD, SPLIT>::STEPS; s0 += QRows<HD, SPLIT>::BATCH) {
         uint4 u[QRows<HD, SPLIT>::BATCH][QRows<HD, SPLIT>::PARTS];
         qr.fetch(p, s0, a.q_vec, u);
@@ -614,21 +654,23 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
         tc_fence_after();
         const int left = lim - (k0 + j * kKeys) - 64 * hf;              // keys of this half tile that the row sees
         const bool cut = __any_sync(0xffffffffu, left < 64);
-        // S is read twice, for the maximum and for the weights: two reads of
-        // tensor memory cost less than 64 registers
-        float top = -INFINITY;
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t s[32];
-          tc_ld32(ts + 64 * hf + 32 * c, s);
-          tc_wait_ld(s);
-          if (cut) mask32(s, left - 32 * c);
-          top = fmaxf(top, max32(s));
-        }
-        top *= sc;
-        if (pair_any(bar, j == 0 || top > m + kSlack)) {
-          // a first or a much larger maximum: agree on the row's over both
-          // halves, scale O (each half its dims) and l to it
+        const float2 sc2 = make_float2(sc, sc);
+        // the row's maximum over this half's keys
+        auto half_top = [&]() {
+          float top = -INFINITY;
+#pragma unroll 1
+          for (int c = 0; c < 2; ++c) {
+            uint32_t s[32];
+            tc_ld32(ts + 64 * hf + 32 * c, s);
+            tc_wait_ld(s);
+            if (cut) mask_from(s, left - 32 * c);
+            top = fmaxf(top, max_of(s));
+          }
+          return top * sc;
+        };
+        // a first or a much larger maximum: agree on the row's over both
+        // halves, scale O (each half its dims) and l to it
+        auto agree = [&](float top) {
           *mine = top;
           pair_sync(bar);
           top = fmaxf(top, *other);
@@ -638,43 +680,97 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
             if (ok) ok = mbar_wait(odone + i, (cnt + j - 1) & 1, p.err, 40);
             __syncwarp();
             tc_fence_after();
-#pragma unroll
-            for (int c = 0; c < HD / 64; ++c) {
-              uint32_t o[32];
-              tc_ld32(to + 32 * c, o);
-              tc_wait_ld(o);
-#pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-              tc_st32(to + 32 * c, o);
-            }
+            scale_cols(to, HD / 2, f);
             l *= f;
           }
           m = mn;
-        }
-        const float bias = kBias - (m == -INFINITY ? 0.0f : m);
-        const float2 sc2 = make_float2(sc, sc), bias2 = make_float2(bias, bias);
-        float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+        };
+        float2 sum[2];
+        if (SPLIT) {
+          // S is read twice, for the maximum and for the weights: the parts of
+          // P take too many registers to be kept until the maximum is known
+          const float top = half_top();
+          if (pair_any(bar, j == 0 || top > m + kSlack)) agree(top);
+          const float bias = kBias - (m == -INFINITY ? 0.0f : m);
+          const float2 bias2 = make_float2(bias, bias);
+          sum[0] = sum[1] = make_float2(0.0f, 0.0f);
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t s[32], hi[16], lo[16];
-          tc_ld32(ts + 64 * hf + 32 * c, s);
-          tc_wait_ld(s);
-          if (cut) mask32(s, left - 32 * c);
+          for (int c = 0; c < 2; ++c) {
+            uint32_t s[32], hi[16], lo[16];
+            tc_ld32(ts + 64 * hf + 32 * c, s);
+            tc_wait_ld(s);
+            if (cut) mask_from(s, left - 32 * c);
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const float2 x = __ffma2_rn(make_float2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), sc2, bias2);
-            const float2 v = !SPLIT && (e & 3) == 3 ? exp2_fma(x) : make_float2(ex2(x.x), ex2(x.y));
-            sum[e & 1] = __fadd2_rn(sum[e & 1], v);
-            if (SPLIT) {
+            for (int e = 0; e < 16; ++e) {
+              const float2 x = __ffma2_rn(make_float2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), sc2, bias2);
+              const float2 v = make_float2(ex2(x.x), ex2(x.y));
+              sum[e & 1] = __fadd2_rn(sum[e & 1], v);
               split_pair(v.x, v.y, hi[e], lo[e]);
-            } else {
-              const __half2 H = __floats2half2_rn(v.x, v.y);
-              hi[e] = *reinterpret_cast<const uint32_t*>(&H);
+            }
+            // over these 32 keys' own S: high parts, then low parts
+            tmem_st16(ts + 64 * hf + 32 * c, hi);
+            tmem_st16(ts + 64 * hf + 32 * c + 16, lo);
+          }
+        } else {
+          // the weights under the maximum so far, and the maximum with them;
+          // P goes over S only once no row of the two halves has outgrown it
+          float top;
+          bool again = j == 0;
+          if (!again) {
+            uint32_t hi[2][16];
+            const float bias = kBias - (m == -INFINITY ? 0.0f : m);
+            const float2 bias2 = make_float2(bias, bias);
+            sum[0] = sum[1] = make_float2(0.0f, 0.0f);
+            top = -INFINITY;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              uint32_t s[16];
+              tc_ld16(ts + 64 * hf + 16 * c, s);
+              tc_wait_ld16(s);
+              if (cut) mask_from(s, left - 16 * c);
+              top = fmaxf(top, max_of(s));
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                const float2 x =
+                    __ffma2_rn(make_float2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), sc2, bias2);
+                const float2 v = kPoly && (e % kPoly) == kPoly - 1 ? exp2_fma(x) : make_float2(ex2(x.x), ex2(x.y));
+                sum[e & 1] = __fadd2_rn(sum[e & 1], v);
+                const __half2 H = __floats2half2_rn(v.x, v.y);
+                hi[c >> 1][8 * (c & 1) + e] = *reinterpret_cast<const uint32_t*>(&H);
+              }
+            }
+            top *= sc;
+            again = pair_any(bar, top > m + kSlack);
+            if (!again) {
+              tmem_st16(ts + 64 * hf, hi[0]);
+              tmem_st16(ts + 64 * hf + 32, hi[1]);
+            }
+          } else {
+            top = half_top();
+          }
+          if (again) {
+            agree(top);
+            const float bias = kBias - (m == -INFINITY ? 0.0f : m);
+            const float2 bias2 = make_float2(bias, bias);
+            sum[0] = sum[1] = make_float2(0.0f, 0.0f);
+#pragma unroll 1
+            for (int c = 0; c < 8; ++c) {                               // 8 keys' P over S that has been read
+              uint32_t s[8], hi[4];
+              tc_ld8(ts + 64 * hf + 8 * c, s);
+              tc_wait_ld8(s);
+              if (cut) mask_from(s, left - 8 * c);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float2 x =
+                    __ffma2_rn(make_float2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), sc2, bias2);
+                const float2 v = make_float2(ex2(x.x), ex2(x.y));
+                sum[0] = __fadd2_rn(sum[0], v);
+                const __half2 H = __floats2half2_rn(v.x, v.y);
+                hi[e] = *reinterpret_cast<const uint32_t*>(&H);
+              }
+              tc_st4(ts + 64 * hf + 32 * (c >> 2) + 4 * (c & 3), hi);
             }
           }
-          // over these 32 keys' own S: high parts, then low parts
-          tmem_st16(ts + 64 * hf + 32 * c, hi);
-          if (SPLIT) tmem_st16(ts + 64 * hf + 32 * c + 16, lo);
         }
         tmem_st_wait();
         tc_fence_before();
@@ -707,7 +803,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
       auto flush = [&](int dim0, int bytes) {
         __syncwarp();
         const int c = lane & 7, dim = dim0 + c * (16 / es);
-#pragma unroll 4
+#pragma unroll 1
         for (int q = 0; q < 8; ++q) {
           const int row = q * 4 + (lane >> 3);
           const long long at = __shfl_sync(0xffffffffu, row_at, row);
@@ -732,7 +828,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
         }
         __syncwarp();
       };
-#pragma unroll
+#pragma unroll 1
       for (int c32 = 0; c32 < HD / 64; ++c32) {
         uint32_t o[32];
         tc_ld32(to + 32 * c32, o);
