@@ -50,7 +50,7 @@ constexpr int kRows = 128;            // rows of a tile
 constexpr int kKeys = 128;            // keys of a tile
 constexpr float kBias = 7.0f;         // log2 of the factor that P carries
 #ifndef TOS_POLY
-#define TOS_POLY 4
+#define TOS_POLY 3
 #endif
 constexpr int kPoly = TOS_POLY;       // one of so many pairs of exponentials goes to the FMA pipe
 constexpr float kSlack = 8.0f;        // log2 by which the maximum may grow unfollowed
