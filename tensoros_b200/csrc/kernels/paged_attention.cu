@@ -57,12 +57,15 @@ struct GenArgs {
 template <int R, int NJ>
 __global__ void __launch_bounds__(kGenThreads) paged_attn_general_kernel(const GenArgs a) {
   constexpr int RI = R / 16, LD = 64 * NJ + 4, LP = kKT + 4;
+  constexpr int NL = kKT * 16 * NJ / kGenThreads;      // 16-byte pieces of K, and of V, a thread a tile
+  constexpr bool AHEAD = NJ <= 2;                      // the next tile waits in registers while this one is worked on
   extern __shared__ float sm[];
   float* sq = sm;                       // [R][LD]
   float* sk = sq + R * LD;              // [kKT][LD]
   float* sv = sk + kKT * LD;            // [kKT][LD]
   float* sp = sv + kKT * LD;            // [R][LP]
   __shared__ int s_bad[R];
+  __shared__ long long s_off[2][kKT];   // where the rows of a tile lie
   const PagedProblem& p = a.p;
   pdl_wait();
   pdl_trigger();
@@ -85,7 +88,27 @@ __global__ void __launch_bounds__(kGenThreads) paged_attn_general_kernel(const G
   }
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
   const int hd4 = (p.hd + 3) / 4;
+  auto place = [&](int kt, int buf) {
+    if (tid < kKT) s_off[buf][tid] = kt + tid < k1 ? kv_off(p, t.table, kt + tid, kvh) : -1;
+  };
+  float4 rk[AHEAD ? NL : 1], rv[AHEAD ? NL : 1];
+  auto piece = [&](int i, int buf, float4& kx, float4& vx) {
+    const int r = i / (16 * NJ), c = i % (16 * NJ);
+    const long long off = s_off[buf][r];
+    kx = vx = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (off >= 0 && c < hd4) {
+      kx = load4_tail(p.k, p.kv_type, off, 4 * c, p.hd, a.kv_vec);
+      vx = load4_tail(p.v, p.kv_type, off, 4 * c, p.hd, a.kv_vec);
+    }
+  };
+  auto put = [&](int i, const float4& kx, const float4& vx) {
+    const int r = i / (16 * NJ), c = i % (16 * NJ);
+    *reinterpret_cast<float4*>(sk + r * LD + 4 * c) = kx;
+    *reinterpret_cast<float4*>(sv + r * LD + 4 * c) = vx;
+  };
+  place(k0, 0);
   for (int i = tid; i < R; i += kGenThreads) s_bad[i] = 0;
+#pragma unroll 4
   for (int i = tid; i < R * 16 * NJ; i += kGenThreads) {
     const int r = i / (16 * NJ), c = i % (16 * NJ);
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -101,7 +124,7 @@ __global__ void __launch_bounds__(kGenThreads) paged_attn_general_kernel(const G
 #pragma unroll
   for (int i = 0; i < RI; ++i) {
     const int r = ty + 16 * i;
-    lim[i] = r < nr ? seen(p, t, (r0 + r) / p.group) : 0;
+    lim[i] = r < nr ? min(k1, seen(p, t, (r0 + r) / p.group)) : 0;
     m[i] = -INFINITY;
     l[i] = 0.0f;
 #pragma unroll
@@ -109,27 +132,35 @@ __global__ void __launch_bounds__(kGenThreads) paged_attn_general_kernel(const G
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[i][j][e] = 0.0f;
   }
-  for (int kt = k0; kt < k1; kt += kKT) {
-    __syncthreads();
-    for (int i = tid; i < kKT * 16 * NJ; i += kGenThreads) {
-      const int r = i / (16 * NJ), c = i % (16 * NJ);
-      float4 kx = make_float4(0.f, 0.f, 0.f, 0.f), vx = kx;
-      if (kt + r < k1 && c < hd4) {
-        const long long off = kv_off(p, t.table, kt + r, kvh);
-        if (off >= 0) {
-          kx = load4_tail(p.k, p.kv_type, off, 4 * c, p.hd, a.kv_vec);
-          vx = load4_tail(p.v, p.kv_type, off, 4 * c, p.hd, a.kv_vec);
-        }
+  __syncthreads();
+  if (AHEAD) {
+#pragma unroll
+    for (int x = 0; x < NL; ++x) piece(tid + x * kGenThreads, 0, rk[AHEAD ? x : 0], rv[AHEAD ? x : 0]);
+  }
+  int buf = 0;
+  for (int kt = k0; kt < k1; kt += kKT, buf ^= 1) {
+    place(kt + kKT, buf ^ 1);
+#pragma unroll
+    for (int x = 0; x < NL; ++x) {
+      if (AHEAD) {
+        put(tid + x * kGenThreads, rk[AHEAD ? x : 0], rv[AHEAD ? x : 0]);
+      } else {
+        float4 kx, vx;
+        piece(tid + x * kGenThreads, buf, kx, vx);
+        put(tid + x * kGenThreads, kx, vx);
       }
-      *reinterpret_cast<float4*>(sk + r * LD + 4 * c) = kx;
-      *reinterpret_cast<float4*>(sv + r * LD + 4 * c) = vx;
     }
     __syncthreads();
+    if (AHEAD && kt + kKT < k1) {
+#pragma unroll
+      for (int x = 0; x < NL; ++x) piece(tid + x * kGenThreads, buf ^ 1, rk[AHEAD ? x : 0], rv[AHEAD ? x : 0]);
+    }
     float s[RI][4];
 #pragma unroll
     for (int i = 0; i < RI; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) s[i][j] = 0.0f;
+#pragma unroll 4
     for (int c = 0; c < hd4; ++c) {
       float4 kx[4];
 #pragma unroll
@@ -147,7 +178,7 @@ __global__ void __launch_bounds__(kGenThreads) paged_attn_general_kernel(const G
       float mx = -INFINITY;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        s[i][j] = kt + tx + 16 * j < min(lim[i], k1) ? s[i][j] * p.scale_log2 : -INFINITY;
+        s[i][j] = kt + tx + 16 * j < lim[i] ? s[i][j] * p.scale_log2 : -INFINITY;
         mx = fmaxf(mx, s[i][j]);
       }
 #pragma unroll
@@ -169,21 +200,28 @@ __global__ void __launch_bounds__(kGenThreads) paged_attn_general_kernel(const G
         for (int e = 0; e < 4; ++e) o[i][j][e] *= c;
     }
     __syncwarp();                               // a row's weights come from its own half warp
-    const int kn = min(kKT, k1 - kt);
-    for (int kk = 0; kk < kn; ++kk) {
+    const int kn = min(kKT, k1 - kt);           // the rows behind are zeros, with weights of zero
+#pragma unroll 2
+    for (int kk = 0; kk < kn; kk += 4) {
+      float4 w[RI];
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        const float4 vx = *reinterpret_cast<const float4*>(sv + kk * LD + 4 * tx + 64 * j);
+      for (int i = 0; i < RI; ++i) w[i] = *reinterpret_cast<const float4*>(sp + (ty + 16 * i) * LP + kk);
 #pragma unroll
-        for (int i = 0; i < RI; ++i) {
-          const float w = sp[(ty + 16 * i) * LP + kk];
-          o[i][j][0] = fmaf(w, vx.x, o[i][j][0]);
-          o[i][j][1] = fmaf(w, vx.y, o[i][j][1]);
-          o[i][j][2] = fmaf(w, vx.z, o[i][j][2]);
-          o[i][j][3] = fmaf(w, vx.w, o[i][j][3]);
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+          const float4 vx = *reinterpret_cast<const float4*>(sv + (kk + e) * LD + 4 * tx + 64 * j);
+#pragma unroll
+          for (int i = 0; i < RI; ++i) {
+            const float we = e == 0 ? w[i].x : e == 1 ? w[i].y : e == 2 ? w[i].z : w[i].w;
+            o[i][j][0] = fmaf(we, vx.x, o[i][j][0]);
+            o[i][j][1] = fmaf(we, vx.y, o[i][j][1]);
+            o[i][j][2] = fmaf(we, vx.z, o[i][j][2]);
+            o[i][j][3] = fmaf(we, vx.w, o[i][j][3]);
+          }
         }
-      }
     }
+    __syncthreads();
   }
 #pragma unroll
   for (int i = 0; i < RI; ++i) {
@@ -235,9 +273,13 @@ struct JoinArgs {
   int pre_splits;              // slots of the prefix, all of them written
   const int* prefix_table;
   int prefix_len;
+  int out_vec;                 // four-element stores to out are aligned
 };
 
+// V elements a lane a round, N rounds
+template <int V, int N>
 __global__ void __launch_bounds__(128) paged_attn_join_kernel(const JoinArgs a) {
+  constexpr int U = V * N <= 4 ? 8 : 4;       // slots whose rows are in flight together
   const PagedProblem& p = a.p;
   pdl_wait();
   pdl_trigger();
@@ -248,40 +290,53 @@ __global__ void __launch_bounds__(128) paged_attn_join_kernel(const JoinArgs a) 
   if (w >= t.qn * p.heads) return;
   const int r = w / p.heads, h = w % p.heads, tok = t.q0 + r;
   const int n = seen(p, t, r);
-  const int own = (n + p.chunk - 1) / p.chunk;
+  const int cnt = a.pre_splits + (n + p.chunk - 1) / p.chunk;
   const long long row = (long long)tok * p.heads + h, step = (long long)p.total_q * p.heads;
-  const int cnt = a.pre_splits + own;
-  float M = -INFINITY;
-  for (int s = lane; s < cnt; s += 32) M = fmaxf(M, p.part_ml[s * step + row].x);
-  for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
-  const float base = M == -INFINITY ? 0.0f : M;
-  float L = 0.0f, o[8];
+  // running over rounds of 32 slots, lane i has slot s0 + i
+  float M = -INFINITY, L = 0.0f, o[N][V];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) o[i] = 0.0f;
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int e = 0; e < V; ++e) o[i][e] = 0.0f;
   for (int s0 = 0; s0 < cnt; s0 += 32) {
-    // lane i: the weight of slot s0 + i; the slots' rows four at a time, so
-    // that their loads are in flight together
-    float c = 0.0f;
-    if (s0 + lane < cnt) {
-      const float2 ml = p.part_ml[(s0 + lane) * step + row];
-      c = exp2f(ml.x - base);
-      L = fmaf(ml.y, c, L);
-    }
-    const int m = min(32, cnt - s0);
-    for (int s = 0; s < m; s += 4) {
-      float x[4][8];
+    float2 ml = make_float2(-INFINITY, 0.0f);
+    if (s0 + lane < cnt) ml = p.part_ml[(s0 + lane) * step + row];
+    float mx = ml.x;
+    for (int x = 16; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+    const float mn = fmaxf(M, mx), base = mn == -INFINITY ? 0.0f : mn;
+    const float f = exp2f(M - base), c = exp2f(ml.x - base);
+    M = mn;
+    L = fmaf(L, f, ml.y * c);
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int e = 0; e < V; ++e) o[i][e] *= f;
+    const int m = min(32, cnt - s0);
+    for (int s = 0; s < m; s += U) {
+      float x[U][N][V];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
         const float* src = p.part_o + ((s0 + s + u) * step + row) * p.hd;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[u][i] = s + u < m && lane + 32 * i < p.hd ? src[lane + 32 * i] : 0.0f;
+        for (int i = 0; i < N; ++i) {
+          const int d = (lane + 32 * i) * V;
+          const bool have = s + u < m && d < p.hd;
+          if constexpr (V == 4) {
+            const float4 q = have ? *reinterpret_cast<const float4*>(src + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+            x[u][i][0] = q.x; x[u][i][1] = q.y; x[u][i][2] = q.z; x[u][i][3] = q.w;
+          } else {
+            x[u][i][0] = have ? src[d] : 0.0f;
+          }
+        }
       }
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
+      for (int u = 0; u < U; ++u) {
         const float cu = __shfl_sync(0xffffffffu, c, (s + u) & 31);
         if (s + u < m) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) o[i] = fmaf(x[u][i], cu, o[i]);
+          for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int e = 0; e < V; ++e) o[i][e] = fmaf(x[u][i][e], cu, o[i][e]);
         }
       }
     }
@@ -291,12 +346,30 @@ __global__ void __launch_bounds__(128) paged_attn_join_kernel(const JoinArgs a) 
   const long long oo = (long long)tok * p.out_stride + (long long)h * p.hd;
   bool bad = false;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float v = o[i] * inv;
-    if (lane + 32 * i < p.hd) {
-      store_elem(p.out, p.type, oo + lane + 32 * i, v);
-      bad |= isnan(v);
+  for (int i = 0; i < N; ++i) {
+    const int d = (lane + 32 * i) * V;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      o[i][e] = L == 0.0f ? 0.0f : o[i][e] * inv;
+      bad |= d < p.hd && isnan(o[i][e]);
     }
+    if (d >= p.hd) continue;
+    if constexpr (V == 4) {
+      if (a.out_vec && p.type == TOSK_F32) {
+        *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.out) + oo + d) = make_float4(o[i][0], o[i][1], o[i][2], o[i][3]);
+        continue;
+      }
+      if (a.out_vec) {
+        const __half2 x = __floats2half2_rn(o[i][0], o[i][1]), y = __floats2half2_rn(o[i][2], o[i][3]);
+        uint2 u;
+        u.x = *reinterpret_cast<const uint32_t*>(&x);
+        u.y = *reinterpret_cast<const uint32_t*>(&y);
+        *reinterpret_cast<uint2*>(reinterpret_cast<__half*>(p.out) + oo + d) = u;
+        continue;
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < V; ++e) store_elem(p.out, p.type, oo + d + e, o[i][e]);
   }
   if (__any_sync(0xffffffffu, bad)) attn_row_plain(p, a.prefix_table, a.prefix_len, t.table, n, tok, h);
 }
@@ -381,10 +454,10 @@ int run_general(const PagedProblem& p, cudaStream_t st) {
   return rows <= 32 ? general_rows<16>(p, st) : general_rows<64>(p, st);
 }
 
-// Splits of a key axis: `rounds` CTAs for every SM, at least 256 keys each.
-int plan_splits(long long tiles, int keys, int rounds) {
+// Splits of a key axis: `rounds` CTAs for every SM, at least `least` keys each.
+int plan_splits(long long tiles, int keys, int rounds, int least) {
   const long long want = (rounds * kSms + tiles - 1) / tiles;
-  const long long most = (keys + 255) / 256;
+  const long long most = (keys + least - 1) / least;
   const long long s = want < most ? want : most;
   return s < 1 ? 1 : (int)s;
 }
@@ -397,10 +470,10 @@ struct DecodePlan {
 DecodePlan plan_decode(int n_seqs, int max_kv, int prefix_len, int heads, int n_kv) {
   DecodePlan d;
   const long long rows = (long long)n_seqs * (heads / n_kv);
-  d.pre = prefix_len > 0 ? plan_splits((rows + 255) / 256 * n_kv, prefix_len, 1) : 0;
+  d.pre = prefix_len > 0 ? plan_splits((rows + 255) / 256 * n_kv, prefix_len, 1, 256) : 0;
   d.pre_chunk = d.pre ? chunk_of(prefix_len, d.pre) : 0;
   if (d.pre) d.pre = (prefix_len + d.pre_chunk - 1) / d.pre_chunk;
-  d.own = max_kv > 0 ? plan_splits((long long)n_seqs * n_kv, max_kv, 12) : 1;
+  d.own = max_kv > 0 ? plan_splits((long long)n_seqs * n_kv, max_kv, 4, 512) : 1;
   d.own_chunk = max_kv > 0 ? chunk_of(max_kv, d.own) : 128;
   if (max_kv > 0) d.own = (max_kv + d.own_chunk - 1) / d.own_chunk;
   if (!d.pre && d.own == 1) d.own = 0;
@@ -415,7 +488,11 @@ int run_join(const PagedProblem& own, int pre, const int* prefix_table, int pref
   j.prefix_len = prefix_len;
   const long long gx = ((long long)own.max_q * own.heads + 3) / 4;
   if (gx > 0x7fffffffll || own.n_seqs > 65535) return (int)cudaErrorInvalidValue;
-  return launch((const void*)paged_attn_join_kernel, dim3((unsigned)gx, own.n_seqs), 128, 0, &j, st);
+  j.out_vec = aligned4(own.out, own.out_stride, own.type, own.hd);
+  const void* f = own.hd % 4   ? (const void*)paged_attn_join_kernel<1, 8>
+                  : own.hd <= 128 ? (const void*)paged_attn_join_kernel<4, 1>
+                                  : (const void*)paged_attn_join_kernel<4, 2>;
+  return launch(f, dim3((unsigned)gx, own.n_seqs), 128, 0, &j, st);
 }
 
 void part_views(PagedProblem& p, void* ws, int slots) {
