@@ -12,7 +12,7 @@
 // group's heads, and walks the keys in tiles of 64 staged in shared memory as
 // fp32.  256 threads as 16 x 16: thread (ty, tx) owns rows ty + 16 i and, for
 // the scores, keys tx + 16 j, for the sums, dims 4 tx + 64 j.  All arithmetic
-// is fp32 FMA.  R = 64 for prompts, 16 where a sequence brings few rows.
+// is fp32 FMA (packed, two at a time).  R = 64 for prompts, 16 where a sequence brings few rows.
 #include <cuda_runtime.h>
 
 #include "paged_common.cuh"
@@ -55,7 +55,7 @@ struct GenArgs {
 };
 
 template <int R, int NJ>
-__global__ void __launch_bounds__(kGenThreads) paged_attn_general_kernel(const GenArgs a) {
+__global__ void __launch_bounds__(kGenThreads) paged_attn_general_kernel(const __grid_constant__ GenArgs a) {
   constexpr int RI = R / 16, LD = 64 * NJ + 4, LP = kKT + 4;
   constexpr int NL = kKT * 16 * NJ / kGenThreads;      // 16-byte pieces of K, and of V, a thread a tile
   constexpr bool AHEAD = NJ <= 2;                      // the next tile waits in registers while this one is worked on
@@ -155,11 +155,12 @@ __global__ void __launch_bounds__(kGenThreads) paged_attn_general_kernel(const G
 #pragma unroll
       for (int x = 0; x < NL; ++x) piece(tid + x * kGenThreads, buf ^ 1, rk[AHEAD ? x : 0], rv[AHEAD ? x : 0]);
     }
+    float2 s2[RI][4];                           // even and odd dims apart: packed FMAs
     float s[RI][4];
 #pragma unroll
     for (int i = 0; i < RI; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) s[i][j] = 0.0f;
+      for (int j = 0; j < 4; ++j) s2[i][j] = make_float2(0.0f, 0.0f);
 #pragma unroll 4
     for (int c = 0; c < hd4; ++c) {
       float4 kx[4];
@@ -169,8 +170,10 @@ __global__ void __launch_bounds__(kGenThreads) paged_attn_general_kernel(const G
       for (int i = 0; i < RI; ++i) {
         const float4 qx = *reinterpret_cast<const float4*>(sq + (ty + 16 * i) * LD + 4 * c);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          s[i][j] = fmaf(qx.w, kx[j].w, fmaf(qx.z, kx[j].z, fmaf(qx.y, kx[j].y, fmaf(qx.x, kx[j].x, s[i][j]))));
+        for (int j = 0; j < 4; ++j) {
+          s2[i][j] = __ffma2_rn(make_float2(qx.x, qx.y), make_float2(kx[j].x, kx[j].y), s2[i][j]);
+          s2[i][j] = __ffma2_rn(make_float2(qx.z, qx.w), make_float2(kx[j].z, kx[j].w), s2[i][j]);
+        }
       }
     }
 #pragma unroll
@@ -178,7 +181,7 @@ __global__ void __launch_bounds__(kGenThreads) paged_attn_general_kernel(const G
       float mx = -INFINITY;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        s[i][j] = kt + tx + 16 * j < lim[i] ? s[i][j] * p.scale_log2 : -INFINITY;
+        s[i][j] = kt + tx + 16 * j < lim[i] ? (s2[i][j].x + s2[i][j].y) * p.scale_log2 : -INFINITY;
         mx = fmaxf(mx, s[i][j]);
       }
 #pragma unroll
@@ -214,10 +217,11 @@ __global__ void __launch_bounds__(kGenThreads) paged_attn_general_kernel(const G
 #pragma unroll
           for (int i = 0; i < RI; ++i) {
             const float we = e == 0 ? w[i].x : e == 1 ? w[i].y : e == 2 ? w[i].z : w[i].w;
-            o[i][j][0] = fmaf(we, vx.x, o[i][j][0]);
-            o[i][j][1] = fmaf(we, vx.y, o[i][j][1]);
-            o[i][j][2] = fmaf(we, vx.z, o[i][j][2]);
-            o[i][j][3] = fmaf(we, vx.w, o[i][j][3]);
+            const float2 w2 = make_float2(we, we);
+            const float2 a0 = __ffma2_rn(w2, make_float2(vx.x, vx.y), make_float2(o[i][j][0], o[i][j][1]));
+            const float2 a1 = __ffma2_rn(w2, make_float2(vx.z, vx.w), make_float2(o[i][j][2], o[i][j][3]));
+            o[i][j][0] = a0.x; o[i][j][1] = a0.y;
+            o[i][j][2] = a1.x; o[i][j][3] = a1.y;
           }
         }
     }
@@ -278,7 +282,7 @@ struct JoinArgs {
 
 // V elements a lane a round, N rounds
 template <int V, int N>
-__global__ void __launch_bounds__(128) paged_attn_join_kernel(const JoinArgs a) {
+__global__ void __launch_bounds__(128) paged_attn_join_kernel(const __grid_constant__ JoinArgs a) {
   constexpr int U = V * N <= 4 ? 8 : 4;       // slots whose rows are in flight together
   const PagedProblem& p = a.p;
   pdl_wait();

@@ -1,6 +1,6 @@
-// paged_decode.cu - attention of single tokens over an fp16 paged cache.
+// paged_decode.cu - attention of single tokens over a paged cache.
 //
-// A CTA takes a chunk of one sequence's keys for one key/value head and the
+// fp16 cache.  A CTA takes a chunk of one sequence's keys for one key/value head and the
 // (up to 8 or 16) query heads that share it; its four warps take every fourth
 // 16-key step each and run alone, without any exchange until the end:
 //   * the step's K and V rows stream through the warp's own ring in shared
@@ -65,7 +65,7 @@ struct DecArgs {
 };
 
 template <int HD, int NQ>
-__global__ void __launch_bounds__(32 * kDecWarps) paged_decode_kernel(const DecArgs a) {
+__global__ void __launch_bounds__(32 * kDecWarps) paged_decode_kernel(const __grid_constant__ DecArgs a) {
   using T = DecShape<HD>;
   extern __shared__ __align__(128) uint8_t sm[];
   const PagedProblem& p = a.p;
@@ -273,20 +273,227 @@ __global__ void __launch_bounds__(32 * kDecWarps) paged_decode_kernel(const DecA
   }
 }
 
+// ---------------------------------------------------------------------------
+// The same over an fp32 cache, in fp32 throughout (packed FMAs: the tensor
+// cores have no fp32 product, and the bytes leave the FMA pipe room for 8
+// query heads a K/V row: 4 FMAs a byte read against the ~5 that HBM lets by).
+// A warp's step is 8 keys.  Scores: lane (key, quarter of the dims), the four
+// quarters added by two shuffles; the weights go through shared memory; sums:
+// a lane has the dims 4 lane .. (64 dims: half the keys too).
+// ---------------------------------------------------------------------------
+template <int HD, int Q>
+struct Dec32Shape {
+  static constexpr int kKeysStep = 8;
+  static constexpr int kRow = HD * 4;
+  static constexpr int kStage = 2 * kKeysStep * kRow;
+  static constexpr int kDepth = HD == 64 ? 6 : 3;
+  static constexpr int kRing = kDecWarps * kDepth * kStage;
+  static constexpr int kSmem = kRing + Q * HD * 4 + kDecWarps * kKeysStep * Q * 4;
+};
+
+template <int HD, int Q>
+__global__ void __launch_bounds__(32 * kDecWarps) paged_decode_f32_kernel(const __grid_constant__ DecArgs a) {
+  using T = Dec32Shape<HD, Q>;
+  constexpr int KS = T::kKeysStep, CH = HD / 4;                  // keys a step, 16-byte pieces of a row
+  constexpr int KG = CH < 32 ? 2 : 1, NC = CH > 32 ? CH / 32 : 1; // key groups of the sums, pieces a lane
+  extern __shared__ __align__(128) uint8_t sm[];
+  const PagedProblem& p = a.p;
+  if (!a.late_wait) {
+    pdl_wait();
+    pdl_trigger();
+  }
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  int b = blockIdx.x;
+  const int qb = b % a.qblocks;
+  b /= a.qblocks;
+  const int kvh = b % p.n_kv;
+  b /= p.n_kv;
+  const int splits = p.splits ? p.splits : 1, split = b % splits, seq = b / splits;
+  const SeqTask t = seq_task(p, seq);
+  int k0 = 0, k1 = t.kvn;
+  if (p.splits) {
+    k0 = split * p.chunk;
+    k1 = min(k1, k0 + p.chunk);
+  }
+  const int h0 = kvh * p.group + qb * Q, nh = min(Q, p.group - qb * Q);
+  if (k0 < k1 || !p.splits) {
+    const int steps = (k1 - k0 + KS - 1) / KS;
+    const uint8_t* ringp = sm + warp * T::kDepth * T::kStage;
+    const uint32_t ring = smem_u32(ringp);
+    float* sq = reinterpret_cast<float*>(sm + T::kRing);                  // [Q][HD]
+    float* sp = sq + Q * HD + warp * KS * Q;                              // [key][query]
+    const float* kb = reinterpret_cast<const float*>(p.k);
+    const float* vb = reinterpret_cast<const float*>(p.v);
+    const int chs = p.hd / 4;
+    auto fetch_row = [&](int st) -> long long {
+      const int key = k0 + st * KS + (lane & 7);
+      return st < steps && key < k1 ? kv_off(p, t.table, key, kvh) : -1;
+    };
+    auto issue = [&](int st, long long row) {
+      if (st < steps) {
+        const uint32_t dst = ring + (st / kDecWarps % T::kDepth) * T::kStage;
+#pragma unroll
+        for (int i = 0; i < KS * CH / 32; ++i) {
+          const int idx = i * 32 + lane, key = idx / CH, c = idx % CH;
+          const long long off = __shfl_sync(0xffffffffu, row, key);
+          const bool have = off >= 0 && c < chs;
+          const long long o = have ? off + 4 * c : 0;
+          const uint32_t d = dst + key * T::kRow + ((c ^ (key & 7)) << 4);
+          cp16(d, kb + o, have);
+          cp16(d + KS * T::kRow, vb + o, have);
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    long long rows[T::kDepth];
+#pragma unroll
+    for (int d = 0; d < T::kDepth; ++d) rows[d] = fetch_row(warp + d * kDecWarps);
+#pragma unroll
+    for (int d = 0; d < T::kDepth - 1; ++d) issue(warp + d * kDecWarps, rows[d]);
+    long long nrow = rows[T::kDepth - 1];
+    for (int i = tid; i < Q * HD; i += 32 * kDecWarps) {
+      const int h = i / HD, d = i % HD;
+      sq[i] = h < nh && d < p.hd ? load_elem(p.q, p.type, (long long)t.q0 * p.q_stride + (long long)(h0 + h) * p.hd + d) : 0.0f;
+    }
+    __syncthreads();
+    float m[Q], l[Q];
+    float2 o[Q][NC][2];
+#pragma unroll
+    for (int n = 0; n < Q; ++n) {
+      m[n] = -INFINITY;
+      l[n] = 0.0f;
+#pragma unroll
+      for (int c = 0; c < NC; ++c) o[n][c][0] = o[n][c][1] = make_float2(0.0f, 0.0f);
+    }
+    const int key = lane & 7, quarter = lane >> 3;
+    for (int st = warp; st < steps; st += kDecWarps) {
+      issue(st + (T::kDepth - 1) * kDecWarps, nrow);
+      nrow = fetch_row(st + T::kDepth * kDecWarps);
+      asm volatile("cp.async.wait_group %0;" ::"n"(T::kDepth - 1) : "memory");
+      __syncwarp();
+      const uint8_t* ks = ringp + (st / kDecWarps % T::kDepth) * T::kStage;
+      const uint8_t* vs = ks + KS * T::kRow;
+      float2 s[Q];
+#pragma unroll
+      for (int n = 0; n < Q; ++n) s[n] = make_float2(0.0f, 0.0f);
+#pragma unroll 4
+      for (int i = 0; i < CH / 4; ++i) {
+        const int c = quarter + 4 * i;
+        const float4 kx = *reinterpret_cast<const float4*>(ks + key * T::kRow + ((c ^ key) << 4));
+#pragma unroll
+        for (int n = 0; n < Q; ++n) {
+          const float4 qx = *reinterpret_cast<const float4*>(sq + n * HD + 4 * c);
+          s[n] = __ffma2_rn(make_float2(qx.x, qx.y), make_float2(kx.x, kx.y), s[n]);
+          s[n] = __ffma2_rn(make_float2(qx.z, qx.w), make_float2(kx.z, kx.w), s[n]);
+        }
+      }
+      const bool counts = key < k1 - (k0 + st * KS);
+#pragma unroll
+      for (int n = 0; n < Q; ++n) {
+        float x = s[n].x + s[n].y;
+        x += __shfl_xor_sync(0xffffffffu, x, 8);
+        x += __shfl_xor_sync(0xffffffffu, x, 16);
+        x = counts ? x * p.scale_log2 : -INFINITY;
+        if (__any_sync(0xffffffffu, x > m[n] + 8.0f)) {
+          float top = x;
+#pragma unroll
+          for (int w = 4; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+          const float mn = fmaxf(m[n], top), f = exp2f(m[n] - mn);   // 0 on the first keys
+          m[n] = mn;
+          l[n] *= f;
+#pragma unroll
+          for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) o[n][c][e] = __fmul2_rn(o[n][c][e], make_float2(f, f));
+        }
+        const float w = ex2(x - (m[n] == -INFINITY ? 0.0f : m[n]));
+        l[n] += w;
+        if (quarter == (n & 3)) sp[key * Q + n] = w;
+      }
+      __syncwarp();
+      // weights of keys behind the end are 0, their values zeros
+#pragma unroll
+      for (int kk = 0; kk < KS / KG; ++kk) {
+        const int ky = kk * KG + (KG == 2 ? lane >> 4 : 0);
+        float w[Q];
+#pragma unroll
+        for (int n = 0; n < Q; ++n) w[n] = sp[ky * Q + n];
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          const int pc = (KG == 2 ? lane & 15 : lane) + 32 * c;
+          const float4 vx = *reinterpret_cast<const float4*>(vs + ky * T::kRow + ((pc ^ (ky & 7)) << 4));
+#pragma unroll
+          for (int n = 0; n < Q; ++n) {
+            o[n][c][0] = __ffma2_rn(make_float2(w[n], w[n]), make_float2(vx.x, vx.y), o[n][c][0]);
+            o[n][c][1] = __ffma2_rn(make_float2(w[n], w[n]), make_float2(vx.z, vx.w), o[n][c][1]);
+          }
+        }
+      }
+      __syncwarp();                                               // the stage and the weights may be written again
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();                                              // the rings are free: join the warps there
+    float* so = reinterpret_cast<float*>(sm);                     // [warp][query][HD]
+    __shared__ float2 sml[kDecWarps][Q];
+#pragma unroll
+    for (int n = 0; n < Q; ++n) {
+#pragma unroll
+      for (int w = 4; w > 0; w >>= 1) l[n] += __shfl_xor_sync(0xffffffffu, l[n], w);
+      if (lane == 0) sml[warp][n] = make_float2(m[n], l[n]);
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        float2 x = o[n][c][0], y = o[n][c][1];
+        if (KG == 2) {
+          x.x += __shfl_xor_sync(0xffffffffu, x.x, 16); x.y += __shfl_xor_sync(0xffffffffu, x.y, 16);
+          y.x += __shfl_xor_sync(0xffffffffu, y.x, 16); y.y += __shfl_xor_sync(0xffffffffu, y.y, 16);
+        }
+        const int pc = (KG == 2 ? lane & 15 : lane) + 32 * c;
+        if (KG == 1 || lane < 16)
+          *reinterpret_cast<float4*>(so + (warp * Q + n) * HD + 4 * pc) = make_float4(x.x, x.y, y.x, y.y);
+      }
+    }
+    __syncthreads();
+    for (int h = warp; h < nh; h += kDecWarps) {
+      float M = -INFINITY, L = 0.0f, f[kDecWarps];
+#pragma unroll
+      for (int w = 0; w < kDecWarps; ++w) M = fmaxf(M, sml[w][h].x);
+#pragma unroll
+      for (int w = 0; w < kDecWarps; ++w) {
+        f[w] = M == -INFINITY ? 0.0f : exp2f(sml[w][h].x - M);
+        L += f[w] * sml[w][h].y;
+      }
+      const int head = h0 + h;
+      const long long part = (long long)(p.slot0 + split) * p.total_q * p.heads + (long long)t.q0 * p.heads + head;
+      const long long oo = (long long)t.q0 * p.out_stride + (long long)head * p.hd;
+      const float inv = p.splits ? 1.0f : L == 0.0f ? 0.0f : 1.0f / L;
+      if (p.splits && lane == 0) p.part_ml[part] = make_float2(M, L);
+      for (int d = lane; d < p.hd; d += 32) {
+        float v = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kDecWarps; ++w) v = fmaf(f[w], so[(w * Q + h) * HD + d], v);
+        if (p.splits) p.part_o[part * p.hd + d] = v;
+        else store_elem(p.out, p.type, oo + d, L == 0.0f ? 0.0f : v * inv);
+      }
+    }
+  }
+  if (a.late_wait) {
+    pdl_trigger();
+    pdl_wait();
+  }
+}
+
 }  // namespace tos
 
 using namespace tos;
 
 namespace {
-template <int HD, int NQ>
-int dec_launch(const DecArgs& a, unsigned grid, cudaStream_t st) {
-  const void* f = (const void*)paged_decode_kernel<HD, NQ>;
-  const cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, DecShape<HD>::kSmem);
+int dec_launch(const void* f, int smem, const DecArgs& a, unsigned grid, cudaStream_t st) {
+  const cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return (int)e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(32 * kDecWarps);
-  cfg.dynamicSmemBytes = DecShape<HD>::kSmem;
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -296,29 +503,45 @@ int dec_launch(const DecArgs& a, unsigned grid, cudaStream_t st) {
   void* args[] = {const_cast<DecArgs*>(&a)};
   return (int)cudaLaunchKernelExC(&cfg, f, args);
 }
+
+template <int HD>
+int dec16(const DecArgs& a, int nq, unsigned n, cudaStream_t st) {
+  if constexpr (HD <= 128)
+    if (nq == 2) return dec_launch((const void*)paged_decode_kernel<HD, 2>, DecShape<HD>::kSmem, a, n, st);
+  return dec_launch((const void*)paged_decode_kernel<HD, 1>, DecShape<HD>::kSmem, a, n, st);
+}
+
+template <int HD>
+int dec32(const DecArgs& a, int q, unsigned n, cudaStream_t st) {
+  if (q == 1) return dec_launch((const void*)paged_decode_f32_kernel<HD, 1>, Dec32Shape<HD, 1>::kSmem, a, n, st);
+  if (q == 4) return dec_launch((const void*)paged_decode_f32_kernel<HD, 4>, Dec32Shape<HD, 4>::kSmem, a, n, st);
+  return dec_launch((const void*)paged_decode_f32_kernel<HD, 8>, Dec32Shape<HD, 8>::kSmem, a, n, st);
+}
 }  // namespace
 
 namespace tos {
 
-// What this kernel takes: an fp16 cache whose rows are whole 16-byte pieces.
+// What these kernels take: a cache whose rows are whole 16-byte pieces.
 bool paged_decode_ok(const PagedProblem& p) {
-  return p.kv_type == TOSK_F16 && p.hd % 8 == 0 && ((uintptr_t)p.k & 15) == 0 && ((uintptr_t)p.v & 15) == 0;
+  return p.hd % (p.kv_type == TOSK_F16 ? 8 : 4) == 0 && ((uintptr_t)p.k & 15) == 0 && ((uintptr_t)p.v & 15) == 0;
 }
 
-// One token a sequence.  Groups of up to 8 query heads in one block of 8,
-// larger ones in blocks of 16 (256 dims: of 8, for the registers).
+// One token a sequence.  fp16: groups of up to 8 query heads in one block of
+// 8, larger ones in blocks of 16 (256 dims: of 8, for the registers).  fp32:
+// blocks of 1, 4 or 8, the smallest that holds the group.
 int paged_decode_run(const PagedProblem& p, int late_wait, cudaStream_t st) {
   DecArgs a;
   a.p = p;
   a.late_wait = late_wait;
+  const bool f16 = p.kv_type == TOSK_F16;
   const int nq = p.group > 8 && p.hd <= 128 ? 2 : 1;
-  a.qblocks = (p.group + 8 * nq - 1) / (8 * nq);
+  const int block = f16 ? 8 * nq : p.group == 1 ? 1 : p.group <= 4 ? 4 : 8;
+  a.qblocks = (p.group + block - 1) / block;
   const long long grid = (long long)a.qblocks * p.n_kv * (p.splits ? p.splits : 1) * p.n_seqs;
   if (grid > 0x7fffffffll) return (int)cudaErrorInvalidValue;
   const unsigned n = (unsigned)grid;
-  if (p.hd <= 64) return nq == 1 ? dec_launch<64, 1>(a, n, st) : dec_launch<64, 2>(a, n, st);
-  if (p.hd <= 128) return nq == 1 ? dec_launch<128, 1>(a, n, st) : dec_launch<128, 2>(a, n, st);
-  return dec_launch<256, 1>(a, n, st);
+  if (f16) return p.hd <= 64 ? dec16<64>(a, nq, n, st) : p.hd <= 128 ? dec16<128>(a, nq, n, st) : dec16<256>(a, nq, n, st);
+  return p.hd <= 64 ? dec32<64>(a, block, n, st) : p.hd <= 128 ? dec32<128>(a, block, n, st) : dec32<256>(a, block, n, st);
 }
 
 }  // namespace tos

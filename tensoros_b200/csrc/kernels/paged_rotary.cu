@@ -265,7 +265,7 @@ __device__ __forceinline__ void do_heads(const RotParams& p, const Pairs<V, NC>&
 
 // V pairs a lane, NC rounds of group * V pairs a head
 template <typename TI, int V, int NC>
-__global__ void __launch_bounds__(32 * kRotWarps, 4) rotary_rows_kernel(const RotParams p) {
+__global__ void __launch_bounds__(32 * kRotWarps, 4) rotary_rows_kernel(const __grid_constant__ RotParams p) {
   const tosk_rotary_args_t& a = p.a;
   __shared__ float2 s_cs[kRotWarps][kMaxPairs];       // magnitude * (cos, -sin) of the warp's token
   __shared__ float s_w[2][2 * kMaxPairs];
