@@ -409,6 +409,9 @@ PagedProblem problem_of(const tosk_paged_attn_t* a) {
   p.kv_type = a->kv.type; p.n_pages = a->kv.n_pages; p.page_size = a->kv.page_size;
   p.n_kv = a->kv.n_kv; p.hd = a->kv.hd;
   p.heads = a->n_heads; p.group = a->n_heads / a->kv.n_kv;
+  p.gshift = -1;
+  for (int i = 0; i < 31; ++i)
+    if (p.group == 1 << i) p.gshift = i;
   p.table = a->kv.table; p.table_stride = a->kv.table_stride;
   p.cu_q = a->cu_q; p.kv_len = a->kv_len;
   p.n_seqs = a->n_seqs; p.total_q = a->total_q; p.max_q = a->max_q; p.max_kv = a->max_kv;

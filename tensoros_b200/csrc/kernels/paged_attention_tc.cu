@@ -289,13 +289,13 @@ struct __align__(16) Work {
 template <int HD, bool SPLIT>
 struct QRows {
   static constexpr int CH = HD / 8, RPS = 32 / CH, STEPS = 16 / RPS, PARTS = SPLIT ? 2 : 1;
-  static constexpr int BATCH = 8 / PARTS < STEPS ? 8 / PARTS : STEPS;
+  static constexpr int BATCH = STEPS;      // all in flight at once
   long long my_at;                    // lane i: element offset of row i (of the warp's 16), -1: none
 
   __device__ __forceinline__ void place(const PagedProblem& p, const Work& w, int row0) {
     const int pr = w.r0 + row0 + (threadIdx.x & 15);
-    my_at = pr < w.rows ? (long long)(w.q0 + pr / p.group) * p.q_stride +
-                              (long long)(w.kvh * p.group + pr % p.group) * p.hd
+    my_at = pr < w.rows ? (long long)(w.q0 + row_token(p, pr)) * p.q_stride +
+                              (long long)(w.kvh * p.group + row_head(p, pr)) * p.hd
                         : -1;
   }
   // the rows' 128-byte lines into L2 (a row's first and second half of the warp each take every other one)
@@ -351,7 +351,7 @@ struct QRows {
 #pragma unroll
         for (int o = CH / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
         const float s2 = pow2_to_2p13(mx), f = sgn * s2;       // exact: powers of two
-        if (c == 0) inv[row] = 1.0f / s2;
+        if (c == 0) inv[row] = pow2_inverse(s2);
         uint32_t hi[4], lo[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) split_pair(x[2 * e] * f, x[2 * e + 1] * f, hi[e], lo[e]);
@@ -442,7 +442,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
           w.off = t.off;
           w.kvn = t.kvn;
           w.k0 = 0;
-          w.k1 = seen(p, t, (min(w.rows, w.r0 + 2 * kRows) - 1) / p.group);
+          w.k1 = seen(p, t, row_token(p, min(w.rows, w.r0 + 2 * kRows) - 1));
           if (p.splits) {
             w.k0 = w.split * p.chunk;
             w.k1 = min(w.k1, w.k0 + p.chunk);
@@ -451,7 +451,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const int last = min(w.rows, w.r0 + (i + 1) * kRows) - 1;
-            const int e = last >= w.r0 + i * kRows ? min(w.k1, seen(p, t, last / p.group)) : 0;
+            const int e = last >= w.r0 + i * kRows ? min(w.k1, seen(p, t, row_token(p, last))) : 0;
             w.nt[i] = e > w.k0 ? (e - w.k0 + kKeys - 1) / kKeys : 0;
           }
         }
@@ -619,7 +619,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
       if (w.seq >= 0) {
         if (lane == 0) mbar_arrive(wempty + (n & 1));
         qr.place(p, w, row0);
-        qr.ask(p);
+        if (n) qr.ask(p);                                                // the first is fetched at once
       }
     };
     take(0);
@@ -642,9 +642,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
       }
       const int pr = w.r0 + i * kRows + r, nt = w.nt[i], k0 = w.k0;
       const bool live = pr < w.rows;
-      const int tok = w.q0 + pr / p.group, head = w.kvh * p.group + pr % p.group, seq = w.seq;
+      const int tok = w.q0 + row_token(p, pr), head = w.kvh * p.group + row_head(p, pr), seq = w.seq;
       const SeqTask st = {w.q0, 0, w.kvn, w.off, nullptr};
-      const int all = live ? seen(p, st, pr / p.group) : 0, lim = min(all, w.k1);   // keys this row sees, here
+      const int all = live ? seen(p, st, row_token(p, pr)) : 0, lim = min(all, w.k1);   // keys this row sees, here
       const long long slot = (long long)(p.slot0 + w.split) * p.total_q * p.heads + (long long)tok * p.heads + head;
       const float sc = fmaxf(fabsf(p.scale_log2) * inv_q, 1.2e-38f);   // not 0: a masked score is -inf * sc
       float m = -INFINITY, l = 0.0f;
@@ -803,7 +803,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
       auto flush = [&](int dim0, int bytes) {
         __syncwarp();
         const int c = lane & 7, dim = dim0 + c * (16 / es);
-#pragma unroll 1
+#pragma unroll 4
         for (int q = 0; q < 8; ++q) {
           const int row = q * 4 + (lane >> 3);
           const long long at = __shfl_sync(0xffffffffu, row_at, row);

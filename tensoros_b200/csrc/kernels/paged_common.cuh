@@ -20,6 +20,7 @@ struct PagedProblem {
   int type;                    // of q and out
   const void *k, *v;
   int kv_type, n_pages, page_size, n_kv, hd, heads, group;   // group = heads / n_kv
+  int gshift;                  // log2 of a group that is a power of two, else -1
   const int *table, *cu_q, *kv_len;
   int n_seqs, total_q, max_q, max_kv, table_stride;
   int fixed_kv;                // >= 0: every sequence's key count (prefix)
@@ -32,6 +33,12 @@ struct PagedProblem {
   float2* part_ml;             // [slot][total_q * heads]: running maximum (base 2), sum
   int* err;
 };
+
+// Token and head of packed row r; a division only where the group needs one.
+__device__ __forceinline__ int row_token(const PagedProblem& p, int r) { return p.gshift >= 0 ? r >> p.gshift : r / p.group; }
+__device__ __forceinline__ int row_head(const PagedProblem& p, int r) {
+  return p.gshift >= 0 ? r & (p.group - 1) : r % p.group;
+}
 
 struct SeqTask {
   int q0, qn, kvn, off;        // first token, tokens, keys; row r sees keys < off + r + 1 (causal) or kvn

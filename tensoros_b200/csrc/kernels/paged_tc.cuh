@@ -91,6 +91,10 @@ __device__ __forceinline__ float pow2_to_2p13(float m) {
   const int k = max(-126, min(126, 13 - (eb - 127)));
   return __uint_as_float((uint32_t)(k + 127) << 23);
 }
+// 1 / s of such a power of two (exponents -126 .. 126)
+__device__ __forceinline__ float pow2_inverse(float s) {
+  return __uint_as_float((254u << 23) - __float_as_uint(s));
+}
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
