@@ -409,9 +409,11 @@ PagedProblem problem_of(const tosk_paged_attn_t* a) {
   p.kv_type = a->kv.type; p.n_pages = a->kv.n_pages; p.page_size = a->kv.page_size;
   p.n_kv = a->kv.n_kv; p.hd = a->kv.hd;
   p.heads = a->n_heads; p.group = a->n_heads / a->kv.n_kv;
-  p.gshift = -1;
-  for (int i = 0; i < 31; ++i)
+  p.gshift = p.pshift = -1;
+  for (int i = 0; i < 31; ++i) {
     if (p.group == 1 << i) p.gshift = i;
+    if (p.page_size == 1 << i) p.pshift = i;
+  }
   p.table = a->kv.table; p.table_stride = a->kv.table_stride;
   p.cu_q = a->cu_q; p.kv_len = a->kv_len;
   p.n_seqs = a->n_seqs; p.total_q = a->total_q; p.max_q = a->max_q; p.max_kv = a->max_kv;
@@ -508,8 +510,27 @@ void part_views(PagedProblem& p, void* ws, int slots) {
   p.part_ml = reinterpret_cast<float2*>(reinterpret_cast<uint8_t*>(ws) + ((rows * p.hd * 4 + 15) & ~(size_t)15));
 }
 
-// Many rows a sequence: the tensor cores where the cache allows it.
-int run_tiles(const PagedProblem& p, cudaStream_t st) { return paged_tc_ok(p) ? paged_tc_run(p, st) : run_general(p, st); }
+// Which kernel takes a problem with several rows a sequence.  The few-rows
+// kernels start faster, but read each K/V row once for every 8 (16) rows; how
+// much of that they may do before the others are ahead is measured, in MB (one
+// sequence, us, others / few rows):
+//   fp32 cache     32 x 128: 67 MB 26.0 / 17.7, 268 MB 44.6 / 45.4
+//                   6 x 48:  75 MB 42.7 / 24.7, 302 MB 48.7 / 80.0
+//   fp16 cache      6 x 48:  38 MB 14.5 / 13.2, 151 MB 20.7 / 26.7
+//     fp32 rows    32 x 128:  8 MB 12.3 / 11.1,  34 MB 12.8 / 13.2, 134 MB 17.8 / 25.3
+//     fp16 rows    32 x 128:  1 MB  8.9 / 10.8
+bool few_rows(const PagedProblem& p) {
+  if (p.fixed_kv >= 0 || !paged_decode_ok(p)) return false;
+  const bool f16 = p.kv_type == TOSK_F16;
+  const long long mb = !f16 ? 150 : p.hd <= 64 ? 40 : p.type == TOSK_F32 ? 30 : 0;
+  // the tensor cores refuse what the few-rows kernel takes (odd pages, 256 dims): the general kernel is the other then
+  const long long most = (f16 && !paged_tc_ok(p) ? 150 : mb) * 1000000;
+  return (long long)p.total_q * p.heads / 8 * p.max_kv * p.hd * (f16 ? 4 : 8) <= most;
+}
+int run_tiles(const PagedProblem& p, cudaStream_t st) {
+  if (few_rows(p)) return paged_decode_run(p, 0, st);
+  return paged_tc_ok(p) ? paged_tc_run(p, st) : run_general(p, st);
+}
 
 // Splits of a prompt call's keys (0: none).  Fewer row tiles than SMs leave
 // SMs without work, so the keys are cut into the number of splits with the

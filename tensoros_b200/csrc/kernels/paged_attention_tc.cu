@@ -413,8 +413,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  pdl_wait();
-  pdl_trigger();
+  // The previous kernel is awaited by those who read or write memory; what
+  // may follow starts after that (the copy warp's word for the CTA).
 
   if (warp >= kCopyWarp) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTcRegsRest));
@@ -422,6 +422,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
       // ------------------------------------------------------------ the plan
       // The pieces, longest first, go round the CTAs there and back, which
       // evens out the CTAs' sums.
+      if (p.fixed_kv < 0) pdl_wait();                  // a prefix is planned from the arguments alone
       bool ok = true, more = true;
       int posted = 0;
       const int splits = p.splits ? p.splits : 1;
@@ -465,6 +466,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
       }
     } else if (warp == kCopyWarp) {
       // ---------------------------------------------------------- K, V tiles
+      pdl_wait();
+      pdl_trigger();
       bool ok = true;
       int used = 0, tails = 0;                        // slots filled; tiles cut off by the key range
       for (int n = 0; ok; ++n) {
@@ -608,6 +611,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
     uint8_t* stage = (T::kStage ? ring + T::kSlots * T::kTile + i * 32768 : q_tile) + (hf * 4 + wq) * 4096;
     bool ok = true;     // a wait that ran out: no more waiting, and all warps of the row tile leave together
     int cnt = 0;                                                        // key tiles so far
+    pdl_wait();
     QRows<HD, SPLIT> qr;
     Work w;
     // the n-th piece of work, and its Q rows on their way to L2

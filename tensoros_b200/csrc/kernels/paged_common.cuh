@@ -20,7 +20,7 @@ struct PagedProblem {
   int type;                    // of q and out
   const void *k, *v;
   int kv_type, n_pages, page_size, n_kv, hd, heads, group;   // group = heads / n_kv
-  int gshift;                  // log2 of a group that is a power of two, else -1
+  int gshift, pshift;          // log2 of a group, a page size that is a power of two, else -1
   const int *table, *cu_q, *kv_len;
   int n_seqs, total_q, max_q, max_kv, table_stride;
   int fixed_kv;                // >= 0: every sequence's key count (prefix)

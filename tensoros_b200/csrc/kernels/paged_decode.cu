@@ -28,11 +28,14 @@ namespace tos {
 constexpr int kDecWarps = 4;
 constexpr int kStep = 16;             // keys a warp step
 
-template <int HD>
+// DEEP: three stages a warp (of 128 dims) and two CTAs an SM, for many keys a
+// CTA; else two stages and three CTAs, which start and end beside one another.
+// (64 sequences of ~256 keys: 47.0 us deep, 41.6 not; 16 of ~2000: 92.8, 96.7.)
+template <int HD, bool DEEP>
 struct DecShape {
   static constexpr int kRow = HD * 2;                            // bytes of a key row in shared memory
   static constexpr int kStage = 2 * kStep * kRow;                // K and V
-  static constexpr int kDepth = HD == 64 ? 6 : 3;
+  static constexpr int kDepth = (HD == 64 ? 2 : 1) * (DEEP || HD == 256 ? 3 : 2);
   static constexpr int kSmem = kDecWarps * kDepth * kStage;
 };
 
@@ -58,15 +61,65 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ int page_of(const PagedProblem& p, int key) {
+  return p.pshift >= 0 ? key >> p.pshift : key / p.page_size;
+}
+// Element offset of a key's row, -1 where its page is none.
+__device__ __forceinline__ long long row_at(const PagedProblem& p, int key, int page, int kvh) {
+  if (page < 0 || page >= p.n_pages) return -1;
+  const int r = p.pshift >= 0 ? key & (p.page_size - 1) : key % p.page_size;
+  return (((long long)page * p.page_size + r) * p.n_kv + kvh) * p.hd;
+}
+
+// K and V rows of the KEYS keys from `first` on into a stage: rows of `rowb`
+// bytes (CH 16-byte pieces, `chs` of them in use, `es` elements each), piece c
+// of row k at c ^ (k & 7); V `voff` bytes behind K.  whole: the keys lie in one
+// page (`page`), else lane k holds key k's.
+template <int KEYS, int CH, typename E>
+__device__ __forceinline__ void copy_step(const PagedProblem& p, int whole, int first, int end, int page, int kvh, int chs,
+                                          int es, uint32_t dst, uint32_t voff, uint32_t rowb, const E* kb, const E* vb) {
+  constexpr int RPI = 32 / CH > 0 ? 32 / CH : 1;                 // rows an instruction (CH 64: half a row)
+  const int lane = threadIdx.x & 31;
+  if (whole) {
+    const long long row = row_at(p, first, page, kvh);
+    const long long step = (long long)p.n_kv * p.hd;
+    const int key0 = lane / CH;
+    long long off = row + key0 * step + (lane % CH) * es;
+#pragma unroll
+    for (int i = 0; i < KEYS * CH / 32; ++i) {
+      const int idx = i * 32 + lane, key = idx / CH, c = idx % CH;
+      const bool have = row >= 0 && c < chs && first + key < end;
+      const long long o = have ? (CH <= 32 ? off + i * RPI * step : row + key * step + c * es) : 0;
+      const uint32_t d = dst + key * rowb + ((c ^ (key & 7)) << 4);
+      cp16(d, kb + o, have);
+      cp16(d + voff, vb + o, have);
+    }
+  } else {
+    const long long row = row_at(p, first + lane, page, kvh);    // lanes < KEYS; -1 behind the end
+#pragma unroll
+    for (int i = 0; i < KEYS * CH / 32; ++i) {
+      const int idx = i * 32 + lane, key = idx / CH, c = idx % CH;
+      const long long off = __shfl_sync(0xffffffffu, row, key);
+      const bool have = off >= 0 && c < chs;
+      const long long o = have ? off + c * es : 0;
+      const uint32_t d = dst + key * rowb + ((c ^ (key & 7)) << 4);
+      cp16(d, kb + o, have);
+      cp16(d + voff, vb + o, have);
+    }
+  }
+}
+
 struct DecArgs {
   PagedProblem p;
-  int qblocks;             // blocks of 8 * NQ query heads of a group
+  int rtiles;              // row tiles of the longest sequence
+  int q_vec;               // pairs of q elements are aligned
+  int whole;               // a page holds whole steps
   int late_wait;           // 1: runs beside the prefix kernel, whose end it awaits at its own end
 };
 
-template <int HD, int NQ>
+template <int HD, int NQ, bool DEEP>
 __global__ void __launch_bounds__(32 * kDecWarps) paged_decode_kernel(const __grid_constant__ DecArgs a) {
-  using T = DecShape<HD>;
+  using T = DecShape<HD, DEEP>;
   extern __shared__ __align__(128) uint8_t sm[];
   const PagedProblem& p = a.p;
   if (!a.late_wait) {
@@ -75,77 +128,80 @@ __global__ void __launch_bounds__(32 * kDecWarps) paged_decode_kernel(const __gr
   }
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
   int b = blockIdx.x;
-  const int qb = b % a.qblocks;
-  b /= a.qblocks;
   const int kvh = b % p.n_kv;
   b /= p.n_kv;
-  const int splits = p.splits ? p.splits : 1, split = b % splits, seq = b / splits;
+  const int splits = p.splits ? p.splits : 1, split = b % splits;
+  b /= splits;
+  const int seq = b % p.n_seqs, r0 = (a.rtiles - 1 - b / p.n_seqs) * 8 * NQ;   // long rows first
   const SeqTask t = seq_task(p, seq);
-  int k0 = 0, k1 = t.kvn;
+  const int nr = min(8 * NQ, t.qn * p.group - r0);                 // rows of this tile
+  int k0 = 0, k1 = nr > 0 ? seen(p, t, row_token(p, r0 + nr - 1)) : 0;
   if (p.splits) {
     k0 = split * p.chunk;
     k1 = min(k1, k0 + p.chunk);
   }
-  const int h0 = kvh * p.group + qb * 8 * NQ;                    // first query head
-  const int nh = min(8 * NQ, p.group - qb * 8 * NQ);
-  if (k0 < k1 || !p.splits) {
+  if (nr > 0 && (k0 < k1 || !p.splits)) {
     const int steps = (k1 - k0 + kStep - 1) / kStep;
     const uint32_t ring = smem_u32(sm) + warp * T::kDepth * T::kStage;
     const __half* kb = reinterpret_cast<const __half*>(p.k);
     const __half* vb = reinterpret_cast<const __half*>(p.v);
     constexpr int CH = HD / 8;                                   // 16-byte pieces of a row
     const int chs = p.hd / 8;
-    // Row offset of key (step, lane): lanes 0..15 hold one each
-    auto fetch_row = [&](int st) -> long long {
-      const int key = k0 + st * kStep + (lane & 15);
-      return st < steps && key < k1 ? kv_off(p, t.table, key, kvh) : -1;
+    // The page of a step (or, where pages are no multiple of a step, of key
+    // `lane` of it).  The entry is not looked at until the step's copies are
+    // issued, so that its load is not waited for a step ahead.
+    auto fetch_page = [&](int st) {
+      const int key = k0 + st * kStep + (a.whole ? 0 : lane & 15);
+      return st < steps && key < k1 ? t.table[page_of(p, key)] : -1;
     };
-    auto issue = [&](int st, long long row) {
+    auto issue = [&](int st, int page) {
       if (st < steps) {
         const uint32_t dst = ring + (st / kDecWarps % T::kDepth) * T::kStage;
-#pragma unroll
-        for (int i = 0; i < kStep * CH / 32; ++i) {
-          const int idx = i * 32 + lane, key = idx / CH, c = idx % CH;
-          const long long off = __shfl_sync(0xffffffffu, row, key);
-          const bool have = off >= 0 && c < chs;
-          const long long o = have ? off + 8 * c : 0;
-          const uint32_t d = dst + key * T::kRow + ((c ^ (key & 7)) << 4);
-          cp16(d, kb + o, have);
-          cp16(d + kStep * T::kRow, vb + o, have);
-        }
+        const int first = k0 + st * kStep;
+        copy_step<kStep, CH>(p, a.whole, first, k1, page, kvh, chs, 8, dst, kStep * T::kRow, T::kRow, kb, vb);
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
     // the ring's first stages, then the queries while they fly
-    long long rows[T::kDepth];
+    int pages[T::kDepth];
 #pragma unroll
-    for (int d = 0; d < T::kDepth; ++d) rows[d] = fetch_row(warp + d * kDecWarps);
+    for (int d = 0; d < T::kDepth; ++d) pages[d] = fetch_page(warp + d * kDecWarps);
 #pragma unroll
-    for (int d = 0; d < T::kDepth - 1; ++d) issue(warp + d * kDecWarps, rows[d]);
-    long long nrow = rows[T::kDepth - 1];
+    for (int d = 0; d < T::kDepth - 1; ++d) issue(warp + d * kDecWarps, pages[d]);
+    int npage = pages[T::kDepth - 1];
 
     uint32_t qa[NQ][HD / 16][4];
     float sc[NQ], m[NQ], l[NQ], o[NQ][HD / 8][4];
+    int lim[NQ];                                                  // keys that this lane's row sees
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
-      const int h = n * 8 + g;                                    // this lane's query
-      const bool live = h < nh;
-      const long long qo = (long long)t.q0 * p.q_stride + (long long)(h0 + (live ? h : 0)) * p.hd;
+      const int r = n * 8 + g, row = r0 + (r < nr ? r : 0);       // this lane's row
+      const bool live = r < nr;
+      lim[n] = live ? min(k1, seen(p, t, row_token(p, row))) : 0;
+      const long long qo = (long long)(t.q0 + row_token(p, row)) * p.q_stride +
+                           (long long)(kvh * p.group + row_head(p, row)) * p.hd;
       float x[HD / 16][4];
       float mx = 0.0f;
 #pragma unroll
       for (int k = 0; k < HD / 16; ++k)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int d = 16 * k + 2 * t4 + (e & 1) + 8 * (e >> 1);
-          x[k][e] = live && d < p.hd ? load_elem(p.q, p.type, qo + d) : 0.0f;
-          mx = fmaxf(mx, fabsf(x[k][e]));
+        for (int e = 0; e < 4; e += 2) {
+          const int d = 16 * k + 2 * t4 + 8 * (e >> 1);           // hd is a multiple of 8
+          float2 f = make_float2(0.0f, 0.0f);
+          if (live && d < p.hd) {
+            if (!a.q_vec) f = make_float2(load_elem(p.q, p.type, qo + d), load_elem(p.q, p.type, qo + d + 1));
+            else if (p.type == TOSK_F32) f = *reinterpret_cast<const float2*>(reinterpret_cast<const float*>(p.q) + qo + d);
+            else f = __half22float2(*reinterpret_cast<const __half2*>(reinterpret_cast<const __half*>(p.q) + qo + d));
+          }
+          x[k][e] = f.x;
+          x[k][e + 1] = f.y;
+          mx = fmaxf(mx, fmaxf(fabsf(f.x), fabsf(f.y)));
         }
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
       const float s2 = pow2_to_2p13(mx);                          // exact scaling of the row
       const float sg = p.scale_log2 < 0.0f ? -s2 : s2;
-      sc[n] = fmaxf(fabsf(p.scale_log2) * (1.0f / s2), 1.2e-38f);  // not 0: a masked score is -inf * sc
+      sc[n] = fmaxf(fabsf(p.scale_log2) * pow2_inverse(s2), 1.2e-38f);  // not 0: a masked score is -inf * sc
 #pragma unroll
       for (int k = 0; k < HD / 16; ++k) {
         split_pair(x[k][0] * sg, x[k][1] * sg, qa[n][k][0], qa[n][k][1]);
@@ -164,8 +220,8 @@ __global__ void __launch_bounds__(32 * kDecWarps) paged_decode_kernel(const __gr
     const int vrow = lane & 15, vch = lane >> 4;
 
     for (int st = warp; st < steps; st += kDecWarps) {
-      issue(st + (T::kDepth - 1) * kDecWarps, nrow);
-      nrow = fetch_row(st + T::kDepth * kDecWarps);
+      issue(st + (T::kDepth - 1) * kDecWarps, npage);
+      npage = fetch_page(st + T::kDepth * kDecWarps);
       asm volatile("cp.async.wait_group %0;" ::"n"(T::kDepth - 1) : "memory");
       __syncwarp();
       const uint32_t kbase = ring + (st / kDecWarps % T::kDepth) * T::kStage, vbase = kbase + kStep * T::kRow;
@@ -186,10 +242,10 @@ __global__ void __launch_bounds__(32 * kDecWarps) paged_decode_kernel(const __gr
           mma16816(s[n][1], qa[n][k], bk[2], bk[3]);
         }
       }
-      const int left = k1 - (k0 + st * kStep);                    // keys of the step that count
       uint32_t pa[NQ][4];
 #pragma unroll
       for (int n = 0; n < NQ; ++n) {
+        const int left = lim[n] - (k0 + st * kStep);              // keys of the step that the row sees
         float w[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -244,27 +300,31 @@ __global__ void __launch_bounds__(32 * kDecWarps) paged_decode_kernel(const __gr
     }
     __syncthreads();
     // a warp a query
-    for (int h = warp; h < nh; h += kDecWarps) {
+    for (int r = warp; r < nr; r += kDecWarps) {
       float M = -INFINITY, L = 0.0f, f[kDecWarps];
 #pragma unroll
-      for (int w = 0; w < kDecWarps; ++w) M = fmaxf(M, sml[w][h].x);
+      for (int w = 0; w < kDecWarps; ++w) M = fmaxf(M, sml[w][r].x);
 #pragma unroll
       for (int w = 0; w < kDecWarps; ++w) {
-        f[w] = M == -INFINITY ? 0.0f : exp2f(sml[w][h].x - M);
-        L += f[w] * sml[w][h].y;
+        f[w] = M == -INFINITY ? 0.0f : exp2f(sml[w][r].x - M);
+        L += f[w] * sml[w][r].y;
       }
-      const int head = h0 + h;
-      const long long part = (long long)(p.slot0 + split) * p.total_q * p.heads + (long long)t.q0 * p.heads + head;
-      const long long oo = (long long)t.q0 * p.out_stride + (long long)head * p.hd;
+      const int tok = t.q0 + row_token(p, r0 + r), head = kvh * p.group + row_head(p, r0 + r);
+      const long long part = (long long)(p.slot0 + split) * p.total_q * p.heads + (long long)tok * p.heads + head;
+      const long long oo = (long long)tok * p.out_stride + (long long)head * p.hd;
       const float inv = p.splits ? 1.0f : L == 0.0f ? 0.0f : 1.0f / L;
       if (p.splits && lane == 0) p.part_ml[part] = make_float2(M, L);
+      bool bad = false;
       for (int d = lane; d < p.hd; d += 32) {
         float v = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kDecWarps; ++w) v = fmaf(f[w], so[(w * NQ * 8 + h) * HD + d], v);
+        for (int w = 0; w < kDecWarps; ++w) v = fmaf(f[w], so[(w * NQ * 8 + r) * HD + d], v);
         if (p.splits) p.part_o[part * p.hd + d] = v;
         else store_elem(p.out, p.type, oo + d, L == 0.0f ? 0.0f : v * inv);
+        bad |= isnan(v);
       }
+      if (!p.splits && __any_sync(0xffffffffu, bad) && L != 0.0f)
+        attn_row_plain(p, nullptr, 0, t.table, seen(p, t, row_token(p, r0 + r)), tok, head);
     }
   }
   if (a.late_wait) {
@@ -304,19 +364,19 @@ __global__ void __launch_bounds__(32 * kDecWarps) paged_decode_f32_kernel(const 
   }
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   int b = blockIdx.x;
-  const int qb = b % a.qblocks;
-  b /= a.qblocks;
   const int kvh = b % p.n_kv;
   b /= p.n_kv;
-  const int splits = p.splits ? p.splits : 1, split = b % splits, seq = b / splits;
+  const int splits = p.splits ? p.splits : 1, split = b % splits;
+  b /= splits;
+  const int seq = b % p.n_seqs, r0 = (a.rtiles - 1 - b / p.n_seqs) * Q;   // long rows first
   const SeqTask t = seq_task(p, seq);
-  int k0 = 0, k1 = t.kvn;
+  const int nr = min(Q, t.qn * p.group - r0);                 // rows of this tile
+  int k0 = 0, k1 = nr > 0 ? seen(p, t, row_token(p, r0 + nr - 1)) : 0;
   if (p.splits) {
     k0 = split * p.chunk;
     k1 = min(k1, k0 + p.chunk);
   }
-  const int h0 = kvh * p.group + qb * Q, nh = min(Q, p.group - qb * Q);
-  if (k0 < k1 || !p.splits) {
+  if (nr > 0 && (k0 < k1 || !p.splits)) {
     const int steps = (k1 - k0 + KS - 1) / KS;
     const uint8_t* ringp = sm + warp * T::kDepth * T::kStage;
     const uint32_t ring = smem_u32(ringp);
@@ -325,50 +385,45 @@ __global__ void __launch_bounds__(32 * kDecWarps) paged_decode_f32_kernel(const 
     const float* kb = reinterpret_cast<const float*>(p.k);
     const float* vb = reinterpret_cast<const float*>(p.v);
     const int chs = p.hd / 4;
-    auto fetch_row = [&](int st) -> long long {
-      const int key = k0 + st * KS + (lane & 7);
-      return st < steps && key < k1 ? kv_off(p, t.table, key, kvh) : -1;
+    auto fetch_page = [&](int st) {
+      const int key = k0 + st * KS + (a.whole ? 0 : lane & 7);
+      return st < steps && key < k1 ? t.table[page_of(p, key)] : -1;
     };
-    auto issue = [&](int st, long long row) {
+    auto issue = [&](int st, int page) {
       if (st < steps) {
         const uint32_t dst = ring + (st / kDecWarps % T::kDepth) * T::kStage;
-#pragma unroll
-        for (int i = 0; i < KS * CH / 32; ++i) {
-          const int idx = i * 32 + lane, key = idx / CH, c = idx % CH;
-          const long long off = __shfl_sync(0xffffffffu, row, key);
-          const bool have = off >= 0 && c < chs;
-          const long long o = have ? off + 4 * c : 0;
-          const uint32_t d = dst + key * T::kRow + ((c ^ (key & 7)) << 4);
-          cp16(d, kb + o, have);
-          cp16(d + KS * T::kRow, vb + o, have);
-        }
+        copy_step<KS, CH>(p, a.whole, k0 + st * KS, k1, page, kvh, chs, 4, dst, KS * T::kRow, T::kRow, kb, vb);
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    long long rows[T::kDepth];
+    int pages[T::kDepth];
 #pragma unroll
-    for (int d = 0; d < T::kDepth; ++d) rows[d] = fetch_row(warp + d * kDecWarps);
+    for (int d = 0; d < T::kDepth; ++d) pages[d] = fetch_page(warp + d * kDecWarps);
 #pragma unroll
-    for (int d = 0; d < T::kDepth - 1; ++d) issue(warp + d * kDecWarps, rows[d]);
-    long long nrow = rows[T::kDepth - 1];
+    for (int d = 0; d < T::kDepth - 1; ++d) issue(warp + d * kDecWarps, pages[d]);
+    int npage = pages[T::kDepth - 1];
     for (int i = tid; i < Q * HD; i += 32 * kDecWarps) {
-      const int h = i / HD, d = i % HD;
-      sq[i] = h < nh && d < p.hd ? load_elem(p.q, p.type, (long long)t.q0 * p.q_stride + (long long)(h0 + h) * p.hd + d) : 0.0f;
+      const int r = i / HD, d = i % HD;
+      sq[i] = r < nr && d < p.hd ? load_elem(p.q, p.type, (long long)(t.q0 + row_token(p, r0 + r)) * p.q_stride +
+                                                              (long long)(kvh * p.group + row_head(p, r0 + r)) * p.hd + d)
+                                 : 0.0f;
     }
     __syncthreads();
     float m[Q], l[Q];
+    int lim[Q];                                                   // keys that the rows see
     float2 o[Q][NC][2];
 #pragma unroll
     for (int n = 0; n < Q; ++n) {
       m[n] = -INFINITY;
       l[n] = 0.0f;
+      lim[n] = n < nr ? min(k1, seen(p, t, row_token(p, r0 + n))) : 0;
 #pragma unroll
       for (int c = 0; c < NC; ++c) o[n][c][0] = o[n][c][1] = make_float2(0.0f, 0.0f);
     }
     const int key = lane & 7, quarter = lane >> 3;
     for (int st = warp; st < steps; st += kDecWarps) {
-      issue(st + (T::kDepth - 1) * kDecWarps, nrow);
-      nrow = fetch_row(st + T::kDepth * kDecWarps);
+      issue(st + (T::kDepth - 1) * kDecWarps, npage);
+      npage = fetch_page(st + T::kDepth * kDecWarps);
       asm volatile("cp.async.wait_group %0;" ::"n"(T::kDepth - 1) : "memory");
       __syncwarp();
       const uint8_t* ks = ringp + (st / kDecWarps % T::kDepth) * T::kStage;
@@ -387,18 +442,25 @@ __global__ void __launch_bounds__(32 * kDecWarps) paged_decode_f32_kernel(const 
           s[n] = __ffma2_rn(make_float2(qx.z, qx.w), make_float2(kx.z, kx.w), s[n]);
         }
       }
-      const bool counts = key < k1 - (k0 + st * KS);
+      float x[Q];
+      bool grown = false;
+#pragma unroll
+      for (int n = 0; n < Q; ++n) x[n] = s[n].x + s[n].y;
+#pragma unroll
+      for (int n = 0; n < Q; ++n) x[n] += __shfl_xor_sync(0xffffffffu, x[n], 8);
 #pragma unroll
       for (int n = 0; n < Q; ++n) {
-        float x = s[n].x + s[n].y;
-        x += __shfl_xor_sync(0xffffffffu, x, 8);
-        x += __shfl_xor_sync(0xffffffffu, x, 16);
-        x = counts ? x * p.scale_log2 : -INFINITY;
-        if (__any_sync(0xffffffffu, x > m[n] + 8.0f)) {
-          float top = x;
+        x[n] += __shfl_xor_sync(0xffffffffu, x[n], 16);
+        x[n] = k0 + st * KS + key < lim[n] ? x[n] * p.scale_log2 : -INFINITY;
+        grown |= x[n] > m[n] + 8.0f;
+      }
+      if (__any_sync(0xffffffffu, grown)) {
+#pragma unroll
+        for (int n = 0; n < Q; ++n) {
+          float top = x[n];
 #pragma unroll
           for (int w = 4; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-          const float mn = fmaxf(m[n], top), f = exp2f(m[n] - mn);   // 0 on the first keys
+          const float mn = fmaxf(m[n], top), f = mn == m[n] ? 1.0f : exp2f(m[n] - mn);   // 0 on the first keys
           m[n] = mn;
           l[n] *= f;
 #pragma unroll
@@ -406,7 +468,10 @@ __global__ void __launch_bounds__(32 * kDecWarps) paged_decode_f32_kernel(const 
 #pragma unroll
             for (int e = 0; e < 2; ++e) o[n][c][e] = __fmul2_rn(o[n][c][e], make_float2(f, f));
         }
-        const float w = ex2(x - (m[n] == -INFINITY ? 0.0f : m[n]));
+      }
+#pragma unroll
+      for (int n = 0; n < Q; ++n) {
+        const float w = ex2(x[n] - (m[n] == -INFINITY ? 0.0f : m[n]));
         l[n] += w;
         if (quarter == (n & 3)) sp[key * Q + n] = w;
       }
@@ -453,27 +518,31 @@ __global__ void __launch_bounds__(32 * kDecWarps) paged_decode_f32_kernel(const 
       }
     }
     __syncthreads();
-    for (int h = warp; h < nh; h += kDecWarps) {
+    for (int r = warp; r < nr; r += kDecWarps) {
       float M = -INFINITY, L = 0.0f, f[kDecWarps];
 #pragma unroll
-      for (int w = 0; w < kDecWarps; ++w) M = fmaxf(M, sml[w][h].x);
+      for (int w = 0; w < kDecWarps; ++w) M = fmaxf(M, sml[w][r].x);
 #pragma unroll
       for (int w = 0; w < kDecWarps; ++w) {
-        f[w] = M == -INFINITY ? 0.0f : exp2f(sml[w][h].x - M);
-        L += f[w] * sml[w][h].y;
+        f[w] = M == -INFINITY ? 0.0f : exp2f(sml[w][r].x - M);
+        L += f[w] * sml[w][r].y;
       }
-      const int head = h0 + h;
-      const long long part = (long long)(p.slot0 + split) * p.total_q * p.heads + (long long)t.q0 * p.heads + head;
-      const long long oo = (long long)t.q0 * p.out_stride + (long long)head * p.hd;
+      const int tok = t.q0 + row_token(p, r0 + r), head = kvh * p.group + row_head(p, r0 + r);
+      const long long part = (long long)(p.slot0 + split) * p.total_q * p.heads + (long long)tok * p.heads + head;
+      const long long oo = (long long)tok * p.out_stride + (long long)head * p.hd;
       const float inv = p.splits ? 1.0f : L == 0.0f ? 0.0f : 1.0f / L;
       if (p.splits && lane == 0) p.part_ml[part] = make_float2(M, L);
+      bool bad = false;
       for (int d = lane; d < p.hd; d += 32) {
         float v = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kDecWarps; ++w) v = fmaf(f[w], so[(w * Q + h) * HD + d], v);
+        for (int w = 0; w < kDecWarps; ++w) v = fmaf(f[w], so[(w * Q + r) * HD + d], v);
         if (p.splits) p.part_o[part * p.hd + d] = v;
         else store_elem(p.out, p.type, oo + d, L == 0.0f ? 0.0f : v * inv);
+        bad |= isnan(v);
       }
+      if (!p.splits && __any_sync(0xffffffffu, bad) && L != 0.0f)
+        attn_row_plain(p, nullptr, 0, t.table, seen(p, t, row_token(p, r0 + r)), tok, head);
     }
   }
   if (a.late_wait) {
@@ -504,11 +573,11 @@ int dec_launch(const void* f, int smem, const DecArgs& a, unsigned grid, cudaStr
   return (int)cudaLaunchKernelExC(&cfg, f, args);
 }
 
-template <int HD>
+template <int HD, bool DEEP>
 int dec16(const DecArgs& a, int nq, unsigned n, cudaStream_t st) {
   if constexpr (HD <= 128)
-    if (nq == 2) return dec_launch((const void*)paged_decode_kernel<HD, 2>, DecShape<HD>::kSmem, a, n, st);
-  return dec_launch((const void*)paged_decode_kernel<HD, 1>, DecShape<HD>::kSmem, a, n, st);
+    if (nq == 2) return dec_launch((const void*)paged_decode_kernel<HD, 2, DEEP>, DecShape<HD, DEEP>::kSmem, a, n, st);
+  return dec_launch((const void*)paged_decode_kernel<HD, 1, DEEP>, DecShape<HD, DEEP>::kSmem, a, n, st);
 }
 
 template <int HD>
@@ -526,21 +595,28 @@ bool paged_decode_ok(const PagedProblem& p) {
   return p.hd % (p.kv_type == TOSK_F16 ? 8 : 4) == 0 && ((uintptr_t)p.k & 15) == 0 && ((uintptr_t)p.v & 15) == 0;
 }
 
-// One token a sequence.  fp16: groups of up to 8 query heads in one block of
-// 8, larger ones in blocks of 16 (256 dims: of 8, for the registers).  fp32:
-// blocks of 1, 4 or 8, the smallest that holds the group.
+// Few rows a sequence (single tokens, short prompts).  fp16: row tiles of 16
+// where a sequence has more than 8 rows (256 dims: of 8, for the registers),
+// else of 8.  fp32: of 1, 4 or 8, the smallest that holds the rows.
 int paged_decode_run(const PagedProblem& p, int late_wait, cudaStream_t st) {
   DecArgs a;
   a.p = p;
   a.late_wait = late_wait;
   const bool f16 = p.kv_type == TOSK_F16;
-  const int nq = p.group > 8 && p.hd <= 128 ? 2 : 1;
-  const int block = f16 ? 8 * nq : p.group == 1 ? 1 : p.group <= 4 ? 4 : 8;
-  a.qblocks = (p.group + block - 1) / block;
-  const long long grid = (long long)a.qblocks * p.n_kv * (p.splits ? p.splits : 1) * p.n_seqs;
+  const long long rows = (long long)p.max_q * p.group;
+  const int nq = rows > 8 && p.hd <= 128 ? 2 : 1;
+  const int block = f16 ? 8 * nq : rows == 1 ? 1 : rows <= 4 ? 4 : 8;
+  const long long rt = (rows + block - 1) / block;
+  const long long grid = rt * p.n_kv * (p.splits ? p.splits : 1) * p.n_seqs;
   if (grid > 0x7fffffffll) return (int)cudaErrorInvalidValue;
+  a.rtiles = (int)rt;
+  a.whole = p.page_size % (f16 ? kStep : 8) == 0;
+  a.q_vec = ((uintptr_t)p.q & (p.type == TOSK_F32 ? 7 : 3)) == 0 && p.q_stride % 2 == 0;
   const unsigned n = (unsigned)grid;
-  if (f16) return p.hd <= 64 ? dec16<64>(a, nq, n, st) : p.hd <= 128 ? dec16<128>(a, nq, n, st) : dec16<256>(a, nq, n, st);
+  const bool deep = (p.splits ? p.chunk : p.max_kv) > 1024;
+  if (f16 && p.hd <= 64) return deep ? dec16<64, true>(a, nq, n, st) : dec16<64, false>(a, nq, n, st);
+  if (f16 && p.hd <= 128) return deep ? dec16<128, true>(a, nq, n, st) : dec16<128, false>(a, nq, n, st);
+  if (f16) return dec16<256, true>(a, nq, n, st);
   return p.hd <= 64 ? dec32<64>(a, block, n, st) : p.hd <= 128 ? dec32<128>(a, block, n, st) : dec32<256>(a, block, n, st);
 }
 

@@ -442,3 +442,101 @@ def test_two_streams_at_once(gpu):
                 outs.append(R.decode(gpu, c, q, c.lens, heads, 0.1)[0])
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(alone, outs))
+
+
+# ------------------------------------- large enough for the tiled kernels
+# (the few-rows kernels take the small calls above: 8 query rows at a time)
+
+@pytest.mark.parametrize("qk,kv", KINDS)
+@pytest.mark.parametrize("heads,n_kv,hd,page,q_lens,hist", [
+    (8, 2, 128, 16, [700, 1, 129], [0, 300, 513]),          # groups of 4: row tiles end inside a token
+    (6, 2, 128, 64, [513, 0, 300], [200, 7, 0]),            # groups of 3
+    (16, 4, 64, 8, [1200, 33], [0, 900]),
+    (12, 12, 48, 32, [900, 517], [0, 7]),
+    (24, 4, 32, 128, [1100, 700], [100, 0]),
+    (16, 2, 96, 256, [600, 31, 1], [0, 511, 1000]),
+    (8, 8, 80, 48, [700], [31]),                            # pages of 48: no tensor-core tiles
+    (4, 2, 200, 16, [500], [0]),
+    (40, 1, 128, 16, [90, 2], [700, 3000]),                 # few row tiles, many keys: the key axis is split
+    (8, 8, 128, 32, [40] * 50, [3 * i for i in range(50)]),  # more sequences than lanes of the plan
+])
+def test_prompt_attention_tiles(gpu, qk, kv, heads, n_kv, hd, page, q_lens, hist):
+    kv_lens = [a + b for a, b in zip(q_lens, hist)]
+    c = Cache(kv_lens, page, n_kv, hd, kv, seed=hd + page)
+    q = randn(sum(q_lens) + 2, heads, hd, seed=17, kind=qk) * 1.5
+    R.check_prompt(gpu, c, q, q_lens, kv_lens, heads)
+
+
+@pytest.mark.parametrize("qk,kv", [(F32, F16), (F16, F16), (F32, F32)])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_tiles_rows_that_see_nothing_and_negative_scale(gpu, qk, kv, hd):
+    q_lens, kv_lens = [900, 300, 40, 512], [700, 0, 40, 511]
+    c = Cache(kv_lens, 16, 4, hd, kv, seed=1)
+    q = randn(sum(q_lens), 16, hd, seed=2, kind=qk)
+    out = R.check_prompt(gpu, c, q, q_lens, kv_lens, 16, scale=-0.2)
+    assert bool((out[:200] == 0).all()) and bool((out[900:1200] == 0).all()) and bool((out[1240] == 0).all())
+    R.check_prompt(gpu, c, q, q_lens, kv_lens, 16, scale=0.0)
+
+
+@pytest.mark.parametrize("qk,kv", [(F32, F16), (F16, F16), (F32, F32)])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("n,hist", [(900, 0), (60, 3000)])
+def test_tiles_unseen_values_do_not_reach_a_row(gpu, qk, kv, hd, n, hist):
+    """As above, over many tiles, and with the keys split."""
+    heads = 16
+    c = Cache([n + hist], 16, 2, hd, kv, seed=5)
+    q = randn(n, heads, hd, seed=6, kind=qk)
+    clean, st = R.prompt(gpu, c, q, [n], [n + hist], heads, hd ** -0.5)
+    assert st == 0
+    pg, r = c.where(c.table[0], n + hist)
+    at, at_k = hist + n // 2, hist + n - 7
+    c.v[pg[at], r[at], 0, 3] = float("inf")
+    c.k[pg[at_k], r[at_k], 1, 7] = float("nan")
+    out, st = R.prompt(gpu, c, q, [n], [n + hist], heads, hd ** -0.5)
+    assert st == 0
+    half = heads // 2
+    assert torch.isfinite(out[:n // 2]).all()
+    assert float((out[:n // 2].double() - clean[:n // 2].double()).abs().max()) < 8 * (2.0 ** -10 if qk == F16 else 1e-5)
+    assert not torch.isfinite(out[n // 2:, :half, 3]).any()
+    assert torch.isnan(out[n - 7:, half:]).all() and torch.isfinite(out[:n - 7, half:]).all()
+
+
+@pytest.mark.parametrize("qk,kv", [(F32, F16), (F16, F16), (F32, F32)])
+def test_tiles_scores_far_apart(gpu, qk, kv):
+    """The running maximum moves in every key tile, up and (reversed) not."""
+    n, heads, hd = 1000, 8, 128
+    c = Cache([n], 16, 2, hd, kv, seed=8)
+    q = randn(n, heads, hd, seed=9, kind=qk)
+    ramp = torch.linspace(0.2, 12.0, n, device="cuda")
+    pg, r = c.where(c.table[0], n)
+    c.k[pg, r] = (c.k[pg, r].float() * ramp[:, None, None]).to(R.DT[kv])
+    R.check_prompt(gpu, c, q, [n], [n], heads)
+    c.k[pg, r] = c.k[pg, r].flip(0)
+    R.check_prompt(gpu, c, q, [n], [n], heads)
+    q[::3] *= 1e-4 if qk == F32 else 1.0          # small rows keep their 22 bits
+    R.check_prompt(gpu, c, q, [n], [n], heads, scale=30.0 if qk == F32 else 0.1)
+
+
+@pytest.mark.parametrize("qk,kv", [(F32, F16), (F16, F16)])
+def test_tiles_unaligned_rows(gpu, qk, kv):
+    """q and out at odd strides from odd elements."""
+    n, heads, hd = 600, 8, 128
+    c = Cache([n], 16, 2, hd, kv, seed=3)
+    w = heads * hd + 3
+    buf, obuf = randn(n * w + 8, seed=4, kind=qk), torch.full((n * w + 8,), 7.0, dtype=R.DT[qk], device="cuda")
+    q = torch.as_strided(buf, (n, heads, hd), (w, hd, 1), 1)
+    out = torch.as_strided(obuf, (n, heads, hd), (w, hd, 1), 5)
+    got, st = R.prompt(gpu, c, q, [n], [n], heads, 0.09, out=out)
+    assert st == 0
+    k, v = c.rows(0)
+    R.assert_rows(got, *R.attend(q, k, v, float(np.float32(0.09)), torch.arange(n, device="cuda") + 1))
+    assert bool((torch.as_strided(obuf, (n, 3), (w, 1), 5 + heads * hd)[:-1] == 7.0).all())
+
+
+def test_prefix_of_many_rows(gpu):
+    """More decode rows than a tile over the prefix, groups that do not
+    divide it, and an empty own part beside full ones."""
+    for qk, kv, hd in ((F32, F16, 128), (F16, F16, 64), (F32, F32, 96), (F16, F16, 256)):
+        lens = [(i * 37) % 200 for i in range(70)]
+        c = Cache(lens, 16, 2, hd, kv, seed=hd, prefix=1025)
+        R.check_decode(gpu, c, randn(70, 10, hd, seed=3, kind=qk), 10)
