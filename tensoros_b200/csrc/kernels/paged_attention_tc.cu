@@ -644,6 +644,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
         inv_q = sx[i * 2 * kRows + r];
         tile_any(kTileBar + i, false);                                   // read by all: sx is free
       }
+      // without a key tile no MMA stands between the warps' Q rows and the
+      // output rows that go to the same place
+      if (w.nt[i] == 0) tile_any(kTileBar + i, false);
       const int pr = w.r0 + i * kRows + r, nt = w.nt[i], k0 = w.k0;
       const bool live = pr < w.rows;
       const int tok = w.q0 + row_token(p, pr), head = w.kvh * p.group + row_head(p, pr), seq = w.seq;
@@ -686,6 +689,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
             tc_fence_after();
             scale_cols(to, HD / 2, f);
             l *= f;
+            // either half's P lets MMAs add to all dims: both halves' O first
+            tmem_st_wait();
+            tc_fence_before();
+            pair_sync(bar);
           }
           m = mn;
         };

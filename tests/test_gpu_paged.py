@@ -540,3 +540,15 @@ def test_prefix_of_many_rows(gpu):
         lens = [(i * 37) % 200 for i in range(70)]
         c = Cache(lens, 16, 2, hd, kv, seed=hd, prefix=1025)
         R.check_decode(gpu, c, randn(70, 10, hd, seed=3, kind=qk), 10)
+
+
+def test_tiles_that_see_nothing_many_times(gpu):
+    """Whole row tiles without a key beside ones with: their rows are written
+    while other warps may still be at the tile's queries."""
+    heads, hd, q_lens, kv_lens = 16, 128, [900, 700, 800], [400, 0, 300]
+    c = Cache(kv_lens, 16, 4, hd, F16, seed=1)
+    q = randn(sum(q_lens), heads, hd, seed=2, kind=F16)
+    first = R.check_prompt(gpu, c, q, q_lens, kv_lens, heads)
+    for _ in range(60):
+        out, st = R.prompt(gpu, c, q, q_lens, kv_lens, heads, hd ** -0.5)
+        assert st == 0 and torch.equal(out, first)
