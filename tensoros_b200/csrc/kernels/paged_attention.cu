@@ -474,7 +474,7 @@ int plan_splits(long long tiles, int keys, int rounds, int least) {
 int chunk_of(int keys, int splits) { return ((keys + splits - 1) / splits + 127) / 128 * 128; }
 
 struct DecodePlan {
-  int own, own_chunk, pre, pre_chunk;   // own 0: straight to out
+  int own, own_chunk, pre, pre_chunk;   // own 0: whole rows, the prefix's added to them
 };
 DecodePlan plan_decode(int n_seqs, int max_kv, int prefix_len, int heads, int n_kv) {
   DecodePlan d;
@@ -485,7 +485,7 @@ DecodePlan plan_decode(int n_seqs, int max_kv, int prefix_len, int heads, int n_
   d.own = max_kv > 0 ? plan_splits((long long)n_seqs * n_kv, max_kv, 4, 512) : 1;
   d.own_chunk = max_kv > 0 ? chunk_of(max_kv, d.own) : 128;
   if (max_kv > 0) d.own = (max_kv + d.own_chunk - 1) / d.own_chunk;
-  if (!d.pre && d.own == 1) d.own = 0;
+  if (d.own == 1) d.own = 0;
   return d;
 }
 
@@ -528,7 +528,7 @@ bool few_rows(const PagedProblem& p) {
   return (long long)p.total_q * p.heads / 8 * p.max_kv * p.hd * (f16 ? 4 : 8) <= most;
 }
 int run_tiles(const PagedProblem& p, cudaStream_t st) {
-  if (few_rows(p)) return paged_decode_run(p, 0, st);
+  if (few_rows(p)) return paged_decode_run(p, PagedPrefix{0, 0, nullptr}, st);
   return paged_tc_ok(p) ? paged_tc_run(p, st) : run_general(p, st);
 }
 
@@ -561,7 +561,8 @@ extern "C" size_t tosk_paged_prompt_ws_bytes(int total_q, int max_kv, int n_head
 
 extern "C" size_t tosk_paged_decode_ws_bytes(int n_seqs, int max_kv, int prefix_len, int n_heads, int n_kv, int hd) {
   const DecodePlan d = plan_decode(n_seqs, max_kv, prefix_len, n_heads, n_kv);
-  return (size_t)(d.own + d.pre) * slot_bytes(n_seqs, n_heads, hd);
+  // the general kernel does not add a prefix: its rows take a slot
+  return (size_t)(d.pre && !d.own ? d.pre + 1 : d.own + d.pre) * slot_bytes(n_seqs, n_heads, hd);
 }
 
 extern "C" int tosk_paged_prompt(const tosk_paged_attn_t* a, cudaStream_t st) {
@@ -576,11 +577,10 @@ extern "C" int tosk_paged_prompt(const tosk_paged_attn_t* a, cudaStream_t st) {
 
 extern "C" int tosk_paged_decode(const tosk_paged_attn_t* a, cudaStream_t st) {
   PagedProblem p = problem_of(a);
-  const DecodePlan d = plan_decode(a->n_seqs, a->max_kv, a->prefix_len, a->n_heads, a->kv.n_kv);
+  DecodePlan d = plan_decode(a->n_seqs, a->max_kv, a->prefix_len, a->n_heads, a->kv.n_kv);
   const bool fast = paged_decode_ok(p);
-  if (!d.own) return fast ? paged_decode_run(p, 0, st) : run_general(p, st);
+  if (!fast && d.pre && !d.own) d.own = 1;
   part_views(p, a->ws, d.own + d.pre);
-  bool beside = false;
   if (d.pre) {
     PagedProblem x = p;
     x.table = a->prefix_table;
@@ -592,14 +592,11 @@ extern "C" int tosk_paged_decode(const tosk_paged_attn_t* a, cudaStream_t st) {
     x.chunk = d.pre_chunk;
     const int e = run_tiles(x, st);
     if (e) return e;
-    beside = true;
   }
   p.splits = d.own;
   p.chunk = d.own_chunk;
   p.slot0 = d.pre;
-  if (a->max_kv > 0) {
-    const int e = fast ? paged_decode_run(p, beside, st) : run_general(p, st);
-    if (e) return e;
-  }
+  const int e = fast ? paged_decode_run(p, PagedPrefix{d.pre, a->prefix_len, a->prefix_table}, st) : run_general(p, st);
+  if (e || !d.own) return e;
   return run_join(p, d.pre, a->prefix_table, a->prefix_len, st);
 }

@@ -115,7 +115,81 @@ struct DecArgs {
   int q_vec;               // pairs of q elements are aligned
   int whole;               // a page holds whole steps
   int late_wait;           // 1: runs beside the prefix kernel, whose end it awaits at its own end
+  int pre;                 // without splits: slots of the prefix to add to each row, 0: none
+  const int* prefix_table;
+  int prefix_len;
 };
+
+// One row at the end of a CTA, by a warp: M, L its maximum (base 2) and sum,
+// v[i] its sum at dim lane + 32 i.  A split's partial row, or the output row:
+// with the prefix's partial rows added to it, and computed again key by key
+// where it shows NaN.
+__device__ __forceinline__ void finish_row(const DecArgs& a, const SeqTask& t, int kvh, int split, int r, float M, float L,
+                                           float (&v)[8]) {
+  const PagedProblem& p = a.p;
+  const int lane = threadIdx.x & 31;
+  const int tok = t.q0 + row_token(p, r), head = kvh * p.group + row_head(p, r);
+  const long long row = (long long)tok * p.heads + head, step = (long long)p.total_q * p.heads;
+  if (p.splits) {
+    const long long part = (p.slot0 + split) * step + row;
+    if (lane == 0) p.part_ml[part] = make_float2(M, L);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (lane + 32 * i < p.hd) p.part_o[part * p.hd + lane + 32 * i] = v[i];
+    return;
+  }
+  for (int s0 = 0; s0 < a.pre; s0 += 32) {               // lane i: slot s0 + i
+    float2 ml = make_float2(-INFINITY, 0.0f);
+    if (s0 + lane < a.pre) ml = p.part_ml[(s0 + lane) * step + row];
+    float mx = ml.x;
+    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    const float mn = fmaxf(M, mx), base = mn == -INFINITY ? 0.0f : mn;
+    const float f = exp2f(M - base), c = exp2f(ml.x - base);
+    float l = ml.y * c;
+    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    M = mn;
+    L = fmaf(L, f, l);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] *= f;
+    const int m = min(32, a.pre - s0);
+    for (int s = 0; s < m; s += 4) {
+      float x[4][8];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          x[u][i] = s + u < m && lane + 32 * i < p.hd ? p.part_o[((s0 + s + u) * step + row) * p.hd + lane + 32 * i] : 0.0f;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const float cu = __shfl_sync(0xffffffffu, c, (s + u) & 31);
+        if (s + u < m) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] = fmaf(x[u][i], cu, v[i]);
+        }
+      }
+    }
+  }
+  const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+  const long long oo = (long long)tok * p.out_stride + (long long)head * p.hd;
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (lane + 32 * i < p.hd) {
+      const float x = L == 0.0f ? 0.0f : v[i] * inv;
+      store_elem(p.out, p.type, oo + lane + 32 * i, x);
+      bad |= isnan(x);
+    }
+  if (__any_sync(0xffffffffu, bad))
+    attn_row_plain(p, a.prefix_table, a.prefix_len, t.table, seen(p, t, row_token(p, r)), tok, head);
+}
+
+// Whether this CTA's rows wait for the prefix kernel's: by all threads, once.
+__device__ __forceinline__ void await_prefix(const DecArgs& a) {
+  if (a.late_wait) {
+    pdl_trigger();
+    pdl_wait();
+  }
+}
 
 template <int HD, int NQ, bool DEEP>
 __global__ void __launch_bounds__(32 * kDecWarps) paged_decode_kernel(const __grid_constant__ DecArgs a) {
@@ -300,8 +374,9 @@ __global__ void __launch_bounds__(32 * kDecWarps) paged_decode_kernel(const __gr
     }
     __syncthreads();
     // a warp a query
+    await_prefix(a);
     for (int r = warp; r < nr; r += kDecWarps) {
-      float M = -INFINITY, L = 0.0f, f[kDecWarps];
+      float M = -INFINITY, L = 0.0f, f[kDecWarps], v[8];
 #pragma unroll
       for (int w = 0; w < kDecWarps; ++w) M = fmaxf(M, sml[w][r].x);
 #pragma unroll
@@ -309,27 +384,19 @@ __global__ void __launch_bounds__(32 * kDecWarps) paged_decode_kernel(const __gr
         f[w] = M == -INFINITY ? 0.0f : exp2f(sml[w][r].x - M);
         L += f[w] * sml[w][r].y;
       }
-      const int tok = t.q0 + row_token(p, r0 + r), head = kvh * p.group + row_head(p, r0 + r);
-      const long long part = (long long)(p.slot0 + split) * p.total_q * p.heads + (long long)tok * p.heads + head;
-      const long long oo = (long long)tok * p.out_stride + (long long)head * p.hd;
-      const float inv = p.splits ? 1.0f : L == 0.0f ? 0.0f : 1.0f / L;
-      if (p.splits && lane == 0) p.part_ml[part] = make_float2(M, L);
-      bool bad = false;
-      for (int d = lane; d < p.hd; d += 32) {
-        float v = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kDecWarps; ++w) v = fmaf(f[w], so[(w * NQ * 8 + r) * HD + d], v);
-        if (p.splits) p.part_o[part * p.hd + d] = v;
-        else store_elem(p.out, p.type, oo + d, L == 0.0f ? 0.0f : v * inv);
-        bad |= isnan(v);
+      for (int i = 0; i < 8; ++i) {
+        const int d = lane + 32 * i;
+        v[i] = 0.0f;
+        if (d < HD) {
+#pragma unroll
+          for (int w = 0; w < kDecWarps; ++w) v[i] = fmaf(f[w], so[(w * NQ * 8 + r) * HD + d], v[i]);
+        }
       }
-      if (!p.splits && __any_sync(0xffffffffu, bad) && L != 0.0f)
-        attn_row_plain(p, nullptr, 0, t.table, seen(p, t, row_token(p, r0 + r)), tok, head);
+      finish_row(a, t, kvh, split, r0 + r, M, L, v);
     }
-  }
-  if (a.late_wait) {
-    pdl_trigger();
-    pdl_wait();
+  } else {
+    await_prefix(a);
   }
 }
 
@@ -518,8 +585,9 @@ __global__ void __launch_bounds__(32 * kDecWarps) paged_decode_f32_kernel(const 
       }
     }
     __syncthreads();
+    await_prefix(a);
     for (int r = warp; r < nr; r += kDecWarps) {
-      float M = -INFINITY, L = 0.0f, f[kDecWarps];
+      float M = -INFINITY, L = 0.0f, f[kDecWarps], v[8];
 #pragma unroll
       for (int w = 0; w < kDecWarps; ++w) M = fmaxf(M, sml[w][r].x);
 #pragma unroll
@@ -527,27 +595,19 @@ __global__ void __launch_bounds__(32 * kDecWarps) paged_decode_f32_kernel(const 
         f[w] = M == -INFINITY ? 0.0f : exp2f(sml[w][r].x - M);
         L += f[w] * sml[w][r].y;
       }
-      const int tok = t.q0 + row_token(p, r0 + r), head = kvh * p.group + row_head(p, r0 + r);
-      const long long part = (long long)(p.slot0 + split) * p.total_q * p.heads + (long long)tok * p.heads + head;
-      const long long oo = (long long)tok * p.out_stride + (long long)head * p.hd;
-      const float inv = p.splits ? 1.0f : L == 0.0f ? 0.0f : 1.0f / L;
-      if (p.splits && lane == 0) p.part_ml[part] = make_float2(M, L);
-      bool bad = false;
-      for (int d = lane; d < p.hd; d += 32) {
-        float v = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kDecWarps; ++w) v = fmaf(f[w], so[(w * Q + r) * HD + d], v);
-        if (p.splits) p.part_o[part * p.hd + d] = v;
-        else store_elem(p.out, p.type, oo + d, L == 0.0f ? 0.0f : v * inv);
-        bad |= isnan(v);
+      for (int i = 0; i < 8; ++i) {
+        const int d = lane + 32 * i;
+        v[i] = 0.0f;
+        if (d < HD) {
+#pragma unroll
+          for (int w = 0; w < kDecWarps; ++w) v[i] = fmaf(f[w], so[(w * Q + r) * HD + d], v[i]);
+        }
       }
-      if (!p.splits && __any_sync(0xffffffffu, bad) && L != 0.0f)
-        attn_row_plain(p, nullptr, 0, t.table, seen(p, t, row_token(p, r0 + r)), tok, head);
+      finish_row(a, t, kvh, split, r0 + r, M, L, v);
     }
-  }
-  if (a.late_wait) {
-    pdl_trigger();
-    pdl_wait();
+  } else {
+    await_prefix(a);
   }
 }
 
@@ -598,10 +658,13 @@ bool paged_decode_ok(const PagedProblem& p) {
 // Few rows a sequence (single tokens, short prompts).  fp16: row tiles of 16
 // where a sequence has more than 8 rows (256 dims: of 8, for the registers),
 // else of 8.  fp32: of 1, 4 or 8, the smallest that holds the rows.
-int paged_decode_run(const PagedProblem& p, int late_wait, cudaStream_t st) {
+int paged_decode_run(const PagedProblem& p, const PagedPrefix& pre, cudaStream_t st) {
   DecArgs a;
   a.p = p;
-  a.late_wait = late_wait;
+  a.late_wait = pre.len > 0;
+  a.pre = p.splits ? 0 : pre.slots;
+  a.prefix_table = pre.table;
+  a.prefix_len = pre.len;
   const bool f16 = p.kv_type == TOSK_F16;
   const long long rows = (long long)p.max_q * p.group;
   const int nq = rows > 8 && p.hd <= 128 ? 2 : 1;

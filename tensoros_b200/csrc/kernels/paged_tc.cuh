@@ -16,7 +16,13 @@ int paged_tc_run(const PagedProblem& p, cudaStream_t st);
 long long paged_tc_tiles(int n_seqs, int total_q, int max_q, int group);
 // paged_decode.cu
 bool paged_decode_ok(const PagedProblem& p);
-int paged_decode_run(const PagedProblem& p, int late_wait, cudaStream_t st);
+// A shared prefix whose partial rows a kernel launched just before brings:
+// `slots` of them, at the slots before the problem's own.
+struct PagedPrefix {
+  int slots, len;
+  const int* table;
+};
+int paged_decode_run(const PagedProblem& p, const PagedPrefix& pre, cudaStream_t st);
 
 #ifdef __CUDACC__
 // Shared-memory operands, rows of 128 bytes swizzled 128 B, eight rows every
