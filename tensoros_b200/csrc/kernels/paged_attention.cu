@@ -424,10 +424,6 @@ PagedProblem problem_of(const tosk_paged_attn_t* a) {
   return p;
 }
 
-size_t slot_bytes(int total_q, int heads, int hd) {
-  return (size_t)total_q * heads * ((size_t)hd * 4 + 8) + 16;
-}
-
 // ------------------------------------------------------------ general kernel
 bool aligned4(const void* p, long long stride, int type, int hd) {
   return ((uintptr_t)p & (type == TOSK_F32 ? 15 : 7)) == 0 && stride % 4 == 0 && hd % 4 == 0;
@@ -504,10 +500,17 @@ int run_join(const PagedProblem& own, int pre, const int* prefix_table, int pref
   return launch(f, dim3((unsigned)gx, own.n_seqs), 128, 0, &j, st);
 }
 
-void part_views(PagedProblem& p, void* ws, int slots) {
+// A workspace: `slots` slots of partial rows, then the tensor-core kernel's sums.
+size_t slots_bytes(int slots, int total_q, int heads, int hd) {
+  const size_t rows = (size_t)slots * total_q * heads;
+  return slots ? ((rows * hd * 4 + 15) & ~(size_t)15) + ((rows * 8 + 15) & ~(size_t)15) : 0;
+}
+void part_views(PagedProblem& p, void* ws, int slots, size_t fold) {
   const size_t rows = (size_t)slots * p.total_q * p.heads;
-  p.part_o = reinterpret_cast<float*>(ws);
-  p.part_ml = reinterpret_cast<float2*>(reinterpret_cast<uint8_t*>(ws) + ((rows * p.hd * 4 + 15) & ~(size_t)15));
+  uint8_t* b = reinterpret_cast<uint8_t*>(ws);
+  p.part_o = reinterpret_cast<float*>(b);
+  p.part_ml = reinterpret_cast<float2*>(b + ((rows * p.hd * 4 + 15) & ~(size_t)15));
+  p.fold = fold ? reinterpret_cast<float*>(b + slots_bytes(slots, p.total_q, p.heads, p.hd)) : nullptr;
 }
 
 // Which kernel takes a problem with several rows a sequence.  The few-rows
@@ -555,24 +558,28 @@ int plan_prompt(int total_q, int max_kv, int heads, int n_kv, int hd) {
 }
 }  // namespace
 
+// Keys of one piece of a prompt's work.
+int prompt_keys(int splits, int max_kv) { return splits ? chunk_of(max_kv, splits) : max_kv; }
+
 extern "C" size_t tosk_paged_prompt_ws_bytes(int total_q, int max_kv, int n_heads, int n_kv, int hd) {
-  return (size_t)plan_prompt(total_q, max_kv, n_heads, n_kv, hd) * slot_bytes(total_q, n_heads, hd);
+  const int splits = plan_prompt(total_q, max_kv, n_heads, n_kv, hd);
+  return slots_bytes(splits, total_q, n_heads, hd) + paged_tc_fold_bytes(prompt_keys(splits, max_kv));
 }
 
 extern "C" size_t tosk_paged_decode_ws_bytes(int n_seqs, int max_kv, int prefix_len, int n_heads, int n_kv, int hd) {
   const DecodePlan d = plan_decode(n_seqs, max_kv, prefix_len, n_heads, n_kv);
   // the general kernel does not add a prefix: its rows take a slot
-  return (size_t)(d.pre && !d.own ? d.pre + 1 : d.own + d.pre) * slot_bytes(n_seqs, n_heads, hd);
+  const int slots = d.pre && !d.own ? d.pre + 1 : d.own + d.pre;
+  return slots_bytes(slots, n_seqs, n_heads, hd) + paged_tc_fold_bytes(d.pre_chunk);
 }
 
 extern "C" int tosk_paged_prompt(const tosk_paged_attn_t* a, cudaStream_t st) {
   PagedProblem p = problem_of(a);
   p.splits = plan_prompt(a->total_q, a->max_kv, a->n_heads, a->kv.n_kv, a->kv.hd);
-  if (!p.splits) return run_tiles(p, st);
-  p.chunk = chunk_of(a->max_kv, p.splits);
-  part_views(p, a->ws, p.splits);
+  p.chunk = prompt_keys(p.splits, a->max_kv);
+  part_views(p, a->ws, p.splits, paged_tc_fold_bytes(p.chunk));
   const int e = run_tiles(p, st);
-  return e ? e : run_join(p, 0, nullptr, 0, st);
+  return e || !p.splits ? e : run_join(p, 0, nullptr, 0, st);
 }
 
 extern "C" int tosk_paged_decode(const tosk_paged_attn_t* a, cudaStream_t st) {
@@ -580,7 +587,7 @@ extern "C" int tosk_paged_decode(const tosk_paged_attn_t* a, cudaStream_t st) {
   DecodePlan d = plan_decode(a->n_seqs, a->max_kv, a->prefix_len, a->n_heads, a->kv.n_kv);
   const bool fast = paged_decode_ok(p);
   if (!fast && d.pre && !d.own) d.own = 1;
-  part_views(p, a->ws, d.own + d.pre);
+  part_views(p, a->ws, d.own + d.pre, paged_tc_fold_bytes(d.pre_chunk));
   if (d.pre) {
     PagedProblem x = p;
     x.table = a->prefix_table;

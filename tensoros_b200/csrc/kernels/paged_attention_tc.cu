@@ -49,10 +49,8 @@ constexpr int kTileBar = 9;            // named barriers: 1..8 pair the two warp
 constexpr int kRows = 128;            // rows of a tile
 constexpr int kKeys = 128;            // keys of a tile
 constexpr float kBias = 7.0f;         // log2 of the factor that P carries
-#ifndef TOS_POLY
-#define TOS_POLY 3
-#endif
-constexpr int kPoly = TOS_POLY;       // one of so many pairs of exponentials goes to the FMA pipe
+constexpr int kPoly = 3;              // of eight pairs of exponentials, those at 2 and 5 go to the FMA pipe
+constexpr int kFold = 3;              // fp32 rows: key tiles whose products one accumulator sums
 constexpr float kSlack = 8.0f;        // log2 by which the maximum may grow unfollowed
 
 struct TcArgs {
@@ -250,6 +248,26 @@ static __device__ __noinline__ void scale_cols(uint32_t addr, int n, float f) {
 #pragma unroll
     for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
     tmem_st16(addr + c, o);
+  }
+}
+// Memory <- s * memory + n columns of this warp's 32 rows in tensor memory (s 0:
+// memory is not read).  Four columns of the 32 rows lie side by side: dst is
+// the lane's first four of n.
+static __device__ __noinline__ void fold_cols(uint32_t addr, int n, float* dst, float s) {
+#pragma unroll 1
+  for (int c = 0; c < n; c += 16, dst += 512) {
+    uint32_t o[16];
+    tc_ld16(addr + c, o);
+    float4 x[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      x[e] = s != 0.0f ? *reinterpret_cast<const float4*>(dst + 128 * e) : make_float4(0.f, 0.f, 0.f, 0.f);
+    tc_wait_ld16(o);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      *reinterpret_cast<float4*>(dst + 128 * e) =
+          make_float4(fmaf(x[e].x, s, __uint_as_float(o[4 * e])), fmaf(x[e].y, s, __uint_as_float(o[4 * e + 1])),
+                      fmaf(x[e].z, s, __uint_as_float(o[4 * e + 2])), fmaf(x[e].w, s, __uint_as_float(o[4 * e + 3])));
   }
 }
 // The two warps that share 32 rows.
@@ -548,11 +566,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
             const uint32_t qd = desc_k(smem_u32(sq + i * (T::kQ / 2)));
             const uint32_t d = tmem + i * kKeys;
 #pragma unroll
-            for (int part = 0; part < (SPLIT ? 2 : 1); ++part)
+            for (int part = 0; part < (SPLIT ? 2 : 1); ++part)          // low parts first: less is cut off small sums
 #pragma unroll
               for (int k = 0; k < HD / 16; ++k) {
                 const uint32_t off = ((k >> 2) * 16384 + (k & 3) * 32) >> 4;
-                mma_f16_ss(d, qd + (part * T::kTile >> 4) + off, kd + off, kIdS, part + k > 0);
+                mma_f16_ss(d, qd + (SPLIT && part == 0 ? T::kTile >> 4 : 0) + off, kd + off, kIdS, part + k > 0);
               }
             mma_commit(sfull + i);
             if (i == 1 || j >= n1) mma_commit(empty + slot);
@@ -582,7 +600,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
 #pragma unroll
                   for (int k = 0; k < kKeys / 32; ++k)
                     mma_f16_ts(d, pa + (k >> 1) * 32 + part * 16 + (k & 1) * 8, vd + (k * 2048 >> 4), kIdO,
-                               part + k > 0 ? true : j + half > 0);
+                               part + k + half > 0 ? true : SPLIT ? j % kFold != 0 : j > 0);
               }
               if (!ok) break;
               mma_commit(odone + i);
@@ -609,6 +627,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
     const uint32_t lanes = (uint32_t)wq << 21;                          // TMEM lane of the warp's first row, << 16
     const uint32_t ts = tmem_at + lanes + i * kKeys, to = tmem_at + lanes + 256 + i * HD + hf * (HD / 2);
     uint8_t* stage = (T::kStage ? ring + T::kSlots * T::kTile + i * 32768 : q_tile) + (hf * 4 + wq) * 4096;
+    float* const fold = p.fold + (size_t)(blockIdx.x * kCopyWarp + warp) * (32 * HD / 2) + lane * 4;
     bool ok = true;     // a wait that ran out: no more waiting, and all warps of the row tile leave together
     int cnt = 0;                                                        // key tiles so far
     pdl_wait();
@@ -652,10 +671,25 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
       const int tok = w.q0 + row_token(p, pr), head = w.kvh * p.group + row_head(p, pr), seq = w.seq;
       const SeqTask st = {w.q0, 0, w.kvn, w.off, nullptr};
       const int all = live ? seen(p, st, row_token(p, pr)) : 0, lim = min(all, w.k1);   // keys this row sees, here
-      const long long slot = (long long)(p.slot0 + w.split) * p.total_q * p.heads + (long long)tok * p.heads + head;
+      const long long slot = (long long)(p.slot0 + (p.splits ? w.split : 0)) * p.total_q * p.heads + (long long)tok * p.heads + head;
       const float sc = fmaxf(fabsf(p.scale_log2) * inv_q, 1.2e-38f);   // not 0: a masked score is -inf * sc
+      // fp32 rows: the sums so far are fold_s * what lies at `fold`
+      float fold_s = 0.0f;
       float m = -INFINITY, l = 0.0f;
       for (int j = 0; j < nt; ++j) {
+        if (SPLIT && j > 0 && j % kFold == 0) {
+          // The tensor cores cut off what their accumulator has no room for,
+          // so a long chain of sums shrinks: by up to 5e-8 of itself a step of
+          // 16 keys, 6e-5 over 9000 keys.  Every kFold tiles the sums are
+          // added up in memory, rounded to nearest, and the chain begins anew.
+          if (ok) ok = mbar_wait(odone + i, (cnt + j - 1) & 1, p.err, 46);
+          __syncwarp();
+          tc_fence_after();
+          fold_cols(to, HD / 2, fold, fold_s);
+          fold_s = 1.0f;
+          tc_fence_before();
+          pair_sync(bar);                                               // the MMAs overwrite all dims
+        }
         if (ok) ok = mbar_wait(sfull + i, (cnt + j) & 1, p.err, 39);
         __syncwarp();
         tc_fence_after();
@@ -689,6 +723,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
             tc_fence_after();
             scale_cols(to, HD / 2, f);
             l *= f;
+            fold_s *= f;
             // either half's P lets MMAs add to all dims: both halves' O first
             tmem_st_wait();
             tc_fence_before();
@@ -744,7 +779,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
               for (int e = 0; e < 8; ++e) {
                 const float2 x =
                     __ffma2_rn(make_float2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), sc2, bias2);
-                const float2 v = kPoly && (e % kPoly) == kPoly - 1 ? exp2_fma(x) : make_float2(ex2(x.x), ex2(x.y));
+                const float2 v = e % kPoly == kPoly - 1 ? exp2_fma(x) : make_float2(ex2(x.x), ex2(x.y));
                 sum[e & 1] = __fadd2_rn(sum[e & 1], v);
                 const __half2 H = __floats2half2_rn(v.x, v.y);
                 hi[c >> 1][8 * (c & 1) + e] = *reinterpret_cast<const uint32_t*>(&H);
@@ -844,6 +879,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
         uint32_t o[32];
         tc_ld32(to + 32 * c32, o);
         tc_wait_ld(o);
+        if (SPLIT && fold_s != 0.0f) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 4) {
+            const float4 x = *reinterpret_cast<const float4*>(fold + (8 * c32 + e / 4) * 128);
+            o[e] = __float_as_uint(fmaf(x.x, fold_s, __uint_as_float(o[e])));
+            o[e + 1] = __float_as_uint(fmaf(x.y, fold_s, __uint_as_float(o[e + 1])));
+            o[e + 2] = __float_as_uint(fmaf(x.z, fold_s, __uint_as_float(o[e + 2])));
+            o[e + 3] = __float_as_uint(fmaf(x.w, fold_s, __uint_as_float(o[e + 3])));
+          }
+        }
 #pragma unroll
         for (int e = 0; e < 32; e += 2) {
           const float2 v = __fmul2_rn(make_float2(__uint_as_float(o[e]), __uint_as_float(o[e + 1])), make_float2(inv, inv));
@@ -957,6 +1002,9 @@ bool paged_tc_ok(const PagedProblem& p) {
 }
 
 // Row tiles of one key/value head that a call can have at most.
+// Bytes of PagedProblem::fold that fp32 rows over so many keys need.
+size_t paged_tc_fold_bytes(int keys) { return keys > kFold * kKeys ? (size_t)kTcCtas * 2 * kRows * 128 * 4 : 0; }
+
 long long paged_tc_tiles(int n_seqs, int total_q, int max_q, int group) {
   const long long each = ((long long)max_q * group + 2 * kRows - 1) / (2 * kRows) * n_seqs;
   const long long all = (long long)total_q * group / (2 * kRows) + n_seqs;
@@ -974,6 +1022,8 @@ int paged_tc_run(const PagedProblem& p, cudaStream_t st) {
   a.out_vec = ((uintptr_t)p.out & 15) == 0 && p.out_stride % (p.type == TOSK_F32 ? 4 : 8) == 0;
   if (!pool_map(&a.mk, p.k, p, a.box_rows) || !pool_map(&a.mv, p.v, p, a.box_rows)) return (int)cudaErrorNotSupported;
   const bool split = p.type == TOSK_F32;
+  const int keys = p.splits ? p.chunk : p.fixed_kv >= 0 ? p.fixed_kv : p.max_kv;
+  if (split && !p.fold && paged_tc_fold_bytes(keys)) return (int)cudaErrorInvalidValue;
   if (p.hd <= 64) return split ? tc_launch<64, true>(a, (unsigned)grid, st) : tc_launch<64, false>(a, (unsigned)grid, st);
   return split ? tc_launch<128, true>(a, (unsigned)grid, st) : tc_launch<128, false>(a, (unsigned)grid, st);
 }

@@ -13,6 +13,7 @@ namespace tos {
 
 bool paged_tc_ok(const PagedProblem& p);
 int paged_tc_run(const PagedProblem& p, cudaStream_t st);
+size_t paged_tc_fold_bytes(int keys);
 long long paged_tc_tiles(int n_seqs, int total_q, int max_q, int group);
 // paged_decode.cu
 bool paged_decode_ok(const PagedProblem& p);

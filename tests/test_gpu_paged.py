@@ -552,3 +552,21 @@ def test_tiles_that_see_nothing_many_times(gpu):
     for _ in range(60):
         out, st = R.prompt(gpu, c, q, q_lens, kv_lens, heads, hd ** -0.5)
         assert st == 0 and torch.equal(out, first)
+
+
+@pytest.mark.parametrize("hist", [700, 9000])
+def test_tiles_long_sums_do_not_shrink(gpu, hist):
+    """fp32 rows over many keys with values of one sign.  A tensor-core sum
+    cuts off up to a unit, 2^-23, a step; steps of 16 keys, high and low parts,
+    in chains of at most 512 keys: 64 2^-23 = 7.6e-6, and scores and weights a
+    tenth of that."""
+    n, heads, hd = 300, 16, 128
+    c = Cache([n + hist], 64, 16, hd, F16, seed=2)
+    pg, r = c.where(c.table[0], n + hist)
+    c.v[pg, r] = 1 + c.v[pg, r] / 16
+    q = randn(n, heads, hd, seed=3)
+    out, st = R.prompt(gpu, c, q, [n], [n + hist], heads, hd ** -0.5)
+    assert st == 0
+    k, v = c.rows(0)
+    ref, _ = R.attend(q, k, v, float(np.float32(hd ** -0.5)), torch.arange(n, device="cuda") + hist + 1)
+    assert float(((out.double() - ref) / ref).abs().max()) < 8.5e-6
