@@ -4,27 +4,45 @@
 //
 //   S = Q K^T,  P = 2^(c S - m),  O += P V,  l += sum P     (128 x 128 tiles)
 //
-// A CTA takes 256 packed rows (token, query head of the group) of one
-// sequence and one key/value head as two tiles of 128 and walks the keys in
-// tiles of 128:
-//   * warp 8 brings K and V tiles, page by page, into a ring of shared memory
+// Persistent CTAs, one an SM, take pieces of work in turn: 256 packed rows
+// (token, query head of the group) of one sequence and one key/value head, as
+// two row tiles of 128, over the keys in tiles of 128.  Twenty warps:
+//   * one plans: which piece is this CTA's next (longest first, dealt there
+//     and back), two ahead;
+//   * one brings K and V tiles, page by page, into a ring of shared memory
 //     slots (TMA boxes of a page's rows x 64 columns, swizzled 128 B; lane i
-//     takes page i of the tile);
-//   * warp 9 issues the MMAs in the order PV0(j) S0(j+1) PV1(j) S1(j+1), so
-//     the tensor cores work on one row tile while the other's softmax runs;
+//     takes page i of the tile), into the next piece where the ring has room;
+//   * one thread issues the MMAs in the order PV0(j) S0(j+1) PV1(j) S1(j+1),
+//     so the tensor cores work on one row tile while the other's softmax runs;
 //     accumulators in tensor memory: S0, S1 (128 columns each), O0, O1;
-//   * warps 0-3 and 4-7 hold one row tile each, a row a thread: S from tensor
-//     memory, the row's maximum and sum without any exchange, P back into
-//     S's columns as the A operand of P V.
+//   * sixteen, eight a row tile, hold a row and half of a tile's keys a thread:
+//     weights under the maximum so far and the new maximum from one pass over
+//     S, a vote of the row's two threads, P over S's columns as the A operand
+//     of P V; at the end of a piece the output rows through shared memory.
 // The maximum in use follows the true one only when that has grown by more
 // than 2^8 (O is then scaled in tensor memory), so O is touched rarely.
 // P carries a factor 2^7, at most 2^15, which keeps small weights out of
 // fp16's subnormals; it cancels in O / l.
 //
+// What bounds it (B200; a piece a SM, 1024 to 8192 keys): a key tile of both
+// row tiles takes 2.4 us for fp16 rows, where a library product's rate would
+// take 1.5, and 4.0 for fp32 rows, whose two-part products are twice the work;
+// a call costs 19 to 26 us beside its tiles.  The row tiles
+// alternate between softmax and MMAs, two of them do not fill the tensor
+// cores, and a third does not fit tensor memory.  Packed fp16 prompts of 6537
+// tokens, 32 / 8 heads x 128: 189 us, 852 TFLOP/s.
+// Steps on the way (the same prompts, us): one warpgroup a row tile 287; queries
+// loaded in batches, registers moved to the softmax warps, halves of P handed
+// on 235; one elected thread for all MMAs 208; four warpgroups 207; persistent
+// 197; weights and maximum from one read of S 194; two pairs of eight
+// exponentials on the FMA pipe 188 (none 197, four pairs 205).
+//
 // Precision.  fp16 rows: P is rounded to fp16 (half a step, 2^-11, of each
 // weight, which is what the output's own rounding costs; sums and maxima are
 // fp32).  fp32 rows: q, scaled by a power of two per row, and P go in as
-// exact fp16 pairs hi + lo (22 bits), two MMAs each, so results are fp32's.
+// fp16 pairs hi + lo (22 bits), two MMAs each, and the accumulators, which cut
+// off instead of rounding, are emptied into memory every kFold key tiles:
+// 1.1e-6 against 64 bits (norm) over 7512 keys.
 //
 // Keys behind a row's last one are masked in S; value rows behind the key
 // range are zeroed in shared memory (a page's unused rows may hold
@@ -40,7 +58,7 @@
 namespace tos {
 
 constexpr int kTcCtas = 148;           // one a SM, each takes pieces of work in turn
-constexpr int kTcThreads = 640;        // four softmax warpgroups; K/V copies, MMAs, two idle warps
+constexpr int kTcThreads = 640;        // four softmax warpgroups; K/V copies, MMAs, plan, an idle warp
 constexpr int kTcRegs = 96;            // a thread at launch, moved to the softmax warps afterwards
 constexpr int kTcRegsSoftmax = 104, kTcRegsRest = 64;
 static_assert(4 * kTcRegsSoftmax + kTcRegsRest <= 5 * kTcRegs, "registers of the launch");
@@ -51,6 +69,7 @@ constexpr int kKeys = 128;            // keys of a tile
 constexpr float kBias = 7.0f;         // log2 of the factor that P carries
 constexpr int kPoly = 3;              // of eight pairs of exponentials, those at 2 and 5 go to the FMA pipe
 constexpr int kFold = 3;              // fp32 rows: key tiles whose products one accumulator sums
+                                      // (512 rows behind 7001 keys, us: 3: 159, 4: 154, 8: 145, never: 138)
 constexpr float kSlack = 8.0f;        // log2 by which the maximum may grow unfollowed
 
 struct TcArgs {
@@ -158,66 +177,89 @@ __device__ __forceinline__ void tma_page(void* dst, const CUtensorMap* m, int x,
 struct TileId {
   int seq, rt;                        // seq < 0: no such tile
 };
+struct PlanCursor {
+  int s0, before;                     // sequences passed, and their tiles
+};
+// Sequences, one a lane, up to which tiles go by length.  One prompt of 2048 to
+// 4096 tokens behind 15 to 30 short ones: 68 to 174 us sorted, 84 to 211 in the
+// order given; with 120 short ones the search costs what it saves (246, 242),
+// and 256 ragged prompts of up to 200 tokens take 268 us sorted, 244 not.
+constexpr int kSortSeqs = 32;
 
-// The f-th row tile of the call in falling order of its key tiles, so that
-// the long ones start first whatever the sequences' order, and no CTA is
-// spent on tiles that the longest sequence would have.  In sequence s the
-// tiles with at least w key tiles are the last count(s, w); the w of rank f
-// is found by bisection over their sum (lanes take sequences), the sequence
-// by a prefix sum.
-__device__ __forceinline__ TileId pick_tile(const PagedProblem& p, int f) {
-  TileId id = {-1, 0};
-  if (p.n_seqs == 1) {
-    const SeqTask t = seq_task(p, 0);
-    const int n = (t.qn * p.group + 2 * kRows - 1) / (2 * kRows);
-    if (f < n) id = {0, n - 1 - f};
-    return id;
-  }
+__device__ __forceinline__ int row_tiles(const PagedProblem& p, const SeqTask& t) {
+  return (t.qn * p.group + 2 * kRows - 1) / (2 * kRows);
+}
+
+// The lane whose running sum over the warp of `n` first passes f: its place,
+// and f less what comes before it.  false: the warp's sum is subtracted.
+__device__ __forceinline__ bool find_lane(int n, int& f, int& at) {
   const int lane = threadIdx.x & 31;
-  auto tiles = [&](const SeqTask& t) { return (t.qn * p.group + 2 * kRows - 1) / (2 * kRows); };
-  const SeqTask none = {0, 0, 0, 0, nullptr};
-  const SeqTask mine = lane < p.n_seqs ? seq_task(p, lane) : none;    // the first 32 sequences stay in registers
-  auto task = [&](int s) { return s < 32 ? mine : s < p.n_seqs ? seq_task(p, s) : none; };
-  auto count = [&](const SeqTask& t, int w) {
-    const int n = tiles(t);
+  int sum = n;
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, sum, o);
+    if (lane >= o) sum += v;
+  }
+  const uint32_t hit = __ballot_sync(0xffffffffu, sum > f);
+  if (hit) {
+    at = __ffs(hit) - 1;
+    f -= __shfl_sync(0xffffffffu, sum - n, at);
+    return true;
+  }
+  f -= __shfl_sync(0xffffffffu, sum, 31);
+  return false;
+}
+
+// The f-th row tile of the call (f grows from call to call of a CTA).
+//
+// Up to kSortSeqs sequences: in falling order of the tiles' key tiles, so that
+// the long ones start first whatever the sequences' order.  In sequence s the
+// tiles with at least w key tiles are the last count(w); the w of rank f is
+// found by bisection over their sum, the sequence by a prefix sum.  More
+// sequences: in their own order, a sequence's long tiles first; the cursor
+// passes each once (4096 ragged prompts: 3.5 ms; a search a tile: 77 ms).
+//
+// Not inlined: the softmax warps' code is slower beside it (194 us for packed
+// prompts against 189).
+__device__ __noinline__ TileId pick_of_many(const PagedProblem& p, int f, PlanCursor& cur) {
+  const int lane = threadIdx.x & 31;
+  int at;
+  if (p.n_seqs > kSortSeqs) {
+    for (; cur.s0 < p.n_seqs; cur.s0 += 32) {
+      const int s = cur.s0 + lane, n = s < p.n_seqs ? row_tiles(p, seq_task(p, s)) : 0;
+      int g = f - cur.before;
+      if (find_lane(n, g, at)) return {cur.s0 + at, __shfl_sync(0xffffffffu, n, at) - 1 - g};
+      cur.before = f - g;
+    }
+    return {-1, 0};
+  }
+  const SeqTask t = lane < p.n_seqs ? seq_task(p, lane) : SeqTask{0, 0, 0, 0, nullptr};
+  const int n = row_tiles(p, t);
+  auto count = [&](int w) {
     if (w <= 0) return n;
     if (kKeys * (w - 1) >= t.kvn) return 0;
     const long long tok = (long long)kKeys * (w - 1) - t.off;    // first token that sees key kKeys (w - 1)
     const long long first = tok <= 0 ? 0 : tok * p.group / (2 * kRows);
     return first >= n ? 0 : n - (int)first;
   };
-  auto total = [&](int w) {
-    int c = count(mine, w);
-    for (int s = lane + 32; s < p.n_seqs; s += 32) c += count(seq_task(p, s), w);
-    return __reduce_add_sync(0xffffffffu, c);
-  };
-  if (f >= total(0)) return id;
+  auto total = [&](int w) { return __reduce_add_sync(0xffffffffu, count(w)); };
+  if (f >= total(0)) return {-1, 0};
   int lo = 0, hi = (p.max_kv + kKeys - 1) / kKeys + 1;            // total(lo) > f >= total(hi)
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
     if (total(mid) > f) lo = mid;
     else hi = mid;
   }
-  f -= total(lo + 1);
-  for (int s0 = 0; s0 < p.n_seqs; s0 += 32) {
-    const int s = s0 + lane;
-    const SeqTask t = task(s);
-    const int c0 = count(t, lo), c1 = count(t, lo + 1);
-    int sum = c0 - c1;
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, sum, o);
-      if (lane >= o) sum += v;
-    }
-    const uint32_t hit = __ballot_sync(0xffffffffu, sum > f);
-    if (hit) {
-      const int w = __ffs(hit) - 1;
-      const int before = __shfl_sync(0xffffffffu, sum - (c0 - c1), w);
-      const int rt = tiles(t) - c0;                               // first tile with that many
-      return {s0 + w, __shfl_sync(0xffffffffu, rt, w) + f - before};
-    }
-    f -= __shfl_sync(0xffffffffu, sum, 31);
+  const int above = count(lo + 1), c = count(lo) - above;         // this lane's tiles of lo key tiles
+  f -= __reduce_add_sync(0xffffffffu, above);
+  if (!find_lane(c, f, at)) return {-1, 0};
+  return {at, __shfl_sync(0xffffffffu, n - above - c, at) + f};
+}
+__device__ __forceinline__ TileId pick_tile(const PagedProblem& p, int f, PlanCursor& cur) {
+  if (p.n_seqs == 1) {
+    const int n = row_tiles(p, seq_task(p, 0));
+    return f < n ? TileId{0, n - 1 - f} : TileId{-1, 0};
   }
-  return id;
+  return pick_of_many(p, f, cur);
 }
 
 // Scores from the n-th on count for nothing.
@@ -443,6 +485,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
       if (p.fixed_kv < 0) pdl_wait();                  // a prefix is planned from the arguments alone
       bool ok = true, more = true;
       int posted = 0;
+      PlanCursor cur = {0, 0};
       const int splits = p.splits ? p.splits : 1;
       for (int k = 0; more && ok; ++k) {
         const int g = k * (int)gridDim.x + (k & 1 ? (int)gridDim.x - 1 - (int)blockIdx.x : (int)blockIdx.x);
@@ -450,7 +493,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
         w.seq = -1;
         w.kvh = g % p.n_kv;
         w.split = g / p.n_kv % splits;
-        const TileId id = pick_tile(p, g / p.n_kv / splits);
+        const TileId id = pick_tile(p, g / p.n_kv / splits, cur);
         more = id.seq >= 0;
         if (more) {
           const SeqTask t = seq_task(p, id.seq);

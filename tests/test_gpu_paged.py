@@ -570,3 +570,14 @@ def test_tiles_long_sums_do_not_shrink(gpu, hist):
     k, v = c.rows(0)
     ref, _ = R.attend(q, k, v, float(np.float32(hd ** -0.5)), torch.arange(n, device="cuda") + hist + 1)
     assert float(((out.double() - ref) / ref).abs().max()) < 8.5e-6
+
+
+@pytest.mark.parametrize("qk,kv", [(F32, F16), (F16, F16), (F32, F32)])
+@pytest.mark.parametrize("hd", [128, 64])
+def test_prompt_of_many_sequences(gpu, qk, kv, hd):
+    """More sequences than the plan sorts, empty ones among them."""
+    q_lens = [(i * 7) % 23 if i % 5 else 0 for i in range(300)]
+    q_lens[150] = 700
+    kv_lens = [n + (i * 13) % 90 for i, n in enumerate(q_lens)]
+    c = Cache(kv_lens, 16, 2, hd, kv, seed=4)
+    R.check_prompt(gpu, c, randn(sum(q_lens), 8, hd, seed=5, kind=qk), q_lens, kv_lens, 8)
