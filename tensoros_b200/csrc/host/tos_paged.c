@@ -10,6 +10,8 @@
 #include "tos_internal.h"
 
 #define MAX_HEAD_DIM 256
+#define MAX_ROWS (1 << 30)   /* keys of a sequence, packed rows of a sequence: 32-bit arithmetic with room */
+#define MAX_SEQS 65535
 
 struct tos_rotary {
     tosk_rotary_t r;
@@ -226,7 +228,7 @@ static int attn_check(const tos_rows_t *out, const tos_rows_t *q, const tos_page
 {
     int rc = paged_check(kv);
     if (rc) return rc;
-    if (n_heads <= 0 || n_heads % kv->n_kv || !isfinite(scale)) return TOS_EINVAL;
+    if (n_heads <= 0 || n_heads % kv->n_kv || !isfinite(scale * 1.5f)) return TOS_EINVAL;
     if (n_heads > (1 << 20)) return TOS_ENOTSUP;
     rc = rows_check(out, n_heads, kv->head_dim);
     if (!rc) rc = rows_check(q, n_heads, kv->head_dim);
@@ -274,6 +276,8 @@ int tos_attention_prompt_paged_dev(const tos_rows_t *out, const tos_rows_t *q, c
     int rc = attn_check(out, q, kv, n_heads, scale);
     if (!rc && (n_seqs < 0 || n_seqs > kv->n_seqs || total_q < 0 || max_q < 0 || max_kv < 0)) rc = TOS_EINVAL;
     if (!rc && n_seqs && (!cu_q || !kv_len || ((uintptr_t)cu_q & 3) || ((uintptr_t)kv_len & 3))) rc = TOS_EINVAL;
+    if (!rc && (max_kv > MAX_ROWS || n_seqs > MAX_SEQS || (int64_t)max_q * (n_heads / kv->n_kv) > MAX_ROWS))
+        rc = TOS_ENOTSUP;
     if (!rc)
         rc = ws_check(ws, ws_bytes, tos_attention_prompt_paged_workspace_bytes(n_seqs, total_q, max_q, max_kv,
                                                                                n_heads, kv->n_kv, kv->head_dim));
@@ -304,6 +308,9 @@ int tos_attention_decode_paged_dev(const tos_rows_t *out, const tos_rows_t *q, c
     if (!rc && (n_seqs < 0 || n_seqs > kv->n_seqs || max_kv < 0 || prefix_len < 0)) rc = TOS_EINVAL;
     if (!rc && n_seqs && (!kv_len || ((uintptr_t)kv_len & 3))) rc = TOS_EINVAL;
     if (!rc && prefix_len && (!prefix_table || ((uintptr_t)prefix_table & 3))) rc = TOS_EINVAL;
+    if (!rc && (max_kv > MAX_ROWS || prefix_len > MAX_ROWS || n_seqs > MAX_SEQS ||
+                (int64_t)n_seqs * (n_heads / kv->n_kv) > MAX_ROWS))
+        rc = TOS_ENOTSUP;
     if (!rc)
         rc = ws_check(ws, ws_bytes, tos_attention_decode_paged_workspace_bytes(n_seqs, max_kv, prefix_len, n_heads,
                                                                                kv->n_kv, kv->head_dim));

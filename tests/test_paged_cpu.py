@@ -120,6 +120,17 @@ def test_attention_refusals(lib):
     assert decode(lib, ws=PTR + 8) == EINVAL
 
 
+def test_attention_limits(lib):
+    """What 32-bit counts of rows and the joining grid do not hold."""
+    assert prompt(lib, mk=(1 << 30) + 1) == ENOTSUP
+    assert prompt(lib, mq=1 << 30, heads=4) == ENOTSUP
+    assert prompt(lib, c=kv(n_seqs=70000), n=70000) == ENOTSUP
+    assert decode(lib, mk=(1 << 30) + 1) == ENOTSUP
+    assert decode(lib, pl=(1 << 30) + 1) == ENOTSUP
+    assert decode(lib, c=kv(n_seqs=70000), n=70000) == ENOTSUP
+    assert decode(lib, scale=3e38) == EINVAL
+
+
 def test_workspace_sizes(lib):
     f = lib.tos_attention_decode_paged_workspace_bytes
     assert f(0, 10, 0, 4, 2, 64) == 0 and f(2, -1, 0, 4, 2, 64) == 0 and f(2, 10, 0, 3, 2, 64) == 0
