@@ -1,23 +1,27 @@
-// paged_decode.cu - attention of single tokens over a paged cache.
+// paged_decode.cu - attention of few rows a sequence over a paged cache:
+// single tokens, and prompts too short for the tiled kernels.
 //
-// fp16 cache.  A CTA takes a chunk of one sequence's keys for one key/value head and the
-// (up to 8 or 16) query heads that share it; its four warps take every fourth
-// 16-key step each and run alone, without any exchange until the end:
+// fp16 cache.  A CTA takes a chunk of one sequence's keys for one key/value
+// head and 8 or 16 packed rows (token, query head of the group); its four
+// warps take every fourth 16-key step each and run alone, without any exchange
+// until the end:
 //   * the step's K and V rows stream through the warp's own ring in shared
-//     memory (cp.async, 16-byte pieces, 8 KB a step at 128 dims; pages by the
+//     memory (cp.async, 16-byte pieces, 8 KB a step at 128 dims; the page's
 //     table entry fetched one step ahead).  Rows past the end and pages that
 //     are none come as zeros;
-//   * S = Q K^T and O += P V by mma.sync m16n8k16: eight queries' fp16 high
+//   * S = Q K^T and O += P V by mma.sync m16n8k16: eight rows' fp16 high
 //     parts are rows 0-7 of A and their low parts rows 8-15, so fp32 queries
 //     and weights cost no extra instruction and the two row halves are added
 //     afterwards.  tcgen05 wants 128 rows; here there are 8 or 16;
-//   * running maximum and sum per query as in the prompt kernel (followed
+//   * running maximum and sum per row as in the prompt kernel (followed
 //     only beyond a factor 2^8, weights biased by 2^7).
 // The four warps' results are joined in shared memory; with a split key axis
-// (or a prefix) the joining kernel adds the chunks.
+// the joining kernel adds the chunks, without one this kernel adds a prefix's.
 //
 // Bound: HBM.  A 16-key step is 8 KB and 32 MMAs (HD 128), ~1/16 of what the
-// tensor pipe does in the time the bytes take.
+// tensor pipe does in the time the bytes take.  Sixteen sequences of 1..4096
+// keys, 32 x 128: 90 to 94 us, 5.2 to 5.4 TB/s.  Short sequences leave the bus
+// idle while CTAs start and end (32 / 8 heads: 64 of 256 keys 29 us, 2.3 TB/s).
 #include <cuda_runtime.h>
 
 #include "paged_common.cuh"
