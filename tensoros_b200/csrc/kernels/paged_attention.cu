@@ -595,6 +595,7 @@ extern "C" int tosk_paged_decode(const tosk_paged_attn_t* a, cudaStream_t st) {
     x.table = a->prefix_table;
     x.n_seqs = 1;
     x.cu_q = nullptr;
+    x.max_q = p.total_q;
     x.fixed_kv = a->prefix_len;
     x.causal = 0;
     x.splits = d.pre;
