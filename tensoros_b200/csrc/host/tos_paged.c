@@ -249,7 +249,7 @@ size_t tos_attention_prompt_paged_workspace_bytes(int n_seqs, int total_q, int m
     if (n_seqs <= 0 || total_q <= 0 || max_q <= 0 || max_kv < 0 || n_heads <= 0 || n_kv <= 0 || n_heads % n_kv ||
         head_dim <= 0 || head_dim > MAX_HEAD_DIM)
         return 0;
-    return tosk_paged_prompt_ws_bytes(total_q, max_kv, n_heads, n_kv, head_dim);
+    return tosk_paged_prompt_ws_bytes(n_seqs, total_q, max_kv, n_heads, n_kv, head_dim);
 }
 
 static tosk_paged_attn_t attn_of(const tos_rows_t *out, const tos_rows_t *q, const tos_paged_kv_t *kv,

@@ -304,7 +304,7 @@ typedef struct {
     size_t ws_bytes;
     int *err;
 } tosk_paged_attn_t;
-size_t tosk_paged_prompt_ws_bytes(int total_q, int max_kv, int n_heads, int n_kv, int hd);
+size_t tosk_paged_prompt_ws_bytes(int n_seqs, int total_q, int max_kv, int n_heads, int n_kv, int hd);
 size_t tosk_paged_decode_ws_bytes(int n_seqs, int max_kv, int prefix_len, int n_heads, int n_kv, int hd);
 int tosk_paged_prompt(const tosk_paged_attn_t *a, cudaStream_t st);
 int tosk_paged_decode(const tosk_paged_attn_t *a, cudaStream_t st);

@@ -537,18 +537,23 @@ int run_tiles(const PagedProblem& p, cudaStream_t st) {
   return paged_tc_ok(p) ? paged_tc_run(p, st) : run_general(p, st);
 }
 
-// Splits of a prompt call's keys (0: none).  Fewer row tiles than SMs leave
-// SMs without work, so the keys are cut into the number of splits with the
-// shortest schedule, counted in key tiles of 128: rounds over the SMs, each
-// its share of the keys and ~3.5 tiles' worth of starting and ending a piece;
-// the joining ~2, and a tile's worth for every 1.1 M elements of partial rows.
-// (Measured: a key tile takes 2.4 us with fp16 rows, 4.0 with fp32 rows.)
-int plan_prompt(int total_q, int max_kv, int heads, int n_kv, int hd) {
-  const long long tiles = ((long long)total_q * (heads / n_kv) + 255) / 256 * n_kv;
-  if (tiles >= kSms) return 0;
+// Splits of a prompt call's keys (0: none).  Up to two rounds of row tiles over
+// the SMs, the keys are cut into the number of splits with the shortest
+// schedule, counted in key tiles of 128: rounds over the SMs, each its share
+// of the keys and ~3.5 tiles' worth of starting and ending a piece; the joining
+// ~2, and a tile's worth for every 1.1 M elements of partial rows.  (A key tile
+// takes 2.4 us with fp16 rows, 4.0 with fp32 rows.)  A sequence has a row tile
+// of its own, however short: 16 sequences of 8 tokens behind 4096 keys take
+// 76 us, 106 where only packed rows are counted; 20 of 16, 122, unsplit 139.
+// The estimate does not see that a causal prompt's row tiles differ in length:
+// 1200 tokens behind 4000 keys, fp16, 169 us, unsplit 160.
+int plan_prompt(int n_seqs, int total_q, int max_kv, int heads, int n_kv, int hd) {
+  const long long packed = ((long long)total_q * (heads / n_kv) + 255) / 256;
+  const long long tiles = (packed > n_seqs ? packed : n_seqs) * n_kv;
+  if (tiles >= 2 * kSms) return 0;
   const float keys = max_kv / 128.0f, rows = (float)total_q * heads * hd / 1.1e6f;
   int best = 1;
-  float cost = keys + 3.5f;
+  float cost = (float)((tiles + kSms - 1) / kSms) * (keys + 3.5f);
   for (int s = 2; s <= 16 && s <= max_kv / 512; ++s) {
     const float c = (float)((s * tiles + kSms - 1) / kSms) * (keys / s + 3.5f) + 2.0f + s * rows;
     if (c < cost) {
@@ -563,8 +568,8 @@ int plan_prompt(int total_q, int max_kv, int heads, int n_kv, int hd) {
 // Keys of one piece of a prompt's work.
 int prompt_keys(int splits, int max_kv) { return splits ? chunk_of(max_kv, splits) : max_kv; }
 
-extern "C" size_t tosk_paged_prompt_ws_bytes(int total_q, int max_kv, int n_heads, int n_kv, int hd) {
-  const int splits = plan_prompt(total_q, max_kv, n_heads, n_kv, hd);
+extern "C" size_t tosk_paged_prompt_ws_bytes(int n_seqs, int total_q, int max_kv, int n_heads, int n_kv, int hd) {
+  const int splits = plan_prompt(n_seqs, total_q, max_kv, n_heads, n_kv, hd);
   return slots_bytes(splits, total_q, n_heads, hd) + paged_tc_fold_bytes(prompt_keys(splits, max_kv));
 }
 
@@ -577,7 +582,7 @@ extern "C" size_t tosk_paged_decode_ws_bytes(int n_seqs, int max_kv, int prefix_
 
 extern "C" int tosk_paged_prompt(const tosk_paged_attn_t* a, cudaStream_t st) {
   PagedProblem p = problem_of(a);
-  p.splits = plan_prompt(a->total_q, a->max_kv, a->n_heads, a->kv.n_kv, a->kv.hd);
+  p.splits = plan_prompt(a->n_seqs, a->total_q, a->max_kv, a->n_heads, a->kv.n_kv, a->kv.hd);
   p.chunk = prompt_keys(p.splits, a->max_kv);
   part_views(p, a->ws, p.splits, paged_tc_fold_bytes(p.chunk));
   const int e = run_tiles(p, st);

@@ -1044,10 +1044,10 @@ bool paged_tc_ok(const PagedProblem& p) {
          (long long)ps * p.n_kv * p.hd * 2 < (1ll << 39);
 }
 
-// Row tiles of one key/value head that a call can have at most.
 // Bytes of PagedProblem::fold that fp32 rows over so many keys need.
 size_t paged_tc_fold_bytes(int keys) { return keys > kFold * kKeys ? (size_t)kTcCtas * 2 * kRows * 128 * 4 : 0; }
 
+// Row tiles of one key/value head that a call can have at most.
 long long paged_tc_tiles(int n_seqs, int total_q, int max_q, int group) {
   const long long each = ((long long)max_q * group + 2 * kRows - 1) / (2 * kRows) * n_seqs;
   const long long all = (long long)total_q * group / (2 * kRows) + n_seqs;
