@@ -178,7 +178,20 @@ int tos_attention_noalloc_dev(float *out, const float *q, const void *k_cache, c
  * captured graphs that may overlap need one each) and give the same bits
  * run to run.  Lengths, positions and tables are device arrays, so a
  * captured call may be replayed after they changed within the bounds given.
- * The calls run on the library's device, whatever the caller's current one. */
+ * The calls run on the library's device, whatever the caller's current one.
+ *
+ * Rows of fp32 are attended to in fp32 (products of two-part fp16 numbers, or
+ * fp32 arithmetic); rows of fp16 may round a weight to fp16, half a step.
+ * Sums, maxima, norms and angles have 32 bits or more.  An attention call has
+ * at most 65535 sequences, 2^25 keys a sequence or prefix and 2^30 rows (tokens
+ * times query heads of a group) a sequence: TOS_ENOTSUP beyond.
+ *
+ * A workspace is 16-byte aligned and has the bytes that its _workspace_bytes
+ * call gives for these very arguments (not fewer for larger ones: they follow
+ * the split of the keys).  Prompts: 19.4 MB for the sums of fp32 rows where a
+ * piece of the keys is longer than 384, and the split's partial rows; decoding:
+ * (splits + prefix splits) * n_seqs * n_heads * (head_dim + 2) * 4 bytes, and
+ * the 19.4 MB.  0: none, NULL will do. */
 
 /* Rows of tokens: token t's heads lie at ptr + t * stride elements, head h
  * at h * head_dim from there.  type: TOS_TYPE_F32 or TOS_TYPE_F16. */

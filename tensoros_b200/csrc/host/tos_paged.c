@@ -10,7 +10,8 @@
 #include "tos_internal.h"
 
 #define MAX_HEAD_DIM 256
-#define MAX_ROWS (1 << 30)   /* keys of a sequence, packed rows of a sequence: 32-bit arithmetic with room */
+#define MAX_ROWS (1 << 30)   /* packed rows of a sequence: 32-bit arithmetic with room */
+#define MAX_KEYS (1 << 25)   /* keys of a sequence: 1 s at 4 us a key tile, the kernels' waits end after 2 s */
 #define MAX_SEQS 65535
 
 struct tos_rotary {
@@ -276,7 +277,7 @@ int tos_attention_prompt_paged_dev(const tos_rows_t *out, const tos_rows_t *q, c
     int rc = attn_check(out, q, kv, n_heads, scale);
     if (!rc && (n_seqs < 0 || n_seqs > kv->n_seqs || total_q < 0 || max_q < 0 || max_kv < 0)) rc = TOS_EINVAL;
     if (!rc && n_seqs && (!cu_q || !kv_len || ((uintptr_t)cu_q & 3) || ((uintptr_t)kv_len & 3))) rc = TOS_EINVAL;
-    if (!rc && (max_kv > MAX_ROWS || n_seqs > MAX_SEQS || (int64_t)max_q * (n_heads / kv->n_kv) > MAX_ROWS))
+    if (!rc && (max_kv > MAX_KEYS || n_seqs > MAX_SEQS || (int64_t)max_q * (n_heads / kv->n_kv) > MAX_ROWS))
         rc = TOS_ENOTSUP;
     if (!rc)
         rc = ws_check(ws, ws_bytes, tos_attention_prompt_paged_workspace_bytes(n_seqs, total_q, max_q, max_kv,
@@ -308,7 +309,7 @@ int tos_attention_decode_paged_dev(const tos_rows_t *out, const tos_rows_t *q, c
     if (!rc && (n_seqs < 0 || n_seqs > kv->n_seqs || max_kv < 0 || prefix_len < 0)) rc = TOS_EINVAL;
     if (!rc && n_seqs && (!kv_len || ((uintptr_t)kv_len & 3))) rc = TOS_EINVAL;
     if (!rc && prefix_len && (!prefix_table || ((uintptr_t)prefix_table & 3))) rc = TOS_EINVAL;
-    if (!rc && (max_kv > MAX_ROWS || prefix_len > MAX_ROWS || n_seqs > MAX_SEQS ||
+    if (!rc && (max_kv > MAX_KEYS || prefix_len > MAX_KEYS || n_seqs > MAX_SEQS ||
                 (int64_t)n_seqs * (n_heads / kv->n_kv) > MAX_ROWS))
         rc = TOS_ENOTSUP;
     if (!rc)

@@ -121,12 +121,12 @@ def test_attention_refusals(lib):
 
 
 def test_attention_limits(lib):
-    """What 32-bit counts of rows and the joining grid do not hold."""
-    assert prompt(lib, mk=(1 << 30) + 1) == ENOTSUP
+    """What 32-bit counts of rows, the joining grid and the kernels' waits do not hold."""
+    assert prompt(lib, mk=(1 << 25) + 1) == ENOTSUP
     assert prompt(lib, mq=1 << 30, heads=4) == ENOTSUP
     assert prompt(lib, c=kv(n_seqs=70000), n=70000) == ENOTSUP
-    assert decode(lib, mk=(1 << 30) + 1) == ENOTSUP
-    assert decode(lib, pl=(1 << 30) + 1) == ENOTSUP
+    assert decode(lib, mk=(1 << 25) + 1) == ENOTSUP
+    assert decode(lib, pl=(1 << 25) + 1) == ENOTSUP
     assert decode(lib, c=kv(n_seqs=70000), n=70000) == ENOTSUP
     assert decode(lib, scale=3e38) == EINVAL
 
