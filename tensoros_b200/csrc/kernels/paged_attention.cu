@@ -524,9 +524,16 @@ void part_views(PagedProblem& p, void* ws, int slots, size_t fold) {
 //   fp16 cache      6 x 48:  38 MB 14.5 / 13.2, 151 MB 20.7 / 26.7
 //     fp32 rows    32 x 128:  8 MB 12.3 / 11.1,  34 MB 12.8 / 13.2, 134 MB 17.8 / 25.3
 //     fp16 rows    32 x 128:  1 MB  8.9 / 10.8
+// A shared prefix goes by its rows a key/value head (all tokens' together), one
+// row tile for fp16 caches; a decode call behind 4096 and 16384 keys (us):
+//   fp32 cache  32 x 128,   8 rows: 142, 576 / 56, 177;  32 rows: 202, 912 / 140, 480;
+//               128 rows: 386 / 493 at 4096;  8 heads, 32 rows: 62, 177 / 50, 120
+//   fp16 cache  32 x 128,   8 rows, fp32: 54, 194 / 32, 73;   fp16: 36, 112 / 32, 73
+//               32 rows, fp32: 71, 206 / 73, 187;  fp16: 52, 124 / 67, 179
 bool few_rows(const PagedProblem& p) {
-  if (p.fixed_kv >= 0 || !paged_decode_ok(p)) return false;
+  if (!paged_decode_ok(p)) return false;
   const bool f16 = p.kv_type == TOSK_F16;
+  if (p.fixed_kv >= 0) return p.total_q * (long long)p.group <= (f16 && paged_tc_ok(p) ? 8 : 32);
   const long long mb = !f16 ? 150 : p.hd <= 64 ? 40 : p.type == TOSK_F32 ? 30 : 0;
   // the tensor cores refuse what the few-rows kernel takes (odd pages, 256 dims): the general kernel is the other then
   const long long most = (f16 && !paged_tc_ok(p) ? 150 : mb) * 1000000;

@@ -581,3 +581,13 @@ def test_prompt_of_many_sequences(gpu, qk, kv, hd):
     kv_lens = [n + (i * 13) % 90 for i, n in enumerate(q_lens)]
     c = Cache(kv_lens, 16, 2, hd, kv, seed=4)
     R.check_prompt(gpu, c, randn(sum(q_lens), 8, hd, seed=5, kind=qk), q_lens, kv_lens, 8)
+
+
+@pytest.mark.parametrize("qk,kv", KINDS)
+@pytest.mark.parametrize("heads,n_kv,hd,page,n", [(8, 4, 128, 16, 4), (8, 4, 128, 16, 5), (4, 4, 64, 64, 32),
+                                                  (4, 4, 64, 64, 33), (12, 1, 256, 5, 2), (6, 6, 48, 32, 1)])
+def test_prefix_around_the_limits_of_a_row_tile(gpu, qk, kv, heads, n_kv, hd, page, n):
+    """8, 10, 32 and 33 rows a key/value head behind prefixes of a page and of many splits."""
+    for prefix in (1, page, 2111):
+        c = Cache([(i * 37) % 150 for i in range(n)], page, n_kv, hd, kv, seed=n + prefix, prefix=prefix)
+        R.check_decode(gpu, c, randn(n, heads, hd, seed=prefix, kind=qk), heads)
