@@ -591,3 +591,15 @@ def test_prefix_around_the_limits_of_a_row_tile(gpu, qk, kv, heads, n_kv, hd, pa
     for prefix in (1, page, 2111):
         c = Cache([(i * 37) % 150 for i in range(n)], page, n_kv, hd, kv, seed=n + prefix, prefix=prefix)
         R.check_decode(gpu, c, randn(n, heads, hd, seed=prefix, kind=qk), heads)
+
+
+@pytest.mark.parametrize("qk,kv", KINDS)
+@pytest.mark.parametrize("heads,n_kv,hd,page", [(71, 1, 64, 256), (128, 1, 128, 512), (28, 4, 120, 24), (9, 1, 96, 100)])
+def test_wide_and_odd_groups(gpu, qk, kv, heads, n_kv, hd, page):
+    """Groups that are no power of two or fill a row tile alone, pages larger than a key tile or across its end."""
+    q_lens = [3, 0, 41]
+    kv_lens = [300, 5, 41]
+    c = Cache(kv_lens, page, n_kv, hd, kv, seed=heads)
+    R.check_prompt(gpu, c, randn(sum(q_lens), heads, hd, seed=8, kind=qk), q_lens, kv_lens, heads)
+    c = Cache(kv_lens, page, n_kv, hd, kv, seed=heads, prefix=777)
+    R.check_decode(gpu, c, randn(3, heads, hd, seed=9, kind=qk), heads)
