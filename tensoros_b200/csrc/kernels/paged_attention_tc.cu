@@ -119,9 +119,17 @@ __device__ __forceinline__ void tc_wait_ld8(uint32_t (&r)[8]) {
 // a clock of the SFU.  x = n + f, |f| <= 1/2: n by adding 1.5 2^23, 2^f by a
 // degree-4 polynomial fitted here for least relative error (2.6e-6, far below
 // the weights' fp16 rounding), 2^n into the exponent.  Below 2^-126: 2^-126.
+// A NaN gives kNanWeight, the largest float: a NaN's bits, 0x7fffffff, and the
+// same shifted by 23 are added.
+constexpr float kNanWeight = 3.402823466e38f;
+__device__ __forceinline__ float max_nan(float x, float y) {
+  float z;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(z) : "f"(x), "f"(y));
+  return z;
+}
 __device__ __forceinline__ float2 exp2_fma(float2 x) {
-  x.x = fmaxf(x.x, -126.0f);
-  x.y = fmaxf(x.y, -126.0f);
+  x.x = max_nan(x.x, -126.0f);
+  x.y = max_nan(x.y, -126.0f);
   const float2 big = make_float2(12582912.0f, 12582912.0f), nbig = make_float2(-12582912.0f, -12582912.0f);
   const float2 n = __fadd2_rn(x, big);
   const float2 r = __fadd2_rn(n, nbig);
@@ -864,7 +872,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
         tmem_st_wait();
         tc_fence_before();
         mbar_arrive(pfull + 2 * i + hf);
-        l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+        const float part = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+        // a NaN score that exp2_fma met makes the row NaN as any other does
+        // (a maximum that keeps NaN costs packed prompts 1%)
+        l += !SPLIT && part >= kNanWeight ? __int_as_float(0x7fffffff) : part;
       }
       cnt += nt;
       take(n + 1);

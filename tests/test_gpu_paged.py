@@ -603,3 +603,29 @@ def test_wide_and_odd_groups(gpu, qk, kv, heads, n_kv, hd, page):
     R.check_prompt(gpu, c, randn(sum(q_lens), heads, hd, seed=8, kind=qk), q_lens, kv_lens, heads)
     c = Cache(kv_lens, page, n_kv, hd, kv, seed=heads, prefix=777)
     R.check_decode(gpu, c, randn(3, heads, hd, seed=9, kind=qk), heads)
+
+
+# ------------------------------------------ keys and values that are not finite
+
+@pytest.mark.parametrize("qk,kv", KINDS)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("n,hist", [(600, 0), (40, 300)])
+def test_seen_nan_key_at_every_place(gpu, qk, kv, hd, n, hist):
+    """A NaN in one key of each head, at all 16 places of a step and all over
+    the last 128 keys: the rows that see it are NaN, the others as without it."""
+    heads = 16
+    c = Cache([n + hist], 16, heads, hd, kv, seed=5)
+    q = randn(n, heads, hd, seed=6, kind=qk)
+    k, v = c.rows(0)
+    pg, r = c.where(c.table[0], n + hist)
+    at = [n + hist - 128 + (17 * h) % 128 for h in range(heads)]
+    for h in range(heads):
+        c.k[pg[at[h]], r[at[h]], h, (5 * h) % hd] = float("nan")
+    out, st = R.prompt(gpu, c, q, [n], [n + hist], heads, hd ** -0.5)
+    assert st == 0
+    lim = torch.arange(n, device="cuda") + hist + 1
+    ref, err = R.attend(q, k, v, float(np.float32(hd ** -0.5)), lim)
+    for h in range(heads):
+        sees = lim > at[h]
+        assert bool(torch.isnan(out[sees, h]).all()), (h, at[h])
+        R.assert_rows(out[~sees, h], ref[~sees, h], err[~sees, h], (h, at[h]))
