@@ -11,7 +11,10 @@
 
 #define MAX_HEAD_DIM 256
 #define MAX_ROWS (1 << 30)   /* packed rows of a sequence: 32-bit arithmetic with room */
-#define MAX_KEYS (1 << 25)   /* keys of a sequence: 1 s at 4 us a key tile, the kernels' waits end after 2 s */
+/* Keys of a sequence: unsplit, a piece of work over them takes 1 s at 4 us a
+ * key tile.  No bounded wait of the kernels spans more than one piece, and they
+ * end after 2 s; what rows with infinities and NaN take comes after the last. */
+#define MAX_KEYS (1 << 25)
 #define MAX_SEQS 65535
 
 struct tos_rotary {

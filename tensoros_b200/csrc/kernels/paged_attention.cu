@@ -68,7 +68,7 @@ __global__ void __launch_bounds__(kGenThreads) paged_attn_general_kernel(const _
   float* sk = sq + R * LD;              // [kKT][LD]
   float* sv = sk + kKT * LD;            // [kKT][LD]
   float* sp = sv + kKT * LD;            // [R][LP]
-  __shared__ int s_bad[R];
+  __shared__ int s_dirty;               // values that are not finite were left out
   __shared__ long long s_off[2][kKT];   // where the rows of a tile lie
   const PagedProblem& p = a.p;
   pdl_wait();
@@ -84,6 +84,7 @@ __global__ void __launch_bounds__(kGenThreads) paged_attn_general_kernel(const _
   const int rows = t.qn * p.group, r0 = rt * R;
   if (r0 >= rows) return;
   const int nr = min(R, rows - r0);
+  const int first = seen(p, t, r0 / p.group);          // keys that all rows see
   int k0 = 0, k1 = seen(p, t, (r0 + nr - 1) / p.group);
   if (p.splits) {
     k0 = split * p.chunk;
@@ -105,13 +106,19 @@ __global__ void __launch_bounds__(kGenThreads) paged_attn_general_kernel(const _
       vx = load4_tail(p.v, p.kv_type, off, 4 * c, p.hd, a.kv_vec);
     }
   };
-  auto put = [&](int i, const float4& kx, const float4& vx) {
+  auto put = [&](int i, int kt, const float4& kx, float4 vx) {
     const int r = i / (16 * NJ), c = i % (16 * NJ);
+    if (kt + r >= first && (not_finite(vx.x) || not_finite(vx.y) || not_finite(vx.z) || not_finite(vx.w))) {
+      uint4 u = make_uint4(__float_as_uint(vx.x), __float_as_uint(vx.y), __float_as_uint(vx.z), __float_as_uint(vx.w));
+      clean_piece<float>(u);
+      vx = make_float4(__uint_as_float(u.x), __uint_as_float(u.y), __uint_as_float(u.z), __uint_as_float(u.w));
+      s_dirty = 1;
+    }
     *reinterpret_cast<float4*>(sk + r * LD + 4 * c) = kx;
     *reinterpret_cast<float4*>(sv + r * LD + 4 * c) = vx;
   };
   place(k0, 0);
-  for (int i = tid; i < R; i += kGenThreads) s_bad[i] = 0;
+  if (tid == 0) s_dirty = 0;
 #pragma unroll 4
   for (int i = tid; i < R * 16 * NJ; i += kGenThreads) {
     const int r = i / (16 * NJ), c = i % (16 * NJ);
@@ -147,11 +154,11 @@ __global__ void __launch_bounds__(kGenThreads) paged_attn_general_kernel(const _
 #pragma unroll
     for (int x = 0; x < NL; ++x) {
       if (AHEAD) {
-        put(tid + x * kGenThreads, rk[AHEAD ? x : 0], rv[AHEAD ? x : 0]);
+        put(tid + x * kGenThreads, kt, rk[AHEAD ? x : 0], rv[AHEAD ? x : 0]);
       } else {
         float4 kx, vx;
         piece(tid + x * kGenThreads, buf, kx, vx);
-        put(tid + x * kGenThreads, kx, vx);
+        put(tid + x * kGenThreads, kt, kx, vx);
       }
     }
     __syncthreads();
@@ -239,6 +246,14 @@ __global__ void __launch_bounds__(kGenThreads) paged_attn_general_kernel(const _
     const int r = ty + 16 * i;
     if (r >= nr) continue;
     const int rr = r0 + r, tok = t.q0 + rr / p.group, h = kvh * p.group + rr % p.group;
+    if (s_dirty) {
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (4 * tx + 64 * j + e < p.hd)
+            o[i][j][e] += bad_value(p, t.table, kvh, max(first, k0), lim[i], 4 * tx + 64 * j + e);
+    }
     if (p.splits) {
       const long long row = (long long)(p.slot0 + split) * p.total_q * p.heads + (long long)tok * p.heads + h;
       if (tx == 0) p.part_ml[row] = make_float2(m[i], sum);
@@ -250,28 +265,13 @@ __global__ void __launch_bounds__(kGenThreads) paged_attn_general_kernel(const _
     } else {
       const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
       const long long oo = (long long)tok * p.out_stride + (long long)h * p.hd;
-      bool bad = false;
 #pragma unroll
       for (int j = 0; j < NJ; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float v = o[i][j][e] * inv;
-          if (4 * tx + 64 * j + e < p.hd) {
-            store_elem(p.out, p.type, oo + 4 * tx + 64 * j + e, v);
-            bad |= isnan(v);
-          }
-        }
-      if (bad) s_bad[r] = 1;
+        for (int e = 0; e < 4; ++e)
+          if (4 * tx + 64 * j + e < p.hd) store_elem(p.out, p.type, oo + 4 * tx + 64 * j + e, o[i][j][e] * inv);
     }
   }
-  if (p.splits) return;
-  __syncthreads();
-  for (int r = tid >> 5; r < nr; r += kGenThreads / 32)
-    if (s_bad[r]) {
-      const int rr = r0 + r;
-      attn_row_plain(p, nullptr, 0, t.table, seen(p, t, rr / p.group), t.q0 + rr / p.group,
-                     kvh * p.group + rr % p.group);
-    }
 }
 
 // Joins the partial rows of a split key axis: o = sum_s 2^(m_s - M) o_s /
@@ -279,8 +279,6 @@ __global__ void __launch_bounds__(kGenThreads) paged_attn_general_kernel(const _
 struct JoinArgs {
   PagedProblem p;              // of the sequences' own keys; splits: slots they have
   int pre_splits;              // slots of the prefix, all of them written
-  const int* prefix_table;
-  int prefix_len;
   int out_vec;                 // four-element stores to out are aligned
 };
 
@@ -352,15 +350,11 @@ __global__ void __launch_bounds__(128) paged_attn_join_kernel(const __grid_const
   for (int x = 16; x > 0; x >>= 1) L += __shfl_xor_sync(0xffffffffu, L, x);
   const float inv = L == 0.0f ? 0.0f : 1.0f / L;
   const long long oo = (long long)tok * p.out_stride + (long long)h * p.hd;
-  bool bad = false;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const int d = (lane + 32 * i) * V;
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      o[i][e] = L == 0.0f ? 0.0f : o[i][e] * inv;
-      bad |= d < p.hd && isnan(o[i][e]);
-    }
+    for (int e = 0; e < V; ++e) o[i][e] = L == 0.0f ? 0.0f : o[i][e] * inv;
     if (d >= p.hd) continue;
     if constexpr (V == 4) {
       if (a.out_vec && p.type == TOSK_F32) {
@@ -379,7 +373,6 @@ __global__ void __launch_bounds__(128) paged_attn_join_kernel(const __grid_const
 #pragma unroll
     for (int e = 0; e < V; ++e) store_elem(p.out, p.type, oo + d + e, o[i][e]);
   }
-  if (__any_sync(0xffffffffu, bad)) attn_row_plain(p, a.prefix_table, a.prefix_len, t.table, n, tok, h);
 }
 
 }  // namespace tos
@@ -489,12 +482,10 @@ DecodePlan plan_decode(int n_seqs, int max_kv, int prefix_len, int heads, int n_
   return d;
 }
 
-int run_join(const PagedProblem& own, int pre, const int* prefix_table, int prefix_len, cudaStream_t st) {
+int run_join(const PagedProblem& own, int pre, cudaStream_t st) {
   JoinArgs j;
   j.p = own;
   j.pre_splits = pre;
-  j.prefix_table = prefix_table;
-  j.prefix_len = prefix_len;
   const long long gx = ((long long)own.max_q * own.heads + 3) / 4;
   if (gx > 0x7fffffffll || own.n_seqs > 65535) return (int)cudaErrorInvalidValue;
   j.out_vec = aligned4(own.out, own.out_stride, own.type, own.hd);
@@ -542,7 +533,7 @@ bool few_rows(const PagedProblem& p) {
   return (long long)p.total_q * p.heads / 8 * p.max_kv * p.hd * (f16 ? 4 : 8) <= most;
 }
 int run_tiles(const PagedProblem& p, cudaStream_t st) {
-  if (few_rows(p)) return paged_decode_run(p, PagedPrefix{0, 0, nullptr}, st);
+  if (few_rows(p)) return paged_decode_run(p, 0, st);
   return paged_tc_ok(p) ? paged_tc_run(p, st) : run_general(p, st);
 }
 
@@ -595,7 +586,7 @@ extern "C" int tosk_paged_prompt(const tosk_paged_attn_t* a, cudaStream_t st) {
   p.chunk = prompt_keys(p.splits, a->max_kv);
   part_views(p, a->ws, p.splits, paged_tc_fold_bytes(p.chunk));
   const int e = run_tiles(p, st);
-  return e || !p.splits ? e : run_join(p, 0, nullptr, 0, st);
+  return e || !p.splits ? e : run_join(p, 0, st);
 }
 
 extern "C" int tosk_paged_decode(const tosk_paged_attn_t* a, cudaStream_t st) {
@@ -620,7 +611,7 @@ extern "C" int tosk_paged_decode(const tosk_paged_attn_t* a, cudaStream_t st) {
   p.splits = d.own;
   p.chunk = d.own_chunk;
   p.slot0 = d.pre;
-  const int e = fast ? paged_decode_run(p, PagedPrefix{d.pre, a->prefix_len, a->prefix_table}, st) : run_general(p, st);
+  const int e = fast ? paged_decode_run(p, d.pre, st) : run_general(p, st);
   if (e || !d.own) return e;
-  return run_join(p, d.pre, a->prefix_table, a->prefix_len, st);
+  return run_join(p, d.pre, st);
 }

@@ -45,9 +45,10 @@
 // 1.1e-6 against 64 bits (norm) over 7512 keys.
 //
 // Keys behind a row's last one are masked in S; value rows behind the key
-// range are zeroed in shared memory (a page's unused rows may hold
-// anything), and a row that shows NaN is computed again key by key
-// (attn_row_plain), so an unseen infinity never reaches it.
+// range (a page's unused rows may hold anything) and, where only some rows see
+// a key, values that are not finite are zeroed in shared memory, so that an
+// unseen infinity never reaches a row.  Rows that do see one get it at the end of
+// the CTA, when the pipeline is done and none of its bounded waits runs (patch_piece).
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <cuda_runtime.h>
@@ -86,7 +87,7 @@ struct TcShape {
   static constexpr int kSlots = HD == 128 ? (SPLIT ? 3 : 5) : 8;
   static constexpr int kBars = 2 * kSlots + 17;
   static constexpr int kStage = kQ >= 16 * 4096 ? 0 : 16 * 4096;     // output rows, where Q's place is too small for them
-  static constexpr int kSmem = kQ + kSlots * kTile + kStage + kBars * 8 + 8 + 2 * 64 + 4 * kRows * 4;
+  static constexpr int kSmem = kQ + kSlots * kTile + kStage + kBars * 8 + 8 + 2 * 64 + 4 * kRows * 4 + 16;
   static_assert(kSmem <= 227 * 1024, "shared memory");
 };
 
@@ -270,6 +271,11 @@ __device__ __forceinline__ TileId pick_tile(const PagedProblem& p, int f, PlanCu
   return pick_of_many(p, f, cur);
 }
 
+// The k-th piece of this CTA: they go round the CTAs there and back.
+__device__ __forceinline__ int piece_of(int k) {
+  return k * (int)gridDim.x + (k & 1 ? (int)gridDim.x - 1 - (int)blockIdx.x : (int)blockIdx.x);
+}
+
 // Scores from the n-th on count for nothing.
 template <int N>
 __device__ __forceinline__ void mask_from(uint32_t (&s)[N], int n) {
@@ -277,15 +283,16 @@ __device__ __forceinline__ void mask_from(uint32_t (&s)[N], int n) {
   for (int e = 0; e < N; ++e)
     if (e >= n) s[e] = 0xff800000u;                                     // -inf
 }
-template <int N>
+template <bool NANS, int N>
 __device__ __forceinline__ float max_of(const uint32_t (&s)[N]) {
-  float a = fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1])), b = fmaxf(__uint_as_float(s[2]), __uint_as_float(s[3]));
+  auto top = [](float x, float y) { return NANS ? max_nan(x, y) : fmaxf(x, y); };
+  float a = top(__uint_as_float(s[0]), __uint_as_float(s[1])), b = top(__uint_as_float(s[2]), __uint_as_float(s[3]));
 #pragma unroll
   for (int e = 4; e < N; e += 4) {
-    a = fmaxf(fmaxf(a, __uint_as_float(s[e])), __uint_as_float(s[e + 1]));
-    b = fmaxf(fmaxf(b, __uint_as_float(s[e + 2])), __uint_as_float(s[e + 3]));
+    a = top(top(a, __uint_as_float(s[e])), __uint_as_float(s[e + 1]));
+    b = top(top(b, __uint_as_float(s[e + 2])), __uint_as_float(s[e + 3]));
   }
-  return fmaxf(a, b);
+  return top(a, b);
 }
 // Multiplies n columns of this warp's 32 rows in tensor memory.  Rarely
 // called: out of line, so that its registers cost the loop around it none.
@@ -348,8 +355,178 @@ struct __align__(16) Work {
   int seq, kvh, split, r0;            // seq < 0: no more
   int rows, q0, off, kvn;             // the sequence's packed rows and first token; its SeqTask's off, kvn
   int k0, k1, nt[2];                  // key tiles of the two row tiles
-  int pad[4];
+  int first;                          // keys that all rows see
+  int pad[3];
 };
+
+// Rows r0 .. r1 - 1 of a tile of values in shared memory: elements that are not
+// finite become zeros.  By a warp; whether any did.
+template <int HALVES>
+static __device__ __noinline__ bool clean_tile(uint8_t* vt, int r0, int r1) {
+  const int lane = threadIdx.x & 31;
+  const __half2 zero = __floats2half2_rn(0.0f, 0.0f);
+  __half2 odd[4] = {zero, zero, zero, zero};             // NaN once one was met
+#pragma unroll 1
+  for (int h = 0; h < HALVES; ++h)
+#pragma unroll 1
+    for (int o = r0 * 128 + lane * 16; o < r1 * 128; o += 8 * 512) {
+      uint4 u[8];
+#pragma unroll
+      for (int x = 0; x < 8; ++x)
+        u[x] = o + x * 512 < r1 * 128 ? *reinterpret_cast<const uint4*>(vt + h * 16384 + o + x * 512) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int x = 0; x < 8; ++x) {
+        const uint32_t w[4] = {u[x].x, u[x].y, u[x].z, u[x].w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) odd[i] = __hfma2(*reinterpret_cast<const __half2*>(&w[i]), zero, odd[i]);
+      }
+    }
+  const float2 f = __half22float2(__hadd2(__hadd2(odd[0], odd[1]), __hadd2(odd[2], odd[3])));
+  if (!__any_sync(0xffffffffu, isnan(f.x) || isnan(f.y))) return false;
+#pragma unroll 1
+  for (int h = 0; h < HALVES; ++h)
+#pragma unroll 1
+    for (int o = r0 * 128 + lane * 16; o < r1 * 128; o += 512) {
+      uint4* at = reinterpret_cast<uint4*>(vt + h * 16384 + o);
+      uint4 u = *at;
+      if (clean_piece<__half>(u)) *at = u;
+    }
+  return true;
+}
+
+constexpr uint32_t kNanRow = 0xffffffffu;    // in a row that is NaN by its weights: a NaN that no arithmetic gives
+
+// A piece that may have met values that are not finite: an element of an output
+// or partial row becomes the sum of those that its row sees, where there are
+// such.  By a warp: a lane looks at eight dims of every KP-th key, 8 KP keys in
+// flight, and adds up what the keys that all rows see have; of the others (at
+// most 255), which were left out, it notes the ones with such a value, and adds
+// them as the rows come to see them.
+template <int HD>
+static __device__ __noinline__ void patch_piece(const PagedProblem& p, const SeqTask& t, int kvh, int split, int r0) {
+  constexpr int PC = HD / 8, KP = 32 / PC, U = 8;
+  const int lane = threadIdx.x & 31, d0 = lane % PC * 8, sub = lane / PC;
+  const bool has = d0 < p.hd;
+  const int rows = min(t.qn * p.group, r0 + 2 * kRows), k0 = p.splits ? split * p.chunk : 0;
+  int k1 = seen(p, t, row_token(p, rows - 1));
+  if (p.splits) k1 = min(k1, k0 + p.chunk);
+  const int first = max(k0, min(k1, seen(p, t, row_token(p, r0))));
+  const __half* vb = reinterpret_cast<const __half*>(p.v) + d0;
+  float s[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) s[e] = 0.0f;
+  auto add = [&](const uint4& u) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      if (not_finite(f.x)) s[2 * i] += f.x;
+      if (not_finite(f.y)) s[2 * i + 1] += f.y;
+    }
+  };
+  uint32_t noted = 0;                                    // lane w: keys first + 32 w ..
+#pragma unroll 1
+  for (int j = k0; j < k1; j += U * KP) {
+    uint4 u[U];
+#pragma unroll
+    for (int x = 0; x < U; ++x) {
+      const int key = j + x * KP + sub;
+      const long long off = has && key < k1 ? kv_off(p, t.table, key, kvh) : -1;
+      u[x] = off >= 0 ? *reinterpret_cast<const uint4*>(vb + off) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int x = 0; x < U; ++x) {
+      uint4 c = u[x];
+      const int key = j + x * KP + sub;
+      const bool bad = clean_piece<__half>(c);
+      if (bad && key < first) add(u[x]);
+      const uint32_t late = __ballot_sync(0xffffffffu, bad && key >= first);
+#pragma unroll
+      for (int q = 0; q < KP; ++q) {
+        const int at = j + x * KP + q - first;
+        if (late >> (q * PC) & ((1u << PC) - 1) && lane == at >> 5) noted |= 1u << (at & 31);
+      }
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    for (int o = PC; o < 32; o <<= 1) s[e] += __shfl_xor_sync(0xffffffffu, s[e], o);
+  bool any = noted != 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) any |= !(s[e] == 0.0f);
+  if (!__any_sync(0xffffffffu, any)) return;
+  const int type = p.splits ? TOSK_F32 : p.type;
+  void* out = p.splits ? p.part_o : p.out;
+  int j = first;
+#pragma unroll 1
+  for (int rb = r0; rb < rows; rb += 32) {
+    // a row a lane: the keys it sees, where it lies, whether it stays as it is
+    const int r = min(rb + lane, rows - 1), tok = t.q0 + row_token(p, r), head = kvh * p.group + row_head(p, r);
+    const long long at =
+        p.splits ? ((long long)(p.slot0 + split) * p.total_q * p.heads + (long long)tok * p.heads + head) * p.hd
+                 : (long long)tok * p.out_stride + (long long)head * p.hd;
+    const int lim = min(k1, seen(p, t, row_token(p, r)));
+    bool stays = lim <= k0;
+    if (!stays)
+      stays = type == TOSK_F32 ? reinterpret_cast<const uint32_t*>(out)[at] == kNanRow
+                               : reinterpret_cast<const uint16_t*>(out)[at] == (uint16_t)kNanRow;
+    const uint32_t skip = __ballot_sync(0xffffffffu, stays);
+#pragma unroll 1
+    for (int x = 0; x < min(32, rows - rb); ++x) {
+      const int l = __shfl_sync(0xffffffffu, lim, x);
+      for (; j < l; ++j)
+        if (__shfl_sync(0xffffffffu, noted, (j - first) >> 5) >> ((j - first) & 31) & 1) {
+          const long long off = has ? kv_off(p, t.table, j, kvh) : -1;
+          if (off >= 0) add(*reinterpret_cast<const uint4*>(vb + off));
+        }
+      const long long to = __shfl_sync(0xffffffffu, at, x) + d0;
+      if (skip >> x & 1 || !has || sub) continue;
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (!(s[e] == 0.0f)) store_elem(out, type, to + e, s[e]);
+    }
+  }
+}
+
+// fp32 rows meet an infinite element of a key as infinity times the high part
+// plus infinity times the low part of q, which is NaN where the low part is
+// zero or of the other sign.  Of 64 keys' scores in tensor memory, those that
+// are NaN by infinite elements alone become the sum of q's elements times them.
+// q: this lane's row, NULL: it has no scores to mend; left: keys it sees.
+static __device__ __noinline__ void infinite_scores(const PagedProblem& p, uint32_t ts, const int* table, int kvh, int key0,
+                                                    int left, const float* q) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll 1
+  for (int c = 0; c < 64; c += 8) {
+    uint32_t s[8];
+    tc_ld8(ts + c, s);
+    tc_wait_ld8(s);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const bool mine = q && c + e < left && isnan(__uint_as_float(s[e]));
+      if (!__any_sync(0xffffffffu, mine)) continue;
+      const long long off = kv_off(p, table, key0 + c + e, kvh);
+      float acc = 0.0f;
+      bool nan = false;
+#pragma unroll 1
+      for (int i = 0; i < p.hd; i += 32) {
+        const float k = off >= 0 && lane + i < p.hd ? load_elem(p.k, p.kv_type, off + lane + i) : 0.0f;
+        nan |= __any_sync(0xffffffffu, isnan(k));
+        uint32_t inf = __ballot_sync(0xffffffffu, isinf(k));
+        while (inf) {
+          const int b = __ffs(inf) - 1;
+          inf &= inf - 1;
+          const float kb = __shfl_sync(0xffffffffu, k, b);
+          if (mine) acc += q[i + b] * kb;
+        }
+      }
+      if (mine && !nan && !(acc == 0.0f)) s[e] = __float_as_uint(p.scale_log2 < 0.0f ? -acc : acc);
+    }
+    tc_st4(ts + c, {s[0], s[1], s[2], s[3]});
+    tc_st4(ts + c + 4, {s[4], s[5], s[6], s[7]});
+  }
+  tmem_st_wait();
+}
 
 // Q rows of a row tile, 16 rows a warp, 8 or 16 lanes a row, eight elements
 // each: asked into L2 early, then through registers into the swizzled K-major
@@ -453,6 +630,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
   static_assert(T::kBars % 2 == 1, "work lies on 16 bytes");
   Work* work = reinterpret_cast<Work*>(tailbar + 2);  // [2]
   float* sx = reinterpret_cast<float*>(work + 2);     // [tile][half of the keys][row]: exchange of the two halves
+  volatile int* odd_seen = reinterpret_cast<int*>(sx + 4 * kRows);   // values that are not finite were left out or met
   const PagedProblem& p = a.p;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (smem_u32(sm) & 1023) {                          // the swizzled tiles need it; the launch gives it
@@ -477,6 +655,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
     }
     mbar_init(tailbar, 1);
     mbar_fence_init();
+    *odd_seen = 0;
   }
   tc_fence_before();
   __syncthreads();
@@ -488,15 +667,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTcRegsRest));
     if (warp == kPlanWarp) {
       // ------------------------------------------------------------ the plan
-      // The pieces, longest first, go round the CTAs there and back, which
-      // evens out the CTAs' sums.
+      // The pieces, longest first, dealt so that the CTAs' sums are even.
       if (p.fixed_kv < 0) pdl_wait();                  // a prefix is planned from the arguments alone
       bool ok = true, more = true;
       int posted = 0;
       PlanCursor cur = {0, 0};
       const int splits = p.splits ? p.splits : 1;
       for (int k = 0; more && ok; ++k) {
-        const int g = k * (int)gridDim.x + (k & 1 ? (int)gridDim.x - 1 - (int)blockIdx.x : (int)blockIdx.x);
+        const int g = piece_of(k);
         Work w;
         w.seq = -1;
         w.kvh = g % p.n_kv;
@@ -513,6 +691,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
           w.kvn = t.kvn;
           w.k0 = 0;
           w.k1 = seen(p, t, row_token(p, min(w.rows, w.r0 + 2 * kRows) - 1));
+          w.first = seen(p, t, row_token(p, w.r0));
           if (p.splits) {
             w.k0 = w.split * p.chunk;
             w.k1 = min(w.k1, w.k0 + p.chunk);
@@ -525,7 +704,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
             w.nt[i] = e > w.k0 ? (e - w.k0 + kKeys - 1) / kKeys : 0;
           }
         }
-        if (posted >= 2) ok = mbar_wait(wempty + (posted & 1), (posted / 2 - 1) & 1, p.err, 42);
+        // for as long as a piece takes: twice the limit
+        if (posted >= 2) {
+          pdl_wait();
+          const uint32_t ph = (posted / 2 - 1) & 1;
+          ok = mbar_wait(wempty + (posted & 1), ph, nullptr, 0) || mbar_wait(wempty + (posted & 1), ph, p.err, 42);
+        }
         ok = __all_sync(0xffffffffu, ok);
         if (ok && lane == 0) {
           work[posted & 1] = w;
@@ -544,7 +728,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         const Work& w = work[n & 1];
-        const int seq = w.seq, kvh = w.kvh, k0 = w.k0, k1 = w.k1, nmax = max(w.nt[0], w.nt[1]);
+        const int seq = w.seq, kvh = w.kvh, k0 = w.k0, k1 = w.k1, first = w.first, nmax = max(w.nt[0], w.nt[1]);
         __syncwarp();
         if (lane == 0) mbar_arrive(wempty + (n & 1));
         if (seq < 0) break;
@@ -563,7 +747,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
             if (used >= T::kSlots) ok = mbar_wait(empty + s, (used / T::kSlots - 1) & 1, p.err, 31);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
-            const bool cut = v && have < kKeys;
+            // value rows behind the key range, and what is not finite where
+            // only some rows see a key, meet weights of 0: zeros instead
+            const bool some = v && kt + have > first, cut = some || (v && have < kKeys);
             uint64_t* bar = cut ? tailbar : full + s;
             if (lane == 0) mbar_arrive_expect_tx(bar, need * a.box_rows * HD * 2);
             __syncwarp();
@@ -574,8 +760,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
                 tma_page(dst + h * 16384, v ? &a.mv : &a.mk, 64 * h, kvh, row, page, bar);
             }
             if (cut) {
-              // value rows behind the key range count with weight 0: they
-              // must be finite
               ok = mbar_wait(tailbar, tails & 1, p.err, 32);
               ok = __all_sync(0xffffffffu, ok);
               if (!ok) break;
@@ -583,6 +767,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
               for (int h = 0; h < T::kHalves; ++h)
                 for (int o = have * 128 + lane * 16; o < kKeys * 128; o += 512)
                   *reinterpret_cast<uint4*>(ring + s * T::kTile + h * 16384 + o) = make_uint4(0, 0, 0, 0);
+              if (some && clean_tile<T::kHalves>(ring + s * T::kTile, max(first - kt, 0), have)) *odd_seen = 1;
               asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
               __syncwarp();
               if (lane == 0) mbar_arrive(full + s);
@@ -600,6 +785,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
         constexpr uint32_t kIdS = (1u << 4) | (8u << 24) | ((uint32_t)(kKeys >> 3) << 17);
         constexpr uint32_t kIdO = (1u << 4) | (8u << 24) | ((uint32_t)(HD >> 3) << 17) | (1u << 16);   // V is N-major
         const uint32_t tmem = tmem_at;
+        pdl_wait();                                   // its own waits are not to count what came before
         bool ok = true;
         int base = 0, c0 = 0, c1 = 0;                 // ring uses and key tiles of the two row tiles before this piece
         for (int n = 0; ok; ++n) {
@@ -756,7 +942,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
             tc_ld32(ts + 64 * hf + 32 * c, s);
             tc_wait_ld(s);
             if (cut) mask_from(s, left - 32 * c);
-            top = fmaxf(top, max_of(s));
+            top = SPLIT ? max_nan(top, max_of<true>(s)) : fmaxf(top, max_of<false>(s));
           }
           return top * sc;
         };
@@ -786,8 +972,18 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
         if (SPLIT) {
           // S is read twice, for the maximum and for the weights: the parts of
           // P take too many registers to be kept until the maximum is known
-          const float top = half_top();
-          if (pair_any(bar, j == 0 || top > m + kSlack)) agree(top);
+          float top = half_top();
+          if (pair_any(bar, j == 0 || !(top <= m + kSlack || isnan(l)))) {
+            if (__any_sync(0xffffffffu, isnan(top) && !isnan(l))) {
+              infinite_scores(p, ts + 64 * hf, p.table + (long long)seq * p.table_stride, head / p.group,
+                              k0 + j * kKeys + 64 * hf, left,
+                              live && !isnan(l) ? reinterpret_cast<const float*>(p.q) + (long long)tok * p.q_stride +
+                                                      (long long)head * p.hd
+                                                : nullptr);
+              top = half_top();
+            }
+            agree(top);
+          }
           const float bias = kBias - (m == -INFINITY ? 0.0f : m);
           const float2 bias2 = make_float2(bias, bias);
           sum[0] = sum[1] = make_float2(0.0f, 0.0f);
@@ -825,7 +1021,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
               tc_ld16(ts + 64 * hf + 16 * c, s);
               tc_wait_ld16(s);
               if (cut) mask_from(s, left - 16 * c);
-              top = fmaxf(top, max_of(s));
+              top = fmaxf(top, max_of<false>(s));
 #pragma unroll
               for (int e = 0; e < 8; ++e) {
                 const float2 x =
@@ -893,12 +1089,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
       if (lim <= k0) l = 0.0f;                                          // sees nothing here, whatever exp2 made of -inf
       const bool f32 = p.splits || p.type == TOSK_F32;
       const int es = f32 ? 4 : 2;
-      const float inv = l == 0.0f || nt == 0 ? 0.0f : p.splits ? 1.0f : 1.0f / l;
+      const float inv = l == 0.0f || nt == 0 ? 0.0f : p.splits && !isnan(l) ? 1.0f : 1.0f / l;
       if (p.splits && live && hf == 0) p.part_ml[slot] = make_float2(m - kBias, l);
       const long long row_at =
           !live ? -1 : p.splits ? slot * p.hd : (long long)tok * p.out_stride + (long long)head * p.hd;
       float2 odd = make_float2(0.0f, 0.0f);                             // NaN once an infinity or NaN was seen
-      const bool none = __any_sync(0xffffffffu, inv == 0.0f);
+      const bool none = __any_sync(0xffffffffu, !(inv > 0.0f));        // or NaN, by the weights
       // the staged rows' `bytes` to dims from dim0 on
       auto flush = [&](int dim0, int bytes) {
         __syncwarp();
@@ -952,7 +1148,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
         }
         if (none) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = inv == 0.0f ? 0u : o[e];
+          for (int e = 0; e < 32; ++e) o[e] = inv == 0.0f ? 0u : isnan(inv) ? kNanRow : o[e];
         }
         if (f32) {
 #pragma unroll
@@ -966,7 +1162,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
               const __half2 H = __floats2half2_rn(__uint_as_float(o[8 * c + 2 * q]), __uint_as_float(o[8 * c + 2 * q + 1]));
-              h[q] = *reinterpret_cast<const uint32_t*>(&H);
+              h[q] = none && isnan(inv) ? kNanRow : *reinterpret_cast<const uint32_t*>(&H);
             }
             *reinterpret_cast<uint4*>(stage + sw128(lane, 4 * c32 + c)) = make_uint4(h[0], h[1], h[2], h[3]);
           }
@@ -974,26 +1170,26 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
       }
       if (!f32) flush(hf * (HD / 2), HD);
       tc_fence_before();                                                // O and S are read: the next piece's MMAs may come
-      const bool bad = live && inv != 0.0f && isnan(odd.x + odd.y);
-      if (!p.splits && pair_any(bar, bad)) {
-        // rows that show one in either half, once both halves are written
-        pair_sync(bar);                                                 // l is read: sx is free
-        *mine = bad ? 1.0f : 0.0f;
-        pair_sync(bar);
-        uint32_t todo = hf == 0 ? __ballot_sync(0xffffffffu, *mine != 0.0f || *other != 0.0f) : 0;
-        while (todo) {
-          const int x = __ffs(todo) - 1;
-          todo &= todo - 1;
-          attn_row_plain(p, nullptr, 0, p.table + (long long)seq * p.table_stride, __shfl_sync(0xffffffffu, all, x),
-                         __shfl_sync(0xffffffffu, tok, x), __shfl_sync(0xffffffffu, head, x));
-        }
-      }
+      if (live && isnan(odd.x + odd.y)) *odd_seen = 1;
     }
   }
   __syncthreads();
   if (warp == kMmaWarp) {
     tc_fence_after();
     tmem_dealloc(tmem_at, 512);
+  }
+  if (warp > kMmaWarp && *odd_seen) {
+    // Values that are not finite were left out or met: the CTA's pieces once
+    // more, by two warps, for whom nobody waits but the end of the CTA.
+    const int splits = p.splits ? p.splits : 1;
+    PlanCursor cur = {0, 0};
+    for (int k = 0;; ++k) {
+      const int g = piece_of(k);
+      const TileId id = pick_tile(p, g / p.n_kv / splits, cur);
+      if (id.seq < 0) break;
+      if ((k ^ warp) & 1) continue;
+      patch_piece<HD>(p, seq_task(p, id.seq), g % p.n_kv, g / p.n_kv % splits, id.rt * 2 * kRows);
+    }
   }
 }
 

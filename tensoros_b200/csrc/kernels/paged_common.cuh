@@ -1,6 +1,6 @@
 // paged_common.cuh - what the paged attention kernels share: the problem as
-// the kernels see it, partial results of a split key axis, and the plain
-// recomputation of single rows.
+// the kernels see it, partial results of a split key axis, and values that are
+// not finite.
 #pragma once
 #include <cuda_fp16.h>
 
@@ -96,47 +96,66 @@ __device__ __forceinline__ void store_elem(void* p, int type, long long i, float
   else reinterpret_cast<__half*>(p)[i] = __float2half_rn(v);
 }
 
-// One output row by one warp, key by key and seen keys only.  The tiled
-// kernels multiply whole key tiles with weights that are zero where a row
-// does not see a key; 0 * inf or 0 * NaN of an unseen value then shows as NaN
-// in the row.  Such rows are computed again here, where an unseen key is not
-// read at all (a row with a NaN of its own gets it again).  prefix: keys
-// before the sequence's own (decode).
-static __device__ __noinline__ void attn_row_plain(const PagedProblem& p, const int* prefix_table, int prefix_len,
-                                            const int* table, int n, int tok, int h) {
-  const int lane = threadIdx.x & 31;
-  const long long qo = (long long)tok * p.q_stride + (long long)h * p.hd;
-  const int kvh = h / p.group;
-  float o[8], m = -INFINITY, l = 0.0f;
+// Values that are not finite.  The kernels multiply whole tiles of values with
+// weights that are zero where a row does not see a key; 0 * inf and 0 * NaN
+// would then be NaN in rows that do not see them.  Of the keys that some of a
+// tile's rows see and others do not, such values are therefore made zeros in
+// shared memory, and what a row does see of them is added to it at the end:
+// whatever its weight, an infinity or NaN is the row's sum.
+__device__ __forceinline__ bool not_finite(float x) { return !(fabsf(x) <= 3.402823466e38f); }
+
+// Elements of 16 bytes that are not finite become zeros; whether any were.
+template <typename E>
+__device__ __forceinline__ bool clean_piece(uint4& u) {
+  uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  bool any = false;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) o[i] = 0.0f;
-  for (int seg = 0; seg < 2; ++seg) {
-    const int* tb = seg ? table : prefix_table;
-    const int cnt = seg ? n : prefix_len;
-    for (int j = 0; j < cnt; ++j) {
-      const long long ko = kv_off(p, tb, j, kvh);
-      float s = 0.0f;
-      if (ko >= 0)
-        for (int d = lane; d < p.hd; d += 32) s = fmaf(load_elem(p.q, p.type, qo + d), load_elem(p.k, p.kv_type, ko + d), s);
-      for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-      s *= p.scale_log2;
-      const float mn = fmaxf(m, s);
-      const float c = mn == -INFINITY ? 1.0f : exp2f(m - mn);
-      const float w = mn == -INFINITY ? 0.0f : exp2f(s - mn);
-      l = fmaf(l, c, w);
-      m = mn;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int d = lane + 32 * i;
-        if (d < p.hd) o[i] = fmaf(o[i], c, ko >= 0 ? w * load_elem(p.v, p.kv_type, ko + d) : 0.0f);
-      }
-    }
+  for (int i = 0; i < 4; ++i) {
+    uint32_t bad;
+    if (sizeof(E) == 2)
+      bad = ((w[i] & 0x7c00u) == 0x7c00u ? 0xffffu : 0u) | ((w[i] & 0x7c000000u) == 0x7c000000u ? 0xffff0000u : 0u);
+    else
+      bad = (w[i] & 0x7f800000u) == 0x7f800000u ? 0xffffffffu : 0u;
+    w[i] &= ~bad;
+    any |= bad != 0;
   }
-  const long long oo = (long long)tok * p.out_stride + (long long)h * p.hd;
+  u = make_uint4(w[0], w[1], w[2], w[3]);
+  return any;
+}
+
+// Sum of the values of one dim at keys [j0, j1) that are not finite; 0: none.
+static __device__ __noinline__ float bad_value(const PagedProblem& p, const int* table, int kvh, int j0, int j1, int d) {
+  float s = 0.0f;
+  for (int j = j0; j < j1; ++j) {
+    const long long off = kv_off(p, table, j, kvh);
+    const float x = off >= 0 ? load_elem(p.v, p.kv_type, off + d) : 0.0f;
+    if (not_finite(x)) s += x;
+  }
+  return s;
+}
+
+// The same by a warp for dims lane + 32 i.
+static __device__ __noinline__ void bad_values(const PagedProblem& p, const int* table, int kvh, int j0, int j1,
+                                               float (&s)[8]) {
+  constexpr int U = 8;
+  const int lane = threadIdx.x & 31;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int d = lane + 32 * i;
-    if (d < p.hd) store_elem(p.out, p.type, oo + d, l == 0.0f ? 0.0f : o[i] / l);
+  for (int i = 0; i < 8; ++i) s[i] = 0.0f;
+  for (int j = j0; j < j1; j += U) {
+    long long off[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) off[u] = j + u < j1 ? kv_off(p, table, j + u, kvh) : -1;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int d = lane + 32 * i;
+      if (32 * i >= p.hd) break;
+      float x[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) x[u] = off[u] >= 0 && d < p.hd ? load_elem(p.v, p.kv_type, off[u] + d) : 0.0f;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (not_finite(x[u])) s[i] += x[u];
+    }
   }
 }
 

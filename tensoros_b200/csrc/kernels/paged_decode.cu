@@ -120,18 +120,46 @@ struct DecArgs {
   int whole;               // a page holds whole steps
   int late_wait;           // 1: runs beside the prefix kernel, whose end it awaits at its own end
   int pre;                 // without splits: slots of the prefix to add to each row, 0: none
-  const int* prefix_table;
-  int prefix_len;
 };
 
+// The values of a step from row r0 on, in shared memory at vs: those that are
+// not finite become zeros.  By a warp; whether any did.
+template <int KEYS, int CH, typename E>
+static __device__ __noinline__ bool clean_step(uint8_t* vs, int r0, int rowb) {
+  bool any = false;
+  for (int i = max(r0, 0) * CH + (int)(threadIdx.x & 31); i < KEYS * CH; i += 32) {
+    uint4* at = reinterpret_cast<uint4*>(vs + i / CH * rowb + i % CH * 16);
+    uint4 u = *at;
+    if (clean_piece<E>(u)) {
+      *at = u;
+      any = true;
+    }
+  }
+  __syncwarp();
+  return __any_sync(0xffffffffu, any);
+}
+
 // One row at the end of a CTA, by a warp: M, L its maximum (base 2) and sum,
-// v[i] its sum at dim lane + 32 i.  A split's partial row, or the output row:
-// with the prefix's partial rows added to it, and computed again key by key
-// where it shows NaN.
+// v[i] its sum at dim lane + 32 i.  A split's partial row, or the output row
+// with the prefix's partial rows added to it.  [k0, k1): the CTA's keys; first:
+// those before are seen by all its rows; dirty: of the others, values that are
+// not finite were left out.  What the row sees of them goes into it here; and
+// where a value met a weight of zero (rounded, or the low part of one), the
+// NaN in v becomes the sum of such values.
 __device__ __forceinline__ void finish_row(const DecArgs& a, const SeqTask& t, int kvh, int split, int r, float M, float L,
-                                           float (&v)[8]) {
+                                           float (&v)[8], int k0, int k1, int first, bool dirty) {
   const PagedProblem& p = a.p;
   const int lane = threadIdx.x & 31;
+  bool nan = false;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) nan |= lane + 32 * i < p.hd && isnan(v[i]);
+  nan = __any_sync(0xffffffffu, nan && !isnan(L));
+  if (nan || dirty) {
+    float s[8];
+    bad_values(p, t.table, kvh, nan ? k0 : max(k0, first), min(k1, seen(p, t, row_token(p, r))), s);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = nan && !(s[i] == 0.0f) ? s[i] : v[i] + s[i];
+  }
   const int tok = t.q0 + row_token(p, r), head = kvh * p.group + row_head(p, r);
   const long long row = (long long)tok * p.heads + head, step = (long long)p.total_q * p.heads;
   if (p.splits) {
@@ -175,17 +203,14 @@ __device__ __forceinline__ void finish_row(const DecArgs& a, const SeqTask& t, i
   }
   const float inv = L == 0.0f ? 0.0f : 1.0f / L;
   const long long oo = (long long)tok * p.out_stride + (long long)head * p.hd;
-  bool bad = false;
 #pragma unroll
   for (int i = 0; i < 8; ++i)
-    if (lane + 32 * i < p.hd) {
-      const float x = L == 0.0f ? 0.0f : v[i] * inv;
-      store_elem(p.out, p.type, oo + lane + 32 * i, x);
-      bad |= isnan(x);
-    }
-  if (__any_sync(0xffffffffu, bad))
-    attn_row_plain(p, a.prefix_table, a.prefix_len, t.table, seen(p, t, row_token(p, r)), tok, head);
+    if (lane + 32 * i < p.hd) store_elem(p.out, p.type, oo + lane + 32 * i, L == 0.0f ? 0.0f : v[i] * inv);
 }
+
+// High and low part's sum.  Beside an infinite high part the low one counts
+// for nothing: it may be zero, or of the other sign, times infinity.
+__device__ __forceinline__ float parts_sum(float hi, float lo) { return isinf(hi) ? hi : hi + lo; }
 
 // Whether this CTA's rows wait for the prefix kernel's: by all threads, once.
 __device__ __forceinline__ void await_prefix(const DecArgs& a) {
@@ -218,6 +243,8 @@ __global__ void __launch_bounds__(32 * kDecWarps) paged_decode_kernel(const __gr
     k0 = split * p.chunk;
     k1 = min(k1, k0 + p.chunk);
   }
+  const int all = nr > 0 ? seen(p, t, row_token(p, r0)) : 0;       // keys that all rows see
+  const int some = all < k1 ? all : 0x7fffffff;                    // the first that only some see, if any
   if (nr > 0 && (k0 < k1 || !p.splits)) {
     const int steps = (k1 - k0 + kStep - 1) / kStep;
     const uint32_t ring = smem_u32(sm) + warp * T::kDepth * T::kStage;
@@ -296,6 +323,7 @@ __global__ void __launch_bounds__(32 * kDecWarps) paged_decode_kernel(const __gr
     // of 16 dims, 16-31 keys 8-15; V (transposed): 0-15 keys, 16-31 the next 8 dims
     const int krow = (lane & 7) + ((lane >> 4) << 3), kch = (lane >> 3) & 1;
     const int vrow = lane & 15, vch = lane >> 4;
+    bool dirty = false;
 
     for (int st = warp; st < steps; st += kDecWarps) {
       issue(st + (T::kDepth - 1) * kDecWarps, npage);
@@ -303,6 +331,8 @@ __global__ void __launch_bounds__(32 * kDecWarps) paged_decode_kernel(const __gr
       asm volatile("cp.async.wait_group %0;" ::"n"(T::kDepth - 1) : "memory");
       __syncwarp();
       const uint32_t kbase = ring + (st / kDecWarps % T::kDepth) * T::kStage, vbase = kbase + kStep * T::kRow;
+      if (k0 + (st + 1) * kStep > some)                           // a prompt's last steps
+        dirty |= clean_step<kStep, CH, __half>(sm + (vbase - smem_u32(sm)), some - k0 - st * kStep, T::kRow);
       float s[NQ][2][4];
 #pragma unroll
       for (int n = 0; n < NQ; ++n)
@@ -328,7 +358,7 @@ __global__ void __launch_bounds__(32 * kDecWarps) paged_decode_kernel(const __gr
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int key = (e >> 1) * 8 + 2 * t4 + (e & 1);
-          w[e] = key < left ? (s[n][e >> 1][e & 1] + s[n][e >> 1][2 + (e & 1)]) * sc[n] : -INFINITY;
+          w[e] = key < left ? parts_sum(s[n][e >> 1][e & 1], s[n][e >> 1][2 + (e & 1)]) * sc[n] : -INFINITY;
         }
         float top = fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3]));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
@@ -374,9 +404,9 @@ __global__ void __launch_bounds__(32 * kDecWarps) paged_decode_kernel(const __gr
 #pragma unroll
       for (int d = 0; d < HD / 8; ++d)
         *reinterpret_cast<float2*>(so + ((warp * NQ + n) * 8 + g) * HD + 8 * d + 2 * t4) =
-            make_float2(o[n][d][0] + o[n][d][2], o[n][d][1] + o[n][d][3]);
+            make_float2(parts_sum(o[n][d][0], o[n][d][2]), parts_sum(o[n][d][1], o[n][d][3]));
     }
-    __syncthreads();
+    dirty = __syncthreads_or(dirty);
     // a warp a query
     await_prefix(a);
     for (int r = warp; r < nr; r += kDecWarps) {
@@ -397,7 +427,7 @@ __global__ void __launch_bounds__(32 * kDecWarps) paged_decode_kernel(const __gr
           for (int w = 0; w < kDecWarps; ++w) v[i] = fmaf(f[w], so[(w * NQ * 8 + r) * HD + d], v[i]);
         }
       }
-      finish_row(a, t, kvh, split, r0 + r, M, L, v);
+      finish_row(a, t, kvh, split, r0 + r, M, L, v, k0, k1, all, dirty);
     }
   } else {
     await_prefix(a);
@@ -447,6 +477,8 @@ __global__ void __launch_bounds__(32 * kDecWarps) paged_decode_f32_kernel(const 
     k0 = split * p.chunk;
     k1 = min(k1, k0 + p.chunk);
   }
+  const int all = nr > 0 ? seen(p, t, row_token(p, r0)) : 0;       // keys that all rows see
+  const int some = all < k1 ? all : 0x7fffffff;                    // the first that only some see, if any
   if (nr > 0 && (k0 < k1 || !p.splits)) {
     const int steps = (k1 - k0 + KS - 1) / KS;
     const uint8_t* ringp = sm + warp * T::kDepth * T::kStage;
@@ -492,6 +524,7 @@ __global__ void __launch_bounds__(32 * kDecWarps) paged_decode_f32_kernel(const 
       for (int c = 0; c < NC; ++c) o[n][c][0] = o[n][c][1] = make_float2(0.0f, 0.0f);
     }
     const int key = lane & 7, quarter = lane >> 3;
+    bool dirty = false;
     for (int st = warp; st < steps; st += kDecWarps) {
       issue(st + (T::kDepth - 1) * kDecWarps, npage);
       npage = fetch_page(st + T::kDepth * kDecWarps);
@@ -499,6 +532,8 @@ __global__ void __launch_bounds__(32 * kDecWarps) paged_decode_f32_kernel(const 
       __syncwarp();
       const uint8_t* ks = ringp + (st / kDecWarps % T::kDepth) * T::kStage;
       const uint8_t* vs = ks + KS * T::kRow;
+      if (k0 + (st + 1) * KS > some)                              // a prompt's last steps
+        dirty |= clean_step<KS, CH, float>(sm + (vs - sm), some - k0 - st * KS, T::kRow);
       float2 s[Q];
 #pragma unroll
       for (int n = 0; n < Q; ++n) s[n] = make_float2(0.0f, 0.0f);
@@ -588,7 +623,7 @@ __global__ void __launch_bounds__(32 * kDecWarps) paged_decode_f32_kernel(const 
           *reinterpret_cast<float4*>(so + (warp * Q + n) * HD + 4 * pc) = make_float4(x.x, x.y, y.x, y.y);
       }
     }
-    __syncthreads();
+    dirty = __syncthreads_or(dirty);
     await_prefix(a);
     for (int r = warp; r < nr; r += kDecWarps) {
       float M = -INFINITY, L = 0.0f, f[kDecWarps], v[8];
@@ -608,7 +643,7 @@ __global__ void __launch_bounds__(32 * kDecWarps) paged_decode_f32_kernel(const 
           for (int w = 0; w < kDecWarps; ++w) v[i] = fmaf(f[w], so[(w * Q + r) * HD + d], v[i]);
         }
       }
-      finish_row(a, t, kvh, split, r0 + r, M, L, v);
+      finish_row(a, t, kvh, split, r0 + r, M, L, v, k0, k1, all, dirty);
     }
   } else {
     await_prefix(a);
@@ -662,13 +697,11 @@ bool paged_decode_ok(const PagedProblem& p) {
 // Few rows a sequence (single tokens, short prompts).  fp16: row tiles of 16
 // where a sequence has more than 8 rows (256 dims: of 8, for the registers),
 // else of 8.  fp32: of 1, 4 or 8, the smallest that holds the rows.
-int paged_decode_run(const PagedProblem& p, const PagedPrefix& pre, cudaStream_t st) {
+int paged_decode_run(const PagedProblem& p, int pre_slots, cudaStream_t st) {
   DecArgs a;
   a.p = p;
-  a.late_wait = pre.len > 0;
-  a.pre = p.splits ? 0 : pre.slots;
-  a.prefix_table = pre.table;
-  a.prefix_len = pre.len;
+  a.late_wait = pre_slots > 0;
+  a.pre = p.splits ? 0 : pre_slots;
   const bool f16 = p.kv_type == TOSK_F16;
   const long long rows = (long long)p.max_q * p.group;
   const int nq = rows > 8 && p.hd <= 128 ? 2 : 1;

@@ -17,13 +17,9 @@ size_t paged_tc_fold_bytes(int keys);
 long long paged_tc_tiles(int n_seqs, int total_q, int max_q, int group);
 // paged_decode.cu
 bool paged_decode_ok(const PagedProblem& p);
-// A shared prefix whose partial rows a kernel launched just before brings:
-// `slots` of them, at the slots before the problem's own.
-struct PagedPrefix {
-  int slots, len;
-  const int* table;
-};
-int paged_decode_run(const PagedProblem& p, const PagedPrefix& pre, cudaStream_t st);
+// pre_slots: partial rows of a shared prefix that a kernel launched just before
+// brings, at the slots before the problem's own.
+int paged_decode_run(const PagedProblem& p, int pre_slots, cudaStream_t st);
 
 #ifdef __CUDACC__
 // Shared-memory operands, rows of 128 bytes swizzled 128 B, eight rows every

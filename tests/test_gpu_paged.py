@@ -629,3 +629,125 @@ def test_seen_nan_key_at_every_place(gpu, qk, kv, hd, n, hist):
         sees = lim > at[h]
         assert bool(torch.isnan(out[sees, h]).all()), (h, at[h])
         R.assert_rows(out[~sees, h], ref[~sees, h], err[~sees, h], (h, at[h]))
+
+
+def fastest(f, times=3):
+    """us of the fastest of some calls, after one"""
+    f()
+    best = float("inf")
+    for _ in range(times):
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        f()
+        b.record()
+        torch.cuda.synchronize()
+        best = min(best, a.elapsed_time(b) * 1e3)
+    return best
+
+
+@pytest.mark.parametrize("qk,kv", KINDS)
+@pytest.mark.parametrize("hd,n,hist,heads,n_kv", [(128, 70, 3000, 16, 4), (64, 300, 1900, 16, 4), (128, 1200, 0, 32, 8),
+                                                  (128, 3, 1500, 8, 4), (200, 40, 700, 4, 2)])
+@pytest.mark.parametrize("what", ["seen nan key", "seen inf value", "unseen nan value"])
+def test_values_that_are_not_finite_cost_no_second_pass(gpu, qk, kv, hd, n, hist, heads, n_kv, what):
+    """A call with a NaN or an infinity takes as long as one without, times a
+    small number: no row is computed again key by key (a microsecond a key)."""
+    c = Cache([n + hist], 16, n_kv, hd, kv, seed=5)
+    q = randn(n, heads, hd, seed=6, kind=qk)
+    args = (gpu, c, q, [n], [n + hist], heads, hd ** -0.5)
+    out, st = R.prompt(*args)
+    assert st == 0
+    ws = torch.empty(64 << 20, dtype=torch.uint8, device="cuda")
+    clean = fastest(lambda: R.prompt(*args, out=out, ws=ws))
+    pg, r = c.where(c.table[0], n + hist)
+    at = n + hist - 1 if what.startswith("unseen") else 5
+    x = c.k if what.endswith("key") else c.v
+    x[pg[at], r[at], :, 3] = float("inf" if "inf" in what else "nan")
+    assert fastest(lambda: R.prompt(*args, out=out, ws=ws)) < 4 * clean + 100
+
+
+@pytest.mark.parametrize("qk,kv", KINDS)
+@pytest.mark.parametrize("hd,n,hist,heads,n_kv", [(128, 300, 700, 16, 4), (64, 513, 0, 16, 16), (128, 1200, 0, 32, 8),
+                                                  (128, 60, 5000, 16, 2), (128, 7, 300, 8, 4), (64, 9, 120, 5, 1),
+                                                  (200, 90, 100, 6, 2), (80, 150, 31, 4, 4), (33, 50, 9, 3, 3)])
+def test_values_that_are_not_finite_reach_the_rows_that_see_them(gpu, qk, kv, hd, n, hist, heads, n_kv):
+    """Infinities of both signs and NaN among the values of the last tokens
+    and of one that all rows see: an element is the sum of those that its row
+    sees, or as if there were none.  And infinite keys, which give a weight of
+    zero or, at +infinity, a NaN."""
+    m = n + hist
+    c = Cache([m], 16, n_kv, hd, kv, seed=5)
+    q = randn(n, heads, hd, seed=6, kind=qk)
+    k, v = c.rows(0)
+    pg, r = c.where(c.table[0], m)
+    inf, nan = float("inf"), float("nan")
+    back = lambda f: m - 1 - int(f * (n - 1))       # tokens of the prompt, from its end
+    plan = [(back(0), 0, 0, nan), (back(.1), 0, 1, inf), (back(.2), 0, 1, inf), (back(.3), 0, 2, -inf),
+            (back(.25), 0, 2, inf), (back(.6), n_kv - 1, hd - 1, -inf), (back(.9), n_kv - 1, hd // 2, nan)]
+    if hist:
+        plan.append((3, n_kv - 1, 5, -inf))
+    extra = torch.zeros(n, heads, hd, dtype=torch.float64, device="cuda")
+    lim = torch.arange(n, device="cuda") + hist + 1
+    g = heads // n_kv
+    for (at, h, d), x in {e[:3]: e[3] for e in plan}.items():       # short prompts: two may name one place
+        c.v[pg[at], r[at], h, d] = x
+        sees = (lim > at).nonzero().flatten()
+        extra[sees, h * g:(h + 1) * g, d] += x
+    out, st = R.prompt(gpu, c, q, [n], [m], heads, hd ** -0.5)
+    assert st == 0
+    ref, err = R.attend(q, k, v, float(np.float32(hd ** -0.5)), lim)
+    # the plan replaced values that rows saw: their elements are infinite or NaN, all others as they were
+    ok = extra == 0
+    R.assert_rows(out[ok], ref[ok], err[ok], "finite")
+    assert torch.equal(torch.isnan(out[~ok]), torch.isnan(extra[~ok])), "NaN"
+    z = ~ok & ~torch.isnan(extra)
+    assert torch.equal(out[z].double(), extra[z]), "infinities"
+
+
+@pytest.mark.parametrize("qk,kv", KINDS)
+@pytest.mark.parametrize("hd,n,hist,heads,n_kv", [(128, 300, 700, 16, 4), (64, 513, 0, 16, 16), (128, 60, 5000, 16, 2),
+                                                  (128, 7, 300, 8, 4), (200, 90, 100, 6, 2)])
+def test_infinite_keys(gpu, qk, kv, hd, n, hist, heads, n_kv):
+    """An infinite element of a key: a score of -infinity weighs nothing, one
+    of +infinity makes the row NaN."""
+    m = n + hist
+    c = Cache([m], 16, n_kv, hd, kv, seed=5)
+    q = randn(n, heads, hd, seed=6, kind=qk)
+    q[:, :, 7] = q[:, :, 7].abs() + 0.01
+    q[:, 0, 7] *= -1
+    k, v = c.rows(0)
+    pg, r = c.where(c.table[0], m)
+    lim = torch.arange(n, device="cuda") + hist + 1
+    ats = [m - 1 - i * max(1, n // 5) for i in range(4)]
+    for at in ats:
+        c.k[pg[at], r[at], :, 7] = float("-inf")
+        k[at, :, 7] = -1e9                             # as good as -infinity in 64 bits
+    out, st = R.prompt(gpu, c, q, [n], [m], heads, hd ** -0.5)
+    assert st == 0
+    ref, _ = R.attend(q, k, v, float(np.float32(hd ** -0.5)), lim)
+    for at in ats:
+        k[at, :, 7] = 0
+    _, err = R.attend(q, k, v, float(np.float32(hd ** -0.5)), lim)
+    R.assert_rows(out[:, 1:], ref[:, 1:], 2 * err[:, 1:], "-inf")
+    sees = lim > min(ats)
+    assert bool(torch.isnan(out[sees, 0]).all()) and bool(torch.isfinite(out[~sees, 0]).all())
+
+
+@pytest.mark.parametrize("qk,heads,n_kv", [(F32, 16, 4), (F16, 16, 4), (F32, 8, 1)])
+def test_nan_value_behind_a_long_history(gpu, qk, heads, n_kv):
+    """200,000 keys: one value that all rows see and one that few see are NaN.
+    The call ends in time, and no other element changes."""
+    n, m, hd = 70, 200000, 128
+    c = Cache([m], 64, n_kv, hd, F16, seed=5)
+    q = randn(n, heads, hd, seed=6, kind=qk)
+    clean, st = R.prompt(gpu, c, q, [n], [m], heads, hd ** -0.5)
+    assert st == 0
+    pg, r = c.where(c.table[0], m)
+    c.v[pg[5], r[5], :, 3] = float("nan")
+    c.v[pg[m - 9], r[m - 9], :, 70] = float("nan")
+    out, st = R.prompt(gpu, c, q, [n], [m], heads, hd ** -0.5)
+    torch.cuda.synchronize()
+    assert st == 0 and gpu.tos_synchronize() == 0
+    assert bool(torch.isnan(out[:, :, 3]).all()) and bool(torch.isnan(out[n - 9:, :, 70]).all())
+    out[:, :, 3], out[n - 9:, :, 70] = clean[:, :, 3], clean[n - 9:, :, 70]
+    assert torch.equal(out, clean)
