@@ -9,10 +9,13 @@
 //     memory (cp.async, 16-byte pieces, 8 KB a step at 128 dims; the page's
 //     table entry fetched one step ahead).  Rows past the end and pages that
 //     are none come as zeros;
-//   * S = Q K^T and O += P V by mma.sync m16n8k16: eight rows' fp16 high
-//     parts are rows 0-7 of A and their low parts rows 8-15, so fp32 queries
-//     and weights cost no extra instruction and the two row halves are added
-//     afterwards.  tcgen05 wants 128 rows; here there are 8 or 16;
+//   * S = Q K^T and P V by mma.sync m16n8k16: eight rows' fp16 high parts are
+//     rows 0-7 of A and their low parts rows 8-15, so fp32 queries and weights
+//     cost no extra instruction and the two row halves are added afterwards.
+//     tcgen05 wants 128 rows; here there are 8 or 16;
+//   * O += P V in fp32 registers, rounded to nearest: an accumulator that the
+//     tensor cores keep is cut off at every step (32,768 keys of one sign
+//     in one chunk came out 5e-5 small);
 //   * running maximum and sum per row as in the prompt kernel (followed
 //     only beyond a factor 2^8, weights biased by 2^7).
 // The four warps' results are joined in shared memory; with a split key axis
@@ -64,6 +67,12 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma16816_zero(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
 }
 __device__ __forceinline__ int page_of(const PagedProblem& p, int key) {
   return p.pshift >= 0 ? key >> p.pshift : key / p.page_size;
@@ -276,7 +285,8 @@ __global__ void __launch_bounds__(32 * kDecWarps) paged_decode_kernel(const __gr
     int npage = pages[T::kDepth - 1];
 
     uint32_t qa[NQ][HD / 16][4];
-    float sc[NQ], m[NQ], l[NQ], o[NQ][HD / 8][4];
+    float sc[NQ], m[NQ], l[NQ];
+    float2 o[NQ][HD / 8];
     int lim[NQ];                                                  // keys that this lane's row sees
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
@@ -315,9 +325,7 @@ __global__ void __launch_bounds__(32 * kDecWarps) paged_decode_kernel(const __gr
       m[n] = -INFINITY;
       l[n] = 0.0f;
 #pragma unroll
-      for (int d = 0; d < HD / 8; ++d)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[n][d][e] = 0.0f;
+      for (int d = 0; d < HD / 8; ++d) o[n][d] = make_float2(0.0f, 0.0f);
     }
     // ldmatrix row addresses: K: lanes 0-7 / 8-15 keys 0-7 at the two halves
     // of 16 dims, 16-31 keys 8-15; V (transposed): 0-15 keys, 16-31 the next 8 dims
@@ -369,9 +377,7 @@ __global__ void __launch_bounds__(32 * kDecWarps) paged_decode_kernel(const __gr
           m[n] = mn;
           l[n] *= f;
 #pragma unroll
-          for (int d = 0; d < HD / 8; ++d)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[n][d][e] *= f;
+          for (int d = 0; d < HD / 8; ++d) o[n][d] = __fmul2_rn(o[n][d], make_float2(f, f));
         }
         const float bias = 7.0f - (m[n] == -INFINITY ? 0.0f : m[n]);
 #pragma unroll
@@ -380,15 +386,32 @@ __global__ void __launch_bounds__(32 * kDecWarps) paged_decode_kernel(const __gr
         split_pair(w[0], w[1], pa[n][0], pa[n][1]);
         split_pair(w[2], w[3], pa[n][2], pa[n][3]);
       }
+      // a few products under way before the first is added: one CTA an SM (256
+      // dims) has no other warps to hide them (8 x 3000 keys: 87 us one by one)
+      constexpr int B = NQ == 1 ? 4 : 2;
 #pragma unroll
-      for (int d = 0; d < HD / 16; ++d) {
-        uint32_t bv[4];
-        ldsm4t(bv, vbase + vrow * T::kRow + (((2 * d + vch) ^ (vrow & 7)) << 4));
+      for (int d0 = 0; d0 < HD / 16; d0 += B) {
+        float c[B][NQ][2][4];
 #pragma unroll
-        for (int n = 0; n < NQ; ++n) {
-          mma16816(o[n][2 * d], pa[n], bv[0], bv[1]);
-          mma16816(o[n][2 * d + 1], pa[n], bv[2], bv[3]);
+        for (int x = 0; x < B; ++x) {
+          uint32_t bv[4];
+          ldsm4t(bv, vbase + vrow * T::kRow + (((2 * (d0 + x) + vch) ^ (vrow & 7)) << 4));
+#pragma unroll
+          for (int n = 0; n < NQ; ++n) {
+            mma16816_zero(c[x][n][0], pa[n], bv[0], bv[1]);
+            mma16816_zero(c[x][n][1], pa[n], bv[2], bv[3]);
+          }
         }
+#pragma unroll
+        for (int x = 0; x < B; ++x)
+#pragma unroll
+          for (int n = 0; n < NQ; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float(&t)[4] = c[x][n][e];
+              float2& to = o[n][2 * (d0 + x) + e];
+              to = __fadd2_rn(to, make_float2(parts_sum(t[0], t[2]), parts_sum(t[1], t[3])));
+            }
       }
       __syncwarp();                                               // the stage may be filled again
     }
@@ -403,8 +426,7 @@ __global__ void __launch_bounds__(32 * kDecWarps) paged_decode_kernel(const __gr
       if (t4 == 0) sml[warp][n * 8 + g] = make_float2(m[n] - 7.0f, l[n]);
 #pragma unroll
       for (int d = 0; d < HD / 8; ++d)
-        *reinterpret_cast<float2*>(so + ((warp * NQ + n) * 8 + g) * HD + 8 * d + 2 * t4) =
-            make_float2(parts_sum(o[n][d][0], o[n][d][2]), parts_sum(o[n][d][1], o[n][d][3]));
+        *reinterpret_cast<float2*>(so + ((warp * NQ + n) * 8 + g) * HD + 8 * d + 2 * t4) = o[n][d];
     }
     dirty = __syncthreads_or(dirty);
     // a warp a query

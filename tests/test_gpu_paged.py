@@ -751,3 +751,34 @@ def test_nan_value_behind_a_long_history(gpu, qk, heads, n_kv):
     assert bool(torch.isnan(out[:, :, 3]).all()) and bool(torch.isnan(out[n - 9:, :, 70]).all())
     out[:, :, 3], out[n - 9:, :, 70] = clean[:, :, 3], clean[n - 9:, :, 70]
     assert torch.equal(out, clean)
+
+
+# ----------------------------------------------- long sums of values of one sign
+# A tensor-core accumulator cuts off what it has no room for, so a long chain of
+# sums comes out small.  Sums rounded to nearest err both ways: N additions to
+# a sum that grows evenly have a standard deviation of u / sqrt(3) sqrt(N / 3),
+# 2^-24 / 3 sqrt(N) of the sum.  The bounds are six of those and, once, what
+# the longest chain between two roundings to nearest may lose.
+
+def one_sign(c, m):
+    """Values of every dim about one number of its own in [1, 2]"""
+    pg, r = c.where(c.table[0], m)
+    x = c.v[pg, r].float() / 16 + 1 + torch.arange(c.hd, device="cuda") / c.hd
+    c.v[pg, r] = x.to(c.v.dtype)
+
+
+def test_decode_long_sums_do_not_shrink(gpu):
+    """640 sequences times heads, so that a CTA has all of one's keys: 512 steps
+    a warp.  The weights' sum and the values' have 512 additions each."""
+    n, heads, hd, m = 40, 16, 128, 32768
+    c = Cache([m], 64, heads, hd, F16, seed=2)
+    one_sign(c, m)
+    k, v = c.rows(0)
+    c.table, c.lens = c.table.expand(n, -1).contiguous(), [m] * n       # all read the same pages
+    q = randn(n, heads, hd, seed=3)
+    out, st = R.decode(gpu, c, q, c.lens, heads, hd ** -0.5)
+    assert st == 0
+    ref, _ = R.attend(q, k, v, float(np.float32(hd ** -0.5)), torch.full((n,), m, device="cuda"))
+    rel = (out.double() - ref) / ref
+    chain = 2 * 2.0 ** -23                                    # one product of 16 keys, two parts
+    assert float(rel.abs().max()) < 6 * 2.0 ** -24 / 3 * (512 + 512) ** 0.5 + chain + 2.0 ** -23
