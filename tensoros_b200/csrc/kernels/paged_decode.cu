@@ -386,9 +386,11 @@ __global__ void __launch_bounds__(32 * kDecWarps) paged_decode_kernel(const __gr
         split_pair(w[0], w[1], pa[n][0], pa[n][1]);
         split_pair(w[2], w[3], pa[n][2], pa[n][3]);
       }
-      // a few products under way before the first is added: one CTA an SM (256
-      // dims) has no other warps to hide them (8 x 3000 keys: 87 us one by one)
-      constexpr int B = NQ == 1 ? 4 : 2;
+      // How many products are under way before the first is added.  One CTA an
+      // SM (256 dims) has no other warps to hide them: 8 x 3000 keys 68.6 us,
+      // 87.0 one by one; 16 rows, 8 tokens behind 300 keys, 22.5, 23.6.  At 8 rows
+      // of 128 dims they cost: 16 sequences of 1 to 4096 keys 106.8, 93.8 one by one.
+      constexpr int B = HD == 256 ? 4 : NQ;
 #pragma unroll
       for (int d0 = 0; d0 < HD / 16; d0 += B) {
         float c[B][NQ][2][4];
