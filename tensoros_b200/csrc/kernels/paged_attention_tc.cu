@@ -40,9 +40,9 @@
 // Precision.  fp16 rows: P is rounded to fp16 (half a step, 2^-11, of each
 // weight, which is what the output's own rounding costs; sums and maxima are
 // fp32).  fp32 rows: q, scaled by a power of two per row, and P go in as
-// fp16 pairs hi + lo (22 bits), two MMAs each, and the accumulators, which cut
-// off instead of rounding, are emptied into memory every kFold key tiles:
-// 1.1e-6 against 64 bits (norm) over 7512 keys.
+// fp16 pairs hi + lo (22 bits), two MMAs each: 1.1e-6 against 64 bits (norm)
+// over 7512 keys.  The accumulators, which cut off instead of rounding, are
+// emptied into memory every few key tiles (fold_tiles).
 //
 // Keys behind a row's last one are masked in S; value rows behind the key
 // range (a page's unused rows may hold anything) and, where only some rows see
@@ -69,8 +69,11 @@ constexpr int kRows = 128;            // rows of a tile
 constexpr int kKeys = 128;            // keys of a tile
 constexpr float kBias = 7.0f;         // log2 of the factor that P carries
 constexpr int kPoly = 3;              // of eight pairs of exponentials, those at 2 and 5 go to the FMA pipe
-constexpr int kFold = 3;              // fp32 rows: key tiles whose products one accumulator sums
-                                      // (512 rows behind 7001 keys, us: 3: 159, 4: 154, 8: 145, never: 138)
+// Key tiles whose products one accumulator sums.  It loses 1e-7 of itself a step
+// of 16 keys.  fp32 rows: 3 (512 rows behind 7001 keys, us: 3: 159, 4: 154, 8: 145,
+// never: 138).  fp16 rows: 32, a loss of 2.6e-5, a twentieth of their rounding
+// (131,072 keys in one chain: 8e-4).
+__host__ __device__ constexpr int fold_tiles(bool split) { return split ? 3 : 32; }
 constexpr float kSlack = 8.0f;        // log2 by which the maximum may grow unfollowed
 
 struct TcArgs {
@@ -307,10 +310,14 @@ static __device__ __noinline__ void scale_cols(uint32_t addr, int n, float f) {
     tmem_st16(addr + c, o);
   }
 }
-// Memory <- s * memory + n columns of this warp's 32 rows in tensor memory (s 0:
-// memory is not read).  Four columns of the 32 rows lie side by side: dst is
-// the lane's first four of n.
-static __device__ __noinline__ void fold_cols(uint32_t addr, int n, float* dst, float s) {
+// The CTA's sums of chains that have ended: four columns of a warp's 32 rows
+// lie side by side, `n` columns a warp.
+__device__ __forceinline__ float* fold_at(const PagedProblem& p, int n) {
+  return p.fold + (size_t)(blockIdx.x * kCopyWarp + (threadIdx.x >> 5)) * (32 * n) + (threadIdx.x & 31) * 4;
+}
+// Adds n columns of this warp's 32 rows in tensor memory to them (first: puts).
+static __device__ __noinline__ void fold_cols(const PagedProblem& p, uint32_t addr, int n, bool first) {
+  float* dst = fold_at(p, n);
 #pragma unroll 1
   for (int c = 0; c < n; c += 16, dst += 512) {
     uint32_t o[16];
@@ -318,13 +325,43 @@ static __device__ __noinline__ void fold_cols(uint32_t addr, int n, float* dst, 
     float4 x[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      x[e] = s != 0.0f ? *reinterpret_cast<const float4*>(dst + 128 * e) : make_float4(0.f, 0.f, 0.f, 0.f);
+      x[e] = first ? make_float4(0.f, 0.f, 0.f, 0.f) : *reinterpret_cast<const float4*>(dst + 128 * e);
     tc_wait_ld16(o);
 #pragma unroll
     for (int e = 0; e < 4; ++e)
       *reinterpret_cast<float4*>(dst + 128 * e) =
-          make_float4(fmaf(x[e].x, s, __uint_as_float(o[4 * e])), fmaf(x[e].y, s, __uint_as_float(o[4 * e + 1])),
-                      fmaf(x[e].z, s, __uint_as_float(o[4 * e + 2])), fmaf(x[e].w, s, __uint_as_float(o[4 * e + 3])));
+          make_float4(x[e].x + __uint_as_float(o[4 * e]), x[e].y + __uint_as_float(o[4 * e + 1]),
+                      x[e].z + __uint_as_float(o[4 * e + 2]), x[e].w + __uint_as_float(o[4 * e + 3]));
+  }
+}
+// And them to the columns, at the end.
+static __device__ __noinline__ void fold_back(const PagedProblem& p, uint32_t addr, int n) {
+  const float* src = fold_at(p, n);
+#pragma unroll 1
+  for (int c = 0; c < n; c += 16, src += 512) {
+    uint32_t o[16];
+    tc_ld16(addr + c, o);
+    float4 x[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = *reinterpret_cast<const float4*>(src + 128 * e);
+    tc_wait_ld16(o);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      o[4 * e] = __float_as_uint(x[e].x + __uint_as_float(o[4 * e]));
+      o[4 * e + 1] = __float_as_uint(x[e].y + __uint_as_float(o[4 * e + 1]));
+      o[4 * e + 2] = __float_as_uint(x[e].z + __uint_as_float(o[4 * e + 2]));
+      o[4 * e + 3] = __float_as_uint(x[e].w + __uint_as_float(o[4 * e + 3]));
+    }
+    tmem_st16(addr + c, o);
+  }
+  tmem_st_wait();
+}
+static __device__ __noinline__ void fold_scale(const PagedProblem& p, int n, float f) {
+  float* dst = fold_at(p, n);
+#pragma unroll 1
+  for (int c = 0; c < n; c += 4, dst += 128) {
+    float4* at = reinterpret_cast<float4*>(dst);
+    *at = make_float4(at->x * f, at->y * f, at->z * f, at->w * f);
   }
 }
 // The two warps that share 32 rows.
@@ -837,7 +874,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
 #pragma unroll
                   for (int k = 0; k < kKeys / 32; ++k)
                     mma_f16_ts(d, pa + (k >> 1) * 32 + part * 16 + (k & 1) * 8, vd + (k * 2048 >> 4), kIdO,
-                               part + k + half > 0 ? true : SPLIT ? j % kFold != 0 : j > 0);
+                               part + k + half > 0 ? true : j % fold_tiles(SPLIT) != 0);
               }
               if (!ok) break;
               mma_commit(odone + i);
@@ -864,7 +901,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
     const uint32_t lanes = (uint32_t)wq << 21;                          // TMEM lane of the warp's first row, << 16
     const uint32_t ts = tmem_at + lanes + i * kKeys, to = tmem_at + lanes + 256 + i * HD + hf * (HD / 2);
     uint8_t* stage = (T::kStage ? ring + T::kSlots * T::kTile + i * 32768 : q_tile) + (hf * 4 + wq) * 4096;
-    float* const fold = p.fold + (size_t)(blockIdx.x * kCopyWarp + warp) * (32 * HD / 2) + lane * 4;
     bool ok = true;     // a wait that ran out: no more waiting, and all warps of the row tile leave together
     int cnt = 0;                                                        // key tiles so far
     pdl_wait();
@@ -910,20 +946,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
       const int all = live ? seen(p, st, row_token(p, pr)) : 0, lim = min(all, w.k1);   // keys this row sees, here
       const long long slot = (long long)(p.slot0 + (p.splits ? w.split : 0)) * p.total_q * p.heads + (long long)tok * p.heads + head;
       const float sc = fmaxf(fabsf(p.scale_log2) * inv_q, 1.2e-38f);   // not 0: a masked score is -inf * sc
-      // fp32 rows: the sums so far are fold_s * what lies at `fold`
-      float fold_s = 0.0f;
       float m = -INFINITY, l = 0.0f;
       for (int j = 0; j < nt; ++j) {
-        if (SPLIT && j > 0 && j % kFold == 0) {
+        if (j > 0 && j % fold_tiles(SPLIT) == 0) {
           // The tensor cores cut off what their accumulator has no room for,
-          // so a long chain of sums shrinks: by up to 5e-8 of itself a step of
-          // 16 keys, 6e-5 over 9000 keys.  Every kFold tiles the sums are
+          // so a long chain of sums shrinks.  Every few tiles the sums are
           // added up in memory, rounded to nearest, and the chain begins anew.
           if (ok) ok = mbar_wait(odone + i, (cnt + j - 1) & 1, p.err, 46);
           __syncwarp();
           tc_fence_after();
-          fold_cols(to, HD / 2, fold, fold_s);
-          fold_s = 1.0f;
+          fold_cols(p, to, HD / 2, j == fold_tiles(SPLIT));
           tc_fence_before();
           pair_sync(bar);                                               // the MMAs overwrite all dims
         }
@@ -960,7 +992,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
             tc_fence_after();
             scale_cols(to, HD / 2, f);
             l *= f;
-            fold_s *= f;
+            if (j >= fold_tiles(SPLIT)) fold_scale(p, HD / 2, f);
             // either half's P lets MMAs add to all dims: both halves' O first
             tmem_st_wait();
             tc_fence_before();
@@ -1124,21 +1156,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
         }
         __syncwarp();
       };
+      if (nt > fold_tiles(SPLIT)) fold_back(p, to, HD / 2);
 #pragma unroll 1
       for (int c32 = 0; c32 < HD / 64; ++c32) {
         uint32_t o[32];
         tc_ld32(to + 32 * c32, o);
         tc_wait_ld(o);
-        if (SPLIT && fold_s != 0.0f) {
-#pragma unroll
-          for (int e = 0; e < 32; e += 4) {
-            const float4 x = *reinterpret_cast<const float4*>(fold + (8 * c32 + e / 4) * 128);
-            o[e] = __float_as_uint(fmaf(x.x, fold_s, __uint_as_float(o[e])));
-            o[e + 1] = __float_as_uint(fmaf(x.y, fold_s, __uint_as_float(o[e + 1])));
-            o[e + 2] = __float_as_uint(fmaf(x.z, fold_s, __uint_as_float(o[e + 2])));
-            o[e + 3] = __float_as_uint(fmaf(x.w, fold_s, __uint_as_float(o[e + 3])));
-          }
-        }
 #pragma unroll
         for (int e = 0; e < 32; e += 2) {
           const float2 v = __fmul2_rn(make_float2(__uint_as_float(o[e]), __uint_as_float(o[e + 1])), make_float2(inv, inv));
@@ -1251,8 +1274,9 @@ bool paged_tc_ok(const PagedProblem& p) {
          (long long)ps * p.n_kv * p.hd * 2 < (1ll << 39);
 }
 
-// Bytes of PagedProblem::fold that fp32 rows over so many keys need.
-size_t paged_tc_fold_bytes(int keys) { return keys > kFold * kKeys ? (size_t)kTcCtas * 2 * kRows * 128 * 4 : 0; }
+// Bytes of PagedProblem::fold that rows over so many keys may need: fp32 rows
+// (fp16 rows, beyond more keys; a call's workspace goes by its sizes alone).
+size_t paged_tc_fold_bytes(int keys) { return keys > fold_tiles(true) * kKeys ? (size_t)kTcCtas * 2 * kRows * 128 * 4 : 0; }
 
 // Row tiles of one key/value head that a call can have at most.
 long long paged_tc_tiles(int n_seqs, int total_q, int max_q, int group) {
@@ -1273,7 +1297,7 @@ int paged_tc_run(const PagedProblem& p, cudaStream_t st) {
   if (!pool_map(&a.mk, p.k, p, a.box_rows) || !pool_map(&a.mv, p.v, p, a.box_rows)) return (int)cudaErrorNotSupported;
   const bool split = p.type == TOSK_F32;
   const int keys = p.splits ? p.chunk : p.fixed_kv >= 0 ? p.fixed_kv : p.max_kv;
-  if (split && !p.fold && paged_tc_fold_bytes(keys)) return (int)cudaErrorInvalidValue;
+  if (!p.fold && keys > fold_tiles(split) * kKeys) return (int)cudaErrorInvalidValue;
   if (p.hd <= 64) return split ? tc_launch<64, true>(a, (unsigned)grid, st) : tc_launch<64, false>(a, (unsigned)grid, st);
   return split ? tc_launch<128, true>(a, (unsigned)grid, st) : tc_launch<128, false>(a, (unsigned)grid, st);
 }

@@ -31,7 +31,7 @@ struct PagedProblem {
   int splits, chunk, slot0;
   float* part_o;               // [slot][total_q * heads][hd], not normalised
   float2* part_ml;             // [slot][total_q * heads]: running maximum (base 2), sum
-  float* fold;                 // tensor-core kernel, fp32 rows, many keys: every CTA's own sums so far
+  float* fold;                 // tensor-core kernel, many keys: every CTA's own sums so far
   int* err;
 };
 

@@ -782,3 +782,42 @@ def test_decode_long_sums_do_not_shrink(gpu):
     rel = (out.double() - ref) / ref
     chain = 2 * 2.0 ** -23                                    # one product of 16 keys, two parts
     assert float(rel.abs().max()) < 6 * 2.0 ** -24 / 3 * (512 + 512) ** 0.5 + chain + 2.0 ** -23
+
+
+@pytest.mark.parametrize("m", [700, 9000])
+def test_prompt_sums_of_one_sign(gpu, m):
+    """fp32 rows: chains of 24 steps of 16 keys, which lose a unit, 2^-23, each;
+    one addition of the weights a key tile, of the values three tiles."""
+    n, heads, hd = 300, 16, 128
+    m += n
+    c = Cache([m], 64, heads, hd, F16, seed=2)
+    one_sign(c, m)
+    k, v = c.rows(0)
+    q = randn(n, heads, hd, seed=3)
+    out, st = R.prompt(gpu, c, q, [n], [m], heads, hd ** -0.5)
+    assert st == 0
+    ref, _ = R.attend(q, k, v, float(np.float32(hd ** -0.5)), torch.arange(n, device="cuda") + m - n + 1)
+    rel = (out.double() - ref) / ref
+    assert float(rel.abs().max()) < 6 * 2.0 ** -24 / 3 * (m / 128 + m / 384) ** 0.5 + 24 * 2.0 ** -23 + 2.0 ** -23
+
+
+@pytest.mark.parametrize("qk", [F32, F16])
+def test_prompt_long_sums_do_not_shrink(gpu, qk):
+    """131,072 keys in one piece (352 row tiles leave nothing to split).  fp32
+    rows as above.  fp16 rows: the mean error of 128 dims' numbers, whose
+    rounding, 2^-11 / sqrt(3) each, averages out, is a twentieth of half a step
+    at most for a chain's loss, and five deviations of the mean."""
+    n, heads, n_kv, hd, m = 700, 128, 16, 128, 131072
+    c = Cache([m], 64, n_kv, hd, F16, seed=2)
+    one_sign(c, m)
+    q = randn(n, heads, hd, seed=3, kind=qk)
+    out, st = R.prompt(gpu, c, q, [n], [m], heads, hd ** -0.5)
+    assert st == 0
+    pick = torch.arange(0, n, 50, device="cuda")
+    k, v = c.rows(0)
+    ref, _ = R.attend(q[pick, :8], k[:, :1], v[:, :1], float(np.float32(hd ** -0.5)), pick + m - n + 1)
+    rel = (out[pick, :8].double() - ref) / ref
+    if qk == F32:
+        assert float(rel.abs().max()) < 6 * 2.0 ** -24 / 3 * (m / 128 + m / 384) ** 0.5 + 24 * 2.0 ** -23 + 2.0 ** -23
+    else:
+        assert abs(float(rel.mean())) < 2.0 ** -11 / 20 + 5 * 2.0 ** -11 / 3 ** 0.5 / 128 ** 0.5
