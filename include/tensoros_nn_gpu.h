@@ -216,23 +216,28 @@ typedef struct {
 
 /* Rotary positions: pair i < rot_dim/2 of a head turns by pos * theta_i,
  * theta_i = base^(-2i/rot_dim) / freq_factors[i]; elements from rot_dim on
- * stay.  LINEAR divides theta_i by `factor`.  YARN (Peng et al. 2023) blends
- * theta_i (fast pairs) with theta_i / factor (slow ones) along the ramp
- * between the pairs that turn beta_fast and beta_slow times in orig_ctx
- * positions, and multiplies the rotated elements by attn_factor * (1 + 0.1
- * ln factor).  Angles are kept as 64-bit fractions of a turn, so far positions
+ * stay.  LINEAR divides theta_i by `factor`.  YARN, as models of that method
+ * (Peng et al. 2023) are trained and released, blends theta_i (fast pairs) with
+ * theta_i / factor (slow ones) linearly in i between two edges: the pairs that
+ * turn beta_fast and beta_slow times in orig_ctx positions, e(b) = rot_dim
+ * ln(orig_ctx / (2 pi b)) / (2 ln base), the first rounded down, the second up,
+ * both kept within [0, rot_dim - 1] (edges that meet: 0.001 apart).
+ * YARN_UNROUNDED takes the edges as they are, for models marked as not
+ * truncating them.  Both multiply the rotated elements by attn_factor * (1 +
+ * 0.1 ln factor).  Angles are kept as 64-bit fractions of a turn, so far positions
  * lose nothing.  (tos_rope_dev keeps the reference's own sine and cosine.) */
 enum { TOS_ROTARY_INTERLEAVED = 0,   /* pairs (2i, 2i + 1), as llm_rope */
        TOS_ROTARY_HALF = 1 };        /* pairs (i, i + rot_dim/2) */
-enum { TOS_ROTARY_SCALE_NONE = 0, TOS_ROTARY_SCALE_LINEAR = 1, TOS_ROTARY_SCALE_YARN = 2 };
+enum { TOS_ROTARY_SCALE_NONE = 0, TOS_ROTARY_SCALE_LINEAR = 1, TOS_ROTARY_SCALE_YARN_UNROUNDED = 2,
+       TOS_ROTARY_SCALE_YARN = 3 };
 typedef struct {
     int rot_dim;             /* even, 2..256 */
     int layout;              /* TOS_ROTARY_INTERLEAVED or TOS_ROTARY_HALF */
     float base;
     int scaling;             /* TOS_ROTARY_SCALE_* */
-    float factor;            /* LINEAR, YARN: >= 1 */
-    int orig_ctx;            /* YARN */
-    float beta_fast, beta_slow, attn_factor;   /* YARN: 32, 1, 1 are usual */
+    float factor;            /* LINEAR, YARN*: >= 1 */
+    int orig_ctx;            /* YARN* */
+    float beta_fast, beta_slow, attn_factor;   /* YARN*: 32, 1, 1 are usual */
     const float *freq_factors;   /* host, rot_dim/2 positive values, or NULL */
 } tos_rotary_desc_t;
 typedef struct tos_rotary tos_rotary_t;

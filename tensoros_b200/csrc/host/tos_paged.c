@@ -86,10 +86,23 @@ static int pair_check(const tos_rows_t *src, const tos_rows_t *dst, int heads, i
 
 /* ------------------------------------------------------------- rotation */
 
+static int is_yarn(int scaling) { return scaling == TOS_ROTARY_SCALE_YARN || scaling == TOS_ROTARY_SCALE_YARN_UNROUNDED; }
+
 /* The pair index at which a rotation makes `turns` turns in ctx positions. */
 static long double yarn_edge(int rot, double base, double turns, int ctx)
 {
     return rot * logl((long double)ctx / (turns * 2.0L * (long double)M_PI)) / (2.0L * logl((long double)base));
+}
+
+/* Where the blend of a YARN rotation begins and ends. */
+static void yarn_edges(const tos_rotary_desc_t *d, long double *lo, long double *hi)
+{
+    *lo = yarn_edge(d->rot_dim, d->base, d->beta_fast, d->orig_ctx);
+    *hi = yarn_edge(d->rot_dim, d->base, d->beta_slow, d->orig_ctx);
+    if (d->scaling == TOS_ROTARY_SCALE_YARN_UNROUNDED) return;
+    *lo = fminl(fmaxl(floorl(*lo), 0), d->rot_dim - 1);
+    *hi = fminl(fmaxl(ceill(*hi), 0), d->rot_dim - 1);
+    if (*lo == *hi) *hi += 0.001L;
 }
 
 static int rotary_desc_ok(const tos_rotary_desc_t *d)
@@ -99,7 +112,7 @@ static int rotary_desc_ok(const tos_rotary_desc_t *d)
     if (!(d->base > 0.0f) || !isfinite(d->base)) return 0;
     if (d->scaling < TOS_ROTARY_SCALE_NONE || d->scaling > TOS_ROTARY_SCALE_YARN) return 0;
     if (d->scaling != TOS_ROTARY_SCALE_NONE && (!(d->factor >= 1.0f) || !isfinite(d->factor))) return 0;
-    if (d->scaling == TOS_ROTARY_SCALE_YARN &&
+    if (is_yarn(d->scaling) &&
         (d->orig_ctx <= 0 || !(d->base > 1.0f) || !(d->beta_slow > 0.0f) || !(d->beta_fast > d->beta_slow) ||
          !isfinite(d->beta_fast) || !isfinite(d->attn_factor)))
         return 0;
@@ -121,9 +134,9 @@ int tos_rotary_create(tos_rotary_t **out, const tos_rotary_desc_t *d)
         long double theta = powl((long double)d->base, -2.0L * i / d->rot_dim);
         if (d->freq_factors) theta /= d->freq_factors[i];
         if (d->scaling == TOS_ROTARY_SCALE_LINEAR) theta /= d->factor;
-        if (d->scaling == TOS_ROTARY_SCALE_YARN) {
-            const long double lo = yarn_edge(d->rot_dim, d->base, d->beta_fast, d->orig_ctx);
-            const long double hi = yarn_edge(d->rot_dim, d->base, d->beta_slow, d->orig_ctx);
+        if (is_yarn(d->scaling)) {
+            long double lo, hi;
+            yarn_edges(d, &lo, &hi);
             long double g = (i - lo) / (hi - lo);
             g = g < 0 ? 0 : g > 1 ? 1 : g;
             theta *= (1 - g) + g / d->factor;
@@ -138,7 +151,7 @@ int tos_rotary_create(tos_rotary_t **out, const tos_rotary_desc_t *d)
     r->rot_dim = d->rot_dim;
     r->r.rot = d->rot_dim;
     r->r.half = d->layout == TOS_ROTARY_HALF;
-    r->r.mag = d->scaling == TOS_ROTARY_SCALE_YARN ? d->attn_factor * (1.0f + 0.1f * logf(d->factor)) : 1.0f;
+    r->r.mag = is_yarn(d->scaling) ? d->attn_factor * (1.0f + 0.1f * logf(d->factor)) : 1.0f;
     int e = cudaMalloc((void **)&r->r.turn, (size_t)n * sizeof(turn[0]));
     if (!e) e = cudaMemcpyAsync(r->r.turn, turn, (size_t)n * sizeof(turn[0]), cudaMemcpyHostToDevice, tos_g.stream);
     if (!e) e = cudaStreamSynchronize(tos_g.stream);

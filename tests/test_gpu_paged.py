@@ -2,6 +2,7 @@
 (paged_ref.py, which derives the tolerances): per-head norm and rotary
 positions, the append, prompt and decode attention, and a run of them."""
 import ctypes as C
+import math
 
 import numpy as np
 import pytest
@@ -821,3 +822,37 @@ def test_prompt_long_sums_do_not_shrink(gpu, qk):
         assert float(rel.abs().max()) < 6 * 2.0 ** -24 / 3 * (m / 128 + m / 384) ** 0.5 + 24 * 2.0 ** -23 + 2.0 ** -23
     else:
         assert abs(float(rel.mean())) < 2.0 ** -11 / 20 + 5 * 2.0 ** -11 / 3 ** 0.5 / 128 ** 0.5
+
+
+# ------------------------------------------------------------------ YaRN's ramp
+
+@pytest.mark.parametrize("rot,base,orig,factor,low,high", [
+    (128, 10000.0, 4096, 4.0, 20, 46),        # 20.94 and 45.03
+    (64, 10000.0, 4096, 40.0, 10, 23),        # 10.47 and 22.51
+    (128, 500000.0, 8192, 8.0, 18, 35),       # 18.08 and 34.98
+    (64, 1000000.0, 32768, 4.0, 11, 20),      # 11.80 and 19.83
+    (64, 10000.0, 100, 8.0, 0, 10),           # -2.43 and 9.61
+    (64, 10000.0, 4, 8.0, 0, 0.001),          # -13.61 and -1.57: all slow but the first
+    (4, 10000.0, 10 ** 9, 8.0, 3, 3.001),     # 3.35 and 4.10: all fast
+])
+def test_yarn_ramp_between_rounded_edges(gpu, rot, base, orig, factor, low, high):
+    """Scaling 3 against the edges, worked out apart from this code: pairs up to
+    the first keep their frequency, from the second on have it divided by the
+    factor, and between them go from one to the other in equal steps."""
+    d = R.rotary_desc(rot, "half", base=base, factor=factor, orig=orig, attn=1.0)
+    d.scaling = 3
+    r = Rotary(gpu, d)
+    pos = torch.tensor([1, 7, 1000, 65535], dtype=torch.int32, device="cuda")
+    x = torch.zeros(4, 1, rot, device="cuda")
+    x[..., :rot // 2] = 1
+    y = torch.empty_like(x)
+    a, b = R.rows(x), R.rows(y)
+    assert gpu.tos_qk_norm_rotary_dev(C.byref(a), C.byref(b), None, None, 4, 1, 0, rot, None, None, 0.0, r.h,
+                                      pos.data_ptr(), R.stream()) == 0
+    mag = 1 + 0.1 * math.log(factor)
+    for i in range(rot // 2):
+        part = 0.0 if i <= low else 1.0 if i >= high else (i - low) / (high - low)
+        angle = pos.double().cpu() * base ** (-2.0 * i / rot) * (1 - part + part / factor)
+        tol = mag * (2.0 ** -22 + 4 * R.U)
+        assert float((y[:, 0, i].double().cpu() - mag * torch.cos(angle)).abs().max()) < tol, i
+        assert float((y[:, 0, i + rot // 2].double().cpu() - mag * torch.sin(angle)).abs().max()) < tol, i

@@ -182,3 +182,14 @@ def test_rotary_factor_refusals(lib):
     assert lib.tos_rotary_create(None, C.byref(d)) == EINVAL
     assert lib.tos_rotary_create(C.byref(h), None) == EINVAL
     lib.tos_rotary_destroy(None)
+
+
+@pytest.mark.parametrize("scaling", [2, 3])
+@pytest.mark.parametrize("o", [dict(orig_ctx=0), dict(beta_fast=1.0), dict(beta_slow=0.0), dict(base=1.0),
+                               dict(factor=0.5), dict(attn_factor=float("inf"))])
+def test_yarn_refusals(lib, scaling, o):
+    a = dict(rot_dim=64, layout=0, base=10000.0, scaling=scaling, factor=2.0, orig_ctx=4096, beta_fast=32.0,
+             beta_slow=1.0, attn_factor=1.0)
+    a.update(o)
+    d, h = _ffi.RotaryDesc(**a), C.c_void_p()
+    assert lib.tos_rotary_create(C.byref(h), C.byref(d)) == EINVAL and not h.value
