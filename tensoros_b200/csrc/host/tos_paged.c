@@ -174,7 +174,7 @@ void tos_rotary_destroy(tos_rotary_t *r)
 static int rotary_args_check(const tos_rotary_t *rot, const int *pos, int hd, const float *qn, const float *kn, float eps)
 {
     if (rot && (rot->rot_dim > hd || !pos)) return TOS_EINVAL;
-    if (((uintptr_t)qn & 3) || ((uintptr_t)kn & 3)) return TOS_EINVAL;
+    if (((uintptr_t)qn & 3) || ((uintptr_t)kn & 3) || ((uintptr_t)pos & 3)) return TOS_EINVAL;
     if ((qn || kn) && !(eps >= 0.0f && isfinite(eps))) return TOS_EINVAL;
     return TOS_OK;
 }
@@ -218,7 +218,7 @@ int tos_kv_append_paged_dev(const tos_paged_kv_t *kv, const tos_rows_t *k, const
     if (!rc) rc = rows_check(v, kv->n_kv, kv->head_dim);
     if (!rc) rc = pair_check(q, q_out, n_heads, kv->head_dim);
     if (!rc) rc = rotary_args_check(rot, pos, kv->head_dim, q_norm, k_norm, eps);
-    if (!rc && n_tokens && (!seq || !slot)) rc = TOS_EINVAL;
+    if (!rc && n_tokens && (!seq || !slot || ((uintptr_t)seq & 3) || ((uintptr_t)slot & 3))) rc = TOS_EINVAL;
     if (!rc && (k->type != v->type || (n_heads && q->type != k->type))) rc = TOS_ENOTSUP;
     if (rc) return tos_set_status(rc);
     int before;

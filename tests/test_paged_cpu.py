@@ -193,3 +193,14 @@ def test_yarn_refusals(lib, scaling, o):
     a.update(o)
     d, h = _ffi.RotaryDesc(**a), C.c_void_p()
     assert lib.tos_rotary_create(C.byref(h), C.byref(d)) == EINVAL and not h.value
+
+
+def test_token_arrays_are_aligned(lib):
+    """Sequences, slots and positions are read as ints."""
+    for o in ("seq", "slot", "pos"):
+        for off in (1, 2, 3):
+            assert append(lib, **{o: PTR + off}) == EINVAL, o
+    q, qo = rows(), rows(ptr=2 * PTR)
+    for off in (1, 2, 3):
+        assert lib.tos_qk_norm_rotary_dev(ref(q), ref(qo), None, None, 3, 4, 0, 64, None, None, 0.0, None, PTR + off,
+                                          None) == EINVAL
