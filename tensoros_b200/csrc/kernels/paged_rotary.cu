@@ -145,60 +145,61 @@ __global__ void __launch_bounds__(32 * kRotWarps) rotary_plain_kernel(const __gr
   const tosk_rotary_args_t& a = p.a;
   const int lane = threadIdx.x & 31, hd = a.hd, rp = a.rot.turn ? a.rot.rot >> 1 : 0;
   const long long t = blockIdx.x;
-  const int g = blockIdx.y * kRotWarps + (threadIdx.x >> 5);          // head of the token: q, k, v
   pdl_wait();
   pdl_trigger();
-  if (g >= a.n_heads + (a.append ? 2 : 1) * a.n_kv) return;
-  const int kind = g < a.n_heads ? 0 : g < a.n_heads + a.n_kv ? 1 : 2;
-  const int h = g - (kind == 0 ? 0 : kind == 1 ? a.n_heads : a.n_heads + a.n_kv);
-  const tosk_rows_t& r = kind == 0 ? a.q : kind == 1 ? a.k : a.v;
-  const TI* src = reinterpret_cast<const TI*>(r.src) + t * r.sstride + (long long)h * hd;
-  const float* w = kind == 0 ? a.q_norm : kind == 1 ? a.k_norm : nullptr;
-  float x[4], y[4], ss = 0.0f;
-  int e0[4], e1[4];
+  const int total = a.n_heads + (a.append ? 2 : 1) * a.n_kv;
+  for (int g = blockIdx.y * kRotWarps + (threadIdx.x >> 5); g < total; g += gridDim.y * kRotWarps) {   // head: q, k, v
+    const int kind = g < a.n_heads ? 0 : g < a.n_heads + a.n_kv ? 1 : 2;
+    const int h = g - (kind == 0 ? 0 : kind == 1 ? a.n_heads : a.n_heads + a.n_kv);
+    const tosk_rows_t& r = kind == 0 ? a.q : kind == 1 ? a.k : a.v;
+    const TI* src = reinterpret_cast<const TI*>(r.src) + t * r.sstride + (long long)h * hd;
+    const float* w = kind == 0 ? a.q_norm : kind == 1 ? a.k_norm : nullptr;
+    float x[4], y[4], ss = 0.0f;
+    int e0[4], e1[4];
 #pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    const int i = lane + 32 * c;
-    const bool half = i < rp && a.rot.half;
-    e0[c] = half ? i : 2 * i;
-    e1[c] = half ? i + rp : 2 * i + 1;
-    x[c] = i < hd >> 1 ? (float)src[e0[c]] : 0.0f;
-    y[c] = i < hd >> 1 ? (float)src[e1[c]] : 0.0f;
-    ss = fmaf(x[c], x[c], fmaf(y[c], y[c], ss));
-  }
-  if (w) {
-    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    const float rs = rsqrtf(fmaf(ss, 1.0f / (float)hd, a.eps));
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
-      if (lane + 32 * c < hd >> 1) {
-        x[c] = x[c] * rs * w[e0[c]];
-        y[c] = y[c] * rs * w[e1[c]];
-      }
-  }
-  void* dst = r.dst;
-  long long off = t * r.dstride + (long long)h * hd;
-  int dtype = r.dtype;
-  if (a.append && kind > 0) {
-    const long long row = cache_row(a, a.seq[t], a.slot[t]);
-    if (row < 0) return;
-    dst = kind == 1 ? a.kv.k : a.kv.v;
-    off = (row + h) * hd;
-    dtype = a.kv.type;
-  }
-#pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    const int i = lane + 32 * c;
-    if (i >= hd >> 1) break;
-    if (kind < 2 && i < rp) {
-      const float2 z = pair_turn(a.rot, i, a.pos[t]);
-      const float u = x[c], v = y[c];
-      x[c] = fmaf(u, z.x, -(v * z.y));
-      y[c] = fmaf(v, z.x, u * z.y);
+    for (int c = 0; c < 4; ++c) {
+      const int i = lane + 32 * c;
+      const bool half = i < rp && a.rot.half;
+      e0[c] = half ? i : 2 * i;
+      e1[c] = half ? i + rp : 2 * i + 1;
+      x[c] = i < hd >> 1 ? (float)src[e0[c]] : 0.0f;
+      y[c] = i < hd >> 1 ? (float)src[e1[c]] : 0.0f;
+      ss = fmaf(x[c], x[c], fmaf(y[c], y[c], ss));
     }
-    const float o0[1] = {x[c]}, o1[1] = {y[c]};
-    store_n<1>(dst, dtype, off + e0[c], o0);
-    store_n<1>(dst, dtype, off + e1[c], o1);
+    if (w) {
+      for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      const float rs = rsqrtf(fmaf(ss, 1.0f / (float)hd, a.eps));
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        if (lane + 32 * c < hd >> 1) {
+          x[c] = x[c] * rs * w[e0[c]];
+          y[c] = y[c] * rs * w[e1[c]];
+        }
+    }
+    void* dst = r.dst;
+    long long off = t * r.dstride + (long long)h * hd;
+    int dtype = r.dtype;
+    if (a.append && kind > 0) {
+      const long long row = cache_row(a, a.seq[t], a.slot[t]);
+      if (row < 0) continue;
+      dst = kind == 1 ? a.kv.k : a.kv.v;
+      off = (row + h) * hd;
+      dtype = a.kv.type;
+    }
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const int i = lane + 32 * c;
+      if (i >= hd >> 1) break;
+      if (kind < 2 && i < rp) {
+        const float2 z = pair_turn(a.rot, i, a.pos[t]);
+        const float u = x[c], v = y[c];
+        x[c] = fmaf(u, z.x, -(v * z.y));
+        y[c] = fmaf(v, z.x, u * z.y);
+      }
+      const float o0[1] = {x[c]}, o1[1] = {y[c]};
+      store_n<1>(dst, dtype, off + e0[c], o0);
+      store_n<1>(dst, dtype, off + e1[c], o1);
+    }
   }
 }
 
@@ -392,7 +393,7 @@ extern "C" int tosk_rotary_rows(const tosk_rotary_args_t* a, cudaStream_t st) {
   if (v == 1) {
     p.group = 32;
     p.parts = (heads + kRotWarps - 1) / kRotWarps;
-    if (p.parts > 65535) return (int)cudaErrorInvalidValue;
+    if (p.parts > 65535) p.parts = 65535;                // the grid's limit; warps go on to further heads
     return launch_rot(f32 ? (const void*)rotary_plain_kernel<float> : (const void*)rotary_plain_kernel<__half>, p,
                       dim3((unsigned)a->n_tokens, p.parts), st);
   }

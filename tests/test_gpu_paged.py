@@ -856,3 +856,36 @@ def test_yarn_ramp_between_rounded_edges(gpu, rot, base, orig, factor, low, high
         tol = mag * (2.0 ** -22 + 4 * R.U)
         assert float((y[:, 0, i].double().cpu() - mag * torch.cos(angle)).abs().max()) < tol, i
         assert float((y[:, 0, i + rot // 2].double().cpu() - mag * torch.sin(angle)).abs().max()) < tol, i
+
+
+# ------------------------------------------------------------- counts of heads
+
+@pytest.mark.parametrize("hd,odd", [(2, 0), (4, 1), (8, 0)])
+def test_rotary_of_very_many_heads(gpu, hd, odd):
+    """More heads than one warp each of the largest grid, element-wise (2 dims,
+    an odd address) and in 16-byte pieces."""
+    heads, n_kv, n = 270001, 263001, 2
+    buf = randn(n * (heads + n_kv) * hd + 8, seed=1)
+    x = torch.as_strided(buf, (n, heads + n_kv, hd), ((heads + n_kv) * hd, hd, 1), odd)
+    q, k = x[:, :heads], x[:, heads:]
+    qo, ko = torch.empty(n, heads, hd, device="cuda"), torch.empty(n, n_kv, hd, device="cuda")
+    d = R.rotary_desc(hd, "interleaved")
+    rot = Rotary(gpu, d)
+    pos = torch.tensor([5, 900], dtype=torch.int32, device="cuda")
+    a = [R.rows(t) for t in (q, qo, k, ko)]
+    assert gpu.tos_qk_norm_rotary_dev(*[C.byref(r) for r in a], n, heads, n_kv, hd, None, None, 0.0, rot.h,
+                                      pos.data_ptr(), R.stream()) == 0
+    R.assert_rows(qo, *R.norm_rotary(q, None, 0.0, d, pos), "q")
+    R.assert_rows(ko, *R.norm_rotary(k, None, 0.0, d, pos), "k")
+
+
+def test_append_of_very_many_heads(gpu):
+    n_kv, hd, page = 140001, 2, 2
+    c = Cache([3], page, n_kv, hd, F32, seed=1, fill=3.0)
+    k, v = randn(2, n_kv, hd, seed=2), randn(2, n_kv, hd, seed=3)
+    seq, slot = (torch.tensor(t, dtype=torch.int32, device="cuda") for t in ([0, 0], [1, 2]))
+    a, desc = [R.rows(t) for t in (k, v)], c.desc()
+    assert gpu.tos_kv_append_paged_dev(C.byref(desc), *[C.byref(r) for r in a], None, None, 2, 0, seq.data_ptr(),
+                                       slot.data_ptr(), None, None, None, 0.0, None, R.stream()) == 0
+    pg, r = c.where(c.table[0], 3)
+    assert torch.equal(c.k[pg[1:], r[1:]], k) and torch.equal(c.v[pg[1:], r[1:]], v)
