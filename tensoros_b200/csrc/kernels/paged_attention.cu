@@ -58,6 +58,33 @@ struct GenArgs {
   int q_vec, kv_vec;         // four-element accesses are aligned
 };
 
+// The values that this thread has just put into a tile, of keys that not all rows
+// see (row r of the tile is key at + r of those): what is not finite becomes
+// zero, and its key is noted.
+template <int NJ>
+static __device__ __noinline__ void clean_values(float* sv, int at, uint32_t* s_odd) {
+#pragma unroll 1
+  for (int i = threadIdx.x; i < kKT * 16 * NJ; i += kGenThreads) {
+    const int r = i / (16 * NJ), c = i % (16 * NJ);
+    uint4* u = reinterpret_cast<uint4*>(sv + r * (64 * NJ + 4) + 4 * c);
+    uint4 x = *u;
+    if (at + r < 0 || !clean_piece<float>(x)) continue;
+    *u = x;
+    atomicOr(&s_odd[(at + r) >> 5], 1u << ((at + r) & 31));
+  }
+}
+// Sum of the values that were left out, of dim d at keys [some, lim).
+static __device__ __noinline__ float left_out(const PagedProblem& p, const int* table, int kvh, const uint32_t* s_odd,
+                                              int some, int lim, int d) {
+  float s = 0.0f;
+  for (int key = some; key < lim && d < p.hd; ++key)
+    if (s_odd[(key - some) >> 5] >> ((key - some) & 31) & 1) {
+      const float x = load_elem(p.v, p.kv_type, kv_off(p, table, key, kvh) + d);
+      if (not_finite(x)) s += x;
+    }
+  return s;
+}
+
 template <int R, int NJ>
 __global__ void __launch_bounds__(kGenThreads) paged_attn_general_kernel(const __grid_constant__ GenArgs a) {
   constexpr int RI = R / 16, LD = 64 * NJ + 4, LP = kKT + 4;
@@ -68,7 +95,7 @@ __global__ void __launch_bounds__(kGenThreads) paged_attn_general_kernel(const _
   float* sk = sq + R * LD;              // [kKT][LD]
   float* sv = sk + kKT * LD;            // [kKT][LD]
   float* sp = sv + kKT * LD;            // [R][LP]
-  __shared__ int s_dirty;               // values that are not finite were left out
+  __shared__ uint32_t s_odd[2];         // keys from `some` on with values that are not finite, which were left out
   __shared__ long long s_off[2][kKT];   // where the rows of a tile lie
   const PagedProblem& p = a.p;
   pdl_wait();
@@ -91,6 +118,8 @@ __global__ void __launch_bounds__(kGenThreads) paged_attn_general_kernel(const _
     k1 = min(k1, k0 + p.chunk);
     if (k0 >= k1) return;               // no row of the tile sees a key of this split
   }
+  // from here on not all rows see a key (of at most 63, a row tile's tokens); none: far behind
+  const int some = first < k1 ? max(first, k0) : 0x7fff0000;
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
   const int hd4 = (p.hd + 3) / 4;
   auto place = [&](int kt, int buf) {
@@ -106,19 +135,13 @@ __global__ void __launch_bounds__(kGenThreads) paged_attn_general_kernel(const _
       vx = load4_tail(p.v, p.kv_type, off, 4 * c, p.hd, a.kv_vec);
     }
   };
-  auto put = [&](int i, int kt, const float4& kx, float4 vx) {
+  auto put = [&](int i, const float4& kx, const float4& vx) {
     const int r = i / (16 * NJ), c = i % (16 * NJ);
-    if (kt + r >= first && (not_finite(vx.x) || not_finite(vx.y) || not_finite(vx.z) || not_finite(vx.w))) {
-      uint4 u = make_uint4(__float_as_uint(vx.x), __float_as_uint(vx.y), __float_as_uint(vx.z), __float_as_uint(vx.w));
-      clean_piece<float>(u);
-      vx = make_float4(__uint_as_float(u.x), __uint_as_float(u.y), __uint_as_float(u.z), __uint_as_float(u.w));
-      s_dirty = 1;
-    }
     *reinterpret_cast<float4*>(sk + r * LD + 4 * c) = kx;
     *reinterpret_cast<float4*>(sv + r * LD + 4 * c) = vx;
   };
   place(k0, 0);
-  if (tid == 0) s_dirty = 0;
+  if (tid < 2) s_odd[tid] = 0;
 #pragma unroll 4
   for (int i = tid; i < R * 16 * NJ; i += kGenThreads) {
     const int r = i / (16 * NJ), c = i % (16 * NJ);
@@ -154,13 +177,14 @@ __global__ void __launch_bounds__(kGenThreads) paged_attn_general_kernel(const _
 #pragma unroll
     for (int x = 0; x < NL; ++x) {
       if (AHEAD) {
-        put(tid + x * kGenThreads, kt, rk[AHEAD ? x : 0], rv[AHEAD ? x : 0]);
+        put(tid + x * kGenThreads, rk[AHEAD ? x : 0], rv[AHEAD ? x : 0]);
       } else {
         float4 kx, vx;
         piece(tid + x * kGenThreads, buf, kx, vx);
-        put(tid + x * kGenThreads, kt, kx, vx);
+        put(tid + x * kGenThreads, kx, vx);
       }
     }
+    if (kt + kKT > some) clean_values<NJ>(sv, kt - some, s_odd);
     __syncthreads();
     if (AHEAD && kt + kKT < k1) {
 #pragma unroll
@@ -246,13 +270,12 @@ __global__ void __launch_bounds__(kGenThreads) paged_attn_general_kernel(const _
     const int r = ty + 16 * i;
     if (r >= nr) continue;
     const int rr = r0 + r, tok = t.q0 + rr / p.group, h = kvh * p.group + rr % p.group;
-    if (s_dirty) {
+    if (s_odd[0] | s_odd[1]) {
 #pragma unroll
       for (int j = 0; j < NJ; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (4 * tx + 64 * j + e < p.hd)
-            o[i][j][e] += bad_value(p, t.table, kvh, max(first, k0), lim[i], 4 * tx + 64 * j + e);
+          o[i][j][e] += left_out(p, t.table, kvh, s_odd, some, lim[i], 4 * tx + 64 * j + e);
     }
     if (p.splits) {
       const long long row = (long long)(p.slot0 + split) * p.total_q * p.heads + (long long)tok * p.heads + h;

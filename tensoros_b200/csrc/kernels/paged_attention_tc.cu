@@ -1181,7 +1181,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
       }
       if (!f32) flush(hf * (HD / 2), HD);
       tc_fence_before();                                                // O and S are read: the next piece's MMAs may come
-      if (live && isnan(odd.x + odd.y)) *odd_seen = 1;
+      if (live && !isnan(l) && isnan(odd.x + odd.y)) *odd_seen = 1;      // not by its weights
     }
   }
   __syncthreads();

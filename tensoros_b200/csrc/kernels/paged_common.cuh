@@ -123,18 +123,8 @@ __device__ __forceinline__ bool clean_piece(uint4& u) {
   return any;
 }
 
-// Sum of the values of one dim at keys [j0, j1) that are not finite; 0: none.
-static __device__ __noinline__ float bad_value(const PagedProblem& p, const int* table, int kvh, int j0, int j1, int d) {
-  float s = 0.0f;
-  for (int j = j0; j < j1; ++j) {
-    const long long off = kv_off(p, table, j, kvh);
-    const float x = off >= 0 ? load_elem(p.v, p.kv_type, off + d) : 0.0f;
-    if (not_finite(x)) s += x;
-  }
-  return s;
-}
-
-// The same by a warp for dims lane + 32 i.
+// Sums of the values at keys [j0, j1) that are not finite, by a warp, at dims
+// lane + 32 i; 0: none.
 static __device__ __noinline__ void bad_values(const PagedProblem& p, const int* table, int kvh, int j0, int j1,
                                                float (&s)[8]) {
   constexpr int U = 8;
