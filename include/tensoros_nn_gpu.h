@@ -275,7 +275,9 @@ int tos_kv_append_paged_dev(const tos_paged_kv_t *kv, const tos_rows_t *k, const
  * computed / not seen).  Rows outside the sequences stay as they were.  Heads
  * are grouped: query head h reads key/value head h / (n_heads / n_kv).  out
  * and q have one type and must not overlap.  Keys and values that a row does
- * not see never reach it, infinities and NaN included. */
+ * not see never reach it, infinities and NaN included; of those that it sees,
+ * a NaN score makes the row NaN, a score of -infinity weighs nothing, and
+ * infinite or NaN values give their element their sum. */
 size_t tos_attention_prompt_paged_workspace_bytes(int n_seqs, int total_q, int max_q, int max_kv, int n_heads,
                                                   int n_kv, int head_dim);
 int tos_attention_prompt_paged_dev(const tos_rows_t *out, const tos_rows_t *q, const tos_paged_kv_t *kv,

@@ -540,6 +540,9 @@ void part_views(PagedProblem& p, void* ws, int slots, size_t fold) {
 //   fp16 cache      6 x 48:  38 MB 14.5 / 13.2, 151 MB 20.7 / 26.7
 //     fp32 rows    32 x 128:  8 MB 12.3 / 11.1,  34 MB 12.8 / 13.2, 134 MB 17.8 / 25.3
 //     fp16 rows    32 x 128:  1 MB  8.9 / 10.8
+// Dims between those, groups and several sequences go by the same rule,
+// unmeasured; max_kv stands for every sequence's length, so a ragged batch
+// counts as if all were the longest.
 // A shared prefix goes by its rows a key/value head (all tokens' together), one
 // row tile for fp16 caches; a decode call behind 4096 and 16384 keys (us):
 //   fp32 cache  32 x 128,   8 rows: 142, 576 / 56, 177;  32 rows: 202, 912 / 140, 480;
@@ -565,7 +568,7 @@ int run_tiles(const PagedProblem& p, cudaStream_t st) {
 // schedule, counted in key tiles of 128: rounds over the SMs, each its share
 // of the keys and ~3.5 tiles' worth of starting and ending a piece; the joining
 // ~2, and a tile's worth for every 1.1 M elements of partial rows.  (A key tile
-// takes 2.4 us with fp16 rows, 4.0 with fp32 rows.)  A sequence has a row tile
+// takes 2.0 us with fp16 rows, 4.0 with fp32 rows.)  A sequence has a row tile
 // of its own, however short: 16 sequences of 8 tokens behind 4096 keys take
 // 76 us, 106 where only packed rows are counted; 20 of 16, 122, unsplit 139.
 // The estimate does not see that a causal prompt's row tiles differ in length:

@@ -25,13 +25,13 @@
 // fp16's subnormals; it cancels in O / l.
 //
 // What bounds it (B200; a piece a SM, 1024 to 8192 keys): a key tile of both
-// row tiles takes 2.4 us for fp16 rows, where a library product's rate would
+// row tiles takes 2.0 us for fp16 rows, where a library product's rate would
 // take 1.5, and 4.0 for fp32 rows, whose two-part products are twice the work;
-// a call costs 19 to 26 us beside its tiles.  The row tiles
+// a call costs 21 to 25 us beside its tiles.  The row tiles
 // alternate between softmax and MMAs, two of them do not fill the tensor
 // cores, and a third does not fit tensor memory.  Packed fp16 prompts of 6537
-// tokens, 32 / 8 heads x 128: 189 us, 852 TFLOP/s.
-// Steps on the way (the same prompts, us): one warpgroup a row tile 287; queries
+// tokens, 32 / 8 heads x 128: 190 us, 846 TFLOP/s.
+// Steps on the way (the same prompts, us, each when it was made): one warpgroup a row tile 287; queries
 // loaded in batches, registers moved to the softmax warps, halves of P handed
 // on 235; one elected thread for all MMAs 208; four warpgroups 207; persistent
 // 197; weights and maximum from one read of S 194; two pairs of eight
@@ -70,9 +70,10 @@ constexpr int kKeys = 128;            // keys of a tile
 constexpr float kBias = 7.0f;         // log2 of the factor that P carries
 constexpr int kPoly = 3;              // of eight pairs of exponentials, those at 2 and 5 go to the FMA pipe
 // Key tiles whose products one accumulator sums.  It loses 1e-7 of itself a step
-// of 16 keys.  fp32 rows: 3 (512 rows behind 7001 keys, us: 3: 159, 4: 154, 8: 145,
-// never: 138).  fp16 rows: 32, a loss of 2.6e-5, a twentieth of their rounding
-// (131,072 keys in one chain: 8e-4).
+// of 16 keys.  fp32 rows: 3 (512 rows behind 7001 keys, us: 3: 157, 4: 152, 8: 144,
+// never: 137).  fp16 rows: 32, a loss of 2.6e-5, a twentieth of their rounding
+// (131,072 keys in one chain: 8e-4; 700 rows behind 20,000 keys, us: 8: 601,
+// 16: 587, 32: 585, 64 and never: 575).
 __host__ __device__ constexpr int fold_tiles(bool split) { return split ? 3 : 32; }
 constexpr float kSlack = 8.0f;        // log2 by which the maximum may grow unfollowed
 

@@ -23,8 +23,8 @@
 //
 // Bound: HBM.  A 16-key step is 8 KB and 32 MMAs (HD 128), ~1/16 of what the
 // tensor pipe does in the time the bytes take.  Sixteen sequences of 1..4096
-// keys, 32 x 128: 90 to 94 us, 5.2 to 5.4 TB/s.  Short sequences leave the bus
-// idle while CTAs start and end (32 / 8 heads: 64 of 256 keys 29 us, 2.3 TB/s).
+// keys, 32 x 128: 91 to 95 us, 5.1 to 5.3 TB/s.  Short sequences leave the bus
+// idle while CTAs start and end (32 / 8 heads: 64 of 256 keys 30 us, 2.3 TB/s).
 #include <cuda_runtime.h>
 
 #include "paged_common.cuh"
