@@ -64,7 +64,8 @@ constexpr int kTcRegs = 96;            // a thread at launch, moved to the softm
 constexpr int kTcRegsSoftmax = 104, kTcRegsRest = 64;
 static_assert(4 * kTcRegsSoftmax + kTcRegsRest <= 5 * kTcRegs, "registers of the launch");
 constexpr int kCopyWarp = 16, kMmaWarp = 17, kPlanWarp = 18;
-constexpr int kTileBar = 9;            // named barriers: 1..8 pair the two warps of 32 rows, 9 and 10 a row tile's eight
+constexpr int kTileBar = 9;            // named barriers: 1..8 pair the two warps of 32 rows, 9 and 10 a row tile's eight,
+constexpr int kEndBar = 11;            // 11 all twenty, when the pipeline is done
 constexpr int kRows = 128;            // rows of a tile
 constexpr int kKeys = 128;            // keys of a tile
 constexpr float kBias = 7.0f;         // log2 of the factor that P carries
@@ -365,6 +366,9 @@ __device__ __forceinline__ bool pair_any(int bar, bool x) {
   return y != 0;
 }
 
+// In both register splits' code: what follows stays within the one or the other.
+__device__ __forceinline__ void end_sync() { asm volatile("bar.sync %0, %1;" ::"n"(kEndBar), "n"(kTcThreads) : "memory"); }
+
 __device__ __forceinline__ bool tile_any(int bar, bool x) {
   uint32_t y;
   asm volatile(
@@ -514,14 +518,31 @@ static __device__ __noinline__ void patch_piece(const PagedProblem& p, const Seq
   }
 }
 
+// Values that are not finite were left out or met: the CTA's pieces once more, by
+// two warps, for whom nobody waits but the end of the CTA.
+template <int HD>
+static __device__ __noinline__ void patch_pieces(const PagedProblem& p, int which) {
+  const int splits = p.splits ? p.splits : 1;
+  PlanCursor cur = {0, 0};
+  for (int k = 0;; ++k) {
+    const int g = piece_of(k);
+    const TileId id = pick_tile(p, g / p.n_kv / splits, cur);
+    if (id.seq < 0) return;
+    if ((k & 1) == which) patch_piece<HD>(p, seq_task(p, id.seq), g % p.n_kv, g / p.n_kv % splits, id.rt * 2 * kRows);
+  }
+}
+
 // fp32 rows meet an infinite element of a key as infinity times the high part
 // plus infinity times the low part of q, which is NaN where the low part is
 // zero or of the other sign.  Of 64 keys' scores in tensor memory, those that
 // are NaN by infinite elements alone become the sum of q's elements times them.
-// q: this lane's row, NULL: it has no scores to mend; left: keys it sees.
-static __device__ __noinline__ void infinite_scores(const PagedProblem& p, uint32_t ts, const int* table, int kvh, int key0,
-                                                    int left, const float* q) {
-  const int lane = threadIdx.x & 31;
+// A row a lane, of token tok and head `head`; left: keys from key0 on that it
+// sees, 0: it has no scores to mend.
+static __device__ __noinline__ void infinite_scores(const PagedProblem& p, uint32_t ts, int seq, int tok, int head, int key0,
+                                                    int left) {
+  const int lane = threadIdx.x & 31, kvh = head / p.group;
+  const int* table = p.table + (long long)seq * p.table_stride;
+  const float* q = reinterpret_cast<const float*>(p.q) + (long long)tok * p.q_stride + (long long)head * p.hd;
 #pragma unroll 1
   for (int c = 0; c < 64; c += 8) {
     uint32_t s[8];
@@ -529,7 +550,7 @@ static __device__ __noinline__ void infinite_scores(const PagedProblem& p, uint3
     tc_wait_ld8(s);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const bool mine = q && c + e < left && isnan(__uint_as_float(s[e]));
+      const bool mine = c + e < left && isnan(__uint_as_float(s[e]));
       if (!__any_sync(0xffffffffu, mine)) continue;
       const long long off = kv_off(p, table, key0 + c + e, kvh);
       float acc = 0.0f;
@@ -759,47 +780,61 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
         if (lane == 0) mbar_arrive(wempty + (n & 1));
         if (seq < 0) break;
         const int* table = p.table + (long long)seq * p.table_stride;
+        // lane i: the page of box i of the next tile, asked for a tile ahead
+        auto page_of_box = [&](int j) {
+          const int key = k0 + j * kKeys + lane * a.box_rows;
+          return lane * a.box_rows < kKeys && key < k1 ? table[p.pshift >= 0 ? key >> p.pshift : key / p.page_size] : -1;
+        };
+        int ahead = page_of_box(0);
         for (int j = 0; j < nmax && ok; ++j) {
           const int kt = k0 + j * kKeys, have = min(kKeys, k1 - kt);
           const int need = (have + a.box_rows - 1) / a.box_rows;
-          int page = -1, row = 0;
-          if (lane < need) {
-            const int key = kt + lane * a.box_rows;
-            page = table[key / p.page_size];
-            row = key % p.page_size;
-          }
-          for (int v = 0; v < 2 && ok; ++v) {
+          const int page = ahead, key = kt + lane * a.box_rows;
+          const int row = p.pshift >= 0 ? key & (p.page_size - 1) : key % p.page_size;
+          ahead = page_of_box(j + 1);
+          // K and V written out, each with its tensor map: chosen in a loop, the
+          // copies of 16-token pages fall behind the MMAs (700 rows behind 20,000
+          // keys 575 us, so 542)
+          auto slot_free = [&]() {
             const int s = used % T::kSlots;
             if (used >= T::kSlots) ok = mbar_wait(empty + s, (used / T::kSlots - 1) & 1, p.err, 31);
             ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-            // value rows behind the key range, and what is not finite where
-            // only some rows see a key, meet weights of 0: zeros instead
-            const bool some = v && kt + have > first, cut = some || (v && have < kKeys);
-            uint64_t* bar = cut ? tailbar : full + s;
+            return s;
+          };
+          auto bring = [&](const CUtensorMap* map, int s, uint64_t* bar) {
             if (lane == 0) mbar_arrive_expect_tx(bar, need * a.box_rows * HD * 2);
             __syncwarp();
             if (lane < need) {
               uint8_t* dst = ring + s * T::kTile + lane * a.box_rows * 128;
 #pragma unroll
-              for (int h = 0; h < T::kHalves; ++h)
-                tma_page(dst + h * 16384, v ? &a.mv : &a.mk, 64 * h, kvh, row, page, bar);
+              for (int h = 0; h < T::kHalves; ++h) tma_page(dst + h * 16384, map, 64 * h, kvh, row, page, bar);
             }
-            if (cut) {
-              ok = mbar_wait(tailbar, tails & 1, p.err, 32);
-              ok = __all_sync(0xffffffffu, ok);
-              if (!ok) break;
-              ++tails;
-              for (int h = 0; h < T::kHalves; ++h)
-                for (int o = have * 128 + lane * 16; o < kKeys * 128; o += 512)
-                  *reinterpret_cast<uint4*>(ring + s * T::kTile + h * 16384 + o) = make_uint4(0, 0, 0, 0);
-              if (some && clean_tile<T::kHalves>(ring + s * T::kTile, max(first - kt, 0), have)) *odd_seen = 1;
-              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-              __syncwarp();
-              if (lane == 0) mbar_arrive(full + s);
-            }
-            ++used;
+          };
+          const int sk = slot_free();
+          if (!ok) break;
+          bring(&a.mk, sk, full + sk);
+          ++used;
+          const int sv = slot_free();
+          if (!ok) break;
+          // value rows behind the key range, and what is not finite where
+          // only some rows see a key, meet weights of 0: zeros instead
+          const bool some = kt + have > first, cut = some || have < kKeys;
+          bring(&a.mv, sv, cut ? tailbar : full + sv);
+          if (cut) {
+            ok = mbar_wait(tailbar, tails & 1, p.err, 32);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            ++tails;
+            uint8_t* tile = ring + sv * T::kTile;
+            for (int h = 0; h < T::kHalves; ++h)
+              for (int o = have * 128 + lane * 16; o < kKeys * 128; o += 512)
+                *reinterpret_cast<uint4*>(tile + h * 16384 + o) = make_uint4(0, 0, 0, 0);
+            if (some && clean_tile<T::kHalves>(tile, max(first - kt, 0), have)) *odd_seen = 1;
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(full + sv);
           }
+          ++used;
         }
       }
       // every copy lands before the CTA may end
@@ -877,6 +912,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
       }
       __syncwarp();
     }
+    end_sync();
+    if (warp == kMmaWarp) {
+      tc_fence_after();
+      tmem_dealloc(tmem_at, 512);
+    }
+    if (warp > kMmaWarp && *odd_seen) patch_pieces<HD>(p, warp & 1);
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kTcRegsSoftmax));
     // --------------------------------------------------------------- softmax
@@ -996,11 +1037,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
           float top = half_top();
           if (pair_any(bar, j == 0 || !(top <= m + kSlack || isnan(l)))) {
             if (__any_sync(0xffffffffu, isnan(top) && !isnan(l))) {
-              infinite_scores(p, ts + 64 * hf, p.table + (long long)seq * p.table_stride, head / p.group,
-                              k0 + j * kKeys + 64 * hf, left,
-                              live && !isnan(l) ? reinterpret_cast<const float*>(p.q) + (long long)tok * p.q_stride +
-                                                      (long long)head * p.hd
-                                                : nullptr);
+              infinite_scores(p, ts + 64 * hf, seq, tok, head, k0 + j * kKeys + 64 * hf, isnan(l) ? 0 : left);
               top = half_top();
             }
             agree(top);
@@ -1184,24 +1221,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
       tc_fence_before();                                                // O and S are read: the next piece's MMAs may come
       if (live && !isnan(l) && isnan(odd.x + odd.y)) *odd_seen = 1;      // not by its weights
     }
-  }
-  __syncthreads();
-  if (warp == kMmaWarp) {
-    tc_fence_after();
-    tmem_dealloc(tmem_at, 512);
-  }
-  if (warp > kMmaWarp && *odd_seen) {
-    // Values that are not finite were left out or met: the CTA's pieces once
-    // more, by two warps, for whom nobody waits but the end of the CTA.
-    const int splits = p.splits ? p.splits : 1;
-    PlanCursor cur = {0, 0};
-    for (int k = 0;; ++k) {
-      const int g = piece_of(k);
-      const TileId id = pick_tile(p, g / p.n_kv / splits, cur);
-      if (id.seq < 0) break;
-      if ((k ^ warp) & 1) continue;
-      patch_piece<HD>(p, seq_task(p, id.seq), g % p.n_kv, g / p.n_kv % splits, id.rt * 2 * kRows);
-    }
+    end_sync();
   }
 }
 
