@@ -305,9 +305,11 @@ struct JoinArgs {
   int out_vec;                 // four-element stores to out are aligned
 };
 
-// V elements a lane a round, N rounds
+// V elements a lane a round, N rounds.  A warp waits on its slots' rows: eight
+// CTAs an SM hide more of that than 94 registers a thread gain (700 tokens of 64
+// heads, 4 slots: 42 us, so 33; with more elements a lane the registers are worth more).
 template <int V, int N>
-__global__ void __launch_bounds__(128) paged_attn_join_kernel(const __grid_constant__ JoinArgs a) {
+__global__ void __launch_bounds__(128, V * N <= 4 ? 8 : 1) paged_attn_join_kernel(const __grid_constant__ JoinArgs a) {
   constexpr int U = V * N <= 4 ? 8 : 4;       // slots whose rows are in flight together
   const PagedProblem& p = a.p;
   pdl_wait();
