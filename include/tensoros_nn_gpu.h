@@ -189,7 +189,7 @@ int tos_attention_noalloc_dev(float *out, const float *q, const void *k_cache, c
  * A workspace is 16-byte aligned and has the bytes that its _workspace_bytes
  * call gives for these very arguments (not fewer for larger ones: they follow
  * the split of the keys).  Prompts: 19.4 MB for the sums of rows where a
- * piece of the keys is longer than 384, and the split's partial rows; decoding:
+ * piece of the keys is longer than 256, and the split's partial rows; decoding:
  * (splits + prefix splits) * n_seqs * n_heads * (head_dim + 2) * 4 bytes, and
  * the 19.4 MB.  0: none, NULL will do. */
 

@@ -70,12 +70,15 @@ constexpr int kRows = 128;            // rows of a tile
 constexpr int kKeys = 128;            // keys of a tile
 constexpr float kBias = 7.0f;         // log2 of the factor that P carries
 constexpr int kPoly = 3;              // of eight pairs of exponentials, those at 2 and 5 go to the FMA pipe
-// Key tiles whose products one accumulator sums.  It loses 1e-7 of itself a step
-// of 16 keys.  fp32 rows: 3 (512 rows behind 7001 keys, us: 3: 157, 4: 152, 8: 144,
-// never: 137).  fp16 rows: 32, a loss of 2.6e-5, a twentieth of their rounding
-// (131,072 keys in one chain: 8e-4; 700 rows behind 20,000 keys, us: 8: 601,
-// 16: 587, 32: 585, 64 and never: 575).
-__host__ __device__ constexpr int fold_tiles(bool split) { return split ? 3 : 32; }
+// Key tiles whose products one accumulator sums, of a row tile's nt.  It loses
+// 1e-7 of itself a step of 16 keys.  fp32 rows: 3 (512 rows behind 7001 keys, us:
+// 2: 174, 3: 157, 4: 152, 8: 144, never: 137; error in norm 1.2e-6, an fp32
+// program's 1.6e-6), and 2 up to 2048 keys, where an fp32 program errs less (90
+// rows behind 400 keys: 8e-7, with 3 1.1e-6, an fp32 program's 5.5e-7).  fp16
+// rows: 32, a loss of 2.6e-5, a twentieth of their rounding (131,072 keys in one
+// chain: 8e-4; 700 rows behind 20,000 keys, us: 8: 553, 16: 535, 32: 531, 64 and
+// never: 520).
+__host__ __device__ constexpr int fold_tiles(bool split, int nt) { return !split ? 32 : nt <= 16 ? 2 : 3; }
 constexpr float kSlack = 8.0f;        // log2 by which the maximum may grow unfollowed
 
 struct TcArgs {
@@ -898,7 +901,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
 #pragma unroll
                   for (int k = 0; k < kKeys / 32; ++k)
                     mma_f16_ts(d, pa + (k >> 1) * 32 + part * 16 + (k & 1) * 8, vd + (k * 2048 >> 4), kIdO,
-                               part + k + half > 0 ? true : j % fold_tiles(SPLIT) != 0);
+                               part + k + half > 0 ? true : j % fold_tiles(SPLIT, i ? n1 : n0) != 0);
               }
               if (!ok) break;
               mma_commit(odone + i);
@@ -977,15 +980,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
       const long long slot = (long long)(p.slot0 + (p.splits ? w.split : 0)) * p.total_q * p.heads + (long long)tok * p.heads + head;
       const float sc = fmaxf(fabsf(p.scale_log2) * inv_q, 1.2e-38f);   // not 0: a masked score is -inf * sc
       float m = -INFINITY, l = 0.0f;
+      const int chain = fold_tiles(SPLIT, nt);
       for (int j = 0; j < nt; ++j) {
-        if (j > 0 && j % fold_tiles(SPLIT) == 0) {
+        if (j > 0 && j % chain == 0) {
           // The tensor cores cut off what their accumulator has no room for,
           // so a long chain of sums shrinks.  Every few tiles the sums are
           // added up in memory, rounded to nearest, and the chain begins anew.
           if (ok) ok = mbar_wait(odone + i, (cnt + j - 1) & 1, p.err, 46);
           __syncwarp();
           tc_fence_after();
-          fold_cols(p, to, HD / 2, j == fold_tiles(SPLIT));
+          fold_cols(p, to, HD / 2, j == chain);
           tc_fence_before();
           pair_sync(bar);                                               // the MMAs overwrite all dims
         }
@@ -1022,7 +1026,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
             tc_fence_after();
             scale_cols(to, HD / 2, f);
             l *= f;
-            if (j >= fold_tiles(SPLIT)) fold_scale(p, HD / 2, f);
+            if (j >= chain) fold_scale(p, HD / 2, f);
             // either half's P lets MMAs add to all dims: both halves' O first
             tmem_st_wait();
             tc_fence_before();
@@ -1182,7 +1186,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
         }
         __syncwarp();
       };
-      if (nt > fold_tiles(SPLIT)) fold_back(p, to, HD / 2);
+      if (nt > chain) fold_back(p, to, HD / 2);
 #pragma unroll 1
       for (int c32 = 0; c32 < HD / 64; ++c32) {
         uint32_t o[32];
@@ -1285,7 +1289,7 @@ bool paged_tc_ok(const PagedProblem& p) {
 
 // Bytes of PagedProblem::fold that rows over so many keys may need: fp32 rows
 // (fp16 rows, beyond more keys; a call's workspace goes by its sizes alone).
-size_t paged_tc_fold_bytes(int keys) { return keys > fold_tiles(true) * kKeys ? (size_t)kTcCtas * 2 * kRows * 128 * 4 : 0; }
+size_t paged_tc_fold_bytes(int keys) { return keys > fold_tiles(true, 0) * kKeys ? (size_t)kTcCtas * 2 * kRows * 128 * 4 : 0; }
 
 // Row tiles of one key/value head that a call can have at most.
 long long paged_tc_tiles(int n_seqs, int total_q, int max_q, int group) {
@@ -1306,7 +1310,7 @@ int paged_tc_run(const PagedProblem& p, cudaStream_t st) {
   if (!pool_map(&a.mk, p.k, p, a.box_rows) || !pool_map(&a.mv, p.v, p, a.box_rows)) return (int)cudaErrorNotSupported;
   const bool split = p.type == TOSK_F32;
   const int keys = p.splits ? p.chunk : p.fixed_kv >= 0 ? p.fixed_kv : p.max_kv;
-  if (!p.fold && keys > fold_tiles(split) * kKeys) return (int)cudaErrorInvalidValue;
+  if (!p.fold && keys > fold_tiles(split, 0) * kKeys) return (int)cudaErrorInvalidValue;
   if (p.hd <= 64) return split ? tc_launch<64, true>(a, (unsigned)grid, st) : tc_launch<64, false>(a, (unsigned)grid, st);
   return split ? tc_launch<128, true>(a, (unsigned)grid, st) : tc_launch<128, false>(a, (unsigned)grid, st);
 }

@@ -889,3 +889,19 @@ def test_append_of_very_many_heads(gpu):
                                        slot.data_ptr(), None, None, None, 0.0, None, R.stream()) == 0
     pg, r = c.where(c.table[0], 3)
     assert torch.equal(c.k[pg[1:], r[1:]], k) and torch.equal(c.v[pg[1:], r[1:]], v)
+
+
+@pytest.mark.parametrize("heads,n_kv,hd", [(32, 8, 128), (16, 4, 96)])
+@pytest.mark.parametrize("n,hist", [(90, 400), (64, 1900)])
+def test_short_prompts_err_little(gpu, n, hist, heads, n_kv, hd):
+    """fp32 rows that see few keys, where an fp32 program errs least.  Chains of
+    two key tiles, 16 steps of high and low parts, each of which loses half a
+    unit, 2^-24, of the sum so far, half of the whole on the average; a tenth of
+    that for all else."""
+    c = Cache([n + hist], 16, n_kv, hd, F16, seed=3)
+    q = randn(n, heads, hd, seed=4)
+    out, st = R.prompt(gpu, c, q, [n], [n + hist], heads, hd ** -0.5)
+    assert st == 0
+    k, v = c.rows(0)
+    ref, _ = R.attend(q, k, v, float(np.float32(hd ** -0.5)), torch.arange(n, device="cuda") + hist + 1)
+    assert float((out.double() - ref).norm() / ref.norm()) < 1.1 * 32 * 2.0 ** -24 / 2
