@@ -40,7 +40,7 @@
 // Precision.  fp16 rows: P is rounded to fp16 (half a step, 2^-11, of each
 // weight, which is what the output's own rounding costs; sums and maxima are
 // fp32).  fp32 rows: q, scaled by a power of two per row, and P go in as
-// fp16 pairs hi + lo (22 bits), two MMAs each: 1.1e-6 against 64 bits (norm)
+// fp16 pairs hi + lo (22 bits), two MMAs each: 1.2e-6 against 64 bits (norm)
 // over 7512 keys.  The accumulators, which cut off instead of rounding, are
 // emptied into memory every few key tiles (fold_tiles).
 //
