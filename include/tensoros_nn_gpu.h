@@ -51,7 +51,9 @@ enum {
     TOS_TYPE_F32 = 0,
     TOS_TYPE_F16 = 1,
     TOS_TYPE_Q4_0 = 2,
-    TOS_TYPE_Q8_0 = 8
+    TOS_TYPE_Q8_0 = 8,
+    TOS_TYPE_I8 = 24,
+    TOS_TYPE_F8_E4M3 = 64   /* not a ggml type: 4 exponent, 3 mantissa bits, up to 448 */
 };
 
 /* attention numerics */
@@ -296,6 +298,74 @@ int tos_attention_decode_paged_dev(const tos_rows_t *out, const tos_rows_t *q, c
                                    const int *kv_len, int n_seqs, int max_kv, const int *prefix_table,
                                    int prefix_len, int n_heads, float scale, void *workspace,
                                    size_t workspace_bytes, void *stream);
+
+/* -------------------------------------------------- paged cache in 8 bits
+ * The same in half the bytes of fp16 (no counterpart in the reference).  What
+ * is said above of streams, replays, workspaces, devices, head groups and
+ * tables holds here too; workspaces are 256-byte aligned.
+ *
+ * An element is a whole number (TOS_TYPE_I8, -127..127) or an e4m3 number
+ * (TOS_TYPE_F8_E4M3); its value is that times a scale, which `block`
+ * neighbouring rows of a sequence share for one head, K and V apart.  Scales
+ * are powers of two, 2^-24..2^9 (I8) or 2^-15..2^7 (F8_E4M3), so values are fp16
+ * numbers, and attention reads them without further rounding.  NaN as a scale
+ * makes the block's values NaN.
+ *
+ * Row r of page p: elements at ((p * page_size + r) * n_kv + head) * head_dim of
+ * k and v, its scales at (p * (page_size / block) + r / block) * n_kv + head of
+ * k_scale and v_scale. */
+typedef struct {
+    void *k, *v;             /* 16-byte aligned */
+    float *k_scale, *v_scale;
+    int type;                /* TOS_TYPE_I8 or TOS_TYPE_F8_E4M3 */
+    int block;               /* a power of two, at most 1024, that divides page_size */
+    int n_pages, page_size, n_kv, head_dim;   /* head_dim <= 256 */
+    const int *table;        /* device, as in tos_paged_kv_t */
+    int n_seqs, table_stride;
+} tos_paged8_kv_t;
+
+/* Stores packed rows: rows cu[i] .. cu[i+1]-1 of k and v become the last rows
+ * of sequence i, which then holds kv_len[i] (device arrays; cu: n_seqs + 1
+ * ascending).  n_tokens: no row from there on is stored.  Keys come rotated
+ * (tos_qk_norm_rotary_dev).  A block's scale is the least power of two with
+ * which the largest magnitude of its rows fits (beyond the limits: held as the
+ * largest value); elements are rounded to nearest, ties to even.  A block that
+ * holds rows before the first new one keeps its scale if that is larger;
+ * otherwise those rows are rounded again under the new one.  A row that is not
+ * finite makes its block's scale NaN, until the block is filled from its first
+ * row again.  Rows of a block behind the last new one lose their meaning when
+ * its scale changes (bytes stay); so a page that sequences share should be
+ * full.  Two sequences of one call must not append to the same block.  Rows of
+ * slots outside the table row, or of pages outside the pool, are not stored. */
+int tos_kv_append_paged8_dev(const tos_paged8_kv_t *kv, const tos_rows_t *k, const tos_rows_t *v, const int *cu,
+                             const int *kv_len, int n_seqs, int n_tokens, void *stream);
+
+/* The other way: the last cu[i+1] - cu[i] rows of sequence i into rows cu[i] ..
+ * of k_out and v_out (either may be NULL; one type), exact in both types.
+ * Rows of pages outside the pool read as zeros; rows outside the sequences, or
+ * of slots outside the table row, stay as they were. */
+int tos_kv_read_paged8_dev(const tos_paged8_kv_t *kv, const tos_rows_t *k_out, const tos_rows_t *v_out, const int *cu,
+                           const int *kv_len, int n_seqs, int n_tokens, void *stream);
+
+/* tos_attention_prompt_paged_dev over this cache.  total_kv: no more keys than
+ * this in all sequences together (keys beyond it may read as zeros).  The
+ * workspace holds an fp16 copy of them, about (total_kv + 128 * n_seqs) * n_kv *
+ * head_dim * 4 bytes, total_kv at most 2^32. */
+size_t tos_attention_prompt_paged8_workspace_bytes(int n_seqs, int total_q, int max_q, int64_t total_kv, int max_kv,
+                                                   int n_heads, int n_kv, int head_dim);
+int tos_attention_prompt_paged8_dev(const tos_rows_t *out, const tos_rows_t *q, const tos_paged8_kv_t *kv,
+                                    const int *cu_q, const int *kv_len, int n_seqs, int total_q, int max_q,
+                                    int64_t total_kv, int max_kv, int n_heads, float scale, void *workspace,
+                                    size_t workspace_bytes, void *stream);
+
+/* Attention of one token for each of n_seqs sequences: row i of q sees the
+ * kv_len[i] rows of sequence i (at most max_kv); none: zeros.  A row that sees a
+ * block of NaN scale is NaN.  head_dim that is no multiple of 16 takes the way
+ * over an fp16 copy, as prompts do (n_seqs * max_kv at most 2^32). */
+size_t tos_attention_decode_paged8_workspace_bytes(int n_seqs, int max_kv, int n_heads, int n_kv, int head_dim);
+int tos_attention_decode_paged8_dev(const tos_rows_t *out, const tos_rows_t *q, const tos_paged8_kv_t *kv,
+                                    const int *kv_len, int n_seqs, int max_kv, int n_heads, float scale,
+                                    void *workspace, size_t workspace_bytes, void *stream);
 
 /* --------------------- host-pointer drop-ins for runtime/nn/llm.c statics */
 void tos_gemv(float *out, const void *weight, const float *x, int out_dim, int in_dim, int type); /* llm.c:329 */

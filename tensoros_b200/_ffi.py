@@ -61,6 +61,13 @@ class PagedKv(C.Structure):
                 ("head_dim", i32), ("table", vp), ("n_seqs", i32), ("table_stride", i32)]
 
 
+class Paged8Kv(C.Structure):
+    """tos_paged8_kv_t"""
+    _fields_ = [("k", vp), ("v", vp), ("k_scale", vp), ("v_scale", vp), ("type", i32), ("block", i32), ("n_pages", i32),
+                ("page_size", i32), ("n_kv", i32), ("head_dim", i32), ("table", vp), ("n_seqs", i32),
+                ("table_stride", i32)]
+
+
 class RotaryDesc(C.Structure):
     """tos_rotary_desc_t"""
     _fields_ = [("rot_dim", i32), ("layout", i32), ("base", f32), ("scaling", i32), ("factor", f32),
@@ -165,6 +172,12 @@ NN_FUNCS = {
     "tos_attention_prompt_paged_dev": (i32, [vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, f32, vp, sz, vp]),
     "tos_attention_decode_paged_workspace_bytes": (sz, [i32] * 6),
     "tos_attention_decode_paged_dev": (i32, [vp, vp, vp, vp, i32, i32, vp, i32, i32, f32, vp, sz, vp]),
+    "tos_kv_append_paged8_dev": (i32, [vp, vp, vp, vp, vp, i32, i32, vp]),
+    "tos_kv_read_paged8_dev": (i32, [vp, vp, vp, vp, vp, i32, i32, vp]),
+    "tos_attention_prompt_paged8_workspace_bytes": (sz, [i32, i32, i32, C.c_int64, i32, i32, i32, i32]),
+    "tos_attention_prompt_paged8_dev": (i32, [vp, vp, vp, vp, vp, i32, i32, i32, C.c_int64, i32, i32, f32, vp, sz, vp]),
+    "tos_attention_decode_paged8_workspace_bytes": (sz, [i32] * 5),
+    "tos_attention_decode_paged8_dev": (i32, [vp, vp, vp, vp, i32, i32, i32, f32, vp, sz, vp]),
     "tos_tf_rmsnorm": (None, [vp, vp, vp, i32]),
     "tos_tf_swiglu_ffn": (None, [vp, vp, vp, vp, vp, i32, i32]),
     "tos_tf_model_create": (i32, [C.POINTER(vp), C.POINTER(TfDesc)]),

@@ -1,7 +1,8 @@
 /*
- * tos_paged.c - entry points of the paged-cache operators: argument checks,
- * the rotation's frequency table, and the hand-over to the tosk_* launchers
- * (paged_rotary.cu, paged_attention.cu).
+ * tos_paged.c - entry points of the paged-cache operators, over caches in
+ * floats and in 8 bits: argument checks, the rotation's frequency table, and
+ * the hand-over to the tosk_* launchers (paged_rotary.cu, paged_attention.cu,
+ * paged8_store.cu, paged8_decode.cu).
  */
 #include <math.h>
 #include <stdlib.h>
@@ -16,6 +17,8 @@
  * end after 2 s; what rows with infinities and NaN take comes after the last. */
 #define MAX_KEYS (1 << 25)
 #define MAX_SEQS 65535
+/* Keys that a call over an 8-bit cache lays out as fp16: pages of 128 in 32-bit arithmetic with room. */
+#define MAX_TOTAL_KEYS ((int64_t)1 << 32)
 
 struct tos_rotary {
     tosk_rotary_t r;
@@ -241,23 +244,33 @@ int tos_kv_append_paged_dev(const tos_paged_kv_t *kv, const tos_rows_t *k, const
 
 /* ------------------------------------------------------------ attention */
 
-static int attn_check(const tos_rows_t *out, const tos_rows_t *q, const tos_paged_kv_t *kv, int n_heads, float scale)
+static int attn_rows_check(const tos_rows_t *out, const tos_rows_t *q, int n_heads, int n_kv, int head_dim, float scale)
 {
-    int rc = paged_check(kv);
-    if (rc) return rc;
-    if (n_heads <= 0 || n_heads % kv->n_kv || !isfinite(scale * 1.5f)) return TOS_EINVAL;
+    if (n_heads <= 0 || n_heads % n_kv || !isfinite(scale * 1.5f)) return TOS_EINVAL;
     if (n_heads > (1 << 20)) return TOS_ENOTSUP;
-    rc = rows_check(out, n_heads, kv->head_dim);
-    if (!rc) rc = rows_check(q, n_heads, kv->head_dim);
+    int rc = rows_check(out, n_heads, head_dim);
+    if (!rc) rc = rows_check(q, n_heads, head_dim);
     if (!rc && out->ptr == q->ptr) rc = TOS_EINVAL;
     if (!rc && out->type != q->type) rc = TOS_ENOTSUP;
     return rc;
+}
+
+static int attn_check(const tos_rows_t *out, const tos_rows_t *q, const tos_paged_kv_t *kv, int n_heads, float scale)
+{
+    int rc = paged_check(kv);
+    return rc ? rc : attn_rows_check(out, q, n_heads, kv->n_kv, kv->head_dim, scale);
 }
 
 static int ws_check(void *ws, size_t bytes, size_t need)
 {
     if (need == 0) return TOS_OK;
     return ws && bytes >= need && ((uintptr_t)ws & 15) == 0 ? TOS_OK : TOS_EINVAL;
+}
+
+/* The 8-bit cache's workspaces begin with pools that are copied from in 16-byte pieces and by TMA. */
+static int ws256_check(void *ws, size_t bytes, size_t need)
+{
+    return ws_check(ws, bytes, need) || (need && ((uintptr_t)ws & 255)) ? TOS_EINVAL : TOS_OK;
 }
 
 size_t tos_attention_prompt_paged_workspace_bytes(int n_seqs, int total_q, int max_q, int max_kv, int n_heads,
@@ -342,4 +355,153 @@ int tos_attention_decode_paged_dev(const tos_rows_t *out, const tos_rows_t *q, c
     a.prefix_table = prefix_table;
     a.prefix_len = prefix_len;
     return device_leave(before, tosk_paged_decode(&a, tos_pick_stream(stream)));
+}
+
+/* --------------------------------------------------------- cache in 8 bits */
+
+static int paged8_check(const tos_paged8_kv_t *c)
+{
+    if (!c || !c->k || !c->v || !c->k_scale || !c->v_scale || !c->table) return TOS_EINVAL;
+    if (c->n_pages <= 0 || c->page_size <= 0 || c->n_kv <= 0 || c->head_dim <= 0 || c->n_seqs < 0 ||
+        c->table_stride <= 0 || c->block <= 0 || (c->block & (c->block - 1)) || c->page_size % c->block)
+        return TOS_EINVAL;
+    if ((c->type != TOS_TYPE_I8 && c->type != TOS_TYPE_F8_E4M3) || c->head_dim > MAX_HEAD_DIM || c->n_kv > (1 << 20) ||
+        c->block > 1024)
+        return TOS_ENOTSUP;
+    if (((uintptr_t)c->k & 15) || ((uintptr_t)c->v & 15) || ((uintptr_t)c->k_scale & 3) || ((uintptr_t)c->v_scale & 3) ||
+        ((uintptr_t)c->table & 3))
+        return TOS_EINVAL;
+    return TOS_OK;
+}
+
+static tosk_paged8_t paged8_of(const tos_paged8_kv_t *c)
+{
+    tosk_paged8_t p = {c->k, c->v, c->k_scale, c->v_scale, c->type, c->block, c->n_pages, c->page_size, c->n_kv,
+                       c->head_dim, c->table, c->n_seqs, c->table_stride};
+    return p;
+}
+
+static int packed_check(const tos_paged8_kv_t *kv, const int *cu, const int *kv_len, int n_seqs, int n_tokens)
+{
+    if (n_seqs < 0 || n_seqs > kv->n_seqs || n_tokens < 0) return TOS_EINVAL;
+    if (n_seqs && (!cu || !kv_len || ((uintptr_t)cu & 3) || ((uintptr_t)kv_len & 3))) return TOS_EINVAL;
+    return n_seqs > MAX_SEQS || n_tokens > MAX_ROWS ? TOS_ENOTSUP : TOS_OK;
+}
+
+int tos_kv_append_paged8_dev(const tos_paged8_kv_t *kv, const tos_rows_t *k, const tos_rows_t *v, const int *cu,
+                             const int *kv_len, int n_seqs, int n_tokens, void *stream)
+{
+    int rc = paged8_check(kv);
+    if (!rc) rc = rows_check(k, kv->n_kv, kv->head_dim);
+    if (!rc) rc = rows_check(v, kv->n_kv, kv->head_dim);
+    if (!rc) rc = packed_check(kv, cu, kv_len, n_seqs, n_tokens);
+    if (!rc && k->type != v->type) rc = TOS_ENOTSUP;
+    if (rc) return tos_set_status(rc);
+    int before;
+    if ((rc = device_enter(&before))) return tos_set_status(rc);
+    if (n_seqs == 0 || n_tokens == 0) return device_leave(before, 0);
+    tosk_paged8_io_t io = {paged8_of(kv), rows_of(k, NULL), rows_of(v, NULL), cu, kv_len, n_seqs, n_tokens};
+    return device_leave(before, tosk_paged8_put(&io, tos_pick_stream(stream)));
+}
+
+int tos_kv_read_paged8_dev(const tos_paged8_kv_t *kv, const tos_rows_t *k_out, const tos_rows_t *v_out, const int *cu,
+                           const int *kv_len, int n_seqs, int n_tokens, void *stream)
+{
+    int rc = paged8_check(kv);
+    if (!rc && !k_out && !v_out) rc = TOS_EINVAL;
+    if (!rc && k_out) rc = rows_check(k_out, kv->n_kv, kv->head_dim);
+    if (!rc && v_out) rc = rows_check(v_out, kv->n_kv, kv->head_dim);
+    if (!rc) rc = packed_check(kv, cu, kv_len, n_seqs, n_tokens);
+    if (!rc && k_out && v_out && k_out->type != v_out->type) rc = TOS_ENOTSUP;
+    if (rc) return tos_set_status(rc);
+    int before;
+    if ((rc = device_enter(&before))) return tos_set_status(rc);
+    if (n_seqs == 0 || n_tokens == 0) return device_leave(before, 0);
+    tosk_paged8_io_t io = {paged8_of(kv), rows_of(NULL, k_out), rows_of(NULL, v_out), cu, kv_len, n_seqs, n_tokens};
+    return device_leave(before, tosk_paged8_get(&io, tos_pick_stream(stream)));
+}
+
+static tosk_paged_attn_t attn8_of(const tos_rows_t *out, const tos_rows_t *q, const int *kv_len, int n_heads, float scale,
+                                  void *ws, size_t ws_bytes)
+{
+    tosk_paged_attn_t a;
+    memset(&a, 0, sizeof(a));
+    a.out = out->ptr; a.out_stride = out->stride;
+    a.q = q->ptr; a.q_stride = q->stride;
+    a.type = q->type;
+    a.kv_len = kv_len;
+    a.n_heads = n_heads;
+    a.scale = scale;
+    a.ws = ws; a.ws_bytes = ws_bytes;
+    a.err = tos_g.err_dev;
+    return a;
+}
+
+size_t tos_attention_prompt_paged8_workspace_bytes(int n_seqs, int total_q, int max_q, int64_t total_kv, int max_kv,
+                                                   int n_heads, int n_kv, int head_dim)
+{
+    if (n_seqs <= 0 || total_q <= 0 || max_q <= 0 || total_kv < 0 || max_kv < 0 || n_heads <= 0 || n_kv <= 0 ||
+        n_heads % n_kv || head_dim <= 0 || head_dim > MAX_HEAD_DIM)
+        return 0;
+    return tosk_paged8_prompt_ws_bytes(n_seqs, total_q, total_kv, max_kv, n_heads, n_kv, head_dim);
+}
+
+int tos_attention_prompt_paged8_dev(const tos_rows_t *out, const tos_rows_t *q, const tos_paged8_kv_t *kv,
+                                    const int *cu_q, const int *kv_len, int n_seqs, int total_q, int max_q,
+                                    int64_t total_kv, int max_kv, int n_heads, float scale, void *ws, size_t ws_bytes,
+                                    void *stream)
+{
+    int rc = paged8_check(kv);
+    if (!rc) rc = attn_rows_check(out, q, n_heads, kv->n_kv, kv->head_dim, scale);
+    if (!rc) rc = packed_check(kv, cu_q, kv_len, n_seqs, total_q);
+    if (!rc && (max_q < 0 || max_kv < 0 || total_kv < 0)) rc = TOS_EINVAL;
+    if (!rc && (max_kv > MAX_KEYS || (int64_t)max_q * (n_heads / kv->n_kv) > MAX_ROWS || total_kv > MAX_TOTAL_KEYS))
+        rc = TOS_ENOTSUP;
+    const int none = n_seqs == 0 || total_q == 0 || max_q == 0;
+    if (!rc && !none)
+        rc = ws256_check(ws, ws_bytes, tos_attention_prompt_paged8_workspace_bytes(n_seqs, total_q, max_q, total_kv, max_kv,
+                                                                                   n_heads, kv->n_kv, kv->head_dim));
+    if (rc) return tos_set_status(rc);
+    int before;
+    if ((rc = device_enter(&before))) return tos_set_status(rc);
+    if (none) return device_leave(before, 0);
+    tosk_paged_attn_t a = attn8_of(out, q, kv_len, n_heads, scale, ws, ws_bytes);
+    a.cu_q = cu_q;
+    a.n_seqs = n_seqs; a.total_q = total_q; a.max_q = max_q; a.max_kv = max_kv;
+    tosk_paged8_t c = paged8_of(kv);
+    return device_leave(before, tosk_paged8_prompt(&a, &c, total_kv, tos_pick_stream(stream)));
+}
+
+size_t tos_attention_decode_paged8_workspace_bytes(int n_seqs, int max_kv, int n_heads, int n_kv, int head_dim)
+{
+    if (n_seqs <= 0 || max_kv < 0 || n_heads <= 0 || n_kv <= 0 || n_heads % n_kv || head_dim <= 0 ||
+        head_dim > MAX_HEAD_DIM)
+        return 0;
+    return tosk_paged8_decode_ws_bytes(n_seqs, max_kv, n_heads, n_kv, head_dim);
+}
+
+int tos_attention_decode_paged8_dev(const tos_rows_t *out, const tos_rows_t *q, const tos_paged8_kv_t *kv,
+                                    const int *kv_len, int n_seqs, int max_kv, int n_heads, float scale, void *ws,
+                                    size_t ws_bytes, void *stream)
+{
+    int rc = paged8_check(kv);
+    if (!rc) rc = attn_rows_check(out, q, n_heads, kv->n_kv, kv->head_dim, scale);
+    if (!rc && (n_seqs < 0 || n_seqs > kv->n_seqs || max_kv < 0)) rc = TOS_EINVAL;
+    if (!rc && n_seqs && (!kv_len || ((uintptr_t)kv_len & 3))) rc = TOS_EINVAL;
+    if (!rc && (max_kv > MAX_KEYS || n_seqs > MAX_SEQS || (int64_t)n_seqs * (n_heads / kv->n_kv) > MAX_ROWS ||
+                (kv->head_dim % 16 && (int64_t)n_seqs * max_kv > MAX_TOTAL_KEYS)))
+        rc = TOS_ENOTSUP;
+    if (!rc)
+        rc = ws256_check(ws, ws_bytes, tos_attention_decode_paged8_workspace_bytes(n_seqs, max_kv, n_heads, kv->n_kv,
+                                                                                   kv->head_dim));
+    if (rc) return tos_set_status(rc);
+    int before;
+    if ((rc = device_enter(&before))) return tos_set_status(rc);
+    if (n_seqs == 0) return device_leave(before, 0);
+    tosk_paged_attn_t a = attn8_of(out, q, kv_len, n_heads, scale, ws, ws_bytes);
+    a.n_seqs = a.total_q = n_seqs;
+    a.max_q = 1;
+    a.max_kv = max_kv;
+    tosk_paged8_t c = paged8_of(kv);
+    return device_leave(before, tosk_paged8_decode(&a, &c, tos_pick_stream(stream)));
 }

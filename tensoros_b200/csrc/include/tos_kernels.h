@@ -19,6 +19,8 @@ extern "C" {
 /* ggml_type_t values, runtime/nn/gguf.h:38-58 */
 #define TOSK_F32 0
 #define TOSK_F16 1
+#define TOSK_I8 24
+#define TOSK_F8 64
 #define TOSK_Q4_0 2
 #define TOSK_Q8_0 8
 
@@ -308,6 +310,34 @@ size_t tosk_paged_prompt_ws_bytes(int n_seqs, int total_q, int max_kv, int n_hea
 size_t tosk_paged_decode_ws_bytes(int n_seqs, int max_kv, int prefix_len, int n_heads, int n_kv, int hd);
 int tosk_paged_prompt(const tosk_paged_attn_t *a, cudaStream_t st);
 int tosk_paged_decode(const tosk_paged_attn_t *a, cudaStream_t st);
+
+/* ---------------------------------------- paged cache in 8 bits (paged8_*.cu) */
+typedef struct {
+    void *k, *v;
+    float *k_scale, *v_scale;
+    int type, block, n_pages, page_size, n_kv, hd;   /* TOSK_I8 or TOSK_F8 */
+    const int *table;
+    int n_seqs, table_stride;
+} tosk_paged8_t;
+
+typedef struct {
+    tosk_paged8_t kv;
+    tosk_rows_t k, v;            /* src: rows to store; dst: rows to fill (NULL: none) */
+    const int *cu, *kv_len;
+    int n_seqs, n_tokens;
+} tosk_paged8_io_t;
+int tosk_paged8_put(const tosk_paged8_io_t *io, cudaStream_t st);
+int tosk_paged8_get(const tosk_paged8_io_t *io, cudaStream_t st);
+/* The keys of n_seqs sequences, at most total_kv in all, as an fp16 cache in ws
+ * (256-byte aligned); *out describes it, *len are its sequences' lengths. */
+size_t tosk_paged8_wide_bytes(int n_seqs, long long total_kv, int max_kv, int n_kv, int hd);
+int tosk_paged8_wide(const tosk_paged8_t *kv, const int *kv_len, int n_seqs, long long total_kv, int max_kv, void *ws,
+                     tosk_paged_t *out, const int **len, cudaStream_t st);
+/* a->kv is not looked at */
+size_t tosk_paged8_prompt_ws_bytes(int n_seqs, int total_q, long long total_kv, int max_kv, int n_heads, int n_kv, int hd);
+int tosk_paged8_prompt(const tosk_paged_attn_t *a, const tosk_paged8_t *kv, long long total_kv, cudaStream_t st);
+size_t tosk_paged8_decode_ws_bytes(int n_seqs, int max_kv, int n_heads, int n_kv, int hd);
+int tosk_paged8_decode(const tosk_paged_attn_t *a, const tosk_paged8_t *kv, cudaStream_t st);
 
 #ifdef __cplusplus
 }

@@ -643,3 +643,11 @@ extern "C" int tosk_paged_decode(const tosk_paged_attn_t* a, cudaStream_t st) {
   if (e || !d.own) return e;
   return run_join(p, d.pre, st);
 }
+
+namespace tos {
+// What the 8-bit cache's decode kernel (paged8_decode.cu) shares.
+PagedProblem paged_problem(const tosk_paged_attn_t* a) { return problem_of(a); }
+size_t paged_slots_bytes(int slots, int total_q, int heads, int hd) { return slots_bytes(slots, total_q, heads, hd); }
+void paged_part_views(PagedProblem& p, void* ws, int slots) { part_views(p, ws, slots, 0); }
+int paged_join(const PagedProblem& p, cudaStream_t st) { return run_join(p, 0, st); }
+}  // namespace tos
