@@ -367,6 +367,34 @@ int tos_attention_decode_paged8_dev(const tos_rows_t *out, const tos_rows_t *q, 
                                     const int *kv_len, int n_seqs, int max_kv, int n_heads, float scale,
                                     void *workspace, size_t workspace_bytes, void *stream);
 
+/* -------------------------------------------------------- sampling a batch
+ * A token for every row of logits (no counterpart in the reference, whose
+ * llm_sample has one row and one fixed recipe: tos_sample).  With the tokens
+ * of a row in order of falling logits (ties by rising index) and w = exp((logit -
+ * largest) / temperature), the first n of them stay:
+ *   top_k    at most k of them (<= 0: all);
+ *   top_p    the least number whose w reach top_p of what the top k have
+ *            (one at least; >= 1: all);
+ *   min_p    those with w >= min_p (<= 0: all; beyond 1 as 1);
+ * and the token is the first whose running sum of w passes u times theirs.
+ * temperature <= 0 (or NaN): the first of the order.  -infinity never stays; a
+ * row with +infinity draws among those; a row of NaN, or of nothing but
+ * -infinity, gives token -1, prob 0, kept 0.  Sums are exact (whole numbers of
+ * 2^-42 of the largest w or finer), so results are the same run to run. */
+typedef struct {             /* device arrays of n_rows, NULL: 1, 0, 1 and 0 */
+    const float *temperature;
+    const int *top_k;
+    const float *top_p, *min_p;
+} tos_sample_params_t;
+
+/* logits: n_rows rows of n_vocab (at most 2^20) elements, F32 or F16; u: n_rows
+ * random numbers in [0, 1) (others: the nearest of those, NaN: 0).  token, and
+ * if not NULL prob (the token's share of what stayed) and kept (how many
+ * stayed), are device arrays of n_rows.  params NULL: all four off.  Runs on
+ * `stream`, allocates nothing, may be captured. */
+int tos_sample_rows_dev(const tos_rows_t *logits, int n_rows, int n_vocab, const tos_sample_params_t *params,
+                        const float *u, int *token, float *prob, int *kept, void *stream);
+
 /* --------------------- host-pointer drop-ins for runtime/nn/llm.c statics */
 void tos_gemv(float *out, const void *weight, const float *x, int out_dim, int in_dim, int type); /* llm.c:329 */
 float tos_vec_dot(const void *weight, const float *x, int n, int type);                           /* llm.c:221 */

@@ -68,6 +68,11 @@ class Paged8Kv(C.Structure):
                 ("table_stride", i32)]
 
 
+class SampleParams(C.Structure):
+    """tos_sample_params_t"""
+    _fields_ = [("temperature", vp), ("top_k", vp), ("top_p", vp), ("min_p", vp)]
+
+
 class RotaryDesc(C.Structure):
     """tos_rotary_desc_t"""
     _fields_ = [("rot_dim", i32), ("layout", i32), ("base", f32), ("scaling", i32), ("factor", f32),
@@ -178,6 +183,7 @@ NN_FUNCS = {
     "tos_attention_prompt_paged8_dev": (i32, [vp, vp, vp, vp, vp, i32, i32, i32, C.c_int64, i32, i32, f32, vp, sz, vp]),
     "tos_attention_decode_paged8_workspace_bytes": (sz, [i32] * 5),
     "tos_attention_decode_paged8_dev": (i32, [vp, vp, vp, vp, i32, i32, i32, f32, vp, sz, vp]),
+    "tos_sample_rows_dev": (i32, [vp, i32, i32, vp, vp, vp, vp, vp, vp]),
     "tos_tf_rmsnorm": (None, [vp, vp, vp, i32]),
     "tos_tf_swiglu_ffn": (None, [vp, vp, vp, vp, vp, i32, i32]),
     "tos_tf_model_create": (i32, [C.POINTER(vp), C.POINTER(TfDesc)]),

@@ -1,8 +1,8 @@
 /*
  * tos_paged.c - entry points of the paged-cache operators, over caches in
- * floats and in 8 bits: argument checks, the rotation's frequency table, and
+ * floats and in 8 bits, and of sampling a batch: argument checks, the rotation's frequency table, and
  * the hand-over to the tosk_* launchers (paged_rotary.cu, paged_attention.cu,
- * paged8_store.cu, paged8_decode.cu).
+ * paged8_store.cu, paged8_decode.cu, sample_rows.cu).
  */
 #include <math.h>
 #include <stdlib.h>
@@ -504,4 +504,30 @@ int tos_attention_decode_paged8_dev(const tos_rows_t *out, const tos_rows_t *q, 
     a.max_kv = max_kv;
     tosk_paged8_t c = paged8_of(kv);
     return device_leave(before, tosk_paged8_decode(&a, &c, tos_pick_stream(stream)));
+}
+
+/* --------------------------------------------------------- sampling a batch */
+
+#define MAX_VOCAB (1 << 20)   /* the sums of weights: 62 bits for as many */
+#define MAX_SAMPLE_ROWS (1 << 24)
+
+int tos_sample_rows_dev(const tos_rows_t *logits, int n_rows, int n_vocab, const tos_sample_params_t *params,
+                        const float *u, int *token, float *prob, int *kept, void *stream)
+{
+    if (n_rows < 0 || n_vocab <= 0) return tos_set_status(TOS_EINVAL);
+    if (n_vocab > MAX_VOCAB || n_rows > MAX_SAMPLE_ROWS) return tos_set_status(TOS_ENOTSUP);
+    int rc = rows_check(logits, 1, n_vocab);
+    if (!rc && n_rows && (!u || !token)) rc = TOS_EINVAL;
+    const tos_sample_params_t none = {NULL, NULL, NULL, NULL};
+    if (!params) params = &none;
+    if (!rc && (((uintptr_t)u | (uintptr_t)token | (uintptr_t)prob | (uintptr_t)kept | (uintptr_t)params->temperature |
+                 (uintptr_t)params->top_k | (uintptr_t)params->top_p | (uintptr_t)params->min_p) & 3))
+        rc = TOS_EINVAL;
+    if (rc) return tos_set_status(rc);
+    int before;
+    if ((rc = device_enter(&before))) return tos_set_status(rc);
+    if (n_rows == 0) return device_leave(before, 0);
+    tosk_sample_t a = {logits->ptr, logits->stride, logits->type, n_rows, n_vocab, params->temperature, params->top_k,
+                       params->top_p, params->min_p, u, token, prob, kept};
+    return device_leave(before, tosk_sample_rows(&a, tos_pick_stream(stream)));
 }

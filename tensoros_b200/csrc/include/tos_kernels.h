@@ -311,6 +311,20 @@ size_t tosk_paged_decode_ws_bytes(int n_seqs, int max_kv, int prefix_len, int n_
 int tosk_paged_prompt(const tosk_paged_attn_t *a, cudaStream_t st);
 int tosk_paged_decode(const tosk_paged_attn_t *a, cudaStream_t st);
 
+/* -------------------------------------- sampling a batch (sample_rows.cu) */
+typedef struct {
+    const void *x;               /* logits, rows `stride` elements apart */
+    long long stride;
+    int type, n_rows, n;
+    const float *temperature;    /* these four: NULL: off */
+    const int *top_k;
+    const float *top_p, *min_p, *u;
+    int *token;
+    float *prob;                 /* may be NULL, kept too */
+    int *kept;
+} tosk_sample_t;
+int tosk_sample_rows(const tosk_sample_t *a, cudaStream_t st);
+
 /* ---------------------------------------- paged cache in 8 bits (paged8_*.cu) */
 typedef struct {
     void *k, *v;
