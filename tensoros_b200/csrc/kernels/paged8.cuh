@@ -127,6 +127,6 @@ Pool8 pool8_of(const tosk_paged8_t& kv);      // paged8_store.cu
 PagedProblem paged_problem(const tosk_paged_attn_t* a);
 size_t paged_slots_bytes(int slots, int total_q, int heads, int hd);
 void paged_part_views(PagedProblem& p, void* ws, int slots);
-int paged_join(const PagedProblem& p, cudaStream_t st);
+int paged_join(const PagedProblem& p, const int* counts, cudaStream_t st);   // counts: see JoinArgs
 
 }  // namespace tos

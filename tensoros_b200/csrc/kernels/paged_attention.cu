@@ -303,6 +303,7 @@ struct JoinArgs {
   PagedProblem p;              // of the sequences' own keys; splits: slots they have
   int pre_splits;              // slots of the prefix, all of them written
   int out_vec;                 // four-element stores to out are aligned
+  const int* counts;           // NULL, or partial rows of every row; where it has one, it is not one but done
 };
 
 // V elements a lane a round, N rounds.  A warp waits on its slots' rows: eight
@@ -321,8 +322,9 @@ __global__ void __launch_bounds__(128, V * N <= 4 ? 8 : 1) paged_attn_join_kerne
   if (w >= t.qn * p.heads) return;
   const int r = w / p.heads, h = w % p.heads, tok = t.q0 + r;
   const int n = seen(p, t, r);
-  const int cnt = a.pre_splits + (n + p.chunk - 1) / p.chunk;
   const long long row = (long long)tok * p.heads + h, step = (long long)p.total_q * p.heads;
+  const int cnt = a.counts ? a.counts[row] : a.pre_splits + (n + p.chunk - 1) / p.chunk;
+  if (a.counts && cnt <= 1) return;
   // running over rounds of 32 slots, lane i has slot s0 + i
   float M = -INFINITY, L = 0.0f, o[N][V];
 #pragma unroll
@@ -507,9 +509,10 @@ DecodePlan plan_decode(int n_seqs, int max_kv, int prefix_len, int heads, int n_
   return d;
 }
 
-int run_join(const PagedProblem& own, int pre, cudaStream_t st) {
+int run_join(const PagedProblem& own, int pre, cudaStream_t st, const int* counts = nullptr) {
   JoinArgs j;
   j.p = own;
+  j.counts = counts;
   j.pre_splits = pre;
   const long long gx = ((long long)own.max_q * own.heads + 3) / 4;
   if (gx > 0x7fffffffll || own.n_seqs > 65535) return (int)cudaErrorInvalidValue;
@@ -649,5 +652,5 @@ namespace tos {
 PagedProblem paged_problem(const tosk_paged_attn_t* a) { return problem_of(a); }
 size_t paged_slots_bytes(int slots, int total_q, int heads, int hd) { return slots_bytes(slots, total_q, heads, hd); }
 void paged_part_views(PagedProblem& p, void* ws, int slots) { part_views(p, ws, slots, 0); }
-int paged_join(const PagedProblem& p, cudaStream_t st) { return run_join(p, 0, st); }
+int paged_join(const PagedProblem& p, const int* counts, cudaStream_t st) { return run_join(p, 0, st, counts); }
 }  // namespace tos

@@ -70,13 +70,15 @@ class Cache8:
         """Rows first .. of sequence i, from their block's first row on, in 64 bits."""
         if rows.shape[0] == 0:
             return
-        pg, r = self.where(i, first, first + rows.shape[0])
-        blk = (first + torch.arange(rows.shape[0], device="cuda")) // self.block
-        for b in blk.unique().tolist():
-            m = blk == b
-            s = needed(rows[m].abs().amax((0, 2)), self.kind)
-            scales[pg[m][0], r[m][0] // self.block] = s.float()
-            pool[pg[m], r[m]] = nearest(rows[m] / s[:, None], self.kind).to(ELEM[self.kind]).view(torch.int8)
+        n, lo = rows.shape[0], first % self.block
+        pg, r = self.where(i, first, first + n)
+        blocks = (lo + n + self.block - 1) // self.block
+        x = rows.new_zeros(blocks * self.block, *rows.shape[1:])
+        x[lo:lo + n] = rows
+        s = needed(x.view(blocks, self.block, *rows.shape[1:]).abs().amax((1, 3)), self.kind)
+        s = s.repeat_interleave(self.block, 0)[lo:lo + n]
+        scales[pg, r // self.block] = s.float()
+        pool[pg, r] = nearest(rows / s[..., None], self.kind).to(ELEM[self.kind]).view(torch.int8)
 
     def rows(self, i, n=None, pool="k"):
         """Values of the first n rows of sequence i in 64 bits, [n][n_kv][hd]"""
@@ -201,12 +203,13 @@ def attend(q, k, v, scale, lim):
     return ref, err + 2.0 ** -32 * sums[lim.long()].repeat_interleave(q.shape[1] // k.shape[1], 1)
 
 
-def check_decode(gpu, c, q, heads, scale=None, kv_lens=None, **o):
+def check_decode(gpu, c, q, heads, scale=None, kv_lens=None, only=None, **o):
     kv_lens = c.lens if kv_lens is None else kv_lens
     scale = c.hd ** -0.5 if scale is None else scale
     out, st = decode(gpu, c, q, kv_lens, heads, scale, **o)
     assert st == 0
-    for i, n in enumerate(kv_lens):
+    for i in range(len(kv_lens)) if only is None else only:
+        n = kv_lens[i]
         lim = torch.tensor([n], device="cuda")
         ref, err = attend(q[i:i + 1], c.rows(i, n), c.rows(i, n, "v"), float(np.float32(scale)), lim)
         R.assert_rows(out[i:i + 1], ref, err, ("decode", i, n))

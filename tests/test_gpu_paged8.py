@@ -223,6 +223,38 @@ def test_decode_split_keys(gpu, kind, q, heads, n_kv, hd):
     P.check_decode(gpu, c, randn(3, heads, hd, seed=1, kind=q), heads, max_kv=5555)
 
 
+def ragged(n, most, seed):
+    """n lengths from 0 to most, a few of them around whole blocks of 128"""
+    g = torch.Generator().manual_seed(seed)
+    lens = (most * torch.rand(n, generator=g) ** 2).int().tolist()
+    for i, v in enumerate([0, 1, 127, 128, 129, most]):
+        lens[(i * 5) % n] = v
+    return lens
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("q,heads,n_kv,hd,page,block,n,most", [
+    (F32, 32, 8, 128, 16, 16, 12, 5000),                    # every CTA takes an even share of the keys
+    (F16, 16, 16, 64, 32, 8, 20, 3000),
+    (F32, 6, 6, 48, 48, 16, 40, 2000),
+    (F32, 32, 2, 128, 64, 64, 40, 4000),                    # 16 rows a tile
+    (F16, 24, 8, 256, 16, 16, 11, 3000),
+    (F32, 8, 4, 96, 24, 8, 30, 4000),                       # by cp.async
+    (F32, 20, 4, 64, 40, 8, 15, 4500),                      # by cp.async, two row tiles of 8
+])
+def test_decode_even_shares(gpu, kind, q, heads, n_kv, hd, page, block, n, most):
+    lens = ragged(n, most, hd + n)
+    c = Cache8(lens, page, block, n_kv, hd, kind, seed=n)
+    P.check_decode(gpu, c, randn(n, heads, hd, seed=1, kind=q), heads)
+
+
+@pytest.mark.parametrize("n", [1024, 1025])
+def test_decode_many_sequences(gpu, n):
+    lens = [(i * 131) % 700 for i in range(n)]
+    c = Cache8(lens, 16, 16, 1, 64, I8, seed=1)
+    P.check_decode(gpu, c, randn(n, 2, 64, seed=1), 2, only=list(range(0, n, 7)) + [n - 1])
+
+
 @pytest.mark.parametrize("kind", KINDS)
 def test_decode_scales_far_apart(gpu, kind):
     """Blocks whose scales span their whole range, the largest I8 ones (which
