@@ -9,7 +9,7 @@
 // written once, so HBM bounds it; at one token a sequence the chain of loads
 // (sequence, table, row, scale) does.
 //
-// Read.  Rows back as fp32 or fp16: a warp a token, 16 elements a lane.
+// Read.  Rows back as fp32 or fp16: 16 elements a thread, four of them in flight.
 // Expand.  The keys and values of a prompt call's sequences as an fp16 pool in
 // a workspace, pages of 128 rows, for the tensor-core kernels; exact, since
 // every value is an fp16 number.  1 byte in, 2 out an element: a few per cent of
@@ -21,7 +21,9 @@
 namespace tos {
 
 constexpr int kPutWarps = 8;
-constexpr int kPutPasses = 8;          // of a warp's rows that stay in registers
+// Passes of a warp's rows that stay in registers: 32 (fp16: 24) warps an SM then.
+template <typename E>
+constexpr int kPutPasses = sizeof(E) == 4 ? 4 : 8;
 
 struct PutArgs {
   Pool8 c;
@@ -62,9 +64,53 @@ struct Piece8 {
 };
 
 __device__ __forceinline__ uint32_t magnitude(uint32_t m, float x) { return max(m, __float_as_uint(x) & 0x7fffffffu); }
+// The largest magnitude of a piece: fp32 bits, or two fp16's.
+template <typename E>
+__device__ __forceinline__ uint32_t piece_max(uint32_t m, const Piece8<E>& y) {
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof(E) / 2); ++i) {
+    const uint32_t w[4] = {y.u[i].x, y.u[i].y, y.u[i].z, y.u[i].w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      m = sizeof(E) == 4 ? max(m, w[e] & 0x7fffffffu) : __vmaxu2(m, w[e] & 0x7fff7fffu);
+  }
+  return m;
+}
+// Its eight elements times inv, a power of two, as bytes.  fp16 in pairs, where inv
+// is an fp16 number: products are exact, or so small that they become 0 either way;
+// I8: 1536 + x rounds x to a whole number, its low byte.
+template <int TYPE, typename E>
+__device__ __forceinline__ uint2 piece_bytes(const Piece8<E>& y, float inv) {
+  if constexpr (sizeof(E) == 2) {
+    if (inv <= 32768.0f) {
+      const __half2 f = __float2half2_rn(inv);
+      const uint32_t w[4] = {y.u[0].x, y.u[0].y, y.u[0].z, y.u[0].w};
+      uint32_t h[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        __half2 x = __hmul2(*reinterpret_cast<const __half2*>(&w[i]), f);
+        if constexpr (TYPE == TOSK_I8) {
+          x = __hmin2(__hmax2(x, __float2half2_rn(-127.0f)), __float2half2_rn(127.0f));
+          x = __hadd2(x, __float2half2_rn(1536.0f));
+          h[i] = *reinterpret_cast<const uint32_t*>(&x);
+        } else {
+          uint16_t b;
+          asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(b) : "r"(*reinterpret_cast<const uint32_t*>(&x)));
+          h[i] = b;
+        }
+      }
+      if constexpr (TYPE == TOSK_I8) return make_uint2(prmt(h[0], h[1], 0x6420u), prmt(h[2], h[3], 0x6420u));
+      return make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
+    }
+  }
+  float f[8];
+  y.get(f);
+  return make_uint2(pack_word<TYPE>(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv),
+                    pack_word<TYPE>(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv));
+}
 
 template <int TYPE, typename E>
-__global__ void __launch_bounds__(32 * kPutWarps) paged8_put_kernel(const __grid_constant__ PutArgs a) {
+__global__ void __launch_bounds__(32 * kPutWarps, sizeof(E) == 4 ? 4 : 3) paged8_put_kernel(const __grid_constant__ PutArgs a) {
   const Pool8& c = a.c;
   __shared__ uint32_t smax[kPutWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = warp & (a.group - 1);
@@ -110,28 +156,22 @@ __global__ void __launch_bounds__(32 * kPutWarps) paged8_put_kernel(const __grid
     const int rpp = 32 >> lshift, p = lane & ((1 << lshift) - 1), rr = lane >> lshift;
     const int stride = rpp * a.group, row0 = r0 + sub * rpp + rr;
     const bool has = live && p < pieces;
-    Piece8<E> x[kPutPasses];
+    constexpr int P = kPutPasses<E>;
+    Piece8<E> x[P];
 #pragma unroll
-    for (int s = 0; s < kPutPasses; ++s) {
+    for (int s = 0; s < P; ++s) {
       const int r = row0 + s * stride;
       x[s].zero();
       if (has && r < r1) x[s].load(src + r * rows.sstride + 8 * p);
     }
 #pragma unroll
-    for (int s = 0; s < kPutPasses; ++s) {
-      float f[8];
-      x[s].get(f);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) m = magnitude(m, f[e]);
-    }
-    for (int r = row0 + kPutPasses * stride; has && r < r1; r += stride) {
+    for (int s = 0; s < P; ++s) m = piece_max(m, x[s]);
+    for (int r = row0 + P * stride; has && r < r1; r += stride) {
       Piece8<E> y;
-      float f[8];
       y.load(src + r * rows.sstride + 8 * p);
-      y.get(f);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) m = magnitude(m, f[e]);
+      m = piece_max(m, y);
     }
+    if constexpr (sizeof(E) == 2) m = __float_as_uint(__half2float(__ushort_as_half((unsigned short)max(m & 0xffffu, m >> 16))));
     m = __reduce_max_sync(0xffffffffu, m);
     if (a.group > 1) {
       if (lane == 0) smax[warp] = m;
@@ -141,19 +181,14 @@ __global__ void __launch_bounds__(32 * kPutWarps) paged8_put_kernel(const __grid
     const float need = scale_for<TYPE>(m), now = isnan(need) || isnan(old) ? __uint_as_float(0x7fffffffu) : fmaxf(need, old);
     const float inv = 1.0f / now;                         // a power of two
     auto put = [&](const Piece8<E>& y, int r) {
-      float f[8];
-      y.get(f);
-      uint2 w;
-      w.x = pack_word<TYPE>(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv);
-      w.y = pack_word<TYPE>(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv);
-      *reinterpret_cast<uint2*>(dst + r * step + 8 * p) = w;
+      *reinterpret_cast<uint2*>(dst + r * step + 8 * p) = piece_bytes<TYPE>(y, inv);
     };
 #pragma unroll
-    for (int s = 0; s < kPutPasses; ++s) {
+    for (int s = 0; s < P; ++s) {
       const int r = row0 + s * stride;
       if (has && r < r1) put(x[s], r);
     }
-    for (int r = row0 + kPutPasses * stride; has && r < r1; r += stride) {
+    for (int r = row0 + P * stride; has && r < r1; r += stride) {
       Piece8<E> y;
       y.load(src + r * rows.sstride + 8 * p);
       put(y, r);
@@ -208,75 +243,122 @@ struct GetArgs {
   tosk_rows_t k, v;
   const int *cu, *kv_len;
   int n_tokens, vec;
+  int tokens;                          // a CTA
 };
 
-// 16 elements, scaled, to a row of E.
+// 16 elements, scaled, to a row of E.  (Values are fp16 numbers: products of pairs
+// are exact.)
 template <int TYPE, typename E>
 __device__ __forceinline__ void put16(E* dst, const uint4& w, float s) {
   const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+  const __half2 f = __float2half2_rn(s);
   uint32_t h[8];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) cvt_word<TYPE>(u[i], h[2 * i], h[2 * i + 1]);
-  float2 f[8];
+  for (int i = 0; i < 4; ++i) {
+    cvt_word<TYPE>(u[i], h[2 * i], h[2 * i + 1]);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    f[i] = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
-    f[i].x *= s;
-    f[i].y *= s;
+    for (int e = 0; e < 2; ++e) {
+      const __half2 x = __hmul2(*reinterpret_cast<const __half2*>(&h[2 * i + e]), f);
+      h[2 * i + e] = *reinterpret_cast<const uint32_t*>(&x);
+    }
   }
   if constexpr (sizeof(E) == 4) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      reinterpret_cast<float4*>(dst)[i] = make_float4(f[2 * i].x, f[2 * i].y, f[2 * i + 1].x, f[2 * i + 1].y);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const __half2 x = __floats2half2_rn(f[i].x, f[i].y);
-      h[i] = *reinterpret_cast<const uint32_t*>(&x);
+    for (int i = 0; i < 4; ++i) {
+      const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&h[2 * i]));
+      const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&h[2 * i + 1]));
+      reinterpret_cast<float4*>(dst)[i] = make_float4(a.x, a.y, b.x, b.y);
     }
+  } else {
     reinterpret_cast<uint4*>(dst)[0] = make_uint4(h[0], h[1], h[2], h[3]);
     reinterpret_cast<uint4*>(dst)[1] = make_uint4(h[4], h[5], h[6], h[7]);
   }
 }
 
-// A token's row of all heads, by a warp: `row` its place, dst its output.
+// A token's row of all heads, by a warp, an element a lane: `row` its place, dst
+// its output.
 template <int TYPE, typename E>
-__device__ __forceinline__ void read_row(const Pool8& c, const Row8& row, const uint8_t* pool, const float* scales, E* dst,
-                                         bool vec) {
-  const int lane = threadIdx.x & 31, n = c.n_kv * c.hd;
-  if (vec) {
-#pragma unroll 4
-    for (int x = lane * 16; x < n; x += 512) {
-      const uint4 w = row.at < 0 ? make_uint4(0, 0, 0, 0) : *reinterpret_cast<const uint4*>(pool + row.at + x);
-      put16<TYPE>(dst + x, w, row.at < 0 ? 0.0f : scales[row.scale + x / c.hd]);
-    }
-  } else {
-    for (int x = lane; x < n; x += 32) {
-      const float f = row.at < 0 ? 0.0f : elem8<TYPE>(pool[row.at + x]) * scales[row.scale + x / c.hd];
-      if constexpr (sizeof(E) == 4) dst[x] = f;
-      else dst[x] = __float2half_rn(f);
-    }
+__device__ __forceinline__ void read_row(const Pool8& c, const Row8& row, const uint8_t* pool, const float* scales, E* dst) {
+  for (int x = threadIdx.x & 31; x < c.n_kv * c.hd; x += 32) {
+    const float f = row.at < 0 ? 0.0f : elem8<TYPE>(pool[row.at + x]) * scales[row.scale + x / c.hd];
+    if constexpr (sizeof(E) == 4) dst[x] = f;
+    else dst[x] = __float2half_rn(f);
   }
 }
 
+// Rows r < n of K and V, rows[r] their places: 16 elements a thread, kWidePieces
+// of them in flight; dst_k, dst_v NULL: not wanted.
+constexpr int kWidePieces = 4;
+constexpr int kMostPieces = 65535;     // of a CTA's rows: its divisions are products then
+__device__ __forceinline__ uint32_t inverse_of(uint32_t d) { return 0xffffffffu / d + 1; }   // d > 1
+__device__ __forceinline__ int divide(uint32_t x, uint32_t d, uint32_t inv) { return d == 1 ? x : __umulhi(x, inv); }   // x, d < 2^16
 template <int TYPE, typename E>
-__global__ void __launch_bounds__(128) paged8_get_kernel(const __grid_constant__ GetArgs a) {
+__device__ __forceinline__ void read_rows(const Pool8& c, const Row8* rows, int n, E* dst_k, long long stride_k, E* dst_v,
+                                          long long stride_v) {
+  const int side = c.n_kv * c.hd / 16, both = dst_k && dst_v ? 2 * side : side, pieces = n * both, per_head = c.hd / 16;
+  const uint32_t inv_both = inverse_of(both), inv_head = inverse_of(per_head);
+  for (int p0 = threadIdx.x; p0 < pieces; p0 += 256 * kWidePieces) {
+    uint4 w[kWidePieces];
+    float s[kWidePieces];
+    E* dst[kWidePieces];
+#pragma unroll
+    for (int x = 0; x < kWidePieces; ++x) {
+      const int p = p0 + 256 * x;
+      w[x] = make_uint4(0, 0, 0, 0);
+      s[x] = 0.0f;
+      dst[x] = nullptr;
+      if (p < pieces) {
+        const int r = divide(p, both, inv_both), q = p - r * both;
+        const bool second = q >= side, is_v = !dst_k || second;
+        const int e = second ? q - side : q;
+        const Row8 row = rows[r];
+        if (row.at < -1) continue;
+        dst[x] = (is_v ? dst_v + r * stride_v : dst_k + r * stride_k) + e * 16;
+        if (row.at >= 0) {
+          w[x] = *reinterpret_cast<const uint4*>((is_v ? c.v : c.k) + row.at + e * 16);
+          s[x] = (is_v ? c.vs : c.ks)[row.scale + divide(e, per_head, inv_head)];
+        }
+      }
+    }
+#pragma unroll
+    for (int x = 0; x < kWidePieces; ++x)
+      if (dst[x]) put16<TYPE>(dst[x], w[x], s[x]);
+  }
+}
+
+constexpr int kGetTokens = 128;        // at most, a CTA
+template <int TYPE, typename E>
+__global__ void __launch_bounds__(256) paged8_get_kernel(const __grid_constant__ GetArgs a) {
   const Pool8& c = a.c;
+  __shared__ Row8 rows[kGetTokens];    // at -1: reads as zeros; -2: stays as it is
   pdl_wait();
   pdl_trigger();
-  const int t = blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (t >= a.n_tokens) return;
-  const int i = find_seq(c.n_seqs, t, [&](int x) { return a.cu[x]; });
-  const int c0 = a.cu[i], c1 = a.cu[i + 1], slot = a.kv_len[i] - c1 + t;
-  if (t < c0 || t >= c1 || slot < 0 || slot >= (long long)c.table_stride * c.page_size) return;
-  const Row8 row = row8(c, slot, c.table[(long long)i * c.table_stride + page_index(c, slot)]);
-  if (a.k.dst) read_row<TYPE>(c, row, c.k, c.ks, reinterpret_cast<E*>(a.k.dst) + t * a.k.dstride, a.vec);
-  if (a.v.dst) read_row<TYPE>(c, row, c.v, c.vs, reinterpret_cast<E*>(a.v.dst) + t * a.v.dstride, a.vec);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int t0 = blockIdx.x * a.tokens, n = min(a.tokens, a.n_tokens - t0);
+  for (int r = warp; r < n; r += 8) {
+    const int t = t0 + r, i = find_seq(c.n_seqs, t, [&](int x) { return a.cu[x]; });
+    const int c0 = a.cu[i], c1 = a.cu[i + 1], slot = a.kv_len[i] - c1 + t;
+    Row8 row = {-2, 0};
+    if (t >= c0 && t < c1 && slot >= 0 && slot < (long long)c.table_stride * c.page_size)
+      row = row8(c, slot, c.table[(long long)i * c.table_stride + page_index(c, slot)]);
+    if (lane == 0) rows[r] = row;
+  }
+  __syncthreads();
+  E* k = a.k.dst ? reinterpret_cast<E*>(a.k.dst) + t0 * a.k.dstride : nullptr;
+  E* v = a.v.dst ? reinterpret_cast<E*>(a.v.dst) + t0 * a.v.dstride : nullptr;
+  if (a.vec) {
+    read_rows<TYPE>(c, rows, n, k, a.k.dstride, v, a.v.dstride);
+    return;
+  }
+  for (int r = warp; r < n; r += 8) {
+    if (rows[r].at < -1) continue;
+    if (k) read_row<TYPE>(c, rows[r], c.k, c.ks, k + r * a.k.dstride);
+    if (v) read_row<TYPE>(c, rows[r], c.v, c.vs, v + r * a.v.dstride);
+  }
 }
 
 // ------------------------------------------------------------------- expand
 constexpr int kWideRows = 128;         // rows of a page of the fp16 pool
-constexpr int kWideKeys = 32;          // keys a CTA
 
 struct WideArgs {
   Pool8 c;
@@ -285,6 +367,7 @@ struct WideArgs {
   int* table;                          // [n_seqs][stride]: the fp16 pool's pages
   int* len;                            // [n_seqs]: kv_len within the rows that the cache's table holds
   int stride, max_kv, cap;             // cap: pages of the fp16 pool
+  int keys;                            // a CTA, a power of two
   int vec;
 };
 
@@ -303,7 +386,7 @@ __global__ void __launch_bounds__(256) paged8_wide_kernel(const __grid_constant_
   if (blockIdx.x == 0)
     for (int s = tid; s < c.n_seqs; s += 256) a.len[s] = (int)min((long long)a.kv_len[s], room);
   // the sequence of page pg: sequences' pages lie one behind the other
-  const int pg = blockIdx.x / (kWideRows / kWideKeys), part = blockIdx.x % (kWideRows / kWideKeys);
+  const int parts = kWideRows / a.keys, pg = blockIdx.x / parts, part = blockIdx.x % parts;
   if (tid == 0) sseq = -1;
   int before = 0;
   for (int s0 = 0; s0 < c.n_seqs; s0 += 256) {
@@ -337,14 +420,18 @@ __global__ void __launch_bounds__(256) paged8_wide_kernel(const __grid_constant_
   if (pg >= a.cap) return;
   const int* table = c.table + (long long)seq * c.table_stride;
   const long long width = (long long)c.n_kv * c.hd;
-#pragma unroll
-  for (int x = 0; x < kWideKeys / 8; ++x) {
-    const int r = part * kWideKeys + x * 8 + warp, key = j * kWideRows + r;
-    if (key >= n) break;
-    const Row8 row = row8(c, key, table[page_index(c, key)]);
-    const long long to = ((long long)pg * kWideRows + r) * width;
-    read_row<TYPE>(c, row, c.k, c.ks, a.k + to, a.vec);
-    read_row<TYPE>(c, row, c.v, c.vs, a.v + to, a.vec);
+  const int r0 = part * a.keys, key0 = j * kWideRows + r0, have = min(a.keys, n - key0);
+  const long long to = ((long long)pg * kWideRows + r0) * width;
+  __shared__ Row8 rows[kWideRows];
+  if (tid < have) rows[tid] = row8(c, key0 + tid, table[page_index(c, key0 + tid)]);
+  __syncthreads();
+  if (a.vec) {
+    read_rows<TYPE>(c, rows, have, a.k + to, width, a.v + to, width);
+    return;
+  }
+  for (int r = warp; r < have; r += 8) {
+    read_row<TYPE>(c, rows[r], c.k, c.ks, a.k + to + r * width);
+    read_row<TYPE>(c, rows[r], c.v, c.vs, a.v + to + r * width);
   }
 }
 
@@ -368,6 +455,17 @@ int launch8(const void* f, long long grid, int threads, const void* arg, cudaStr
   void* args[] = {const_cast<void*>(arg)};
   return (int)cudaLaunchKernelExC(&cfg, f, args);
 }
+
+// Rows that a CTA of 256 threads reads back, a power of two up to 128: as many as
+// give four CTAs an SM, so that few rows go to many CTAs and of many rows a CTA's
+// beginning is soon paid for.
+int rows_a_cta(long long rows) {
+  int n = 1;
+  while (n < 128 && n * 4 * 148 < rows) n *= 2;
+  return n;
+}
+
+bool few_pieces(int rows, const tosk_paged8_t& kv) { return (long long)rows * kv.n_kv * kv.hd / 8 <= kMostPieces; }
 
 bool rows_on(const void* p, long long stride, int type, int bytes) {
   return ((uintptr_t)p & (bytes - 1)) == 0 && stride * (type == TOSK_F32 ? 4 : 2) % bytes == 0;
@@ -412,7 +510,8 @@ extern "C" int tosk_paged8_put(const tosk_paged8_io_t* io, cudaStream_t st) {
   // warps a block: as many as keep their rows in registers
   const long long elems = (long long)io->kv.block * io->kv.hd;
   a.group = 1;
-  while (a.group < kPutWarps && elems > (long long)a.group * kPutPasses * 256) a.group *= 2;
+  const int passes = type == TOSK_F32 ? kPutPasses<float> : kPutPasses<__half>;
+  while (a.group < kPutWarps && elems > (long long)a.group * passes * 256) a.group *= 2;
   const long long groups = units * io->kv.n_kv * 2, grid = (groups * a.group + kPutWarps - 1) / kPutWarps;
   const void* f = io->kv.type == TOSK_I8
                       ? type == TOSK_F32 ? (const void*)paged8_put_kernel<TOSK_I8, float> : (const void*)paged8_put_kernel<TOSK_I8, __half>
@@ -428,11 +527,12 @@ extern "C" int tosk_paged8_get(const tosk_paged8_io_t* io, cudaStream_t st) {
   a.cu = io->cu; a.kv_len = io->kv_len;
   a.n_tokens = io->n_tokens;
   const int type = io->k.dst ? io->k.dtype : io->v.dtype;
-  a.vec = io->kv.hd % 16 == 0 && rows_on(io->k.dst, io->k.dstride, type, 16) && rows_on(io->v.dst, io->v.dstride, type, 16);
+  a.tokens = rows_a_cta(io->n_tokens);
+  a.vec = io->kv.hd % 16 == 0 && few_pieces(a.tokens, io->kv) && rows_on(io->k.dst, io->k.dstride, type, 16) && rows_on(io->v.dst, io->v.dstride, type, 16);
   const void* f = io->kv.type == TOSK_I8
                       ? type == TOSK_F32 ? (const void*)paged8_get_kernel<TOSK_I8, float> : (const void*)paged8_get_kernel<TOSK_I8, __half>
                       : type == TOSK_F32 ? (const void*)paged8_get_kernel<TOSK_F8, float> : (const void*)paged8_get_kernel<TOSK_F8, __half>;
-  return launch8(f, ((long long)io->n_tokens + 3) / 4, 128, &a, st);
+  return launch8(f, ((long long)io->n_tokens + a.tokens - 1) / a.tokens, 256, &a, st);
 }
 
 namespace {
@@ -449,7 +549,8 @@ extern "C" size_t tosk_paged8_wide_bytes(int n_seqs, long long total_kv, int max
 extern "C" int tosk_paged8_wide(const tosk_paged8_t* kv, const int* kv_len, int n_seqs, long long total_kv, int max_kv, void* ws,
                                 tosk_paged_t* out, const int** len, cudaStream_t st) {
   const long long pages = wide_pages(n_seqs, total_kv);
-  if (pages > 0x7fffffffll / (kWideRows / kWideKeys)) return (int)cudaErrorInvalidValue;
+  const int keys = rows_a_cta(total_kv);
+  if (pages > 0x7fffffffll / (kWideRows / keys)) return (int)cudaErrorInvalidValue;
   const size_t pool = wide_pool_bytes(pages, kv->n_kv, kv->hd);
   WideArgs a;
   a.c = pool8_of(*kv);
@@ -463,7 +564,8 @@ extern "C" int tosk_paged8_wide(const tosk_paged8_t* kv, const int* kv_len, int 
   *len = a.len;
   a.max_kv = max_kv;
   a.cap = (int)pages;
-  a.vec = kv->hd % 16 == 0;
+  a.keys = keys;
+  a.vec = kv->hd % 16 == 0 && few_pieces(keys, *kv);
   memset(out, 0, sizeof(*out));
   out->k = a.k; out->v = a.v;
   out->type = TOSK_F16;
@@ -474,5 +576,5 @@ extern "C" int tosk_paged8_wide(const tosk_paged8_t* kv, const int* kv_len, int 
   out->n_seqs = n_seqs;
   out->table_stride = a.stride;
   const void* f = kv->type == TOSK_I8 ? (const void*)paged8_wide_kernel<TOSK_I8> : (const void*)paged8_wide_kernel<TOSK_F8>;
-  return launch8(f, pages * (kWideRows / kWideKeys), 256, &a, st);
+  return launch8(f, pages * (kWideRows / keys), 256, &a, st);
 }
