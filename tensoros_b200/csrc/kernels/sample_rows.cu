@@ -7,11 +7,11 @@
 //
 // All three filters and the draw cut one order, so nothing is sorted but what
 // lies around a cut.  A cluster of up to eight CTAs takes a row:
-//   max (and argmax)  ->  histogram of (max - x) / T, 64 bins an e-fold: counts
-//   and weights  ->  prefix sums in the cluster's first CTA give the bins of the
-//   cuts  ->  the bins down to the last cut, if they hold at most kCap tokens,
-//   or else the bins of the cuts one after the other, go to the first CTA's
-//   shared memory, are sorted there and resolved.
+//   max  ->  histogram of (max - x) / T, 123 bins an e-fold down to a weight of
+//   2^-24: counts and weights  ->  prefix sums in the cluster's first CTA give the
+//   bins of the cuts  ->  the bins down to the last cut, if they hold at most
+//   kCap tokens, or else the bins of the cuts one after the other, go to the first
+//   CTA's shared memory, are sorted there and resolved.
 // A bin of more than kCap tokens is cut into 2048 finer ones; one of those that
 // still holds too many (ties, all but always) is searched by bisection of the
 // values, then of the indexes.
@@ -74,19 +74,20 @@ struct CutBin {                         // where a cut falls in a histogram
 enum { kBinK, kBinP, kBinM, kBinCuts };
 
 struct SampleShared {
-  unsigned lo[kBins], hi[kBins], cnt[kBins];     // a histogram: weights in two words, counts
-  u64 list[kCap];                       // first CTA: tokens to sort, value over inverted index
+  unsigned lo[kBins], hi[kBins], cnt[kBins];     // this CTA's histogram: weights in two words, counts
+  u64 cum_w[kBins];                     // first CTA: all CTAs' histograms, then their inclusive sums
+  unsigned cum_n[kBins];
+  u64 list[kCap];                       // first CTA: tokens to sort, value over inverted index; or finer bins' weights
+  unsigned fine_n[kBins];               // and their counts
   double pow2[32];
   u64 wsum[kSmpThreads / 32];
   unsigned wcnt[kSmpThreads / 32];
   u64 part_w[2][2];                     // this CTA's sums, two rounds apart
   unsigned part_n[2][2];
-  u64 best[kSmpThreads / 32];
-  u64 top;                              // this CTA's best token
-  int nan;
+  float best[kSmpThreads / 32];
+  float top;                            // this CTA's largest logit; NaN: it has one
+  unsigned first;                       // its first place
   unsigned listed;
-  u64 total_w;                          // first CTA
-  unsigned total_n;
   CutBin cut[kBinCuts];                 // first CTA
   Found found;                          // first CTA
 };
@@ -99,6 +100,11 @@ __device__ __forceinline__ unsigned order_key(float x) {
 __device__ __forceinline__ float key_value(unsigned k) {
   return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
+
+// Bins.  The first kBins - 1 are for weights of 2^-24 and more, the last for all
+// that are less; cut finer, those have 41 bins an e-fold.
+constexpr float kBinsFold = (kBins - 1) / (24 * 0.69314718f);
+constexpr float kFineLast = 41.0f / kBinsFold;
 
 struct Row {
   const void* x;
@@ -113,66 +119,87 @@ struct Row {
   __device__ __forceinline__ float place(float v) const { return below(v) * scale; }
   __device__ __forceinline__ int bin(float v) const { return min(__float2int_rd(place(v)), kBins - 1); }
   __device__ __forceinline__ int fine(float v, int b) const {
-    return min(__float2int_rd((place(v) - (float)b) * kBins), kBins - 1);
+    return min(__float2int_rd((place(v) - (float)b) * (b == kBins - 1 ? kFineLast : (float)kBins)), kBins - 1);
   }
-  // 2^(shift - (top - v) rate) to the nearest whole number: 2^(n/32) from a
-  // table, 2^r, |r| <= 1/64, by its Taylor sum (next term 2e-15)
+  // 2^(shift - (top - v) rate) to the nearest whole number: 2^(m/32) from a table,
+  // 2^r, |r| <= 1/64, by its Taylor sum (next term 2e-15).  Whole numbers come of
+  // adding 1.5 2^52, 2^52.  In the last bin fp32 will do: each weight is below 2^-24
+  // and off by 3e-6 of itself.
   __device__ __forceinline__ u64 weight(float v) const {
     if (v == top) return 1ull << shift;
-    const double y = fma(-((double)top - (double)v), rate, (double)shift);
-    if (!(y > -2.0)) return 0;
-    const int m = __double2int_rn(y * 32.0);
-    const double r = fma((double)m, -1.0 / 32, y) * 0.6931471805599453;
-    double p = fma(r, 1.0 / 120, 1.0 / 24);
-    p = fma(p, r, 1.0 / 6);
-    p = fma(p, r, 0.5);
-    p = fma(p, r, 1.0);
+    const float d = top - v;
+    if (isinf(d)) return 0;                               // below an infinity, whatever T
+    if (d * scale >= (float)(kBins - 1)) {
+      float y;
+      asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(fmaf(-d, (float)rate, (float)shift)));
+      return __float2uint_rn(y);
+    }
+    const double y = fma((double)v - (double)top, rate, (double)shift);
+    if (!(y > -1.0)) return 0;                            // T so small that the bins' scale has its limit
+    const double big = fma(y, 32.0, 6755399441055744.0);
+    const int m = __double2loint(big);
+    const double r = fma(big - 6755399441055744.0, -1.0 / 32, y);
+    constexpr double c1 = 0.6931471805599453, c2 = c1 * c1 / 2, c3 = c1 * c1 * c1 / 6, c4 = c2 * c2 / 6, c5 = c2 * c3 / 10;
+    double p = fma(r, c5, c4);
+    p = fma(p, r, c3);
+    p = fma(p, r, c2);
+    p = fma(p, r, c1);
     p = fma(p, r, 1.0) * pow2[m & 31];
-    return __double2ull_rn(__longlong_as_double(__double_as_longlong(p) + ((long long)(m >> 5) << 52)));
+    p = __hiloint2double(__double2hiint(p) + ((m >> 5) << 20), __double2loint(p));
+    return (u64)__double_as_longlong(p + 4503599627370496.0) & 0xfffffffffffffull;
   }
 };
 
-// f(value, index, valid) of this CTA's elements; a warp's lanes go together.
+// f(values, index of the first) of this CTA's pieces of 16 bytes; a warp's lanes go
+// together; -infinity behind the row's end.
 template <typename E, typename F>
 __device__ __forceinline__ void sweep(const Row& r, F f) {
-  constexpr int P = 16 / sizeof(E), U = 2;
-  const int pieces = (r.n + P - 1) / P, lane = threadIdx.x & 31;
+  constexpr int P = 16 / sizeof(E), U = 4;
+  const int pieces = (r.n + P - 1) / P, lane = threadIdx.x & 31, step = r.ctas * kSmpThreads;
   const E* x = reinterpret_cast<const E*>(r.x);
-  for (int p0 = r.rank * kSmpThreads + (threadIdx.x & ~31); p0 < pieces; p0 += U * r.ctas * kSmpThreads) {
-    float v[U][P];
+  for (int p0 = r.rank * kSmpThreads + (threadIdx.x & ~31); p0 < pieces; p0 += U * step) {
+    uint4 w[U];
 #pragma unroll
     for (int q = 0; q < U; ++q) {
-      const int i = (p0 + q * r.ctas * kSmpThreads + lane) * P;
+      const int i = (p0 + q * step + lane) * P;
+      constexpr uint32_t none = sizeof(E) == 4 ? 0xff800000u : 0xfc00fc00u;
+      w[q] = make_uint4(none, none, none, none);
       if (r.vec && i + P <= r.n) {
-        const uint4 w = *reinterpret_cast<const uint4*>(x + i);
-        if constexpr (sizeof(E) == 4) {
-          v[q][0] = __uint_as_float(w.x); v[q][1] = __uint_as_float(w.y);
-          v[q][2] = __uint_as_float(w.z); v[q][3] = __uint_as_float(w.w);
-        } else {
-          const uint32_t h[4] = {w.x, w.y, w.z, w.w};
+        w[q] = *reinterpret_cast<const uint4*>(x + i);
+      } else if (i < r.n) {
+        uint32_t h[4] = {none, none, none, none};
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float2 g = __half22float2(*reinterpret_cast<const __half2*>(&h[e]));
-            v[q][2 * e] = g.x;
-            v[q][2 * e + 1] = g.y;
+        for (int e = 0; e < P; ++e)
+          if (i + e < r.n) {
+            if constexpr (sizeof(E) == 4) h[e] = __float_as_uint((float)x[i + e]);
+            else h[e / 2] = e & 1 ? (h[e / 2] & 0xffffu) | (uint32_t)reinterpret_cast<const uint16_t*>(x)[i + e] << 16
+                                  : (h[e / 2] & 0xffff0000u) | reinterpret_cast<const uint16_t*>(x)[i + e];
           }
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < P; ++e) v[q][e] = i >= 0 && i + e < r.n ? (float)x[i + e] : 0.0f;
+        w[q] = make_uint4(h[0], h[1], h[2], h[3]);
       }
     }
 #pragma unroll
     for (int q = 0; q < U; ++q) {
-      const int i = (p0 + q * r.ctas * kSmpThreads + lane) * P;
+      if (p0 + q * step >= pieces) break;
+      float v[P];
+      const uint32_t h[4] = {w[q].x, w[q].y, w[q].z, w[q].w};
 #pragma unroll
-      for (int e = 0; e < P; ++e) f(v[q][e], i + e, i >= 0 && i + e < r.n);
+      for (int e = 0; e < 4; ++e) {
+        if constexpr (sizeof(E) == 4) {
+          v[e] = __uint_as_float(h[e]);
+        } else {
+          const float2 g = __half22float2(*reinterpret_cast<const __half2*>(&h[e]));
+          v[2 * e] = g.x;
+          v[2 * e + 1] = g.y;
+        }
+      }
+      f(v, (p0 + q * step + lane) * P);
     }
   }
 }
 
-__device__ __forceinline__ void add_weight(SampleShared& s, int b, u64 w) {
-  atomicAdd(&s.cnt[b], 1u);
+__device__ __forceinline__ void add_weight(SampleShared& s, int b, u64 w, unsigned n = 1) {
+  atomicAdd(&s.cnt[b], n);
   const unsigned l = (unsigned)w;
   const unsigned old = l ? atomicAdd(&s.lo[b], l) : 0u;
   const unsigned h = (unsigned)(w >> 32) + (old + l < old ? 1u : 0u);
@@ -221,26 +248,36 @@ __device__ __forceinline__ void clear_bins(SampleShared& s) {
   for (int b = threadIdx.x; b < kBins; b += kSmpThreads) s.lo[b] = s.hi[b] = s.cnt[b] = 0;
 }
 
-// First CTA: the sums of all CTAs' bins this thread has (kPerThread neighbours),
-// inclusive within the thread.
-__device__ __forceinline__ void merge_bins(cg::cluster_group& cl, SampleShared& s, u64 (&w)[kPerThread], unsigned (&n)[kPerThread]) {
-  const int b0 = threadIdx.x * kPerThread;
-#pragma unroll
-  for (int i = 0; i < kPerThread; ++i) w[i] = n[i] = 0;
-  for (unsigned c = 0; c < cl.num_blocks(); ++c) {
-    const SampleShared* o = cl.map_shared_rank(&s, c);
-#pragma unroll
-    for (int i = 0; i < kPerThread; ++i) {
-      w[i] += (u64)o->hi[b0 + i] << 32;
-      w[i] += o->lo[b0 + i];
-      n[i] += o->cnt[b0 + i];
+// Adds this CTA's bins to the first one's sums.  By atomics that return nothing, so
+// that none is waited for.
+__device__ __forceinline__ void push_bins(SampleShared& s, u64* w, unsigned* n) {
+  for (int b = threadIdx.x; b < kBins; b += kSmpThreads)
+    if (const unsigned c = s.cnt[b]) {
+      atomicAdd(n + b, c);
+      if (const u64 x = ((u64)s.hi[b] << 32) + s.lo[b]) atomicAdd(w + b, x);
     }
-  }
+}
+// First CTA: its sums, inclusive from (w0, n0) on.
+__device__ __forceinline__ void scan_bins(SampleShared& s, u64* w, unsigned* n, u64 w0, unsigned n0) {
+  const int b0 = threadIdx.x * kPerThread;
+  u64 x[kPerThread], all;
+  unsigned y[kPerThread], alln;
 #pragma unroll
-  for (int i = 1; i < kPerThread; ++i) {
-    w[i] += w[i - 1];
-    n[i] += n[i - 1];
+  for (int i = 0; i < kPerThread; ++i) {
+    x[i] = w[b0 + i] + (i ? x[i - 1] : 0);
+    y[i] = n[b0 + i] + (i ? y[i - 1] : 0);
   }
+  u64 sum = x[kPerThread - 1];
+  unsigned sn = y[kPerThread - 1];
+  block_scan(s, sum, sn, all, alln);
+  sum += w0 - x[kPerThread - 1];
+  sn += n0 - y[kPerThread - 1];
+#pragma unroll
+  for (int i = 0; i < kPerThread; ++i) {
+    w[b0 + i] = sum + x[i];
+    n[b0 + i] = sn + y[i];
+  }
+  __syncthreads();
 }
 
 // First CTA: the list sorted, falling.
@@ -298,32 +335,41 @@ __device__ __forceinline__ Found find_listed(SampleShared& s, const u64 (&cum)[k
   return s.found;
 }
 
-// First CTA: the first bin past the cut; w, n: the sums before this thread's bins
-// and theirs, inclusive.
-__device__ __forceinline__ void find_bin(CutBin& to, const Cut& c, u64 w0, unsigned n0, const u64 (&w)[kPerThread],
-                                         const unsigned (&n)[kPerThread]) {
+// First CTA: the first bin past the cut, of inclusive sums from (w0, n0) on.
+__device__ __forceinline__ void find_bin(CutBin& to, const Cut& c, const u64* w, const unsigned* n, u64 w0, unsigned n0) {
 #pragma unroll
   for (int i = 0; i < kPerThread; ++i) {
-    const u64 wb = w0 + (i ? w[i - 1] : 0);
-    const unsigned nb = n0 + (i ? n[i - 1] : 0);
-    if (n0 + n[i] > nb && past(c, n0 + n[i], w0 + w[i]) && (nb == 0 || !past(c, nb, wb)))
-      to = {(int)threadIdx.x * kPerThread + i, nb, n0 + n[i] - nb, wb, w0 + w[i]};
+    const int b = threadIdx.x * kPerThread + i;
+    const u64 wb = b ? w[b - 1] : w0;
+    const unsigned nb = b ? n[b - 1] : n0;
+    if (n[b] > nb && past(c, n[b], w[b]) && (nb == 0 || !past(c, nb, wb))) to = {b, nb, n[b] - nb, wb, w[b]};
   }
 }
 
 // Tokens for which keep(value) go to the first CTA's list.
 template <typename E, typename F>
-__device__ __forceinline__ void collect(cg::cluster_group& cl, SampleShared& s, const Row& r, F keep) {
-  SampleShared* lead = cl.map_shared_rank(&s, 0);
+__device__ __forceinline__ void collect(SampleShared* lead, const Row& r, F keep) {
   const int lane = threadIdx.x & 31;
-  sweep<E>(r, [&](float v, int i, bool valid) {
-    const bool take = valid && v > -INFINITY && keep(v);
-    const unsigned hit = __ballot_sync(0xffffffffu, take);
-    if (hit == 0) return;
-    unsigned at = 0;
-    if (lane == 0) at = atomicAdd(&lead->listed, (unsigned)__popc(hit));
-    at = __shfl_sync(0xffffffffu, at, 0) + __popc(hit & ((1u << lane) - 1));
-    if (take && at < kCap) lead->list[at] = (u64)order_key(v) << 32 | ~(unsigned)i;
+  sweep<E>(r, [&](const auto& v, int i) {
+    constexpr int P = 16 / sizeof(E);
+    unsigned mine = 0;
+#pragma unroll
+    for (int e = 0; e < P; ++e) mine |= (v[e] > -INFINITY && keep(v[e]) ? 1u : 0u) << e;
+    if (!__any_sync(0xffffffffu, mine != 0)) return;
+    unsigned at = __popc(mine);                           // a place for each in the list
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned x = __shfl_up_sync(0xffffffffu, at, o);
+      if (lane >= o) at += x;
+    }
+    unsigned base = 0;
+    if (lane == 31) base = atomicAdd(&lead->listed, at);
+    at += __shfl_sync(0xffffffffu, base, 31) - __popc(mine);
+#pragma unroll
+    for (int e = 0; e < P; ++e)
+      if (mine >> e & 1) {
+        if (at < kCap) lead->list[at] = (u64)order_key(v[e]) << 32 | ~(unsigned)(i + e);
+        ++at;
+      }
   });
 }
 
@@ -334,11 +380,14 @@ __device__ __forceinline__ void count_row(cg::cluster_group& cl, SampleShared& s
                                           unsigned& n) {
   w = 0;
   n = 0;
-  sweep<E>(r, [&](float v, int i, bool valid) {
-    if (valid && v > -INFINITY && keep(v, i)) {
-      w += r.weight(v);
-      ++n;
-    }
+  sweep<E>(r, [&](const auto& v, int i) {
+    constexpr int P = 16 / sizeof(E);
+#pragma unroll 1
+    for (int e = 0; e < P; ++e)
+      if (v[e] > -INFINITY && keep(v[e], i + e)) {
+        w += r.weight(v[e]);
+        ++n;
+      }
   });
   block_sum(s, w, n);
   if (threadIdx.x == 0) {
@@ -363,21 +412,26 @@ __device__ __noinline__ Found resolve(cg::cluster_group& cl, SampleShared& s, co
   int f = -1;                                             // the finer bin, if any
   if (at.count > kCap) {
     clear_bins(s);
-    __syncthreads();
-    sweep<E>(r, [&](float v, int, bool valid) {
-      if (valid && v > -INFINITY && r.bin(v) == b) add_weight(s, r.fine(v, b), r.weight(v));
+    if (r.rank == 0)
+      for (int i = threadIdx.x; i < kBins; i += kSmpThreads) {
+        s.list[i] = 0;
+        s.fine_n[i] = 0;
+      }
+    cl.sync();
+    sweep<E>(r, [&](const auto& v, int) {
+      constexpr int P = 16 / sizeof(E);
+#pragma unroll 1
+      for (int e = 0; e < P; ++e)
+        if (v[e] > -INFINITY && r.bin(v[e]) == b) add_weight(s, r.fine(v[e], b), r.weight(v[e]));
     });
+    __syncthreads();
+    push_bins(s, lead->list, lead->fine_n);
     cl.sync();
     if (r.rank == 0) {
-      u64 w[kPerThread], all;
-      unsigned n[kPerThread], alln;
-      merge_bins(cl, s, w, n);
-      u64 sum = w[kPerThread - 1];
-      unsigned sn = n[kPerThread - 1];
-      block_scan(s, sum, sn, all, alln);
+      scan_bins(s, s.list, s.fine_n, at.w0, at.n0);
       // nb == 0 in find_bin stands for the very first token: past is monotone, so
       // with tokens before the bin the test of what comes before holds
-      find_bin(s.cut[kBinK], c, at.w0 + sum - w[kPerThread - 1], at.n0 + sn - n[kPerThread - 1], w, n);
+      find_bin(s.cut[kBinK], c, s.list, s.fine_n, at.w0, at.n0);
     }
     cl.sync();
     at = lead->cut[kBinK];
@@ -392,7 +446,7 @@ __device__ __noinline__ Found resolve(cg::cluster_group& cl, SampleShared& s, co
     cl.sync();
     if (r.rank == 0 && threadIdx.x == 0) s.listed = 0;
     cl.sync();
-    collect<E>(cl, s, r, mine);
+    collect<E>(lead, r, mine);
     cl.sync();
     if (r.rank == 0) {
       sort_list(s, cnt);
@@ -443,7 +497,7 @@ __device__ __noinline__ Found resolve(cg::cluster_group& cl, SampleShared& s, co
 }
 
 template <typename E>
-__global__ void __launch_bounds__(kSmpThreads, 1) sample_rows_kernel(const __grid_constant__ SampleArgs a) {
+__global__ void __launch_bounds__(kSmpThreads, 2) sample_rows_kernel(const __grid_constant__ SampleArgs a) {
   extern __shared__ __align__(16) uint8_t raw[];
   SampleShared& s = *reinterpret_cast<SampleShared*>(raw);
   cg::cluster_group cl = cg::this_cluster();
@@ -462,54 +516,59 @@ __global__ void __launch_bounds__(kSmpThreads, 1) sample_rows_kernel(const __gri
   SampleShared* lead = cl.map_shared_rank(&s, 0);
 
   clear_bins(s);
+  if (r.rank == 0)
+    for (int i = tid; i < kBins; i += kSmpThreads) {
+      s.cum_w[i] = 0;
+      s.cum_n[i] = 0;
+    }
   if (tid < 32) s.pow2[tid] = exp2((double)tid / 32.0);
   if (tid == 0) {
     s.listed = 0;
-    s.nan = 0;
+    s.first = 0xffffffffu;
   }
-  __syncthreads();
-  // the largest, and the first of its kind
+  // the largest; NaN if there is one
+  auto top_nan = [](float x, float y) {
+    float z;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(z) : "f"(x), "f"(y));
+    return z;
+  };
   float best = -INFINITY;
-  int at = 0x7fffffff;
-  bool nan = false;
-  sweep<E>(r, [&](float v, int i, bool valid) {
-    if (!valid) return;
-    nan |= isnan(v);
-    if (v > best || (v == best && i < at)) {
-      best = v;
-      at = i;
-    }
+  sweep<E>(r, [&](const auto& v, int) {
+    constexpr int P = 16 / sizeof(E);
+    float m = top_nan(v[0], v[1]);
+#pragma unroll
+    for (int e = 2; e < P; e += 2) m = top_nan(m, top_nan(v[e], v[e + 1]));
+    best = top_nan(best, m);
   });
-  u64 top = (u64)order_key(best) << 32 | ~(unsigned)at;
-  for (int o = 16; o > 0; o >>= 1) {
-    const u64 b = __shfl_xor_sync(0xffffffffu, top, o);
-    top = b > top ? b : top;
-  }
-  nan = __any_sync(0xffffffffu, nan);
-  if (lane == 0) {
-    s.best[warp] = top;
-    if (nan) s.nan = 1;
-  }
+  for (int o = 16; o > 0; o >>= 1) best = top_nan(best, __shfl_xor_sync(0xffffffffu, best, o));
+  if (lane == 0) s.best[warp] = best;
   __syncthreads();
-  if (tid == 0) {
-    for (int i = 1; i < kSmpThreads / 32; ++i) top = s.best[i] > top ? s.best[i] : top;
-    s.top = top;
+  if (warp == 0) {
+    best = s.best[lane & (kSmpThreads / 32 - 1)];
+    for (int o = kSmpThreads / 64; o > 0; o >>= 1) best = top_nan(best, __shfl_xor_sync(0xffffffffu, best, o));
+    if (lane == 0) s.top = best;
   }
   cl.sync();
-  top = 0;
-  nan = false;
-  for (int c = 0; c < r.ctas; ++c) {
-    const SampleShared* o = cl.map_shared_rank(&s, c);
-    const u64 b = o->top;
-    top = b > top ? b : top;
-    nan |= o->nan != 0;
-  }
-  r.top = key_value((unsigned)(top >> 32));
+  best = -INFINITY;
+  for (int c = 0; c < r.ctas; ++c) best = top_nan(best, cl.map_shared_rank(&s, c)->top);
+  r.top = best;
   const float T = a.temperature ? a.temperature[row] : 1.0f;
-  const bool none = nan || r.top == -INFINITY;            // nothing to choose from
+  const bool none = isnan(r.top) || r.top == -INFINITY;   // nothing to choose from
   if (none || !(T > 0.0f)) {
+    if (!none) {                                          // the first of the largest
+      unsigned at = 0xffffffffu;
+      sweep<E>(r, [&](const auto& v, int i) {
+        constexpr int P = 16 / sizeof(E);
+#pragma unroll
+        for (int e = 0; e < P; ++e)
+          if (v[e] == r.top) at = min(at, (unsigned)(i + e));
+      });
+      at = __reduce_min_sync(0xffffffffu, at);
+      if (lane == 0 && at != 0xffffffffu) atomicMin(&lead->first, at);
+      cl.sync();
+    }
     if (r.rank == 0 && tid == 0) {
-      a.token[row] = none ? -1 : (int)~(unsigned)top;
+      a.token[row] = none ? -1 : (int)s.first;
       if (a.prob) a.prob[row] = none ? 0.0f : 1.0f;
       if (a.kept) a.kept[row] = none ? 0 : 1;
     }
@@ -517,22 +576,38 @@ __global__ void __launch_bounds__(kSmpThreads, 1) sample_rows_kernel(const __gri
     return;
   }
   r.rate = 1.4426950408889634 / (double)T;
-  r.scale = fminf(64.0f / T, 1e30f);
+  r.scale = fminf(kBinsFold / T, 1e30f);
 
   const float pf = a.top_p ? a.top_p[row] : 1.0f, mf = a.min_p ? a.min_p[row] : 0.0f;
   const bool by_p = pf < 1.0f, by_m = mf > 0.0f;
-  const double p = pf, m = fmin((double)mf, 1.0) * (double)(1ull << r.shift);
-  u64 wm = 0;
-  unsigned nm = 0;
-  sweep<E>(r, [&](float v, int, bool valid) {
-    if (!valid || v == -INFINITY) return;
-    const u64 w = r.weight(v);
-    if (by_m && (double)w >= m) {
-      wm += w;
-      ++nm;
+  const double p = pf;
+  const u64 m = (u64)ceil(fmin((double)mf, 1.0) * (double)(1ull << r.shift));
+  u64 wm = 0, wl = 0;                                     // of the tokens that min-p keeps, of the last bin's
+  unsigned nm = 0, nl = 0;
+  sweep<E>(r, [&](const auto& v, int) {
+    constexpr int P = 16 / sizeof(E);
+#pragma unroll
+    for (int e = 0; e < P; ++e) {
+      if (v[e] == -INFINITY) continue;
+      const u64 w = r.weight(v[e]);
+      if (by_m && w >= m) {
+        wm += w;
+        ++nm;
+      }
+      const int b = r.bin(v[e]);
+      if (b == kBins - 1) {
+        wl += w;
+        ++nl;
+      } else {
+        add_weight(s, b, w);
+      }
     }
-    add_weight(s, r.bin(v), w);
   });
+  for (int o = 16; o > 0; o >>= 1) {
+    wl += __shfl_xor_sync(0xffffffffu, wl, o);
+    nl += __shfl_xor_sync(0xffffffffu, nl, o);
+  }
+  if (lane == 0 && nl) add_weight(s, kBins - 1, wl, nl);
   if (by_m) {
     block_sum(s, wm, nm);
     if (tid == 0) {
@@ -540,6 +615,8 @@ __global__ void __launch_bounds__(kSmpThreads, 1) sample_rows_kernel(const __gri
       s.part_n[0][1] = nm;
     }
   }
+  __syncthreads();
+  push_bins(s, lead->cum_w, lead->cum_n);
   cl.sync();
   if (by_m) {
     wm = 0;
@@ -551,27 +628,16 @@ __global__ void __launch_bounds__(kSmpThreads, 1) sample_rows_kernel(const __gri
     }
   }
   const int k = a.top_k ? a.top_k[row] : 0;
-  // what this thread of the first CTA has of the bins' sums
-  u64 bw[kPerThread] = {}, bw0 = 0, total_w = 0;
-  unsigned bn[kPerThread] = {}, bn0 = 0, total_n = 0;
   if (r.rank == 0) {
-    merge_bins(cl, s, bw, bn);
-    bw0 = bw[kPerThread - 1];
-    bn0 = bn[kPerThread - 1];
-    block_scan(s, bw0, bn0, total_w, total_n);
-    bw0 -= bw[kPerThread - 1];
-    bn0 -= bn[kPerThread - 1];
-    if (tid == 0) {
-      s.total_w = total_w;
-      s.total_n = total_n;
-    }
-    if (k > 0 && (unsigned)k < total_n) find_bin(s.cut[kBinK], {kByCount, (unsigned)k, 0.0}, bw0, bn0, bw, bn);
-    else if (by_p) find_bin(s.cut[kBinP], {kReach, 0, p * (double)total_w}, bw0, bn0, bw, bn);
-    if (by_m) find_bin(s.cut[kBinM], {kByCount, nm, 0.0}, bw0, bn0, bw, bn);
+    scan_bins(s, s.cum_w, s.cum_n, 0, 0);
+    const u64 all = s.cum_w[kBins - 1];
+    if (k > 0 && (unsigned)k < s.cum_n[kBins - 1]) find_bin(s.cut[kBinK], {kByCount, (unsigned)k, 0.0}, s.cum_w, s.cum_n, 0, 0);
+    else if (by_p) find_bin(s.cut[kBinP], {kReach, 0, p * (double)all}, s.cum_w, s.cum_n, 0, 0);
+    if (by_m) find_bin(s.cut[kBinM], {kByCount, nm, 0.0}, s.cum_w, s.cum_n, 0, 0);
   }
   cl.sync();
-  total_w = lead->total_w;
-  total_n = lead->total_n;
+  const u64 total_w = lead->cum_w[kBins - 1];
+  const unsigned total_n = lead->cum_n[kBins - 1];
   const bool by_k = k > 0 && (unsigned)k < total_n;
   const Cut cut_k = {kByCount, (unsigned)k, 0.0};
   float uf = a.u[row];
@@ -590,7 +656,7 @@ __global__ void __launch_bounds__(kSmpThreads, 1) sample_rows_kernel(const __gri
   else if (by_p) down_to(lead->cut[kBinP]);
   if (by_m && !(by_k && by_p)) down_to(lead->cut[kBinM]);
   if (upto <= kCap) {
-    collect<E>(cl, s, r, [&](float v) { return r.bin(v) <= last; });
+    collect<E>(lead, r, [&](float v) { return r.bin(v) <= last; });
     cl.sync();
     if (r.rank == 0) {
       sort_list(s, (int)upto);
@@ -617,7 +683,7 @@ __global__ void __launch_bounds__(kSmpThreads, 1) sample_rows_kernel(const __gri
   }
   // one cut after the other
   auto cut_at = [&](const Cut& c) {
-    if (r.rank == 0) find_bin(s.cut[kBinP], c, bw0, bn0, bw, bn);
+    if (r.rank == 0) find_bin(s.cut[kBinP], c, s.cum_w, s.cum_n, 0, 0);
     cl.sync();
     return resolve<E>(cl, s, r, c, lead->cut[kBinP]);
   };
@@ -663,7 +729,7 @@ extern "C" int tosk_sample_rows(const tosk_sample_t* t, cudaStream_t st) {
   a.vec = ((uintptr_t)t->x & 15) == 0 && t->stride * es % 16 == 0;
   int lg = 0;
   while ((1ll << lg) < t->n) ++lg;
-  a.shift = 62 - lg;
+  a.shift = lg < 11 ? 51 : 62 - lg;              // weights below 2^52, their sum below 2^62
   a.temperature = t->temperature;
   a.top_k = t->top_k;
   a.top_p = t->top_p; a.min_p = t->min_p; a.u = t->u;
