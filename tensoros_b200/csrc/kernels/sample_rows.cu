@@ -8,10 +8,10 @@
 // All three filters and the draw cut one order, so nothing is sorted but what
 // lies around a cut.  A cluster of up to eight CTAs takes a row:
 //   max  ->  histogram of (max - x) / T, 123 bins an e-fold down to a weight of
-//   2^-24: counts and weights  ->  prefix sums in the cluster's first CTA give the
-//   bins of the cuts  ->  the bins down to the last cut, if they hold at most
-//   kCap tokens, or else the bins of the cuts one after the other, go to the first
-//   CTA's shared memory, are sorted there and resolved.
+//   2^-24: counts and weights, summed over the cluster  ->  prefix sums give the
+//   bins of the cuts  ->  the tokens of the bins down to the last cut, if they are
+//   at most kCap, or else of the cuts' bins one after the other, go to the first
+//   CTA's shared memory; there a cut's bin is sorted and the cut found in it.
 // A bin of more than kCap tokens is cut into 2048 finer ones; one of those that
 // still holds too many (ties, all but always) is searched by bisection of the
 // values, then of the indexes.
@@ -34,7 +34,7 @@ namespace tos {
 
 constexpr int kSmpThreads = 512;
 constexpr int kBins = 2048;
-constexpr int kCap = 2048;              // tokens that are sorted in shared memory
+constexpr int kCap = 4096;              // tokens that are listed, and sorted, in shared memory
 constexpr int kPerThread = kBins / kSmpThreads;
 typedef unsigned long long u64;
 
@@ -71,14 +71,27 @@ struct CutBin {                         // where a cut falls in a histogram
   unsigned n0, count;                   // tokens before the bin, in it
   u64 w0, w;                            // weight before it, up to its end
 };
-enum { kBinK, kBinP, kBinM, kBinCuts };
 
+// A histogram: weights in two words, counts; or, in the same place, inclusive sums.
+struct Hist {
+  union {
+    struct {
+      alignas(16) unsigned lo[kBins], hi[kBins];
+    };
+    u64 w[kBins];
+  };
+  alignas(16) unsigned n[kBins];
+};
 struct SampleShared {
-  unsigned lo[kBins], hi[kBins], cnt[kBins];     // this CTA's histogram: weights in two words, counts
-  u64 cum_w[kBins];                     // first CTA: all CTAs' histograms, then their inclusive sums
-  unsigned cum_n[kBins];
-  u64 list[kCap];                       // first CTA: tokens to sort, value over inverted index; or finer bins' weights
-  unsigned fine_n[kBins];               // and their counts
+  Hist hist;                            // this CTA's, then all CTAs' inclusive sums
+  union {
+    Hist all;                           // a part of the bins, all CTAs' (all_bins)
+    u64 sorted[kCap];                   // first CTA: a cut's bin
+  };
+  union {
+    u64 list[kCap];                     // first CTA: tokens, value over inverted index
+    Hist fine;                          // a bin cut finer, as hist
+  };
   double pow2[32];
   u64 wsum[kSmpThreads / 32];
   unsigned wcnt[kSmpThreads / 32];
@@ -87,9 +100,10 @@ struct SampleShared {
   float best[kSmpThreads / 32];
   float top;                            // this CTA's largest logit; NaN: it has one
   unsigned first;                       // its first place
-  unsigned listed;
-  CutBin cut[kBinCuts];                 // first CTA
-  Found found;                          // first CTA
+  unsigned listed[4];                   // first CTA: tokens listed for the first, second .. time
+  unsigned picked;
+  CutBin cut[3];
+  Found found;
 };
 
 // Order-preserving bits of a float; -0 as +0.
@@ -102,7 +116,8 @@ __device__ __forceinline__ float key_value(unsigned k) {
 }
 
 // Bins.  The first kBins - 1 are for weights of 2^-24 and more, the last for all
-// that are less; cut finer, those have 41 bins an e-fold.
+// that are less (and summed apart, without atomics); cut finer, those have 41 bins
+// an e-fold.
 constexpr float kBinsFold = (kBins - 1) / (24 * 0.69314718f);
 constexpr float kFineLast = 41.0f / kBinsFold;
 
@@ -111,31 +126,21 @@ struct Row {
   int n, vec, shift;
   int rank, ctas;
   float top;                            // the largest logit
+  bool inf;                             // that was +infinity: such count as 0, all others as far below (and T as 1)
   double rate;                          // log2(e) / T
   float scale;                          // bins per unit of max - x
   const double* pow2;
-  // how far below the top
-  __device__ __forceinline__ float below(float v) const { return v == top ? 0.0f : top - v; }
-  __device__ __forceinline__ float place(float v) const { return below(v) * scale; }
+  __device__ __forceinline__ float place(float v) const { return (top - v) * scale; }
   __device__ __forceinline__ int bin(float v) const { return min(__float2int_rd(place(v)), kBins - 1); }
   __device__ __forceinline__ int fine(float v, int b) const {
     return min(__float2int_rd((place(v) - (float)b) * (b == kBins - 1 ? kFineLast : (float)kBins)), kBins - 1);
   }
   // 2^(shift - (top - v) rate) to the nearest whole number: 2^(m/32) from a table,
   // 2^r, |r| <= 1/64, by its Taylor sum (next term 2e-15).  Whole numbers come of
-  // adding 1.5 2^52, 2^52.  In the last bin fp32 will do: each weight is below 2^-24
-  // and off by 3e-6 of itself.
+  // adding 1.5 2^52, 2^52.  No branches: a warp's lanes would take both sides.
   __device__ __forceinline__ u64 weight(float v) const {
-    if (v == top) return 1ull << shift;
-    const float d = top - v;
-    if (isinf(d)) return 0;                               // below an infinity, whatever T
-    if (d * scale >= (float)(kBins - 1)) {
-      float y;
-      asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(fmaf(-d, (float)rate, (float)shift)));
-      return __float2uint_rn(y);
-    }
-    const double y = fma((double)v - (double)top, rate, (double)shift);
-    if (!(y > -1.0)) return 0;                            // T so small that the bins' scale has its limit
+    double y = fma((double)v - (double)top, rate, (double)shift);
+    y = y > -2.0 ? y : -2.0;                              // 0, as is NaN (-infinity at T infinite)
     const double big = fma(y, 32.0, 6755399441055744.0);
     const int m = __double2loint(big);
     const double r = fma(big - 6755399441055744.0, -1.0 / 32, y);
@@ -193,13 +198,17 @@ __device__ __forceinline__ void sweep(const Row& r, F f) {
           v[2 * e + 1] = g.y;
         }
       }
+      if (r.inf) {
+#pragma unroll
+        for (int e = 0; e < P; ++e) v[e] = v[e] == INFINITY ? 0.0f : fminf(v[e], -1e30f);
+      }
       f(v, (p0 + q * step + lane) * P);
     }
   }
 }
 
-__device__ __forceinline__ void add_weight(SampleShared& s, int b, u64 w, unsigned n = 1) {
-  atomicAdd(&s.cnt[b], n);
+__device__ __forceinline__ void add_weight(Hist& s, int b, u64 w, unsigned n) {
+  atomicAdd(&s.n[b], n);
   const unsigned l = (unsigned)w;
   const unsigned old = l ? atomicAdd(&s.lo[b], l) : 0u;
   const unsigned h = (unsigned)(w >> 32) + (old + l < old ? 1u : 0u);
@@ -244,28 +253,53 @@ __device__ __forceinline__ void block_sum(SampleShared& s, u64& w, unsigned& n) 
   n = b;
 }
 
-__device__ __forceinline__ void clear_bins(SampleShared& s) {
-  for (int b = threadIdx.x; b < kBins; b += kSmpThreads) s.lo[b] = s.hi[b] = s.cnt[b] = 0;
+__device__ __forceinline__ void clear(Hist& s) {
+  for (int b = threadIdx.x; b < kBins; b += kSmpThreads) s.lo[b] = s.hi[b] = s.n[b] = 0;
 }
 
-// Adds this CTA's bins to the first one's sums.  By atomics that return nothing, so
-// that none is waited for.
-__device__ __forceinline__ void push_bins(SampleShared& s, u64* w, unsigned* n) {
-  for (int b = threadIdx.x; b < kBins; b += kSmpThreads)
-    if (const unsigned c = s.cnt[b]) {
-      atomicAdd(n + b, c);
-      if (const u64 x = ((u64)s.hi[b] << 32) + s.lo[b]) atomicAdd(w + b, x);
+// All CTAs' histograms, from (w0, n0) on, as inclusive sums in each one's `h`.  A CTA
+// adds up its share of the bins, four of one CTA a thread and the CTAs' by shuffles
+// (by remote atomics: 12,000 cycles, so 6,500); then each reads all of them.
+__device__ __forceinline__ void all_bins(cg::cluster_group& cl, SampleShared& s, Hist& h, u64 w0, unsigned n0) {
+  const int ctas = (int)cl.num_blocks(), each = kBins / ctas, from = (int)threadIdx.x % ctas;
+  const int mine = (int)cl.block_rank() * each + (int)threadIdx.x / ctas * kPerThread;
+  cl.sync();
+  {
+    const Hist& g = &h == &s.hist ? cl.map_shared_rank(&s, from)->hist : cl.map_shared_rank(&s, from)->fine;
+    const uint4 lo = *reinterpret_cast<const uint4*>(g.lo + mine), hi = *reinterpret_cast<const uint4*>(g.hi + mine);
+    const uint4 cn = *reinterpret_cast<const uint4*>(g.n + mine);
+    u64 w[4] = {((u64)hi.x << 32) + lo.x, ((u64)hi.y << 32) + lo.y, ((u64)hi.z << 32) + lo.z, ((u64)hi.w << 32) + lo.w};
+    unsigned n[4] = {cn.x, cn.y, cn.z, cn.w};
+    static_assert(kPerThread == 4, "a uint4 of bins");
+    for (int x = 1; x < ctas; x <<= 1)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        w[i] += __shfl_xor_sync(0xffffffffu, w[i], x);
+        n[i] += __shfl_xor_sync(0xffffffffu, n[i], x);
+      }
+    if (from == 0) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        s.all.w[mine + i] = w[i];
+        s.all.n[mine + i] = n[i];
+      }
     }
-}
-// First CTA: its sums, inclusive from (w0, n0) on.
-__device__ __forceinline__ void scan_bins(SampleShared& s, u64* w, unsigned* n, u64 w0, unsigned n0) {
+  }
+  cl.sync();
   const int b0 = threadIdx.x * kPerThread;
+  const SampleShared* o = cl.map_shared_rank(&s, b0 / each);
   u64 x[kPerThread], all;
   unsigned y[kPerThread], alln;
+  {
+    const ulonglong2 p = *reinterpret_cast<const ulonglong2*>(o->all.w + b0), q = *reinterpret_cast<const ulonglong2*>(o->all.w + b0 + 2);
+    const uint4 c = *reinterpret_cast<const uint4*>(o->all.n + b0);
+    x[0] = p.x; x[1] = p.y; x[2] = q.x; x[3] = q.y;
+    y[0] = c.x; y[1] = c.y; y[2] = c.z; y[3] = c.w;
+  }
 #pragma unroll
-  for (int i = 0; i < kPerThread; ++i) {
-    x[i] = w[b0 + i] + (i ? x[i - 1] : 0);
-    y[i] = n[b0 + i] + (i ? y[i - 1] : 0);
+  for (int i = 1; i < kPerThread; ++i) {
+    x[i] += x[i - 1];
+    y[i] += y[i - 1];
   }
   u64 sum = x[kPerThread - 1];
   unsigned sn = y[kPerThread - 1];
@@ -274,87 +308,62 @@ __device__ __forceinline__ void scan_bins(SampleShared& s, u64* w, unsigned* n, 
   sn += n0 - y[kPerThread - 1];
 #pragma unroll
   for (int i = 0; i < kPerThread; ++i) {
-    w[b0 + i] = sum + x[i];
-    n[b0 + i] = sn + y[i];
+    h.w[b0 + i] = sum + x[i];
+    h.n[b0 + i] = sn + y[i];
   }
   __syncthreads();
 }
 
-// First CTA: the list sorted, falling.
-__device__ __forceinline__ void sort_list(SampleShared& s, int count) {
-  int m = 2;
-  while (m < count) m <<= 1;
-  for (int i = count + threadIdx.x; i < m; i += kSmpThreads) s.list[i] = 0;
-  __syncthreads();
-  for (int k = 2; k <= m; k <<= 1)
-    for (int j = k >> 1; j > 0; j >>= 1) {
-      for (int i = threadIdx.x; i < m / 2; i += kSmpThreads) {
-        const int a = 2 * i - (i & (j - 1)), b = a + j;
-        const u64 x = s.list[a], y = s.list[b];
-        if ((x < y) == ((a & k) == 0)) {
-          s.list[a] = y;
-          s.list[b] = x;
-        }
-      }
-      __syncthreads();
-    }
-}
-
-// First CTA: inclusive sums over the sorted list, from (w0, n0) on, this thread's
-// entries threadIdx.x * 4 ..; own: their weights.
-constexpr int kListed = kCap / kSmpThreads;
-__device__ __forceinline__ void scan_list(SampleShared& s, const Row& r, int count, u64 w0, unsigned n0, u64 (&cum)[kListed],
-                                          u64 (&own)[kListed]) {
-  u64 sum = 0, all;
-  unsigned n = 0, alln;
-#pragma unroll
-  for (int i = 0; i < kListed; ++i) {
-    const int at = threadIdx.x * kListed + i;
-    own[i] = at < count ? r.weight(key_value((unsigned)(s.list[at] >> 32))) : 0;
-    sum += own[i];
-    cum[i] = sum;
-  }
-  u64 incl = sum;
-  block_scan(s, incl, n, all, alln);
-#pragma unroll
-  for (int i = 0; i < kListed; ++i) cum[i] += w0 + incl - sum;
-}
-// First CTA: the first entry of the list past the cut, or `other`.
-__device__ __forceinline__ Found find_listed(SampleShared& s, const u64 (&cum)[kListed], const u64 (&own)[kListed], int count,
-                                             unsigned n0, const Cut& c, const Found& other) {
-  __syncthreads();
-  if (threadIdx.x == 0) s.found = other;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < kListed; ++i) {
-    const int at = threadIdx.x * kListed + i;
-    if (at < count && past(c, n0 + at + 1, cum[i]) && (at == 0 || !past(c, n0 + at, cum[i] - own[i])))
-      s.found = {n0 + at + 1, cum[i], own[i], (int)~(unsigned)s.list[at]};
-  }
-  __syncthreads();
-  return s.found;
-}
-
-// First CTA: the first bin past the cut, of inclusive sums from (w0, n0) on.
-__device__ __forceinline__ void find_bin(CutBin& to, const Cut& c, const u64* w, const unsigned* n, u64 w0, unsigned n0) {
+// The first bin past the cut, of inclusive sums from (w0, n0) on; by all threads,
+// to be read behind a barrier.  (nb == 0 stands for the very first token: past is
+// monotone, so with tokens before the bin the test of what comes before holds.)
+__device__ __forceinline__ void find_bin(CutBin& to, const Cut& c, const Hist& h, u64 w0, unsigned n0) {
 #pragma unroll
   for (int i = 0; i < kPerThread; ++i) {
     const int b = threadIdx.x * kPerThread + i;
-    const u64 wb = b ? w[b - 1] : w0;
-    const unsigned nb = b ? n[b - 1] : n0;
-    if (n[b] > nb && past(c, n[b], w[b]) && (nb == 0 || !past(c, nb, wb))) to = {b, nb, n[b] - nb, wb, w[b]};
+    const u64 wb = b ? h.w[b - 1] : w0;
+    const unsigned nb = b ? h.n[b - 1] : n0;
+    if (h.n[b] > nb && past(c, h.n[b], h.w[b]) && (nb == 0 || !past(c, nb, wb))) to = {b, nb, h.n[b] - nb, wb, h.w[b]};
   }
 }
 
-// Tokens for which keep(value) go to the first CTA's list.
-template <typename E, typename F>
-__device__ __forceinline__ void collect(SampleShared* lead, const Row& r, F keep) {
+// Which values lie in bins from[i] to to[i] for some i, of the fine ones of bin
+// from[0] in `f` alone (f < 0: in all).
+template <int N>
+struct Ranges {
+  Row r;
+  int from[N], to[N], f;
+  bool plain;
+  __device__ __forceinline__ Ranges(const Row& row, int fine) : r(row), f(fine), plain(fine < 0 && row.scale > 0.0f) {}
+  __device__ __forceinline__ void set(int i, int a, int b) {
+    from[i] = a;
+    to[i] = b;
+    plain &= b < kBins - 1;
+  }
+  __device__ __forceinline__ bool has(float v) const {
+    bool in = false;
+    if (plain) {                                          // -infinity, and what lies further than floats go: not in any
+      const float x = r.place(v);
+#pragma unroll
+      for (int i = 0; i < N; ++i) in |= x >= (float)from[i] && x < (float)(to[i] + 1);
+      return in;
+    }
+    const int b = r.bin(v);
+#pragma unroll
+    for (int i = 0; i < N; ++i) in |= b >= from[i] && b <= to[i];
+    return in && v > -INFINITY && (f < 0 || r.fine(v, from[0]) == f);
+  }
+};
+
+// Tokens of a range go to the first CTA's list.
+template <typename E, typename G>
+__device__ __forceinline__ void collect(SampleShared* lead, const Row& r, const G& g, unsigned* listed) {
   const int lane = threadIdx.x & 31;
   sweep<E>(r, [&](const auto& v, int i) {
     constexpr int P = 16 / sizeof(E);
     unsigned mine = 0;
 #pragma unroll
-    for (int e = 0; e < P; ++e) mine |= (v[e] > -INFINITY && keep(v[e]) ? 1u : 0u) << e;
+    for (int e = 0; e < P; ++e) mine |= (g.has(v[e]) ? 1u : 0u) << e;
     if (!__any_sync(0xffffffffu, mine != 0)) return;
     unsigned at = __popc(mine);                           // a place for each in the list
     for (int o = 1; o < 32; o <<= 1) {
@@ -362,7 +371,7 @@ __device__ __forceinline__ void collect(SampleShared* lead, const Row& r, F keep
       if (lane >= o) at += x;
     }
     unsigned base = 0;
-    if (lane == 31) base = atomicAdd(&lead->listed, at);
+    if (lane == 31) base = atomicAdd(listed, at);
     at += __shfl_sync(0xffffffffu, base, 31) - __popc(mine);
 #pragma unroll
     for (int e = 0; e < P; ++e)
@@ -371,6 +380,62 @@ __device__ __forceinline__ void collect(SampleShared* lead, const Row& r, F keep
         ++at;
       }
   });
+}
+
+// First CTA: the list's tokens of a cut's bin (all: the list has no others), sorted,
+// falling, and the first past the cut.
+__device__ __noinline__ Found find_listed(SampleShared& s, const Row& r, const Cut& c, const CutBin& at, int listed, bool all) {
+  const int tid = threadIdx.x, count = (int)at.count;
+  if (tid == 0) s.picked = 0;
+  int m = 2;
+  while (m < count) m <<= 1;
+  for (int i = count + tid; i < m; i += kSmpThreads) s.sorted[i] = 0;
+  __syncthreads();
+  for (int i = tid; i < listed; i += kSmpThreads) {
+    const u64 x = s.list[i];
+    if (all) s.sorted[i] = x;
+    else if (r.bin(key_value((unsigned)(x >> 32))) == at.bin) s.sorted[atomicAdd(&s.picked, 1u)] = x;
+  }
+  __syncthreads();
+  auto stage = [&](int k, int j, int i) {
+    const int a = 2 * i - (i & (j - 1)), b = a + j;
+    const u64 x = s.sorted[a], y = s.sorted[b];
+    if ((x < y) == ((a & k) == 0)) {
+      s.sorted[a] = y;
+      s.sorted[b] = x;
+    }
+  };
+  if (m <= 64) {                                          // a warp's work
+    if (tid < 32)
+      for (int k = 2; k <= m; k <<= 1)
+        for (int j = k >> 1; j > 0; j >>= 1) {
+          if (tid < m / 2) stage(k, j, tid);
+          __syncwarp();
+        }
+    __syncthreads();
+  } else {
+    for (int k = 2; k <= m; k <<= 1)
+      for (int j = k >> 1; j > 0; j >>= 1) {
+        for (int i = tid; i < m / 2; i += kSmpThreads) stage(k, j, i);
+        __syncthreads();
+      }
+  }
+  // sums from (w0, n0) on, a run of tokens a thread
+  const int run = (count + kSmpThreads - 1) / kSmpThreads, i0 = tid * run, i1 = min(i0 + run, count);
+  u64 sum = 0, total;
+  unsigned none = 0, nonen;
+  for (int i = i0; i < i1; ++i) sum += r.weight(key_value((unsigned)(s.sorted[i] >> 32)));
+  u64 w = sum;
+  block_scan(s, w, none, total, nonen);
+  w += at.w0 - sum;
+  for (int i = i0; i < i1; ++i) {
+    const u64 own = r.weight(key_value((unsigned)(s.sorted[i] >> 32))), before = w;
+    w += own;
+    const unsigned n = at.n0 + i;
+    if (past(c, n + 1, w) && (n == 0 || !past(c, n, before))) s.found = {n + 1, w, own, (int)~(unsigned)s.sorted[i]};
+  }
+  __syncthreads();
+  return s.found;
 }
 
 // Count and weight over the row of the tokens for which keep(value, index), the
@@ -404,72 +469,56 @@ __device__ __forceinline__ void count_row(cg::cluster_group& cl, SampleShared& s
   }
 }
 
-// The token at which a cut falls, in the bin where it does; the same in every CTA.
+// The token at which a cut falls, in the bin where it does; the same in every CTA
+// (last: in the first, the others need not know).  time: 0, 1 .. of a row.
 template <typename E>
-__device__ __noinline__ Found resolve(cg::cluster_group& cl, SampleShared& s, const Row& r, const Cut& c, CutBin at) {
+__device__ __noinline__ Found resolve(cg::cluster_group& cl, SampleShared& s, const Row& r, const Cut& c, CutBin at, int time,
+                                      bool last) {
   SampleShared* lead = cl.map_shared_rank(&s, 0);
   const int b = at.bin;
   int f = -1;                                             // the finer bin, if any
   if (at.count > kCap) {
-    clear_bins(s);
-    if (r.rank == 0)
-      for (int i = threadIdx.x; i < kBins; i += kSmpThreads) {
-        s.list[i] = 0;
-        s.fine_n[i] = 0;
-      }
-    cl.sync();
+    cl.sync();                                            // what was read of `all`, what was sorted there, the list are done with
+    clear(s.fine);
+    __syncthreads();
     sweep<E>(r, [&](const auto& v, int) {
       constexpr int P = 16 / sizeof(E);
 #pragma unroll 1
       for (int e = 0; e < P; ++e)
-        if (v[e] > -INFINITY && r.bin(v[e]) == b) add_weight(s, r.fine(v[e], b), r.weight(v[e]));
+        if (v[e] > -INFINITY && r.bin(v[e]) == b) add_weight(s.fine, r.fine(v[e], b), r.weight(v[e]), 1);
     });
+    all_bins(cl, s, s.fine, at.w0, at.n0);
+    find_bin(s.cut[2], c, s.fine, at.w0, at.n0);
     __syncthreads();
-    push_bins(s, lead->list, lead->fine_n);
-    cl.sync();
-    if (r.rank == 0) {
-      scan_bins(s, s.list, s.fine_n, at.w0, at.n0);
-      // nb == 0 in find_bin stands for the very first token: past is monotone, so
-      // with tokens before the bin the test of what comes before holds
-      find_bin(s.cut[kBinK], c, s.list, s.fine_n, at.w0, at.n0);
-    }
-    cl.sync();
-    at = lead->cut[kBinK];
+    at = s.cut[2];
     f = at.bin;
+    cl.sync();                                            // `all` is read, `fine` makes way for the list
   }
-  const int cnt = (int)at.count;
-  const u64 w0 = at.w0;
-  const unsigned n0 = at.n0;
-  auto mine = [&](float v) { return r.bin(v) == b && (f < 0 || r.fine(v, b) == f); };
+  Ranges<1> g(r, f);
+  g.set(0, b, b);
   Found got;
-  if (cnt <= kCap) {
+  if (at.count <= kCap) {
+    collect<E>(lead, r, g, &lead->listed[time]);
     cl.sync();
-    if (r.rank == 0 && threadIdx.x == 0) s.listed = 0;
+    if (r.rank == 0) got = find_listed(s, r, c, at, (int)at.count, true);
+    if (last) return got;
     cl.sync();
-    collect<E>(lead, r, mine);
-    cl.sync();
-    if (r.rank == 0) {
-      sort_list(s, cnt);
-      u64 cum[kListed], own[kListed];
-      scan_list(s, r, cnt, w0, n0, cum, own);
-      find_listed(s, cum, own, cnt, n0, c, Found{});
-    }
-    cl.sync();
-    got = lead->found;
-    return got;
+    return lead->found;
   }
   // bisection: the largest key k such that what is not below it is past the cut
+  const u64 w0 = at.w0;
+  const unsigned n0 = at.n0;
   unsigned lo = 0, hi = 0xffffffffu;
   int round = 0;
   u64 w;
   unsigned n;
   while (lo < hi) {
     const unsigned mid = lo + (hi - lo) / 2 + 1;
-    count_row<E>(cl, s, r, round ^= 1, [&](float v, int) { return order_key(v) >= mid && mine(v); }, w, n);
+    count_row<E>(cl, s, r, round ^= 1, [&](float v, int) { return order_key(v) >= mid && g.has(v); }, w, n);
     if (past(c, n0 + n, w0 + w)) lo = mid;
     else hi = mid - 1;
   }
-  count_row<E>(cl, s, r, round ^= 1, [&](float v, int) { return order_key(v) > lo && mine(v); }, w, n);
+  count_row<E>(cl, s, r, round ^= 1, [&](float v, int) { return order_key(v) > lo && g.has(v); }, w, n);
   w += w0;
   n += n0;
   const u64 own = r.weight(key_value(lo));
@@ -501,8 +550,7 @@ __global__ void __launch_bounds__(kSmpThreads, 2) sample_rows_kernel(const __gri
   extern __shared__ __align__(16) uint8_t raw[];
   SampleShared& s = *reinterpret_cast<SampleShared*>(raw);
   cg::cluster_group cl = cg::this_cluster();
-  pdl_wait();
-  pdl_trigger();
+  constexpr int P = 16 / sizeof(E);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   Row r;
   r.rank = (int)cl.block_rank();
@@ -512,20 +560,16 @@ __global__ void __launch_bounds__(kSmpThreads, 2) sample_rows_kernel(const __gri
   r.n = a.n;
   r.vec = a.vec;
   r.shift = a.shift;
+  r.inf = false;
   r.pow2 = s.pow2;
   SampleShared* lead = cl.map_shared_rank(&s, 0);
-
-  clear_bins(s);
-  if (r.rank == 0)
-    for (int i = tid; i < kBins; i += kSmpThreads) {
-      s.cum_w[i] = 0;
-      s.cum_n[i] = 0;
-    }
+  clear(s.hist);
   if (tid < 32) s.pow2[tid] = exp2((double)tid / 32.0);
-  if (tid == 0) {
-    s.listed = 0;
-    s.first = 0xffffffffu;
-  }
+  if (tid < 4) s.listed[tid] = 0;
+  if (tid == 0) s.first = 0xffffffffu;
+  pdl_wait();
+  pdl_trigger();
+
   // the largest; NaN if there is one
   auto top_nan = [](float x, float y) {
     float z;
@@ -534,7 +578,6 @@ __global__ void __launch_bounds__(kSmpThreads, 2) sample_rows_kernel(const __gri
   };
   float best = -INFINITY;
   sweep<E>(r, [&](const auto& v, int) {
-    constexpr int P = 16 / sizeof(E);
     float m = top_nan(v[0], v[1]);
 #pragma unroll
     for (int e = 2; e < P; e += 2) m = top_nan(m, top_nan(v[e], v[e + 1]));
@@ -549,16 +592,15 @@ __global__ void __launch_bounds__(kSmpThreads, 2) sample_rows_kernel(const __gri
     if (lane == 0) s.top = best;
   }
   cl.sync();
-  best = -INFINITY;
-  for (int c = 0; c < r.ctas; ++c) best = top_nan(best, cl.map_shared_rank(&s, c)->top);
-  r.top = best;
+  best = lane < r.ctas ? cl.map_shared_rank(&s, lane)->top : -INFINITY;
+  for (int o = 4; o > 0; o >>= 1) best = top_nan(best, __shfl_xor_sync(0xffffffffu, best, o));
+  r.top = __shfl_sync(0xffffffffu, best, 0);
   const float T = a.temperature ? a.temperature[row] : 1.0f;
   const bool none = isnan(r.top) || r.top == -INFINITY;   // nothing to choose from
   if (none || !(T > 0.0f)) {
     if (!none) {                                          // the first of the largest
       unsigned at = 0xffffffffu;
       sweep<E>(r, [&](const auto& v, int i) {
-        constexpr int P = 16 / sizeof(E);
 #pragma unroll
         for (int e = 0; e < P; ++e)
           if (v[e] == r.top) at = min(at, (unsigned)(i + e));
@@ -575,8 +617,10 @@ __global__ void __launch_bounds__(kSmpThreads, 2) sample_rows_kernel(const __gri
     cl.sync();                                            // nobody leaves while its memory is read
     return;
   }
-  r.rate = 1.4426950408889634 / (double)T;
-  r.scale = fminf(kBinsFold / T, 1e30f);
+  r.inf = isinf(r.top);
+  if (r.inf) r.top = 0.0f;
+  r.rate = r.inf ? 1.0 : 1.4426950408889634 / (double)T;
+  r.scale = r.inf ? 1.0f : fminf(kBinsFold / T, 1e30f);
 
   const float pf = a.top_p ? a.top_p[row] : 1.0f, mf = a.min_p ? a.min_p[row] : 0.0f;
   const bool by_p = pf < 1.0f, by_m = mf > 0.0f;
@@ -585,21 +629,38 @@ __global__ void __launch_bounds__(kSmpThreads, 2) sample_rows_kernel(const __gri
   u64 wm = 0, wl = 0;                                     // of the tokens that min-p keeps, of the last bin's
   unsigned nm = 0, nl = 0;
   sweep<E>(r, [&](const auto& v, int) {
-    constexpr int P = 16 / sizeof(E);
+    // two at a time (four spill registers): their weights, then their atomics
 #pragma unroll
-    for (int e = 0; e < P; ++e) {
-      if (v[e] == -INFINITY) continue;
-      const u64 w = r.weight(v[e]);
-      if (by_m && w >= m) {
-        wm += w;
-        ++nm;
+    for (int e0 = 0; e0 < P; e0 += 2) {
+      u64 w[2];
+      int b[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        w[e] = r.weight(v[e0 + e]);
+        b[e] = r.bin(v[e0 + e]);
       }
-      const int b = r.bin(v[e]);
-      if (b == kBins - 1) {
-        wl += w;
-        ++nl;
-      } else {
-        add_weight(s, b, w);
+      unsigned old[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        old[e] = 0;
+        if (v[e0 + e] == -INFINITY) {
+          b[e] = kBins;
+        } else if (b[e] == kBins - 1) {
+          wl += w[e];
+          ++nl;
+        } else {
+          atomicAdd(&s.hist.n[b[e]], 1u);
+          old[e] = atomicAdd(&s.hist.lo[b[e]], (unsigned)w[e]);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const unsigned h = (unsigned)(w[e] >> 32) + (old[e] + (unsigned)w[e] < old[e] ? 1u : 0u);
+        if (b[e] < kBins - 1 && h) atomicAdd(&s.hist.hi[b[e]], h);
+        if (by_m && w[e] >= m && b[e] < kBins) {
+          wm += w[e];
+          ++nm;
+        }
       }
     }
   });
@@ -607,7 +668,7 @@ __global__ void __launch_bounds__(kSmpThreads, 2) sample_rows_kernel(const __gri
     wl += __shfl_xor_sync(0xffffffffu, wl, o);
     nl += __shfl_xor_sync(0xffffffffu, nl, o);
   }
-  if (lane == 0 && nl) add_weight(s, kBins - 1, wl, nl);
+  if (lane == 0 && nl) add_weight(s.hist, kBins - 1, wl, nl);
   if (by_m) {
     block_sum(s, wm, nm);
     if (tid == 0) {
@@ -615,9 +676,7 @@ __global__ void __launch_bounds__(kSmpThreads, 2) sample_rows_kernel(const __gri
       s.part_n[0][1] = nm;
     }
   }
-  __syncthreads();
-  push_bins(s, lead->cum_w, lead->cum_n);
-  cl.sync();
+  all_bins(cl, s, s.hist, 0, 0);
   if (by_m) {
     wm = 0;
     nm = 0;
@@ -627,21 +686,18 @@ __global__ void __launch_bounds__(kSmpThreads, 2) sample_rows_kernel(const __gri
       nm += o->part_n[0][1];
     }
   }
+  // every CTA has the same sums and finds the same bins
+  const u64 total_w = s.hist.w[kBins - 1];
+  const unsigned total_n = s.hist.n[kBins - 1];
   const int k = a.top_k ? a.top_k[row] : 0;
-  if (r.rank == 0) {
-    scan_bins(s, s.cum_w, s.cum_n, 0, 0);
-    const u64 all = s.cum_w[kBins - 1];
-    if (k > 0 && (unsigned)k < s.cum_n[kBins - 1]) find_bin(s.cut[kBinK], {kByCount, (unsigned)k, 0.0}, s.cum_w, s.cum_n, 0, 0);
-    else if (by_p) find_bin(s.cut[kBinP], {kReach, 0, p * (double)all}, s.cum_w, s.cum_n, 0, 0);
-    if (by_m) find_bin(s.cut[kBinM], {kByCount, nm, 0.0}, s.cum_w, s.cum_n, 0, 0);
-  }
-  cl.sync();
-  const u64 total_w = lead->cum_w[kBins - 1];
-  const unsigned total_n = lead->cum_n[kBins - 1];
   const bool by_k = k > 0 && (unsigned)k < total_n;
   const Cut cut_k = {kByCount, (unsigned)k, 0.0};
   float uf = a.u[row];
   uf = uf >= 0.0f ? fminf(uf, 0.99999994f) : 0.0f;        // NaN: 0
+  if (by_k) find_bin(s.cut[0], cut_k, s.hist, 0, 0);
+  else if (by_p) find_bin(s.cut[0], {kReach, 0, p * (double)total_w}, s.hist, 0, 0);
+  if (by_m) find_bin(s.cut[1], {kByCount, nm, 0.0}, s.hist, 0, 0);
+  __syncthreads();
 
   // the bins down to the last cut; a top-p of the top k needs all of those
   int last = kBins - 1;
@@ -652,52 +708,80 @@ __global__ void __launch_bounds__(kSmpThreads, 2) sample_rows_kernel(const __gri
       upto = c.n0 + c.count;
     }
   };
-  if (by_k) down_to(lead->cut[kBinK]);
-  else if (by_p) down_to(lead->cut[kBinP]);
-  if (by_m && !(by_k && by_p)) down_to(lead->cut[kBinM]);
-  if (upto <= kCap) {
-    collect<E>(lead, r, [&](float v) { return r.bin(v) <= last; });
-    cl.sync();
-    if (r.rank == 0) {
-      sort_list(s, (int)upto);
-      u64 cum[kListed], own[kListed];
-      scan_list(s, r, (int)upto, 0, 0, cum, own);
-      Found f = {total_n, total_w, 0, 0};                 // of a cut that lies behind the list: min-p's does not
-      if (by_k) f = find_listed(s, cum, own, (int)upto, 0, cut_k, f);
-      if (by_p) f = find_listed(s, cum, own, (int)upto, 0, {kReach, 0, p * (double)f.w}, f);
-      if (by_m && nm < f.n) {
-        f.n = nm;
-        f.w = wm;
-      }
-      const unsigned n = f.n;
-      const u64 wn = f.w;
-      f = find_listed(s, cum, own, (int)upto, 0, {kPass, 0, (double)uf * (double)wn}, f);
-      if (tid == 0) {
-        a.token[row] = f.index;
-        if (a.prob) a.prob[row] = (float)((double)f.own / (double)wn);
-        if (a.kept) a.kept[row] = (int)n;
-      }
+  const CutBin first_cut = s.cut[0];
+  if (by_k || by_p) down_to(first_cut);
+  if (by_m && !(by_k && by_p)) down_to(s.cut[1]);
+  // Few tokens: all of them.  Else the bins that the cuts may fall in: k's is known,
+  // p's and the draw's as closely as the weight down to the cut before is.
+  Ranges<3> g(r, -1);
+  bool few = upto <= kCap;
+  g.set(0, 0, last);
+  g.set(1, 0, last);
+  g.set(2, 0, last);
+  if (!few) {
+    double lo = (double)total_w, hi = lo;
+    int b0 = kBins - 1, b1 = b0;
+    if (by_k) {
+      lo = (double)first_cut.w0;
+      hi = (double)first_cut.w;
+      b0 = b1 = first_cut.bin;
     }
-    cl.sync();
-    return;
+    unsigned count = 0;
+    auto between = [&](int mode, double x, double y) {    // the bins of the cuts at x and at y
+      __syncthreads();
+      find_bin(s.cut[0], {mode, 0, x}, s.hist, 0, 0);
+      find_bin(s.cut[2], {mode, 0, y}, s.hist, 0, 0);
+      __syncthreads();
+      count += s.cut[2].n0 + s.cut[2].count - s.cut[0].n0;
+      b0 = s.cut[0].bin;
+      b1 = s.cut[2].bin;
+    };
+    if (by_k) count += first_cut.count;
+    g.set(0, by_k ? b0 : -1, by_k ? b1 : -1);
+    g.set(1, -1, -1);
+    if (by_p) {
+      between(kReach, p * lo, p * hi);
+      g.set(1, b0, b1);
+      lo = (double)s.cut[0].w0;
+      hi = (double)s.cut[2].w;
+    }
+    if (by_m) lo = fmin(lo, (double)wm);
+    between(kPass, (double)uf * lo, (double)uf * hi);
+    g.set(2, b0, b1);
+    few = count <= kCap;
   }
-  // one cut after the other
-  auto cut_at = [&](const Cut& c) {
-    if (r.rank == 0) find_bin(s.cut[kBinP], c, s.cum_w, s.cum_n, 0, 0);
+  if (few) {
+    collect<E>(lead, r, g, &lead->listed[0]);
     cl.sync();
-    return resolve<E>(cl, s, r, c, lead->cut[kBinP]);
+    if (r.rank != 0) {
+      cl.sync();
+      return;
+    }
+  }
+  const int listed = (int)s.listed[0];
+  // One cut after the other; where the bins are listed, in the first CTA alone.
+  // Of two that are bins apart only the nearer is looked for.
+  int time = 0;
+  auto cut_at = [&](const Cut& c, bool final) {
+    __syncthreads();
+    find_bin(s.cut[0], c, s.hist, 0, 0);
+    __syncthreads();
+    const CutBin at = s.cut[0];
+    if (few) return find_listed(s, r, c, at, listed, false);
+    return resolve<E>(cl, s, r, c, at, time++, final);
   };
   unsigned n = total_n;
   u64 wn = total_w;
-  if (by_k) {
-    const CutBin b = lead->cut[kBinK];
+  const bool m_nearer = by_m && !(by_k && by_p) && nm < n;
+  if (by_k && !(m_nearer && nm <= (unsigned)k)) {
     n = (unsigned)k;
-    wn = b.w;
+    wn = first_cut.w;
     // a bin that ends with the cut, or weighs nothing, need not be looked at
-    if (b.n0 + b.count != n && b.w != b.w0) wn = resolve<E>(cl, s, r, cut_k, b).w;
+    if (first_cut.n0 + first_cut.count != n && first_cut.w != first_cut.w0)
+      wn = few ? find_listed(s, r, cut_k, first_cut, listed, false).w : resolve<E>(cl, s, r, cut_k, first_cut, time++, false).w;
   }
-  if (by_p) {
-    const Found f = cut_at({kReach, 0, p * (double)wn});
+  if (by_p && !(m_nearer && nm <= first_cut.n0)) {
+    const Found f = cut_at({kReach, 0, p * (double)wn}, false);
     if (f.n < n) {
       n = f.n;
       wn = f.w;
@@ -707,7 +791,7 @@ __global__ void __launch_bounds__(kSmpThreads, 2) sample_rows_kernel(const __gri
     n = nm;
     wn = wm;
   }
-  const Found f = cut_at({kPass, 0, (double)uf * (double)wn});
+  const Found f = cut_at({kPass, 0, (double)uf * (double)wn}, true);
   if (r.rank == 0 && tid == 0) {
     a.token[row] = f.index;
     if (a.prob) a.prob[row] = (float)((double)f.own / (double)wn);
