@@ -545,8 +545,10 @@ __device__ __noinline__ Found resolve(cg::cluster_group& cl, SampleShared& s, co
   return got;
 }
 
+// One CTA an SM: two, of 64 registers a thread, spill (one row 21.7 us, 18.1; 64 x
+// 131072 77.0, 71.3).
 template <typename E>
-__global__ void __launch_bounds__(kSmpThreads, 2) sample_rows_kernel(const __grid_constant__ SampleArgs a) {
+__global__ void __launch_bounds__(kSmpThreads, 1) sample_rows_kernel(const __grid_constant__ SampleArgs a) {
   extern __shared__ __align__(16) uint8_t raw[];
   SampleShared& s = *reinterpret_cast<SampleShared*>(raw);
   cg::cluster_group cl = cg::this_cluster();
@@ -629,19 +631,19 @@ __global__ void __launch_bounds__(kSmpThreads, 2) sample_rows_kernel(const __gri
   u64 wm = 0, wl = 0;                                     // of the tokens that min-p keeps, of the last bin's
   unsigned nm = 0, nl = 0;
   sweep<E>(r, [&](const auto& v, int) {
-    // two at a time (four spill registers): their weights, then their atomics
+    // four at a time: their weights, then their atomics
 #pragma unroll
-    for (int e0 = 0; e0 < P; e0 += 2) {
-      u64 w[2];
-      int b[2];
+    for (int e0 = 0; e0 < P; e0 += 4) {
+      u64 w[4];
+      int b[4];
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
+      for (int e = 0; e < 4; ++e) {
         w[e] = r.weight(v[e0 + e]);
         b[e] = r.bin(v[e0 + e]);
       }
-      unsigned old[2];
+      unsigned old[4];
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
+      for (int e = 0; e < 4; ++e) {
         old[e] = 0;
         if (v[e0 + e] == -INFINITY) {
           b[e] = kBins;
@@ -654,7 +656,7 @@ __global__ void __launch_bounds__(kSmpThreads, 2) sample_rows_kernel(const __gri
         }
       }
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
+      for (int e = 0; e < 4; ++e) {
         const unsigned h = (unsigned)(w[e] >> 32) + (old[e] + (unsigned)w[e] < old[e] ? 1u : 0u);
         if (b[e] < kBins - 1 && h) atomicAdd(&s.hist.hi[b[e]], h);
         if (by_m && w[e] >= m && b[e] < kBins) {
@@ -820,8 +822,10 @@ extern "C" int tosk_sample_rows(const tosk_sample_t* t, cudaStream_t st) {
   a.token = t->token;
   a.prob = t->prob;
   a.kept = t->kept;
+  // A cluster's SMs are neighbours, so that not every count of them fits at once:
+  // 16 clusters of eight take two rounds (39.4 us; of four 25.9).
   int ctas = 8;
-  while (ctas > 1 && (long long)t->n_rows * ctas > 2 * 148) ctas /= 2;
+  while (ctas > 1 && (long long)t->n_rows * ctas > (ctas == 8 ? 104 : ctas == 4 ? 136 : 148)) ctas /= 2;
   while (ctas > 1 && t->n < 1024 * ctas) ctas /= 2;
   const long long grid = (long long)t->n_rows * ctas;
   if (grid > 0x7fffffffll) return (int)cudaErrorInvalidValue;
