@@ -6,14 +6,17 @@
 // rows keeps the larger of its own and that, and rounds the older rows anew only
 // if it grew.  Elements are x / 2^e (exact) rounded to nearest.  Each source
 // element is read once (eight passes of a warp stay in registers) and each byte
-// written once, so HBM bounds it; at one token a sequence the chain of loads
-// (sequence, table, row, scale) does.
+// written once, so HBM bounds it (8191 fp16 tokens, 8 heads x 128, K and V: 50 MB
+// in 13.4 us, 3.8 TB/s, launch and last wave included; with fp32 arithmetic for
+// fp16 rows 17.6); at one token a sequence the chain of loads (sequence, table, row,
+// scale) does.
 //
-// Read.  Rows back as fp32 or fp16: 16 elements a thread, four of them in flight.
+// Read.  Rows back as fp32 or fp16: 16 elements a thread, four of them in flight (the
+// same tokens in 15 us, 3.4 TB/s; 256 tokens 6.8, where a warp a row took 17.5).
 // Expand.  The keys and values of a prompt call's sequences as an fp16 pool in
 // a workspace, pages of 128 rows, for the tensor-core kernels; exact, since
-// every value is an fp16 number.  1 byte in, 2 out an element: a few per cent of
-// the attention that reads it.
+// every value is an fp16 number.  1 byte in, 2 out an element: 17 us for 8191 such
+// tokens, where the attention that reads them takes 182.
 #include <cuda_runtime.h>
 
 #include "paged8.cuh"
@@ -528,7 +531,8 @@ extern "C" int tosk_paged8_get(const tosk_paged8_io_t* io, cudaStream_t st) {
   a.n_tokens = io->n_tokens;
   const int type = io->k.dst ? io->k.dtype : io->v.dtype;
   a.tokens = rows_a_cta(io->n_tokens);
-  a.vec = io->kv.hd % 16 == 0 && few_pieces(a.tokens, io->kv) && rows_on(io->k.dst, io->k.dstride, type, 16) && rows_on(io->v.dst, io->v.dstride, type, 16);
+  a.vec = io->kv.hd % 16 == 0 && few_pieces(a.tokens, io->kv) && rows_on(io->k.dst, io->k.dstride, type, 16) &&
+          rows_on(io->v.dst, io->v.dstride, type, 16);
   const void* f = io->kv.type == TOSK_I8
                       ? type == TOSK_F32 ? (const void*)paged8_get_kernel<TOSK_I8, float> : (const void*)paged8_get_kernel<TOSK_I8, __half>
                       : type == TOSK_F32 ? (const void*)paged8_get_kernel<TOSK_F8, float> : (const void*)paged8_get_kernel<TOSK_F8, __half>;

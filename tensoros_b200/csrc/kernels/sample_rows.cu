@@ -21,7 +21,11 @@
 // depend on it, and a token differs from an exact evaluation's only where u
 // falls within ~1e-12 of a border.
 //
-// Bound: one read from HBM; the further passes find the row in L2.
+// Bound: for few rows the chain of passes and of the cluster's waits (1 x 32000,
+// temperature and top-p: 18 us; 16 of them 26; with top-k and min-p in some 41); for
+// many the histogram's atomics and fp64 weights, about half of the time, and the
+// collecting (64 x 131072: 71 us, one read of HBM would be 5; the further passes find
+// the row in L2).
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
@@ -89,7 +93,7 @@ struct SampleShared {
     u64 sorted[kCap];                   // first CTA: a cut's bin
   };
   union {
-    u64 list[kCap];                     // first CTA: tokens, value over inverted index
+    u64 list[kCap];                     // tokens, value over inverted index; first CTA: all CTAs'
     Hist fine;                          // a bin cut finer, as hist
   };
   double pow2[32];
@@ -100,8 +104,9 @@ struct SampleShared {
   float best[kSmpThreads / 32];
   float top;                            // this CTA's largest logit; NaN: it has one
   unsigned first;                       // its first place
-  unsigned listed[4];                   // first CTA: tokens listed for the first, second .. time
-  unsigned picked;
+  unsigned listed[4];                   // tokens that this CTA has listed for the first, second .. time
+  unsigned pushed[4];                   // first CTA: tokens that the others have, from the list's end on
+  unsigned picked, base;
   CutBin cut[3];
   Found found;
 };
@@ -355,44 +360,86 @@ struct Ranges {
   }
 };
 
-// Tokens of a range go to the first CTA's list.
+// Tokens of a range go to the first CTA's list, by way of this CTA's: its own from the
+// front, the others' from the end.  (An atomic add in another CTA's memory for every
+// piece with a token took 64 x 131072 20,000 cycles, so PLACEHOLDER.)
 template <typename E, typename G>
-__device__ __forceinline__ void collect(SampleShared* lead, const Row& r, const G& g, unsigned* listed) {
-  const int lane = threadIdx.x & 31;
+__device__ __forceinline__ void collect(SampleShared& s, SampleShared* lead, const Row& r, const G& g, int time) {
   sweep<E>(r, [&](const auto& v, int i) {
     constexpr int P = 16 / sizeof(E);
     unsigned mine = 0;
 #pragma unroll
     for (int e = 0; e < P; ++e) mine |= (g.has(v[e]) ? 1u : 0u) << e;
-    if (!__any_sync(0xffffffffu, mine != 0)) return;
-    unsigned at = __popc(mine);                           // a place for each in the list
-    for (int o = 1; o < 32; o <<= 1) {
-      const unsigned x = __shfl_up_sync(0xffffffffu, at, o);
-      if (lane >= o) at += x;
-    }
-    unsigned base = 0;
-    if (lane == 31) base = atomicAdd(listed, at);
-    at += __shfl_sync(0xffffffffu, base, 31) - __popc(mine);
+    if (!mine) return;
+    unsigned at = atomicAdd(&s.listed[time], __popc(mine));
 #pragma unroll
     for (int e = 0; e < P; ++e)
       if (mine >> e & 1) {
-        if (at < kCap) lead->list[at] = (u64)order_key(v[e]) << 32 | ~(unsigned)(i + e);
+        if (at < kCap) s.list[at] = (u64)order_key(v[e]) << 32 | ~(unsigned)(i + e);
         ++at;
       }
   });
+  if (r.rank == 0) return;
+  __syncthreads();
+  const unsigned n = min(s.listed[time], (unsigned)kCap);
+  if (threadIdx.x == 0) s.base = atomicAdd(&lead->pushed[time], n);
+  __syncthreads();
+  for (unsigned i = threadIdx.x; i < n; i += kSmpThreads)
+    if (s.base + i < kCap) lead->list[kCap - 1 - (s.base + i)] = s.list[i];
 }
 
-// First CTA: the list's tokens of a cut's bin (all: the list has no others), sorted,
-// falling, and the first past the cut.
-__device__ __noinline__ Found find_listed(SampleShared& s, const Row& r, const Cut& c, const CutBin& at, int listed, bool all) {
-  const int tid = threadIdx.x, count = (int)at.count;
+// First CTA: of the list's tokens of a cut's bin (all: it has no others), in falling
+// order, the first past the cut.
+constexpr int kQuick = 128;
+__device__ __noinline__ Found find_listed(SampleShared& s, const Row& r, const Cut& c, const CutBin& at, int time, bool all) {
+  const int tid = threadIdx.x, count = (int)at.count, front = (int)s.listed[time], listed = front + (int)s.pushed[time];
+  auto token = [&](int i) { return s.list[i < front ? i : kCap - 1 - (i - front)]; };
   if (tid == 0) s.picked = 0;
-  int m = 2;
+  if (count <= kQuick) {
+    // Each token's place and the weight before it, by comparing it with all: 4 to 32
+    // lanes a token.  (One token sorted, weighed and summed as below: 5,000 cycles, so
+    // PLACEHOLDER.)
+    u64* weights = s.sorted + kCap / 2;
+    __syncthreads();
+    for (int i = tid; i < listed; i += kSmpThreads) {
+      const u64 x = token(i);
+      const float v = key_value((unsigned)(x >> 32));
+      if (!all && r.bin(v) != at.bin) continue;
+      const unsigned to = atomicAdd(&s.picked, 1u);
+      s.sorted[to] = x;
+      weights[to] = r.weight(v);
+    }
+    __syncthreads();
+    int lanes = 32;
+    while (lanes * count > kSmpThreads) lanes >>= 1;
+    const int i = tid / lanes;
+    u64 w = 0;
+    unsigned n = 0;
+    if (i < count) {
+      const u64 x = s.sorted[i];
+      for (int j = tid & (lanes - 1); j < count; j += lanes)
+        if (s.sorted[j] > x) {
+          w += weights[j];
+          ++n;
+        }
+    }
+    for (int o = lanes >> 1; o > 0; o >>= 1) {
+      w += __shfl_xor_sync(0xffffffffu, w, o);
+      n += __shfl_xor_sync(0xffffffffu, n, o);
+    }
+    w += at.w0;
+    n += at.n0;
+    if (i < count && (tid & (lanes - 1)) == 0 && past(c, n + 1, w + weights[i]) && (n == 0 || !past(c, n, w)))
+      s.found = {n + 1, w + weights[i], weights[i], (int)~(unsigned)s.sorted[i]};
+    __syncthreads();
+    return s.found;
+  }
+  int m = 2 * kQuick;
   while (m < count) m <<= 1;
   for (int i = count + tid; i < m; i += kSmpThreads) s.sorted[i] = 0;
   __syncthreads();
   for (int i = tid; i < listed; i += kSmpThreads) {
-    const u64 x = s.list[i];
+    const u64 x = token(i);
     if (all) s.sorted[i] = x;
     else if (r.bin(key_value((unsigned)(x >> 32))) == at.bin) s.sorted[atomicAdd(&s.picked, 1u)] = x;
   }
@@ -405,21 +452,11 @@ __device__ __noinline__ Found find_listed(SampleShared& s, const Row& r, const C
       s.sorted[b] = x;
     }
   };
-  if (m <= 64) {                                          // a warp's work
-    if (tid < 32)
-      for (int k = 2; k <= m; k <<= 1)
-        for (int j = k >> 1; j > 0; j >>= 1) {
-          if (tid < m / 2) stage(k, j, tid);
-          __syncwarp();
-        }
-    __syncthreads();
-  } else {
-    for (int k = 2; k <= m; k <<= 1)
-      for (int j = k >> 1; j > 0; j >>= 1) {
-        for (int i = tid; i < m / 2; i += kSmpThreads) stage(k, j, i);
-        __syncthreads();
-      }
-  }
+  for (int k = 2; k <= m; k <<= 1)
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      for (int i = tid; i < m / 2; i += kSmpThreads) stage(k, j, i);
+      __syncthreads();
+    }
   // sums from (w0, n0) on, a run of tokens a thread
   const int run = (count + kSmpThreads - 1) / kSmpThreads, i0 = tid * run, i1 = min(i0 + run, count);
   u64 sum = 0, total;
@@ -498,9 +535,9 @@ __device__ __noinline__ Found resolve(cg::cluster_group& cl, SampleShared& s, co
   g.set(0, b, b);
   Found got;
   if (at.count <= kCap) {
-    collect<E>(lead, r, g, &lead->listed[time]);
+    collect<E>(s, lead, r, g, time);
     cl.sync();
-    if (r.rank == 0) got = find_listed(s, r, c, at, (int)at.count, true);
+    if (r.rank == 0) got = find_listed(s, r, c, at, time, true);
     if (last) return got;
     cl.sync();
     return lead->found;
@@ -567,7 +604,7 @@ __global__ void __launch_bounds__(kSmpThreads, 1) sample_rows_kernel(const __gri
   SampleShared* lead = cl.map_shared_rank(&s, 0);
   clear(s.hist);
   if (tid < 32) s.pow2[tid] = exp2((double)tid / 32.0);
-  if (tid < 4) s.listed[tid] = 0;
+  if (tid < 4) s.listed[tid] = s.pushed[tid] = 0;
   if (tid == 0) s.first = 0xffffffffu;
   pdl_wait();
   pdl_trigger();
@@ -753,14 +790,13 @@ __global__ void __launch_bounds__(kSmpThreads, 1) sample_rows_kernel(const __gri
     few = count <= kCap;
   }
   if (few) {
-    collect<E>(lead, r, g, &lead->listed[0]);
+    collect<E>(s, lead, r, g, 0);
     cl.sync();
     if (r.rank != 0) {
       cl.sync();
       return;
     }
   }
-  const int listed = (int)s.listed[0];
   // One cut after the other; where the bins are listed, in the first CTA alone.
   // Of two that are bins apart only the nearer is looked for.
   int time = 0;
@@ -769,7 +805,7 @@ __global__ void __launch_bounds__(kSmpThreads, 1) sample_rows_kernel(const __gri
     find_bin(s.cut[0], c, s.hist, 0, 0);
     __syncthreads();
     const CutBin at = s.cut[0];
-    if (few) return find_listed(s, r, c, at, listed, false);
+    if (few) return find_listed(s, r, c, at, 0, false);
     return resolve<E>(cl, s, r, c, at, time++, final);
   };
   unsigned n = total_n;
@@ -780,7 +816,7 @@ __global__ void __launch_bounds__(kSmpThreads, 1) sample_rows_kernel(const __gri
     wn = first_cut.w;
     // a bin that ends with the cut, or weighs nothing, need not be looked at
     if (first_cut.n0 + first_cut.count != n && first_cut.w != first_cut.w0)
-      wn = few ? find_listed(s, r, cut_k, first_cut, listed, false).w : resolve<E>(cl, s, r, cut_k, first_cut, time++, false).w;
+      wn = few ? find_listed(s, r, cut_k, first_cut, 0, false).w : resolve<E>(cl, s, r, cut_k, first_cut, time++, false).w;
   }
   if (by_p && !(m_nearer && nm <= first_cut.n0)) {
     const Found f = cut_at({kReach, 0, p * (double)wn}, false);
