@@ -54,17 +54,16 @@ struct SampleArgs {
   int* kept;
 };
 
-// What a cut is: the first token at which the count is `count`, or the sum of
-// weights reaches (passes) `sum`.
-enum { kByCount, kReach, kPass };
+// What a cut is: the first token at which the count is `count` and the sum of weights
+// `sum`, one of them for what the cut asks, the other the least there is.
 struct Cut {
-  int mode;
   unsigned count;
-  double sum;
+  u64 sum;
 };
-__device__ __forceinline__ bool past(const Cut& c, unsigned n, u64 w) {
-  return c.mode == kByCount ? n >= c.count : c.mode == kReach ? (double)w >= c.sum : (double)w > c.sum;
-}
+__device__ __forceinline__ Cut by_count(unsigned n) { return {n, 0}; }
+__device__ __forceinline__ Cut reaches(double w) { return {1, w > 0.0 ? (u64)ceil(w) : 0}; }
+__device__ __forceinline__ Cut passes(double w) { return {1, (u64)floor(w) + 1}; }    // w >= 0
+__device__ __forceinline__ bool past(const Cut& c, unsigned n, u64 w) { return n >= c.count && w >= c.sum; }
 struct Found {
   unsigned n;                           // tokens up to and with it
   u64 w, own;                           // their weight, its own
@@ -320,15 +319,14 @@ __device__ __forceinline__ void all_bins(cg::cluster_group& cl, SampleShared& s,
 }
 
 // The first bin past the cut, of inclusive sums from (w0, n0) on; by all threads,
-// to be read behind a barrier.  (nb == 0 stands for the very first token: past is
-// monotone, so with tokens before the bin the test of what comes before holds.)
+// to be read behind a barrier.
 __device__ __forceinline__ void find_bin(CutBin& to, const Cut& c, const Hist& h, u64 w0, unsigned n0) {
 #pragma unroll
   for (int i = 0; i < kPerThread; ++i) {
     const int b = threadIdx.x * kPerThread + i;
     const u64 wb = b ? h.w[b - 1] : w0;
     const unsigned nb = b ? h.n[b - 1] : n0;
-    if (h.n[b] > nb && past(c, h.n[b], h.w[b]) && (nb == 0 || !past(c, nb, wb))) to = {b, nb, h.n[b] - nb, wb, h.w[b]};
+    if (past(c, h.n[b], h.w[b]) && !past(c, nb, wb)) to = {b, nb, h.n[b] - nb, wb, h.w[b]};
   }
 }
 
@@ -410,9 +408,9 @@ __device__ __noinline__ Found find_listed(SampleShared& s, const Row& r, const C
       weights[to] = r.weight(v);
     }
     __syncthreads();
-    int lanes = 32;
-    while (lanes * count > kSmpThreads) lanes >>= 1;
-    const int i = tid / lanes;
+    int lg = 5;                                           // of the lanes a token
+    while (count << lg > kSmpThreads) --lg;
+    const int lanes = 1 << lg, i = tid >> lg;
     u64 w = 0;
     unsigned n = 0;
     if (i < count) {
@@ -429,7 +427,7 @@ __device__ __noinline__ Found find_listed(SampleShared& s, const Row& r, const C
     }
     w += at.w0;
     n += at.n0;
-    if (i < count && (tid & (lanes - 1)) == 0 && past(c, n + 1, w + weights[i]) && (n == 0 || !past(c, n, w)))
+    if (i < count && (tid & (lanes - 1)) == 0 && past(c, n + 1, w + weights[i]) && !past(c, n, w))
       s.found = {n + 1, w + weights[i], weights[i], (int)~(unsigned)s.sorted[i]};
     __syncthreads();
     return s.found;
@@ -469,7 +467,7 @@ __device__ __noinline__ Found find_listed(SampleShared& s, const Row& r, const C
     const u64 own = r.weight(key_value((unsigned)(s.sorted[i] >> 32))), before = w;
     w += own;
     const unsigned n = at.n0 + i;
-    if (past(c, n + 1, w) && (n == 0 || !past(c, n, before))) s.found = {n + 1, w, own, (int)~(unsigned)s.sorted[i]};
+    if (past(c, n + 1, w) && !past(c, n, before)) s.found = {n + 1, w, own, (int)~(unsigned)s.sorted[i]};
   }
   __syncthreads();
   return s.found;
@@ -560,15 +558,8 @@ __device__ __noinline__ Found resolve(cg::cluster_group& cl, SampleShared& s, co
   n += n0;
   const u64 own = r.weight(key_value(lo));
   // the ties it takes
-  unsigned t;
-  if (c.mode == kByCount) {
-    t = c.count - n;
-  } else {
-    const double q = floor((c.sum - (double)w) / (double)own);
-    t = q < 1.0 ? 1u : (unsigned)fmin(q, 1e9);
-    while (t > 1 && past(c, 0, w + (t - 1) * own)) --t;
-    while (!past(c, 0, w + t * own)) ++t;
-  }
+  unsigned t = c.count > n ? c.count - n : 1;
+  if (c.sum > w + t * own) t = (unsigned)((c.sum - w + own - 1) / own);
   unsigned a = 0, z = (unsigned)r.n - 1;                  // the t-th of them by index
   while (a < z) {
     const unsigned mid = a + (z - a) / 2;
@@ -730,12 +721,12 @@ __global__ void __launch_bounds__(kSmpThreads, 1) sample_rows_kernel(const __gri
   const unsigned total_n = s.hist.n[kBins - 1];
   const int k = a.top_k ? a.top_k[row] : 0;
   const bool by_k = k > 0 && (unsigned)k < total_n;
-  const Cut cut_k = {kByCount, (unsigned)k, 0.0};
+  const Cut cut_k = by_count((unsigned)k);
   float uf = a.u[row];
   uf = uf >= 0.0f ? fminf(uf, 0.99999994f) : 0.0f;        // NaN: 0
   if (by_k) find_bin(s.cut[0], cut_k, s.hist, 0, 0);
-  else if (by_p) find_bin(s.cut[0], {kReach, 0, p * (double)total_w}, s.hist, 0, 0);
-  if (by_m) find_bin(s.cut[1], {kByCount, nm, 0.0}, s.hist, 0, 0);
+  else if (by_p) find_bin(s.cut[0], reaches(p * (double)total_w), s.hist, 0, 0);
+  if (by_m) find_bin(s.cut[1], by_count(nm), s.hist, 0, 0);
   __syncthreads();
 
   // the bins down to the last cut; a top-p of the top k needs all of those
@@ -766,10 +757,10 @@ __global__ void __launch_bounds__(kSmpThreads, 1) sample_rows_kernel(const __gri
       b0 = b1 = first_cut.bin;
     }
     unsigned count = 0;
-    auto between = [&](int mode, double x, double y) {    // the bins of the cuts at x and at y
+    auto between = [&](const Cut& x, const Cut& y) {    // the bins of the cuts at x and at y
       __syncthreads();
-      find_bin(s.cut[0], {mode, 0, x}, s.hist, 0, 0);
-      find_bin(s.cut[2], {mode, 0, y}, s.hist, 0, 0);
+      find_bin(s.cut[0], x, s.hist, 0, 0);
+      find_bin(s.cut[2], y, s.hist, 0, 0);
       __syncthreads();
       count += s.cut[2].n0 + s.cut[2].count - s.cut[0].n0;
       b0 = s.cut[0].bin;
@@ -779,13 +770,13 @@ __global__ void __launch_bounds__(kSmpThreads, 1) sample_rows_kernel(const __gri
     g.set(0, by_k ? b0 : -1, by_k ? b1 : -1);
     g.set(1, -1, -1);
     if (by_p) {
-      between(kReach, p * lo, p * hi);
+      between(reaches(p * lo), reaches(p * hi));
       g.set(1, b0, b1);
       lo = (double)s.cut[0].w0;
       hi = (double)s.cut[2].w;
     }
     if (by_m) lo = fmin(lo, (double)wm);
-    between(kPass, (double)uf * lo, (double)uf * hi);
+    between(passes((double)uf * lo), passes((double)uf * hi));
     g.set(2, b0, b1);
     few = count <= kCap;
   }
@@ -819,7 +810,7 @@ __global__ void __launch_bounds__(kSmpThreads, 1) sample_rows_kernel(const __gri
       wn = few ? find_listed(s, r, cut_k, first_cut, 0, false).w : resolve<E>(cl, s, r, cut_k, first_cut, time++, false).w;
   }
   if (by_p && !(m_nearer && nm <= first_cut.n0)) {
-    const Found f = cut_at({kReach, 0, p * (double)wn}, false);
+    const Found f = cut_at(reaches(p * (double)wn), false);
     if (f.n < n) {
       n = f.n;
       wn = f.w;
@@ -829,7 +820,7 @@ __global__ void __launch_bounds__(kSmpThreads, 1) sample_rows_kernel(const __gri
     n = nm;
     wn = wm;
   }
-  const Found f = cut_at({kPass, 0, (double)uf * (double)wn}, true);
+  const Found f = cut_at(passes((double)uf * (double)wn), true);
   if (r.rank == 0 && tid == 0) {
     a.token[row] = f.index;
     if (a.prob) a.prob[row] = (float)((double)f.own / (double)wn);

@@ -143,6 +143,17 @@ def test_bins_that_overflow(gpu, what, o):
     check(gpu, x, uniform(rows, 5), **o)
 
 
+@pytest.mark.parametrize("o", [dict(p=0.0), dict(p=-1.0), dict(p=1e-30), dict(k=20000, p=0.0), dict(p=0.0, m=0.5)])
+@pytest.mark.parametrize("n", [1, 50, 32000])
+def test_one_token_at_least_stays(gpu, n, o):
+    """No top-p is too small for the first token, of very many ties too."""
+    x = torch.zeros(4, n, device="cuda")
+    x[1] = logits(1, n, 7)[0]
+    x[2, : n // 2] = -1.0
+    x[3] = (logits(1, n, 8)[0] / 4).round()
+    check(gpu, x, uniform(4), **o)
+
+
 @pytest.mark.parametrize("t", [1e-30, 1e-4, 100.0, 1e6, 1e38, float("inf")])
 @pytest.mark.parametrize("o", [dict(), dict(k=9000, p=0.7), dict(m=0.9)])
 def test_extreme_temperatures(gpu, t, o):
