@@ -379,8 +379,9 @@ int tos_attention_decode_paged8_dev(const tos_rows_t *out, const tos_rows_t *q, 
  * and the token is the first whose running sum of w passes u times theirs.
  * temperature <= 0 (or NaN): the first of the order.  -infinity never stays; a
  * row with +infinity draws among those; a row of NaN, or of nothing but
- * -infinity, gives token -1, prob 0, kept 0.  Sums are exact (whole numbers of
- * 2^-42 of the largest w or finer), so results are the same run to run. */
+ * -infinity, gives token -1, prob 0, kept 0.  Sums are those of w as whole numbers
+ * of 2^-42 of the largest (2^-51 for small vocabularies) and exact, so results are
+ * the same run to run. */
 typedef struct {             /* device arrays of n_rows, NULL: 1, 0, 1 and 0 */
     const float *temperature;
     const int *top_k;

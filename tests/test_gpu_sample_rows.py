@@ -154,6 +154,14 @@ def test_one_token_at_least_stays(gpu, n, o):
     check(gpu, x, uniform(4), **o)
 
 
+@pytest.mark.parametrize("m", [0.3, 1e-6, 1e-12, 1e-18])
+def test_tokens_around_min_p(gpu, m):
+    """Steps of 1e-5 around the least weight, however small that is."""
+    x = math.log(m) + 1e-5 * torch.arange(-2000, 2001, device="cuda", dtype=torch.float64)
+    x = torch.cat([x.new_zeros(1), x]).float()[None]
+    check(gpu, x.expand(3, -1).contiguous(), torch.tensor([0.2, 0.999, 0.9999999], device="cuda"), m=m)
+
+
 @pytest.mark.parametrize("t", [1e-30, 1e-4, 100.0, 1e6, 1e38, float("inf")])
 @pytest.mark.parametrize("o", [dict(), dict(k=9000, p=0.7), dict(m=0.9)])
 def test_extreme_temperatures(gpu, t, o):
