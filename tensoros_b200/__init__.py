@@ -8,6 +8,7 @@ for host numpy buffers (`ops`), and generates seeded workloads (`workloads`).
 from . import _ffi  # noqa: F401
 
 TYPE_F32, TYPE_F16, TYPE_Q4_0, TYPE_Q8_0 = 0, 1, 2, 8
+TYPE_I8, TYPE_F8_E4M3 = 24, 64        # elements of an 8-bit paged cache
 ATTN_EXACT, ATTN_FAST = 0, 1
 
 TOS_OK, TOS_EINVAL, TOS_ENOMEM, TOS_ECUDA, TOS_ENCCL, TOS_ETIMEOUT, TOS_ENOTSUP, TOS_ENODEV = (

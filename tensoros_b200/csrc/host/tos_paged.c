@@ -1,8 +1,8 @@
 /*
- * tos_paged.c - entry points of the paged-cache operators, over caches in
- * floats and in 8 bits, and of sampling a batch: argument checks, the rotation's frequency table, and
- * the hand-over to the tosk_* launchers (paged_rotary.cu, paged_attention.cu,
- * paged8_store.cu, paged8_decode.cu, sample_rows.cu).
+ * tos_paged.c - entry points of the paged-cache operators, over caches in floats
+ * and in 8 bits, and of sampling a batch: argument checks, the rotation's
+ * frequency table, and the hand-over to the tosk_* launchers (paged_rotary.cu,
+ * paged_attention.cu, paged8_store.cu, paged8_decode.cu, sample_rows.cu).
  */
 #include <math.h>
 #include <stdlib.h>

@@ -22,9 +22,9 @@
 // falls within ~1e-12 of a border.
 //
 // Bound: for few rows the chain of passes and of the cluster's waits (1 x 32000,
-// temperature and top-p: 18 us; 16 of them 26; with top-k and min-p in some 41); for
-// many the histogram's atomics and fp64 weights, about half of the time, and the
-// collecting (64 x 131072: 71 us, one read of HBM would be 5; the further passes find
+// top-k and top-p: 17 us; 16 of them, top-p 22; 33 x 50001 fp16, each with filters of its
+// own, 37); for many the histogram's instructions, about half of the time, and the
+// collecting (64 x 131072: 63 us, one read of HBM would be 5; the further passes find
 // the row in L2).
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
