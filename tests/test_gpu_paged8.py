@@ -531,6 +531,31 @@ def test_graph_replay_with_changed_lengths(gpu, hd):
                 assert torch.equal(kb[i].double(), k[-1])
 
 
+@pytest.mark.parametrize("n", [5, 20])
+def test_graph_replay_shares_the_keys_anew(gpu, n):
+    """Decode whose keys are dealt by the lengths (equal pieces; even shares), captured
+    once: each replay deals those that are there then, and gives an eager call's bits."""
+    heads, n_kv, hd, most = 32, 8, 128, 5000
+    c = Cache8([most] * n, 16, 16, n_kv, hd, I8, seed=n)
+    q = randn(n, heads, hd, seed=1)
+    out, kl = torch.empty_like(q), P.ints([most] * n)
+    size = gpu.tos_attention_decode_paged8_workspace_bytes(n, most, heads, n_kv, hd)
+    ws = torch.full((size,), 255, dtype=torch.uint8, device="cuda")
+    d, rq, ro = c.desc(), R.rows(q), R.rows(out)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        assert gpu.tos_attention_decode_paged8_dev(C.byref(ro), C.byref(rq), C.byref(d), kl.data_ptr(), n, most, heads, 0.1,
+                                                   ws.data_ptr(), size, torch.cuda.current_stream().cuda_stream) == 0
+    for step, lens in enumerate([ragged(n, most, 1), [0] * n, [most] + [0] * (n - 1), [1] * n, ragged(n, 700, 2), [most] * n]):
+        kl.copy_(P.ints(lens))
+        out.fill_(7.0)
+        g.replay()
+        want = P.check_decode(gpu, c, q, heads, scale=0.1, kv_lens=lens, max_kv=most, only=[0, n // 2, n - 1])
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), step
+
+
 def test_two_streams_at_once(gpu):
     """Calls on two streams beside one another, each with its own workspace."""
     c = Cache8([6000, 900], 16, 16, 2, 128, I8, seed=1)
