@@ -299,6 +299,7 @@ typedef struct {
     const int *cu_q;             /* NULL: one row a sequence (decode) */
     const int *kv_len;
     int n_seqs, total_q, max_q, max_kv, n_heads;
+    int room;                    /* > 0: keys of a sequence at most, whatever kv_len says and kv's table holds */
     const int *prefix_table;     /* decode */
     int prefix_len;
     float scale;
@@ -343,10 +344,11 @@ typedef struct {
 int tosk_paged8_put(const tosk_paged8_io_t *io, cudaStream_t st);
 int tosk_paged8_get(const tosk_paged8_io_t *io, cudaStream_t st);
 /* The keys of n_seqs sequences, at most total_kv in all, as an fp16 cache in ws
- * (256-byte aligned); *out describes it, *len are its sequences' lengths. */
+ * (256-byte aligned); *out describes it.  A sequence has those of its kv_len, max_kv
+ * and the rows that kv's table holds (tosk_paged_attn_t's room, for its readers) at most. */
 size_t tosk_paged8_wide_bytes(int n_seqs, long long total_kv, int max_kv, int n_kv, int hd);
 int tosk_paged8_wide(const tosk_paged8_t *kv, const int *kv_len, int n_seqs, long long total_kv, int max_kv, void *ws,
-                     tosk_paged_t *out, const int **len, cudaStream_t st);
+                     tosk_paged_t *out, cudaStream_t st);
 /* a->kv is not looked at */
 size_t tosk_paged8_prompt_ws_bytes(int n_seqs, int total_q, long long total_kv, int max_kv, int n_heads, int n_kv, int hd);
 int tosk_paged8_prompt(const tosk_paged_attn_t *a, const tosk_paged8_t *kv, long long total_kv, cudaStream_t st);

@@ -867,6 +867,19 @@ Plan8 plan8(int n_seqs, int max_kv, int heads, int n_kv, int hd) {
 bool direct(int hd) { return hd % 16 == 0; }
 size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 
+// A call over the cache's fp16 copy, which lies in front of its workspace.  The
+// copy's pages have room for more keys than the cache's table row may hold: keys end
+// there, while kv_len still says where the rows are.
+int over_copy(tosk_paged_attn_t& x, const tosk_paged8_t* kv, long long total_kv, cudaStream_t st) {
+  const size_t wide = tosk_paged8_wide_bytes(x.n_seqs, total_kv, x.max_kv, kv->n_kv, kv->hd);
+  const int e = tosk_paged8_wide(kv, x.kv_len, x.n_seqs, total_kv, x.max_kv, x.ws, &x.kv, st);
+  const long long room = (long long)kv->table_stride * kv->page_size;
+  x.room = (int)(room < x.max_kv ? room : x.max_kv);
+  x.ws = reinterpret_cast<uint8_t*>(x.ws) + wide;
+  x.ws_bytes -= wide;
+  return e;
+}
+
 }  // namespace
 
 extern "C" size_t tosk_paged8_decode_ws_bytes(int n_seqs, int max_kv, int n_heads, int n_kv, int hd) {
@@ -881,13 +894,8 @@ extern "C" size_t tosk_paged8_decode_ws_bytes(int n_seqs, int max_kv, int n_head
 extern "C" int tosk_paged8_decode(const tosk_paged_attn_t* t, const tosk_paged8_t* kv, cudaStream_t st) {
   tosk_paged_attn_t x = *t;
   if (!direct(kv->hd)) {
-    const long long total = (long long)x.n_seqs * x.max_kv;
-    const size_t wide = tosk_paged8_wide_bytes(x.n_seqs, total, x.max_kv, kv->n_kv, kv->hd);
-    const int e = tosk_paged8_wide(kv, x.kv_len, x.n_seqs, total, x.max_kv, x.ws, &x.kv, &x.kv_len, st);
-    if (e) return e;
-    x.ws = reinterpret_cast<uint8_t*>(x.ws) + wide;
-    x.ws_bytes -= wide;
-    return tosk_paged_decode(&x, st);
+    const int e = over_copy(x, kv, (long long)x.n_seqs * x.max_kv, st);
+    return e ? e : tosk_paged_decode(&x, st);
   }
   Dec8Args a;
   a.c = pool8_of(*kv);
@@ -932,10 +940,6 @@ extern "C" size_t tosk_paged8_prompt_ws_bytes(int n_seqs, int total_q, long long
 
 extern "C" int tosk_paged8_prompt(const tosk_paged_attn_t* t, const tosk_paged8_t* kv, long long total_kv, cudaStream_t st) {
   tosk_paged_attn_t x = *t;
-  const size_t wide = tosk_paged8_wide_bytes(x.n_seqs, total_kv, x.max_kv, kv->n_kv, kv->hd);
-  const int e = tosk_paged8_wide(kv, x.kv_len, x.n_seqs, total_kv, x.max_kv, x.ws, &x.kv, &x.kv_len, st);
-  if (e) return e;
-  x.ws = reinterpret_cast<uint8_t*>(x.ws) + wide;
-  x.ws_bytes -= wide;
-  return tosk_paged_prompt(&x, st);
+  const int e = over_copy(x, kv, total_kv, st);
+  return e ? e : tosk_paged_prompt(&x, st);
 }

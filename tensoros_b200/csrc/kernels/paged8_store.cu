@@ -368,7 +368,6 @@ struct WideArgs {
   const int* kv_len;
   __half *k, *v;
   int* table;                          // [n_seqs][stride]: the fp16 pool's pages
-  int* len;                            // [n_seqs]: kv_len within the rows that the cache's table holds
   int stride, max_kv, cap;             // cap: pages of the fp16 pool
   int keys;                            // a CTA, a power of two
   int vec;
@@ -386,8 +385,6 @@ __global__ void __launch_bounds__(256) paged8_wide_kernel(const __grid_constant_
     const int n = min(a.kv_len[s], a.max_kv);
     return (int)max(0ll, min((long long)n, room));
   };
-  if (blockIdx.x == 0)
-    for (int s = tid; s < c.n_seqs; s += 256) a.len[s] = (int)min((long long)a.kv_len[s], room);
   // the sequence of page pg: sequences' pages lie one behind the other
   const int parts = kWideRows / a.keys, pg = blockIdx.x / parts, part = blockIdx.x % parts;
   if (tid == 0) sseq = -1;
@@ -547,11 +544,11 @@ size_t wide_pool_bytes(long long pages, int n_kv, int hd) { return up256((size_t
 
 extern "C" size_t tosk_paged8_wide_bytes(int n_seqs, long long total_kv, int max_kv, int n_kv, int hd) {
   return 2 * wide_pool_bytes(wide_pages(n_seqs, total_kv), n_kv, hd) +
-         up256((size_t)n_seqs * ((size_t)max_kv / kWideRows + 1) * 4) + up256((size_t)n_seqs * 4);
+         up256((size_t)n_seqs * ((size_t)max_kv / kWideRows + 1) * 4);
 }
 
 extern "C" int tosk_paged8_wide(const tosk_paged8_t* kv, const int* kv_len, int n_seqs, long long total_kv, int max_kv, void* ws,
-                                tosk_paged_t* out, const int** len, cudaStream_t st) {
+                                tosk_paged_t* out, cudaStream_t st) {
   const long long pages = wide_pages(n_seqs, total_kv);
   const int keys = rows_a_cta(total_kv);
   if (pages > 0x7fffffffll / (kWideRows / keys)) return (int)cudaErrorInvalidValue;
@@ -564,8 +561,6 @@ extern "C" int tosk_paged8_wide(const tosk_paged8_t* kv, const int* kv_len, int 
   a.v = reinterpret_cast<__half*>(reinterpret_cast<uint8_t*>(ws) + pool);
   a.table = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(ws) + 2 * pool);
   a.stride = max_kv / kWideRows + 1;
-  a.len = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(a.table) + up256((size_t)n_seqs * a.stride * 4));
-  *len = a.len;
   a.max_kv = max_kv;
   a.cap = (int)pages;
   a.keys = keys;

@@ -440,7 +440,8 @@ PagedProblem problem_of(const tosk_paged_attn_t* a) {
   }
   p.table = a->kv.table; p.table_stride = a->kv.table_stride;
   p.cu_q = a->cu_q; p.kv_len = a->kv_len;
-  p.n_seqs = a->n_seqs; p.total_q = a->total_q; p.max_q = a->max_q; p.max_kv = a->max_kv;
+  p.n_seqs = a->n_seqs; p.total_q = a->total_q; p.max_q = a->max_q;
+  p.max_kv = a->room > 0 && a->room < a->max_kv ? a->room : a->max_kv;
   p.fixed_kv = -1;
   p.causal = 1;
   p.scale_log2 = a->scale * 1.4426950408889634f;
