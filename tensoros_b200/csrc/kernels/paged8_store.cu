@@ -368,7 +368,7 @@ struct WideArgs {
   const int* kv_len;
   __half *k, *v;
   int* table;                          // [n_seqs][stride]: the fp16 pool's pages
-  int stride, max_kv, cap;             // cap: pages of the fp16 pool
+  int stride, max_kv, cap;             // cap: pages of the fp16 pool, and of the grid
   int keys;                            // a CTA, a power of two
   int vec;
 };
@@ -387,6 +387,9 @@ __global__ void __launch_bounds__(256) paged8_wide_kernel(const __grid_constant_
   };
   // the sequence of page pg: sequences' pages lie one behind the other
   const int parts = kWideRows / a.keys, pg = blockIdx.x / parts, part = blockIdx.x % parts;
+  // where the pool has no room for all of them, the last CTA makes the table say so:
+  // an earlier call's page numbers may lie there
+  const bool marks = blockIdx.x == gridDim.x - 1;
   if (tid == 0) sseq = -1;
   int before = 0;
   for (int s0 = 0; s0 < c.n_seqs; s0 += 256) {
@@ -410,14 +413,22 @@ __global__ void __launch_bounds__(256) paged8_wide_kernel(const __grid_constant_
       sfirst = sum - n;
     }
     before += all;
-    if (before > pg) break;                               // the same for every thread
+    if (marks) {
+      for (uint32_t over = __ballot_sync(0xffffffffu, n > 0 && sum > a.cap); over; over &= over - 1) {
+        const int o = __ffs(over) - 1, no = __shfl_sync(0xffffffffu, n, o), first = __shfl_sync(0xffffffffu, sum, o) - no;
+        int* row = a.table + (long long)(s0 + warp * 32 + o) * a.stride;
+        for (int j = max(0, a.cap - first) + lane; j < no; j += 32) row[j] = -1;
+      }
+      before = min(before, a.cap);                        // 32 bits may not hold them all
+    } else if (before > pg) {                             // the same for every thread
+      break;
+    }
   }
   __syncthreads();
   const int seq = sseq;
   if (seq < 0) return;
   const int j = pg - sfirst, n = keys(seq);
-  if (part == 0 && tid == 0) a.table[(long long)seq * a.stride + j] = pg < a.cap ? pg : -1;
-  if (pg >= a.cap) return;
+  if (part == 0 && tid == 0) a.table[(long long)seq * a.stride + j] = pg;
   const int* table = c.table + (long long)seq * c.table_stride;
   const long long width = (long long)c.n_kv * c.hd;
   const int r0 = part * a.keys, key0 = j * kWideRows + r0, have = min(a.keys, n - key0);
