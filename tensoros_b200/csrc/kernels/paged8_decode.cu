@@ -443,12 +443,13 @@ __global__ void __launch_bounds__(32 * kD8Warps, HD == 256 || NQ == 2 ? 2 : TMA 
     auto ask_v = [&](int first, int slot) { copy(first, slot, c.v, &a.mv, c.vs); };
     auto arrived = [&](int slot) {
       asm volatile("cp.async.wait_group 2;" ::: "memory");          // all but the two tiles asked for last
-      bool ok = true;
+      __syncwarp();                                                 // what the other lanes' copies brought is read too
       if constexpr (TMA) {
-        ok = mbar_wait(bars + slot, phases >> slot & 1, p.err, 62);
+        const bool ok = mbar_wait(bars + slot, phases >> slot & 1, p.err, 62);
         phases ^= 1u << slot;
+        return __all_sync(0xffffffffu, ok) != 0;
       }
-      return __all_sync(0xffffffffu, ok) != 0;
+      return true;
     };
     // this lane's share of its query's row, asked for ahead of the keys
     float x[NQ][HD / 16][4];
