@@ -467,16 +467,17 @@ int launch8(const void* f, long long grid, int threads, const void* arg, cudaStr
   return (int)cudaLaunchKernelExC(&cfg, f, args);
 }
 
+bool few_pieces(int rows, const tosk_paged8_t& kv) { return (long long)rows * kv.n_kv * kv.hd / 8 <= kMostPieces; }
+
 // Rows that a CTA of 256 threads reads back, a power of two up to 128: as many as
 // give four CTAs an SM, so that few rows go to many CTAs and of many rows a CTA's
-// beginning is soon paid for.
-int rows_a_cta(long long rows) {
+// beginning is soon paid for; but no more than its 16-byte pieces may be (40,000
+// rows of 32 heads x 128: 64 a CTA 188 us; 128, which goes an element a lane, 1546).
+int rows_a_cta(long long rows, const tosk_paged8_t& kv) {
   int n = 1;
-  while (n < 128 && n * 4 * 148 < rows) n *= 2;
+  while (n < 128 && n * 4 * 148 < rows && few_pieces(2 * n, kv)) n *= 2;
   return n;
 }
-
-bool few_pieces(int rows, const tosk_paged8_t& kv) { return (long long)rows * kv.n_kv * kv.hd / 8 <= kMostPieces; }
 
 bool rows_on(const void* p, long long stride, int type, int bytes) {
   return ((uintptr_t)p & (bytes - 1)) == 0 && stride * (type == TOSK_F32 ? 4 : 2) % bytes == 0;
@@ -538,7 +539,7 @@ extern "C" int tosk_paged8_get(const tosk_paged8_io_t* io, cudaStream_t st) {
   a.cu = io->cu; a.kv_len = io->kv_len;
   a.n_tokens = io->n_tokens;
   const int type = io->k.dst ? io->k.dtype : io->v.dtype;
-  a.tokens = rows_a_cta(io->n_tokens);
+  a.tokens = rows_a_cta(io->n_tokens, io->kv);
   a.vec = io->kv.hd % 16 == 0 && few_pieces(a.tokens, io->kv) && rows_on(io->k.dst, io->k.dstride, type, 16) &&
           rows_on(io->v.dst, io->v.dstride, type, 16);
   const void* f = io->kv.type == TOSK_I8
@@ -561,7 +562,7 @@ extern "C" size_t tosk_paged8_wide_bytes(int n_seqs, long long total_kv, int max
 extern "C" int tosk_paged8_wide(const tosk_paged8_t* kv, const int* kv_len, int n_seqs, long long total_kv, int max_kv, void* ws,
                                 tosk_paged_t* out, cudaStream_t st) {
   const long long pages = wide_pages(n_seqs, total_kv);
-  const int keys = rows_a_cta(total_kv);
+  const int keys = rows_a_cta(total_kv, *kv);
   if (pages > 0x7fffffffll / (kWideRows / keys)) return (int)cudaErrorInvalidValue;
   const size_t pool = wide_pool_bytes(pages, kv->n_kv, kv->hd);
   WideArgs a;
