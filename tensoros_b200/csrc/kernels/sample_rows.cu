@@ -134,7 +134,9 @@ struct Row {
   double rate;                          // log2(e) / T
   float scale;                          // bins per unit of max - x
   const double* pow2;
-  __device__ __forceinline__ float place(float v) const { return (top - v) * scale; }
+  // Rounded before it is used, whatever the compiler may fuse: fine() takes a bin's
+  // number, which is this rounded down, from it, and that must not become negative.
+  __device__ __forceinline__ float place(float v) const { return __fmul_rn(top - v, scale); }
   __device__ __forceinline__ int bin(float v) const { return min(__float2int_rd(place(v)), kBins - 1); }
   __device__ __forceinline__ int fine(float v, int b) const {
     return min(__float2int_rd((place(v) - (float)b) * (b == kBins - 1 ? kFineLast : (float)kBins)), kBins - 1);
