@@ -347,7 +347,8 @@ int tos_kv_append_paged8_dev(const tos_paged8_kv_t *kv, const tos_rows_t *k, con
 int tos_kv_read_paged8_dev(const tos_paged8_kv_t *kv, const tos_rows_t *k_out, const tos_rows_t *v_out, const int *cu,
                            const int *kv_len, int n_seqs, int n_tokens, void *stream);
 
-/* tos_attention_prompt_paged_dev over this cache.  total_kv: no more keys than
+/* tos_attention_prompt_paged_dev over this cache.  kv_len may exceed what the table
+ * row holds: positions follow it, keys end with the row.  total_kv: no more keys than
  * this in all sequences together (keys beyond it may read as zeros).  The
  * workspace holds an fp16 copy of them, about (total_kv + 128 * n_seqs) * n_kv *
  * head_dim * 4 bytes, total_kv at most 2^32. */

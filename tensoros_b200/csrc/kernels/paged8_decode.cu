@@ -305,7 +305,9 @@ __device__ __forceinline__ void share_out(Share8& w, int n_seqs, int kinds, int 
 }
 
 // Four CTAs an SM at 128 registers a thread: sixteen warps (twelve, with 168: 4.1
-// TB/s over long sequences, sixteen 5.5; with spills in the loop 3.8).
+// TB/s over long sequences, sixteen 5.5; with the loop's operands spilled 3.8).  Some
+// instances keep a little in local memory: of 128 dims by TMA 36 bytes a thread (I8) and
+// 40 (F8).
 template <int HD, int NQ, int TYPE, bool TMA>
 __global__ void __launch_bounds__(32 * kD8Warps, HD == 256 || NQ == 2 ? 2 : TMA ? 4 : 3)
     paged8_decode_kernel(const __grid_constant__ Dec8Args a) {
